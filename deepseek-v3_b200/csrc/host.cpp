@@ -872,6 +872,8 @@ PyObject* py_drop_workspaces(PyObject*, PyObject*) {
     Py_RETURN_NONE;
 }
 
+#include "host_latent.inl"
+
 PyMethodDef methods[] = {
     {"set_error_class", py_set_error_class, METH_O, "class raised for a non-zero status: cls(status, message)"},
     {"act_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_act_quant)), METH_FASTCALL, "(x, block_size, scale_fmt)"},
@@ -894,6 +896,14 @@ PyMethodDef methods[] = {
      "(experts, x, weights, indices, n_routed, assume_no_inplace, shared)"},
     {"weights_pending", py_weights_pending, METH_O, "whether `combine` of this result still reads the experts' weights"},
     {"combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_combine)), METH_FASTCALL, "(routed, z)"},
+    {"latent_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_latent_write)), METH_FASTCALL,
+     "(latent, rope, scale, kv, weight, freqs, positions, slots, eps)"},
+    {"latent_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_latent_read)), METH_FASTCALL,
+     "(latent, rope, scale, block_table, cu_seqlens, total)"},
+    {"latent_keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_latent_keep)), METH_FASTCALL,
+     "(latent, rope, scale, block_table, first, path, count)"},
+    {"latent_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_latent_attention)), METH_FASTCALL,
+     "(q_latent, q_rope, latent, rope, scale, block_table, seq_lens, softmax_scale, cu_seqlens_q, tree_mask, return_lse)"},
     {"set_stats", py_set_stats, METH_O, "dict whose counters linear() keeps"},
     {"forget", py_forget, METH_NOARGS, "drop the remembered quantisations"},
     {"drop_workspaces", py_drop_workspaces, METH_NOARGS, "give the split-K workspaces back"},

@@ -312,6 +312,86 @@ int dsv3_few_down(const void* table2, int n, const void* route, const void* h, i
                   const dsv3_few_shared_t* shared, const void* z, void* y, dsv3_stream_t stream);
 
 /*
+ * The latent cache of MLA in 8 bits, and the attention that reads it -- what MLA.forward keeps of a token and what it does with it,
+ * model.py:468-472, 480-495 (there: bf16 buffers, and einsums over the whole prefix).
+ *
+ * A cached token is
+ *   latent : e4m3 [512]   the normalised latent divided by `scale`
+ *   rope   : bf16 [64]    the rotated key divided by `scale`
+ *   scale  : fp32         s, the least power of two with max(amax, 1e-4) <= 448 s, amax being the largest |latent|
+ * (e4m3 has its own exponent: a finer grid of scales would gain at most one bit at the bottom of the range, and a power of two costs
+ * the rotated values nothing).  A token with a value that is not finite has zero bytes and scale NaN: a query that sees it becomes NaN, one that does
+ * not is not touched by it.
+ * Tokens lie in pages of a pool: latent [n_pages, page_size, 512], rope [n_pages, page_size, 64], scale [n_pages, page_size], contiguous, latent and rope
+ * 16-byte aligned; page_size is a power of two from 16 on; n_pages * page_size < 2^31.  A token's slot is page * page_size + its place in the page.
+ * pages: int32 [n_seqs, pages_width], rows pages_stride apart: the pages of a sequence in order of position.  Entries behind a sequence's last
+ * token are not read; one that names no page of the pool makes its tokens absent (attention does not see them, read returns zeros, keep does not move them).
+ */
+#define DSV3_LATENT_DIM 512
+#define DSV3_ROPE_DIM 64
+typedef struct dsv3_latent_cache {
+    void* latent;
+    void* rope;
+    float* scale;
+    int64_t n_pages;
+    int page_size;
+    const int32_t* pages; /* not used by dsv3_latent_write */
+    int64_t pages_stride, pages_width;
+    int n_seqs;
+} dsv3_latent_cache_t;
+
+/*
+ * New tokens -- `kv, k_pe = split(wkv_a(x))`, kv_norm, apply_rotary_emb and the two stores of model.py:469-471, 484-485 in one launch.
+ *   kv        : bf16 [tokens, 576] with rows kv_stride apart (a multiple of 8; 16-byte aligned): 512 latent values, then 64 to rotate
+ *   weight    : [512] of the norm, bf16 or fp32 (weight_fp32); latent = kv / sqrt(mean(kv^2) + eps) * weight, in fp32
+ *   freqs     : complex64 [n_positions, 32], cos + i sin of every angle; pair j of a token's rotated values is multiplied by freqs[position, j]
+ *   positions : int64 [tokens]; a token whose position the table does not hold is stored as one that is not finite
+ *   slots     : int64 [tokens], all different; a token whose slot lies outside the pool is not stored
+ */
+int dsv3_latent_write(const dsv3_latent_cache_t* cache, const void* kv, int64_t kv_stride, const void* weight, int weight_fp32, float eps,
+                      const float* freqs, int64_t n_positions, const int64_t* positions, const int64_t* slots, int64_t tokens,
+                      dsv3_stream_t stream);
+
+/*
+ * The first cu_seqlens[b + 1] - cu_seqlens[b] tokens of every sequence, packed: latent bf16 [total, 512] and rope bf16 [total, 64], each value the exact
+ * product of what is stored and its scale (rounded to bf16 where it is too small for one).  cu_seqlens: int32 [n_seqs + 1] in device memory,
+ * starting at 0, not decreasing; rows at and beyond its last are left as they are.
+ */
+int dsv3_latent_read(const dsv3_latent_cache_t* cache, const int32_t* cu_seqlens, int64_t total, void* latent, void* rope,
+                     dsv3_stream_t stream);
+
+/*
+ * What is left of drafted tokens after their verification: of sequence b, which had first[b] tokens before the drafts, draft path[b, j] moves to
+ * position first[b] + j, for j < count[b].  path: int32 [n_seqs, drafts], rows path_stride apart, strictly ascending in its
+ * first count[b] entries (a path down a tree whose nodes are numbered parents first).  The pages that hold a sequence's drafts
+ * are no other sequence's (those of a shared prefix may be).
+ */
+int dsv3_latent_keep(const dsv3_latent_cache_t* cache, const int32_t* first, const int32_t* path, int64_t path_stride, int drafts,
+                     const int32_t* count, dsv3_stream_t stream);
+
+/*
+ * Attention of absorbed queries over the cache -- the scores, softmax and weighted sum of model.py:486-494:
+ *   out[t, h] = sum over the tokens p that t sees of softmax_p(softmax_scale * (q_latent[t, h] . c_p + q_rope[t, h] . k_p)) c_p
+ *   lse[t, h] = log of the sum of exp(softmax_scale * ...) (natural; optional: null)
+ *   q_latent : bf16 [tokens, heads, 512], q_rope : bf16 [tokens, heads, 64]; any strides of tokens and heads that are multiples of 8
+ *              elements, 16-byte aligned; 1 <= heads <= 1024
+ *   seq_lens : int32 [n_seqs] in device memory, tokens of each sequence in the cache, the queries' own among them; a length that its row of pages cannot hold is
+ *              taken as what that holds
+ *   cu_seqlens_q : int32 [n_seqs + 1] in device memory, starting at 0, not decreasing: sequence b owns queries [cu[b], cu[b + 1]); rows of out at
+ *              and beyond cu[n_seqs] are left as they are.  Null: tokens / n_seqs queries each.
+ *   tree_mask : null: the queries of a sequence are its last tokens, each sees itself and all before it.  Else int64 [tokens], a word per query: the
+ *              queries' own tokens are still the last ones of their sequence; a query sees all before them, and of them those whose bit is
+ *              set (bit j: the j-th; from the 64th on none is seen).
+ *   out      : bf16 [tokens, heads, 512], lse : fp32 [tokens, heads].  A query that sees nothing: zeros, and -inf.
+ * workspace: dsv3_latent_attention_workspace_bytes() bytes, 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
+ */
+size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest);
+int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
+                          const void* q_rope, int64_t q_rope_token_stride, int64_t q_rope_head_stride, int64_t tokens, int heads,
+                          const int32_t* seq_lens, const int32_t* cu_seqlens_q, const int64_t* tree_mask, float softmax_scale, void* out,
+                          float* lse, void* workspace, size_t workspace_bytes, dsv3_stream_t stream);
+
+/*
  * One-shot all-reduce of a decode-sized bf16 tensor over peer-mapped buffers -- replaces `dist.all_reduce(y)` after
  * a row-parallel Linear and after the MoE expert loop (model.py:263-264, 691-692) for small y, where a ring or tree
  * collective is bound by latency.  One process per GPU; every rank
