@@ -1,71 +1,831 @@
 // Attention of absorbed MLA queries over the 8-bit latent cache (see include/dsv3_b200.h).
+//
+//   x[r, p] = q_latent[r] . c8[p] + q_rope[r] . k16[p]           r: a query head, p: a cached token, c8 and k16 as stored (divided by s[p])
+//   y[r, p] = x[r, p] * s[p] * k[r] + log2 s[p]                   k[r]: softmax_scale, log2(e) and the row's own scale
+//   out[r]  = sum_p 2^(y - m) c8[p] / sum_p 2^(y - m) / s[p]      m: the row's running maximum of y
+//
+// Both products run on e4m3 operands as they lie in the cache: nothing is converted to 16 bits on the way, which would cost a conversion and a
+// trip through shared memory per cached value.  What is not 8 bits wide is split in two e4m3 values: a bf16 query has 8 significant bits, so that
+// hi = e4m3(q), lo = e4m3(q - hi) is the query itself (scaled by a power of two per row, and down to 2^-18 of the row's largest value); a weight 2^(y - m) is off by
+// at most 2^-8 of itself, what rounding it to bf16 would cost.  Two e4m3 products take the time of one in bf16, and half the operand bytes.
+//   The token's scale is a factor of its scores and, taken into the exponent as log2 s, of its weight in the second product.
+//   Rounding of small weights: lo is stored times 16, so that its grid is 2^-13 of a scale on which the row's largest weight lies in [2^7, 2^8); what is
+// below half of that would round to zero, and thousands of tokens that each weigh 2^-21 of one first token do matter.  So a fixed offset
+// per token, evenly spread over a step of the grid, is added before rounding: sums of small weights stay what they are.
+//
+// The tokens are the rows of both MMAs (128 of them) and the query heads the columns: with 16 query heads (one decoding sequence on one rank of
+// eight) nothing is padded, and a tile costs what its 128 x 32 bytes per step take to be read from shared memory.
+//   S^T [128 tokens, hi | lo]  = C [128, 512] Q^T,  S_rope^T [128, R] = K [128, 64] Q_rope^T (bf16),  O^T [4 x 128 dims, hi | lo] += C^T P^T
+// hi and lo stand side by side as columns, which reads C once for both.  C is the MMA's A operand in both products, K-major in the first and transposed
+// (MN-major) in the second, from the same bytes.
+#include <cuda.h>
+
 #include "latent_cache.cuh"
+#include "tc_wait.cuh"
 
 namespace dsv3 {
+
+int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows);
+
 namespace {
+
+constexpr int kTokens = 128;              // of a tile: MMA M of the first product, K of the second
+constexpr int kUnitBytes = kTokens * 128; // 128 bytes of each of a tile's tokens: a quarter of the latents, or the rotated values
+constexpr int kTileUnits = 5;
+constexpr int kSoftmaxWarps = 8, kFirstSoftmaxWarp = 4;
+constexpr int kAttnThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
+constexpr int kScaleSlots = 4;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// The running maximum moves when a score exceeds it by more than kSlack, and stands for 2^kTop: the largest weight is 2^8.
+constexpr float kSlack = 1.0f, kTop = 7.0f;
+constexpr float kLoScale = 16.0f;         // the largest remainder is 2^-4 of 2^8
 
 struct Queries {
     const __nv_bfloat16 *latent, *rope;
     int64_t latent_token, latent_head, rope_token, rope_head;   // strides in elements
-    int64_t tokens;
-    int heads;
-    const int32_t *seq_lens, *cu;       // cu: null for tokens / n_seqs queries a sequence
+    int tokens, heads;
+    const int32_t *seq_lens, *cu;         // cu: null for `per` queries a sequence
+    int per;
     const int64_t* tree;
     float scale;
     __nv_bfloat16* out;
     float* lse;
+    // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
+    int head_blocks, block_shift;
+    float* partial;                       // [2 * grid][R, 512]
+    float* partial_lse;                   // [2 * grid][R]
+    int4* cut;                            // [grid]: the item that begins in a CTA and ends in a later one
 };
 
-// A warp to a query head, a token at a time with a running maximum and sum.
-__global__ void __launch_bounds__(128) latent_attention_simple_kernel(LatentCache c, Queries q) {
+template <int R>
+struct Cfg {
+    static constexpr int kUnits = R == 16 ? 12 : 10;
+    static constexpr int kQChunk = 2 * R * 128;                 // hi and lo rows of 128 latents
+    static constexpr int kQBytes = 4 * kQChunk + R * 128;
+    static constexpr int kPBytes = kTokens * 2 * R;
+    static constexpr int kRows = R / 2;                         // of a softmax warp
+    static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
+    static constexpr int kTmemO = 2 * kTmemS;
+    static constexpr int kTmemCols = R == 16 ? 256 : 512;
+    static_assert(kTmemO + 8 * R <= kTmemCols, "TMEM");
+};
+
+template <int R>
+struct Small {                                                  // shared memory beside the operand tiles
+    float scales[kScaleSlots][kTokens];
+    float factor[2][R];                                         // k[r] by item parity
+    int64_t tree[2][R];
+    int place[2][R];                                            // query * heads + head, -1 for a row that is none
+    int limit[2][R];                                            // last position that a row sees (a tree: of those before the queries)
+    float top[2][2][4][R / 2];                                  // [tile parity][half][warp][row]
+    float sum[2][4][R / 2];
+    float row[kSoftmaxWarps][R / 2], row2[kSoftmaxWarps][R / 2];
+    uint64_t full[Cfg<R>::kUnits], empty[Cfg<R>::kUnits];
+    uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
+    Control ctl;
+    int64_t warp_sum[kAttnThreads / 32];
+    int64_t start_offset;
+    int start_seq;
+};
+
+template <int R>
+constexpr int smem_bytes() {
+    return 1024 + Cfg<R>::kUnits * kUnitBytes + Cfg<R>::kQBytes + 2 * Cfg<R>::kPBytes + static_cast<int>(sizeof(Small<R>));
+}
+static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
+
+// ---------------------------------------------------------------- PTX
+__device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t* r) {
+    static_assert(N == 8 || N == 16, "columns");
+    if constexpr (N == 8) tc_ld_x8(taddr, r);
+    else tc_ld_x16(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t* r) {
+    static_assert(N == 8 || N == 16, "columns");
+    if constexpr (N == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                     "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+    else
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                     "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                     "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                     : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Operand descriptor of a transposed (MN-major) tile with rows of kWidth bytes, one row per step of K, swizzled over kWidth bytes: groups of eight rows are
+// 8 * kWidth bytes apart.  The tile is one swizzle atom wide, so that the offset between atoms is not used.
+template <int kWidth>
+__device__ __forceinline__ uint64_t umma_desc_mn_major(uint32_t smem_addr) {
+    static_assert(kWidth == 32 || kWidth == 64 || kWidth == 128, "swizzle width");
+    constexpr uint64_t layout = kWidth == 128 ? 2 : kWidth == 64 ? 4 : 6;
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(8 * kWidth >> 4) << 16;
+    d |= static_cast<uint64_t>(8 * kWidth >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= layout << 61;
+    return d;
+}
+constexpr uint32_t kIdescTransposed = (1u << 15) | (1u << 16);                      // A and B MN-major
+constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f32(m, n) | (1u << 7) | (1u << 10); }
+
+// ---------------------------------------------------------------- who works on what
+// The work is a list of tiles: for every sequence, block of its query heads and 128 cached tokens that some row of the block sees one (at least one
+// per block, which writes the zeros of rows that see nothing).  A CTA takes an equal, contiguous share of the list, whatever the lengths are; a block's
+// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  Every role walks the
+// list by itself.
+struct Seq {
+    int len, queries, first;              // cached tokens, queries, index of the first query
+};
+__device__ __forceinline__ Seq load_seq(const LatentCache& c, const Queries& q, int s) {
+    const int64_t cap = static_cast<int64_t>(c.pages_width) << c.page_shift;
+    Seq r;
+    r.len = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(q.seq_lens[s]), cap)));
+    r.first = q.cu ? q.cu[s] : s * q.per;
+    // (offsets that lead out of the queries are cut off)
+    const int end = q.cu ? q.cu[s + 1] : r.first + q.per;
+    r.first = max(0, min(r.first, q.tokens));
+    r.queries = max(0, min(end, q.tokens) - r.first);
+    return r;
+}
+__device__ __forceinline__ int tiles_of(int tokens) { return tokens <= kTokens ? 1 : (tokens - 1) / kTokens + 1; }
+__device__ __forceinline__ int blocks_of(const Queries& q, const Seq& s) { return (s.queries + (1 << q.block_shift) - 1) >> q.block_shift; }
+// Tiles that a block of tokens sees: all, or those up to its last token's own position
+__device__ __forceinline__ int block_tiles(const Queries& q, const Seq& s, int block) {
+    if (q.tree) return tiles_of(s.len);
+    return tiles_of(s.len - s.queries + min((block + 1) << q.block_shift, s.queries));
+}
+// sum over j = 1 .. x of max(1, ceil(j / m)); x <= 0: what is to be subtracted for j = x + 1 .. 0
+__device__ __forceinline__ int64_t ramp(int64_t x, int shift) {
+    if (x <= 0) return x;
+    const int64_t m = 1ll << shift, n = x >> shift;
+    return m * (n * (n + 1) / 2) + (x - (n << shift)) * (n + 1);
+}
+// Tiles of a sequence's first n blocks of tokens (of one block of heads).  Block i sees base + (i + 1) 2^b tokens (the last one: all); with m = 128 / 2^b that
+// is ceil((u + i + 1) / m) tiles, where u = ceil(base / 2^b).
+__device__ __forceinline__ int64_t tiles_before(const Queries& q, const Seq& s, int n, int blocks) {
+    if (n == 0) return 0;
+    if (q.tree) return static_cast<int64_t>(n) * tiles_of(s.len);
+    const int64_t u = (static_cast<int64_t>(s.len) - s.queries + (1 << q.block_shift) - 1) >> q.block_shift;
+    const int shift = 7 - q.block_shift;
+    const int whole = n == blocks ? n - 1 : n;
+    return ramp(u + whole, shift) - ramp(u, shift) + (n == blocks ? tiles_of(s.len) : 0);
+}
+
+struct Walk {
+    Seq s;
+    int seq, block, head_block;
+    int tile, n, tiles;                   // first tile of the item, how many, how many the whole block has
+    int64_t left;                         // of the CTA's share, behind this item
+
+    __device__ void settle(const Queries& q) {
+        tiles = block_tiles(q, s, block);
+        n = static_cast<int>(min(static_cast<int64_t>(tiles - tile), left));
+        left -= n;
+    }
+    // the share starts at tile `offset` of sequence `sq`
+    __device__ void begin(const LatentCache& c, const Queries& q, int sq, int64_t offset, int64_t share) {
+        seq = sq;
+        s = load_seq(c, q, sq);
+        const int blocks = blocks_of(q, s);
+        int lo = 0, hi = blocks;          // largest block whose tiles begin at or before the offset
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (tiles_before(q, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
+            else hi = mid;
+        }
+        offset -= tiles_before(q, s, lo, blocks) * q.head_blocks;
+        block = lo;
+        const int t = block_tiles(q, s, lo);
+        head_block = static_cast<int>(offset / t);
+        tile = static_cast<int>(offset - static_cast<int64_t>(head_block) * t);
+        left = share;
+        settle(q);
+    }
+    __device__ bool next(const LatentCache& c, const Queries& q) {
+        if (left == 0) return false;
+        tile = 0;
+        if (++head_block == q.head_blocks) {
+            head_block = 0;
+            if (++block >= blocks_of(q, s)) {
+                block = 0;
+                do s = load_seq(c, q, ++seq);
+                while (s.queries == 0);
+            }
+        }
+        settle(q);
+        return true;
+    }
+};
+
+// All threads: this CTA's share [*first, *first + share) of the list, and where in which sequence it starts.
+template <typename Sm>
+__device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, int64_t* total_out, int64_t* first_out) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const auto mine = [&](int s) -> int64_t {
+        if (s >= c.n_seqs) return 0;
+        const Seq x = load_seq(c, q, s);
+        const int b = blocks_of(q, x);
+        return tiles_before(q, x, b, b) * q.head_blocks;
+    };
+    const int64_t kept = mine(threadIdx.x);
+    const auto scan = [&](int64_t v, int64_t* sum) -> int64_t {       // tiles of the threads before this one; *sum: of all
+        int64_t run = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += u;
+        }
+        __syncthreads();
+        if (lane == 31) sm.warp_sum[warp] = run;
+        __syncthreads();
+        int64_t before = run - v, all = 0;
+        for (int w = 0; w < kAttnThreads / 32; ++w) {
+            if (w < warp) before += sm.warp_sum[w];
+            all += sm.warp_sum[w];
+        }
+        *sum = all;
+        return before;
+    };
+    int64_t total, sum;
+    const int64_t kept_before = scan(kept, &total);
+    for (int s0 = kAttnThreads; s0 < c.n_seqs; s0 += kAttnThreads) {
+        scan(mine(s0 + threadIdx.x), &sum);
+        total += sum;
+    }
+    // (no CTA between two that work on the same block is without a tile)
+    const int64_t ctas = min(total, static_cast<int64_t>(gridDim.x)), at_cta = min(static_cast<int64_t>(blockIdx.x), ctas);
+    const int64_t first = ctas ? total * at_cta / ctas : 0, share = at_cta < ctas ? total * (at_cta + 1) / ctas - first : 0;
+    *total_out = total;
+    *first_out = first;
+    if (share == 0) return 0;
+    int64_t at = 0;
+    for (int s0 = 0; s0 < c.n_seqs && at <= first; s0 += kAttnThreads) {
+        const int64_t v = s0 ? mine(s0 + threadIdx.x) : kept;
+        int64_t before = kept_before;
+        sum = 0;
+        if (s0 || c.n_seqs > kAttnThreads) before = scan(v, &sum) + at;
+        if (before <= first && first < before + v) {
+            sm.start_seq = s0 + threadIdx.x;
+            sm.start_offset = first - before;
+        }
+        at += sum;
+        if (c.n_seqs <= kAttnThreads) break;
+    }
+    __syncthreads();
+    return share;
+}
+
+// ---------------------------------------------------------------- reductions over a tile's tokens
+// v[i] of 32 lanes, i < N rows: afterwards every lane holds the reduction of row own_row<N>() over the lanes.  Every exchange halves the rows that a lane
+// goes on with: N - 1 + log2(32 / N) shuffles instead of 5 N.
+template <int N>
+__device__ __forceinline__ int own_row() { return (threadIdx.x & 31) / (32 / N); }
+template <int N, typename Op>
+__device__ __forceinline__ float reduce_rows(float (&v)[N], Op op) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = N / 2, o = 16; half >= 1; half >>= 1, o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float keep = up ? v[i + half] : v[i], give = up ? v[i] : v[i + half];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+    }
+#pragma unroll
+    for (int o = 16 / N; o >= 1; o >>= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    return v[0];
+}
+
+template <int N>
+__device__ __forceinline__ void broadcast_rows(float* to, float own, float (&v)[N]) {     // `to`: N floats of this warp
+    __syncwarp();
+    if ((threadIdx.x & 31) % (32 / N) == 0) to[own_row<N>()] = own;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(to + i);
+        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+}
+
+// ---------------------------------------------------------------- the kernel
+// Warp 0 loads, warp 1 issues the MMAs, warps 4 to 11 do the softmax: four of them (one per quarter of the 128 TMEM lanes, a lane a token) for each half of the rows.
+template <int R>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __grid_constant__ CUtensorMap map_rope, const LatentCache c, const Queries q,
+                        unsigned int* status) {
+    using C = Cfg<R>;
+    constexpr int N = C::kRows;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* const units = smem;
+    uint8_t* const qs = units + C::kUnits * kUnitBytes;
+    uint8_t* const ps = qs + C::kQBytes;
+    Small<R>& sm = *reinterpret_cast<Small<R>*>(ps + 2 * C::kPBytes);
+    Control* const ctl = &sm.ctl;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const auto bar = [](const uint64_t& b) { return smem_u32(&b); };
+
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kUnits; ++i) {
+            mbar_init(bar(sm.full[i]), 1);
+            mbar_init(bar(sm.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(sm.s_full[i]), 1);
+            mbar_init(bar(sm.s_empty[i]), kSoftmaxWarps);
+            mbar_init(bar(sm.p_full[i]), kSoftmaxWarps);
+            mbar_init(bar(sm.p_empty[i]), 1);
+        }
+        mbar_init(bar(sm.q_full), kSoftmaxWarps);
+        mbar_init(bar(sm.o_empty), kSoftmaxWarps);
+        mbar_fence_init();
+        ctl->abort_flag = 0;
+    }
+    if (warp == 1) tc_alloc(smem_u32(&ctl->tmem_base), C::kTmemCols);
+    if (warp == 0) {
+        tma_prefetch_desc(&map_latent);
+        tma_prefetch_desc(&map_rope);
+    }
+    griddep_wait();
+    int64_t total, first;
+    const int64_t share = find_share(c, q, sm, &total, &first);     // (its barriers also publish what was set up above)
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    if (threadIdx.x == 32 * kFirstSoftmaxWarp && q.cut) q.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+
+    Walk w;
+    if (share > 0) w.begin(c, q, sm.start_seq, sm.start_offset, share);
+
+    if (share == 0) {
+        // nothing to do
+    } else if (warp == 0) {
+        // ------------------------------------------------------------ loads: a lane to each box of a tile's tokens
+        const int page_rows = 1 << c.page_shift, rows = min(page_rows, kTokens);
+        const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
+        uint32_t unit = 0;
+        bool ok = true;
+        int slot = 0, tile_count = 0;
+        do {
+            for (int t = 0; t < w.n && ok; ++t, ++tile_count) {
+                const int p0 = (w.tile + t) * kTokens + lane * rows;
+                const bool here = lane < kTokens / rows && p0 < w.s.len;
+                const int boxes = __popc(__ballot_sync(0xffffffffu, here));
+                const int at = here ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -1;
+                const int present = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                const int y = static_cast<int>(at >= 0 ? static_cast<uint32_t>(at) : outside);
+                float* const scales = sm.scales[tile_count & (kScaleSlots - 1)] + lane * rows;
+                for (int u = 0; u < kTileUnits; ++u) {
+                    const uint32_t full = bar(sm.full[slot]);
+                    uint32_t free = 1;
+                    if (lane == 0) free = bounded_wait(bar(sm.empty[slot]), ((unit / C::kUnits) & 1) ^ 1, ctl, status, 1, unit);
+                    free = __shfl_sync(0xffffffffu, free, 0);
+                    ok = free != 0;
+                    if (!ok) break;
+                    if (u == 0) {
+                        if (here && at < 0)                                    // an absent page: its tokens have no scale
+                            for (int i = 0; i < rows; ++i) scales[i] = 0.0f;
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(full, boxes * rows * 128 + (u == 0 ? present * rows * 4 : 0));
+                    __syncwarp();
+                    if (here) {
+                        const uint32_t dst = smem_u32(units + slot * kUnitBytes) + lane * rows * 128;
+                        if (u < 4) tma_load_2d(dst, &map_latent, u * 128, y, full);
+                        else tma_load_2d(dst, &map_rope, 0, y, full);
+                        if (u == 0 && at >= 0) bulk_load(smem_u32(scales), c.scale + at, rows * 4, full);
+                    }
+                    ++unit;
+                    if (++slot == C::kUnits) slot = 0;
+                }
+            }
+        } while (ok && w.next(c, q));
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMAs: one elected lane
+        if (elect_one()) {
+            constexpr uint32_t idesc_s = umma_idesc_e4m3_f32(kTokens, 2 * R), idesc_r = idesc_bf16(kTokens, R);
+            constexpr uint32_t idesc_o = idesc_s | kIdescTransposed;
+            const uint32_t units_at = smem_u32(units), q_at = smem_u32(qs), p_at = smem_u32(ps);
+            uint32_t s_count = 0, p_count = 0, item = 0;                       // tiles whose scores, whose sums have been issued
+            // scores of tile s_count, in the ring from unit 5 * s_count on
+            const auto scores = [&]() -> bool {
+                const uint32_t b = s_count & 1, d = tmem + b * C::kTmemS;
+                if (!bounded_wait(bar(sm.s_empty[b]), ((s_count >> 1) & 1) ^ 1, ctl, status, 3, s_count)) return false;
+                tc_fence_after();
+                for (int u = 0; u < kTileUnits; ++u) {
+                    const uint32_t unit = s_count * kTileUnits + u, at = unit % C::kUnits;
+                    if (!bounded_wait(bar(sm.full[at]), (unit / C::kUnits) & 1, ctl, status, 2, unit)) return false;
+                    const uint64_t da = umma_desc_k_major_sw128(units_at + at * kUnitBytes);
+                    const uint64_t db = umma_desc_k_major_sw128(q_at + u * C::kQChunk);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {                              // 32 bytes of K a step
+                        if (u < 4) tc_mma_f8(d, da + 2 * k, db + 2 * k, idesc_s, (u | k) != 0);
+                        else tc_mma_bf16(d + 2 * R, da + 2 * k, db + 2 * k, idesc_r, k != 0);
+                    }
+                    if (u == 4) {
+                        tc_commit(bar(sm.empty[at]));
+                        tc_commit(bar(sm.s_full[b]));
+                    }
+                }
+                ++s_count;
+                return true;
+            };
+            const auto sums = [&](bool fresh) -> bool {
+                const uint32_t b = p_count & 1;
+                if (!bounded_wait(bar(sm.p_full[b]), (p_count >> 1) & 1, ctl, status, 11, p_count)) return false;
+                tc_fence_after();
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t at = (p_count * kTileUnits + u) % C::kUnits;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)                                // 32 tokens a step
+                        tc_mma_f8(tmem + C::kTmemO + u * 2 * R, umma_desc_mn_major<128>(units_at + at * kUnitBytes + k * 32 * 128),
+                                  umma_desc_mn_major<2 * R>(p_at + b * C::kPBytes + k * 32 * 2 * R), idesc_o, !fresh || k != 0);
+                    tc_commit(bar(sm.empty[at]));
+                }
+                tc_commit(bar(sm.p_empty[b]));
+                ++p_count;
+                return true;
+            };
+            bool ok = true;
+            do {
+                ok = bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item);
+                ok = ok && scores();
+                for (int t = 0; t < w.n && ok; ++t) {
+                    if (t + 1 < w.n) ok = scores();
+                    // (the first sums of an item overwrite those of the item before it)
+                    if (ok && t == 0) ok = bounded_wait(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, 12, item);
+                    ok = ok && sums(t == 0);
+                }
+                ++item;
+            } while (ok && w.next(c, q));
+        }
+        __syncwarp();
+    } else if (warp >= kFirstSoftmaxWarp) {
+        // ------------------------------------------------------------ softmax
+        const int sw = warp - kFirstSoftmaxWarp, half = sw >> 2, quarter = sw & 3;
+        const int token = quarter * 32 + lane;                                 // of the tile: this thread's TMEM lane
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const float dither = static_cast<float>((token * 79) & 127) * 0x1p-16f - 0x1.fcp-11f;   // evenly over (-2^-10, 2^-10), half a step either side
+        uint32_t tile_count = 0, item = 0;
+        bool ok = true;                                                        // the same in all lanes of a warp
+        const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t counter) -> bool {
+            return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, counter));
+        };
+        do {
+            const uint32_t par = item & 1;
+            // -------- the block's rows: a warp to every eighth row
+            for (int r = sw; r < R; r += kSoftmaxWarps) {
+                int tok = w.block << q.block_shift, head = w.head_block * R + r;
+                if (q.head_blocks == 1) {
+                    tok += r / q.heads;
+                    head = r % q.heads;
+                }
+                const bool valid = head < q.heads && tok < w.s.queries && (q.head_blocks > 1 || r < q.heads << q.block_shift);
+                uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                uint32_t pair = 0;
+                if (valid) {
+                    const int64_t row = w.s.first + tok;
+                    const uint4* src = reinterpret_cast<const uint4*>(q.latent + row * q.latent_token + head * q.latent_head);
+                    v[0] = src[lane * 2], v[1] = src[lane * 2 + 1];
+                    pair = reinterpret_cast<const uint32_t*>(q.rope + row * q.rope_token + head * q.rope_head)[lane];
+                }
+                float x[16], top = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t word = reinterpret_cast<const uint32_t*>(v)[i];
+                    x[2 * i] = bf16_bits_to_float(word & 0xFFFFu);
+                    x[2 * i + 1] = __uint_as_float(word & 0xFFFF0000u);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    top = fmaxf(top, fabsf(x[i]));
+                    finite = finite && fabsf(x[i]) < INFINITY;
+                }
+                float re = bf16_bits_to_float(pair & 0xFFFFu), im = __uint_as_float(pair & 0xFFFF0000u);
+                finite = __all_sync(0xffffffffu, finite && fabsf(re) < INFINITY && fabsf(im) < INFINITY);
+                // (the rotated half is held divided by the same scale, in bf16: the scale is kept from being too small for that)
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(re), fabsf(im)) * 0x1p-40f), 0x1p-100f);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float s = finite ? power_scale(top) : 1.0f, inv = finite ? power_reciprocal(s) : 0.0f;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = finite ? x[2 * i] * inv : 0.0f, b = finite ? x[2 * i + 1] * inv : 0.0f;
+                    const uint16_t h = cvt_e4m3x2(a, b);
+                    const float2 f = e4m3x2_to_float2(h);
+                    const uint16_t l = cvt_e4m3x2(a - f.x, b - f.y);
+                    if (i & 1) hi[i / 2] |= static_cast<uint32_t>(h) << 16, lo[i / 2] |= static_cast<uint32_t>(l) << 16;
+                    else hi[i / 2] = h, lo[i / 2] = l;
+                }
+                uint8_t* const chunk = qs + (lane >> 3) * C::kQChunk + (((lane & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(chunk + r * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(chunk + (R + r) * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint32_t*>(qs + 4 * C::kQChunk + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) =
+                    finite ? pack_bf16x2(re * inv, im * inv) : 0u;
+                if (lane == 0) {
+                    const int base = w.s.len - w.s.queries;
+                    sm.place[par][r] = valid ? (w.s.first + tok) * q.heads + head : -1;
+                    sm.factor[par][r] = !valid ? 0.0f : finite ? s * q.scale * kLog2e : __uint_as_float(0x7FC00000u);
+                    sm.limit[par][r] = q.tree ? base - 1 : base + tok;
+                    sm.tree[par][r] = q.tree && valid ? q.tree[w.s.first + tok] : 0;
+                }
+            }
+            fence_proxy_async_shared();
+            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);                       // factors and limits of all rows
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(bar(sm.q_full));
+
+            float l[N], m = -INFINITY;                                         // m: of row own_row<N>()
+#pragma unroll
+            for (int i = 0; i < N; ++i) l[i] = 0.0f;
+            const int base = w.s.len - w.s.queries;                            // position of the first query's token
+            for (int t = 0; t < w.n; ++t, ++tile_count) {
+                const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
+                const uint32_t unit = tile_count * kTileUnits;
+                const int p = (w.tile + t) * kTokens + token;
+                ok = ok && wait(sm.full[unit % C::kUnits], (unit / C::kUnits) & 1, 2, unit);
+                const float sc = sm.scales[tile_count & (kScaleSlots - 1)][token];
+                ok = ok && wait(sm.s_full[b], phase, 4, tile_count);
+                tc_fence_after();
+                float y[N];
+                {
+                    uint32_t hi[N], lo[N], ro[N];
+                    const uint32_t at = tmem + lanes + b * C::kTmemS + half * N;
+                    tc_ld<N>(at, hi);
+                    tc_ld<N>(at + R, lo);
+                    tc_ld<N>(at + 2 * R, ro);
+                    tc_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(sm.s_empty[b]));
+                    const float e = static_cast<float>(static_cast<int>(__float_as_uint(sc) >> 23) - 127);     // log2 of a power of two
+                    const float4* const k = reinterpret_cast<const float4*>(sm.factor[par] + half * N);
+#pragma unroll
+                    for (int i = 0; i < N; i += 4) {
+                        const float4 f = k[i / 4];
+                        const float g[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            y[i + j] = fmaf((__uint_as_float(hi[i + j]) + __uint_as_float(lo[i + j])) + __uint_as_float(ro[i + j]), sc * g[j], e);
+                    }
+                }
+                const bool present = p < w.s.len && sc != 0.0f;
+                if (!__all_sync(0xffffffffu, present && p < base)) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int r = half * N + i;
+                        bool seen = p <= sm.limit[par][r];
+                        if (q.tree) seen = seen || (p >= base && p - base < 64 && ((sm.tree[par][r] >> (p - base)) & 1));
+                        if (!present || !seen) y[i] = -INFINITY;
+                    }
+                }
+                float mv[N];
+                bool moved;
+                float old = m;
+                {
+                    float v[N];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[i] = y[i];
+                    const float top = reduce_rows<N>(v, [](float a, float b2) { return fmaxf(a, b2); });
+                    if (lane % (32 / N) == 0) sm.top[b][half][quarter][own_row<N>()] = top;
+                    ok = barrier_all<128>(1 + half, ok);
+                    if (!ok) break;
+                    float all = sm.top[b][half][0][own_row<N>()];
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) all = fmaxf(all, sm.top[b][half][i][own_row<N>()]);
+                    moved = all > m + kSlack || (m == -INFINITY && all > m);
+                    if (moved) m = all;
+                    broadcast_rows<N>(sm.row[sw], m == -INFINITY ? 0.0f : m - kTop, mv);
+                }
+                // -------- sums so far take the new maximum
+                if (t > 0 && __any_sync(0xffffffffu, moved && old != -INFINITY)) {
+                    float f[N];
+                    broadcast_rows<N>(sm.row2[sw], moved ? ex2(old - m) : 1.0f, f);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) l[i] *= f[i];
+                    const uint32_t before = tile_count - 1;
+                    ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
+                    tc_fence_after();
+                    if (ok) {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {                          // hi and lo of four times 128 dimensions
+                            uint32_t o[N];
+                            const uint32_t at = tmem + lanes + C::kTmemO + u * R + half * N;
+                            tc_ld<N>(at, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < N; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[i]);
+                            tc_st<N>(at, o);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                // -------- weights: hi and lo, to shared memory
+                if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, 12, tile_count);
+                if (ok) {
+                    const float inv = present ? power_reciprocal(sc) : 0.0f;
+                    uint32_t hi[N / 4], lo[N / 4];
+#pragma unroll
+                    for (int i = 0; i < N; i += 2) {
+                        const float a = ex2(y[i] - mv[i]), d = ex2(y[i + 1] - mv[i + 1]);
+                        l[i] = fmaf(a, inv, l[i]);
+                        l[i + 1] = fmaf(d, inv, l[i + 1]);
+                        const uint16_t h = cvt_e4m3x2(a, d);
+                        const float2 f = e4m3x2_to_float2(h);
+                        const uint16_t g = cvt_e4m3x2(fmaf(a - f.x, kLoScale, a > 0.0f ? dither : 0.0f), fmaf(d - f.y, kLoScale, d > 0.0f ? dither : 0.0f));
+                        if ((i & 2) == 0) hi[i / 4] = h, lo[i / 4] = g;
+                        else hi[i / 4] |= static_cast<uint32_t>(h) << 16, lo[i / 4] |= static_cast<uint32_t>(g) << 16;
+                    }
+                    uint8_t* const row = ps + b * C::kPBytes + token * 2 * R;
+                    if constexpr (R == 32) {                                   // four 16-byte places a token: hi of either half, lo of either half
+                        const int turn = (token >> 1) & 3;
+                        *reinterpret_cast<uint4*>(row + ((half ^ turn) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(row + (((2 + half) ^ turn) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    } else {                                                   // two: hi, lo
+                        const int turn = (token >> 2) & 1;
+                        *reinterpret_cast<uint2*>(row + (turn << 4) + half * 8) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(row + ((1 ^ turn) << 4) + half * 8) = make_uint2(lo[0], lo[1]);
+                    }
+                    // Behind the sequence's end lie other sequences' bytes, or none at all; no weight, but 0 x NaN is not 0.
+                    if (__any_sync(0xffffffffu, p >= w.s.len)) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t mine = unit + half * 2 + u, at = mine % C::kUnits;
+                            ok = ok && wait(sm.full[at], (mine / C::kUnits) & 1, 2, mine);
+                            if (ok && p >= w.s.len) {
+                                uint4* const v = reinterpret_cast<uint4*>(units + at * kUnitBytes + token * 128);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(sm.p_full[b]));
+                }
+            }
+            // -------- the item's result
+            float sum;
+            {
+                sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
+                if (lane % (32 / N) == 0) sm.sum[half][quarter][own_row<N>()] = sum;
+                ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
+                if (!ok) break;
+                sum = (sm.sum[half][0][own_row<N>()] + sm.sum[half][1][own_row<N>()]) + (sm.sum[half][2][own_row<N>()] + sm.sum[half][3][own_row<N>()]);
+            }
+            float inv[N];
+            broadcast_rows<N>(sm.row[sw], sum == 0.0f ? 0.0f : 1.0f / sum, inv);
+            const uint32_t last = tile_count - 1;
+            ok = wait(sm.p_empty[last & 1], (last >> 1) & 1, 12, last);
+            tc_fence_after();
+            const bool begins = w.tile == 0, ends = w.tile + w.n == w.tiles, whole = begins && ends;
+            const int part = 2 * blockIdx.x + (begins ? 1 : 0);
+            if (ok) {
+                const float lse2 = sum == 0.0f ? -INFINITY : m - kTop + __log2f(sum);
+                if (quarter == 0 && lane % (32 / N) == 0 && !whole) q.partial_lse[static_cast<int64_t>(part) * R + half * N + own_row<N>()] = lse2;
+                if (threadIdx.x == 32 * kFirstSoftmaxWarp && begins && !ends) {
+                    const int64_t end = first + (share - w.left) - w.n + w.tiles;          // of the block's tiles, in the list
+                    q.cut[blockIdx.x] = make_int4(w.seq, w.block, w.head_block, static_cast<int>((end * min(total, static_cast<int64_t>(gridDim.x)) - 1) / total));
+                }
+                const int* const place = sm.place[par] + half * N;
+                if (whole && q.lse && quarter == 0 && lane % (32 / N) == 0) {
+                    const int to = place[own_row<N>()];
+                    if (to >= 0) q.lse[to] = lse2 * kLn2;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t hi[N], lo[N];
+                    const uint32_t at = tmem + lanes + C::kTmemO + u * 2 * R + half * N;
+                    tc_ld<N>(at, hi);
+                    tc_ld<N>(at + R, lo);
+                    tc_wait_ld();
+                    const int dim = u * 128 + token;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float o = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
+                        if (whole) {
+                            const int to = place[i];
+                            if (to >= 0) q.out[static_cast<int64_t>(to) * kLatent + dim] = __float2bfloat16_rn(o);
+                        } else {
+                            q.partial[(static_cast<int64_t>(part) * R + half * N + i) * kLatent + dim] = o;
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(sm.o_empty));
+            ++item;
+        } while (w.next(c, q));
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (ctl->abort_flag) {
+        // give copies and MMAs that were already issued time to land before shared memory and TMEM are released
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tc_dealloc(tmem, C::kTmemCols);
+    }
+}
+
+// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  A block of threads to kCombineRows rows of a cut block, which is
+// named by the CTA that it begins in.
+constexpr int kCombineThreads = 256, kCombineRows = 2;
+template <int R>
+__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const LatentCache c, const Queries q) {
     griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= q.tokens * q.heads) return;
-    const int64_t t = row / q.heads;
-    const int h = static_cast<int>(row - t * q.heads);
-    int seq = 0;
-    int64_t begin, end;
-    if (q.cu) {
-        while (seq < c.n_seqs && q.cu[seq + 1] <= t) ++seq;
-        if (seq == c.n_seqs) return;
-        begin = q.cu[seq], end = q.cu[seq + 1];
-    } else {
-        const int64_t per = q.tokens / c.n_seqs;
-        seq = static_cast<int>(t / per);
-        begin = seq * per, end = begin + per;
+    const int4 cut = q.cut[blockIdx.x];
+    if (cut.x < 0) return;
+    const int r = blockIdx.y * kCombineRows + threadIdx.x / 128;
+    const Seq s = load_seq(c, q, cut.x);
+    int tok = cut.y << q.block_shift, head = cut.z * R + r;
+    if (q.head_blocks == 1) {
+        tok += r / q.heads;
+        head = r % q.heads;
     }
-    const int64_t cap = static_cast<int64_t>(c.pages_width) << c.page_shift;
-    const int64_t len = max(static_cast<int64_t>(0), min(static_cast<int64_t>(q.seq_lens[seq]), cap));
-    const int64_t base = len - (end - begin);           // position of the sequence's first query
-    float ql[16], qr[2], acc[16], m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < 16; ++i) ql[i] = __bfloat162float(q.latent[t * q.latent_token + h * q.latent_head + lane * 16 + i]), acc[i] = 0.0f;
-    for (int i = 0; i < 2; ++i) qr[i] = __bfloat162float(q.rope[t * q.rope_token + h * q.rope_head + lane * 2 + i]);
-    const int64_t last = q.tree ? len : min(len, base + (t - begin) + 1);
-    for (int64_t p = 0; p < last; ++p) {
-        if (q.tree && p >= base && (p - base >= 64 || !((q.tree[t] >> (p - base)) & 1))) continue;
-        const int64_t slot = slot_of(c, seq, static_cast<uint32_t>(p));
-        if (slot < 0) continue;
-        float v[16], d = 0.0f;
-        const uint4 w = *reinterpret_cast<const uint4*>(c.latent + slot * kLatent + lane * 16);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-        for (int i = 0; i < 8; ++i) {
-            const float2 f = e4m3x2_to_float2(static_cast<uint16_t>(ww[i / 2] >> (16 * (i & 1))));
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
-        for (int i = 0; i < 16; ++i) d = fmaf(ql[i], v[i], d);
-        for (int i = 0; i < 2; ++i) d = fmaf(qr[i], __bfloat162float(c.rope[slot * kRope + lane * 2 + i]), d);
-        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        const float s = c.scale[slot], x = d * s * q.scale;
-        const float mn = fmaxf(m, x), old = exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * 1.44269504f), pr = exp2f((x - mn) * 1.44269504f);
-        l = l * old + pr;
-        for (int i = 0; i < 16; ++i) acc[i] = acc[i] * old + pr * s * v[i];
-        m = mn;
+    if (head >= q.heads || tok >= s.queries || (q.head_blocks == 1 && r >= q.heads << q.block_shift)) return;
+    const int parts = cut.w - static_cast<int>(blockIdx.x) + 1;
+    const auto part = [&](int i) { return static_cast<int64_t>(2 * (static_cast<int>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * R + r; };
+    float top = -INFINITY;
+    bool nan = false;
+    for (int i = threadIdx.x & 31; i < parts; i += 32) {
+        const float v = q.partial_lse[part(i)];
+        nan = nan || isnan(v);
+        top = fmaxf(top, v);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int i = 0; i < 16; ++i) q.out[row * kLatent + lane * 16 + i] = __float2bfloat16_rn(acc[i] * inv);
-    if (q.lse && lane == 0) q.lse[row] = l == 0.0f ? -INFINITY : m + logf(l);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    nan = __any_sync(0xffffffffu, nan);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float f = ex2(q.partial_lse[part(i)] - ref);
+        const float4 v = reinterpret_cast<const float4*>(q.partial + part(i) * kLatent)[threadIdx.x & 127];
+        sum += f;
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+    const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t to = (static_cast<int64_t>(s.first) + tok) * q.heads + head;
+    reinterpret_cast<uint2*>(q.out + to * kLatent)[threadIdx.x & 127] =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (q.lse && (threadIdx.x & 127) == 0) q.lse[to] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+}
+
+// Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
+int block_rows(int64_t tokens, int heads, int n_seqs) { return (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32; }
+
+size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + sizeof(int4)); }
+
+template <int R>
+int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool cut, unsigned int* status,
+           cudaStream_t stream) {
+    const auto kern = latent_attention_kernel<R>;
+    DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
+    DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    if (cut)
+        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / kCombineRows), dim3(kCombineThreads), 0, stream, c, q));
+    return DSV3_OK;
 }
 
 }  // namespace
@@ -75,7 +835,10 @@ using namespace dsv3;
 
 extern "C" {
 
-size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest) { return 0; }
+size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest) {
+    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || longest <= kTokens) return 0;      // (a block of one tile is never cut)
+    return partial_bytes(block_rows(tokens, heads, n_seqs), num_sms());
+}
 
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
                           const void* q_rope, int64_t q_rope_token_stride, int64_t q_rope_head_stride, int64_t tokens, int heads,
@@ -88,8 +851,8 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
         return DSV3_ERR_INVALID_ARGUMENT;
     }
     if (tokens == 0 || heads == 0) return DSV3_OK;
-    if (!q_latent || !q_rope || !seq_lens || !out) {
-        set_last_error("latent_attention: null pointer");
+    if (!q_latent || !q_rope || !seq_lens || !out || c.n_pages == 0) {
+        set_last_error("latent_attention: null pointer, or a pool without pages");
         return DSV3_ERR_INVALID_ARGUMENT;
     }
     if (c.n_seqs == 0 || (!cu_seqlens_q && tokens % c.n_seqs != 0)) {
@@ -97,21 +860,40 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
         return DSV3_ERR_INVALID_ARGUMENT;
     }
     const int64_t strides = q_latent_token_stride | q_latent_head_stride | q_rope_token_stride | q_rope_head_stride;
-    if (strides % 8 != 0 || (reinterpret_cast<uintptr_t>(q_latent) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
-        set_last_error("latent_attention: rows of the queries and out must be 16-byte aligned");
+    if (strides % 8 != 0 || (reinterpret_cast<uintptr_t>(q_latent) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(out)) % 16 != 0 ||
+        reinterpret_cast<uintptr_t>(c.scale) % 16 != 0) {
+        set_last_error("latent_attention: rows of the queries and out, and the cache's scales, must be 16-byte aligned");
         return DSV3_ERR_UNSUPPORTED;
     }
     if (heads > 1024 || tokens > 0x7FFFFFFFll / heads) {
         set_last_error("latent_attention: takes at most 1024 heads and 2^31 query heads");
         return DSV3_ERR_UNSUPPORTED;
     }
-    Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
-                 q_rope_token_stride, q_rope_head_stride, tokens, heads, seq_lens, cu_seqlens_q, tree_mask, softmax_scale,
-                 static_cast<__nv_bfloat16*>(out), lse};
-    const int64_t rows = tokens * heads;
-    DSV3_CUDA_TRY(launch_dependent(latent_attention_simple_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0,
-                                   static_cast<cudaStream_t>(stream), c, q));
-    return DSV3_OK;
+    const int grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
+    const bool cut = (static_cast<int64_t>(c.pages_width) << c.page_shift) > kTokens;
+    if (cut && (!workspace || workspace_bytes < partial_bytes(rows, grid) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
+        set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, grid));
+        return DSV3_ERR_WORKSPACE;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    unsigned int* const status = status_device_ptr();
+    if (!status) return DSV3_ERR_CUDA;
+    const int64_t slots = static_cast<int64_t>(c.n_pages) << c.page_shift;
+    const int box = c.page_shift < 7 ? 1 << c.page_shift : kTokens;
+    CUtensorMap map_latent, map_rope;
+    if (const int rc = make_tmap(&map_latent, c.latent, slots, kLatent, box); rc != DSV3_OK) return rc;
+    if (const int rc = make_tmap(&map_rope, c.rope, slots, 2 * kRope, box); rc != DSV3_OK) return rc;
+    // tokens to a block: a power of two, so that the tiles of a causal sequence can be counted without adding them up
+    int shift = 0;
+    while ((heads << (shift + 1)) <= rows) ++shift;
+    float* const partial = static_cast<float*>(workspace);
+    float* const partial_lse = cut ? partial + static_cast<size_t>(grid) * 2 * rows * kLatent : nullptr;
+    int4* const list = cut ? reinterpret_cast<int4*>(partial_lse + static_cast<size_t>(grid) * 2 * rows) : nullptr;
+    const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
+                       q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
+                       cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
+                       (heads + rows - 1) / rows, shift, partial, partial_lse, list};
+    return rows == 16 ? launch<16>(c, q, map_latent, map_rope, grid, cut, status, st) : launch<32>(c, q, map_latent, map_rope, grid, cut, status, st);
 }
 
 }  // extern "C"
