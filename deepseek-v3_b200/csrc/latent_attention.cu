@@ -38,6 +38,7 @@ constexpr int kScaleSlots = 4;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // The running maximum moves when a score exceeds it by more than kSlack, and stands for 2^kTop: the largest weight is 2^8.
 constexpr float kSlack = 1.0f, kTop = 7.0f;
+constexpr float kNothing = -3.0e38f;      // below every finite score, and no infinity: -inf less this is -inf
 constexpr float kLoScale = 16.0f;         // the largest remainder is 2^-4 of 2^8
 
 struct Queries {
@@ -85,7 +86,7 @@ struct Small {                                                  // shared memory
     Control ctl;
     int64_t warp_sum[kAttnThreads / 32];
     int64_t start_offset;
-    int start_seq;
+    int4 start;                                                 // sequence, its cached tokens, queries, first query
 };
 
 template <int R>
@@ -207,9 +208,9 @@ struct Walk {
         left -= n;
     }
     // the share starts at tile `offset` of sequence `sq`
-    __device__ void begin(const LatentCache& c, const Queries& q, int sq, int64_t offset, int64_t share) {
-        seq = sq;
-        s = load_seq(c, q, sq);
+    __device__ void begin(const Queries& q, const int4& start, int64_t offset, int64_t share) {
+        seq = start.x;
+        s = {start.y, start.z, start.w};
         const int blocks = blocks_of(q, s);
         int lo = 0, hi = blocks;          // largest block whose tiles begin at or before the offset
         while (hi - lo > 1) {
@@ -241,13 +242,25 @@ struct Walk {
     }
 };
 
+// Row r of an item's block: query * heads + head, or -1 where it is none.
+__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) {
+    int token = w.block << q.block_shift, head = w.head_block * rows + r;
+    if (q.head_blocks == 1) {
+        if (r >= q.heads << q.block_shift) return -1;
+        token += r / q.heads;
+        head = r % q.heads;
+    }
+    return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
+}
+
 // All threads: this CTA's share [*first, *first + share) of the list, and where in which sequence it starts.
 template <typename Sm>
 __device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, int64_t* total_out, int64_t* first_out) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Seq x;
     const auto mine = [&](int s) -> int64_t {
         if (s >= c.n_seqs) return 0;
-        const Seq x = load_seq(c, q, s);
+        x = load_seq(c, q, s);
         const int b = blocks_of(q, x);
         return tiles_before(q, x, b, b) * q.head_blocks;
     };
@@ -284,12 +297,12 @@ __device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, in
     if (share == 0) return 0;
     int64_t at = 0;
     for (int s0 = 0; s0 < c.n_seqs && at <= first; s0 += kAttnThreads) {
-        const int64_t v = s0 ? mine(s0 + threadIdx.x) : kept;
+        const int64_t v = s0 || c.n_seqs > kAttnThreads ? mine(s0 + threadIdx.x) : kept;
         int64_t before = kept_before;
         sum = 0;
         if (s0 || c.n_seqs > kAttnThreads) before = scan(v, &sum) + at;
         if (before <= first && first < before + v) {
-            sm.start_seq = s0 + threadIdx.x;
+            sm.start = make_int4(s0 + threadIdx.x, x.len, x.queries, x.first);
             sm.start_offset = first - before;
         }
         at += sum;
@@ -383,145 +396,173 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     if (threadIdx.x == 32 * kFirstSoftmaxWarp && q.cut) q.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
     Walk w;
-    if (share > 0) w.begin(c, q, sm.start_seq, sm.start_offset, share);
+    if (share > 0) w.begin(q, sm.start, sm.start_offset, share);
 
     if (share == 0) {
         // nothing to do
     } else if (warp == 0) {
-        // ------------------------------------------------------------ loads: a lane to each box of a tile's tokens
-        const int page_rows = 1 << c.page_shift, rows = min(page_rows, kTokens);
+        // ------------------------------------------------------------ loads.  The lanes look up a tile's pages together, one tile ahead; one lane issues, with
+        // coordinates that the warp has in common: copies issued by the lanes of several pages cost 490 cycles a unit.
+        const int rows = min(1 << c.page_shift, kTokens), boxes_max = kTokens / rows;
         const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
-        uint32_t unit = 0;
+        uint32_t unit = 0, slot = 0, turn = 1, tile_count = 0;
         bool ok = true;
-        int slot = 0, tile_count = 0;
-        do {
-            for (int t = 0; t < w.n && ok; ++t, ++tile_count) {
-                const int p0 = (w.tile + t) * kTokens + lane * rows;
-                const bool here = lane < kTokens / rows && p0 < w.s.len;
-                const int boxes = __popc(__ballot_sync(0xffffffffu, here));
-                const int at = here ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -1;
-                const int present = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                const int y = static_cast<int>(at >= 0 ? static_cast<uint32_t>(at) : outside);
-                float* const scales = sm.scales[tile_count & (kScaleSlots - 1)] + lane * rows;
-                for (int u = 0; u < kTileUnits; ++u) {
-                    const uint32_t full = bar(sm.full[slot]);
-                    uint32_t free = 1;
-                    if (lane == 0) free = bounded_wait(bar(sm.empty[slot]), ((unit / C::kUnits) & 1) ^ 1, ctl, status, 1, unit);
-                    free = __shfl_sync(0xffffffffu, free, 0);
-                    ok = free != 0;
+        // the slot where this lane's box of a tile begins; absent: -1, behind the sequence's end: -2
+        const auto look_up = [&](const Walk& at, int t) -> int {
+            const int64_t p0 = static_cast<int64_t>(at.tile + t) * kTokens + lane * rows;
+            return lane < boxes_max && p0 < at.s.len ? slot_of(c, at.seq, static_cast<uint32_t>(p0)) : -2;
+        };
+        int mine = look_up(w, 0);
+        bool more = true;
+        while (more) {
+            const int n = w.n;
+            for (int t = 0; t < n && ok; ++t, ++tile_count) {
+                const int at = mine;
+                if (t + 1 < n) {
+                    mine = look_up(w, t + 1);
+                } else {
+                    more = w.next(c, q);
+                    if (more) mine = look_up(w, 0);
+                }
+                const int boxes = __popc(__ballot_sync(0xffffffffu, at > -2)), present = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                float* const scales = sm.scales[tile_count & (kScaleSlots - 1)];
+                for (int u = 0; u < kTileUnits; ++u, ++unit) {
+                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), turn, ctl, status, 1, unit));
                     if (!ok) break;
-                    if (u == 0) {
-                        if (here && at < 0)                                    // an absent page: its tokens have no scale
-                            for (int i = 0; i < rows; ++i) scales[i] = 0.0f;
+                    if (u == 0 && boxes != present) {                          // an absent page: its tokens have no scale
+                        if (at == -1)
+                            for (int i = 0; i < rows; ++i) scales[lane * rows + i] = 0.0f;
                         __syncwarp();
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(full, boxes * rows * 128 + (u == 0 ? present * rows * 4 : 0));
-                    __syncwarp();
-                    if (here) {
-                        const uint32_t dst = smem_u32(units + slot * kUnitBytes) + lane * rows * 128;
-                        if (u < 4) tma_load_2d(dst, &map_latent, u * 128, y, full);
-                        else tma_load_2d(dst, &map_rope, 0, y, full);
-                        if (u == 0 && at >= 0) bulk_load(smem_u32(scales), c.scale + at, rows * 4, full);
+                    const uint32_t full = bar(sm.full[slot]), dst = smem_u32(units) + slot * kUnitBytes;
+                    if (elect_one()) mbar_arrive_expect_tx(full, boxes * rows * 128 + (u == 0 ? present * rows * 4 : 0));
+                    for (int i = 0; i < boxes; ++i) {
+                        const int from = __shfl_sync(0xffffffffu, at, i);
+                        const int y = from >= 0 ? from : static_cast<int>(outside);
+                        if (elect_one()) {
+                            if (u < 4) tma_load_2d(dst + i * rows * 128, &map_latent, u * 128, y, full);
+                            else tma_load_2d(dst + i * rows * 128, &map_rope, 0, y, full);
+                            if (u == 0 && from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
+                        }
+                        __syncwarp();
                     }
-                    ++unit;
+                    if (++slot == C::kUnits) slot = 0, turn ^= 1;
+                }
+            }
+            more = more && ok;
+        }
+        // none of the commits onto empty[] may be in flight when the CTA leaves its shared memory to another
+        for (uint32_t u = unit > C::kUnits ? unit - C::kUnits : 0u; ok && u < unit; ++u)
+            ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[u % C::kUnits]), (u / C::kUnits) & 1, ctl, status, 1, u));
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ scores.  The warp stays converged and elects a lane for the MMAs alone: addresses and
+        // descriptors then stay in uniform registers.  The sums have an issuer of their own: in one thread, a tile whose weights are there waits behind
+        // the next tile's loads, which wait for the room that its sums make.
+        constexpr uint32_t idesc_s = umma_idesc_e4m3_f32(kTokens, 2 * R), idesc_r = idesc_bf16(kTokens, R);
+        const uint32_t units_at = smem_u32(units), q_at = smem_u32(qs);
+        uint32_t slot = 0, turn = 0, count = 0, item = 0;                      // ring position and its parity, tiles, items
+        bool ok = true;
+        do {
+            ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item));
+            for (int t = 0; t < w.n && ok; ++t, ++count) {
+                const uint32_t b = count & 1, d = tmem + b * C::kTmemS;
+                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.s_empty[b]), ((count >> 1) & 1) ^ 1, ctl, status, 3, count));
+                for (int u = 0; u < kTileUnits && ok; ++u) {
+                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.full[slot]), turn, ctl, status, 2, count));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = umma_desc_k_major_sw128(units_at + slot * kUnitBytes), db = umma_desc_k_major_sw128(q_at + u * C::kQChunk);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {                          // 32 bytes of K a step
+                            if (u < 4) tc_mma_f8(d, da + 2 * k, db + 2 * k, idesc_s, (u | k) != 0);
+                            else tc_mma_bf16(d + 2 * R, da + 2 * k, db + 2 * k, idesc_r, k != 0);
+                        }
+                        if (u == 4) {
+                            tc_commit(bar(sm.empty[slot]));
+                            tc_commit(bar(sm.s_full[b]));
+                        }
+                    }
+                    __syncwarp();
+                    if (++slot == C::kUnits) slot = 0, turn ^= 1;
+                }
+            }
+            ++item;
+        } while (ok && w.next(c, q));
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ sums
+        constexpr uint32_t idesc_o = umma_idesc_e4m3_f32(kTokens, 2 * R) | kIdescTransposed;
+        const uint32_t units_at = smem_u32(units), p_at = smem_u32(ps);
+        uint32_t slot = 0, count = 0, item = 0;
+        bool ok = true;
+        do {
+            for (int t = 0; t < w.n && ok; ++t, ++count) {
+                const uint32_t b = count & 1;
+                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.p_full[b]), (count >> 1) & 1, ctl, status, 11, count));
+                // (an item's first sums overwrite those of the item before it)
+                if (ok && t == 0) ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, 12, item));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t db = umma_desc_mn_major<2 * R>(p_at + b * C::kPBytes);
+#pragma unroll
+                for (int u = 0; u < kTileUnits; ++u) {
+                    if (u < 4) {
+                        const uint64_t da = umma_desc_mn_major<128>(units_at + slot * kUnitBytes);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)                        // 32 tokens a step
+                                tc_mma_f8(tmem + C::kTmemO + u * 2 * R, da + (k * 32 * 128 >> 4), db + (k * 32 * 2 * R >> 4), idesc_o, (t | k) != 0);
+                            tc_commit(bar(sm.empty[slot]));
+                            if (u == 3) tc_commit(bar(sm.p_empty[b]));
+                        }
+                        __syncwarp();
+                    }
                     if (++slot == C::kUnits) slot = 0;
                 }
             }
+            ++item;
         } while (ok && w.next(c, q));
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMAs: one elected lane
-        if (elect_one()) {
-            constexpr uint32_t idesc_s = umma_idesc_e4m3_f32(kTokens, 2 * R), idesc_r = idesc_bf16(kTokens, R);
-            constexpr uint32_t idesc_o = idesc_s | kIdescTransposed;
-            const uint32_t units_at = smem_u32(units), q_at = smem_u32(qs), p_at = smem_u32(ps);
-            uint32_t s_count = 0, p_count = 0, item = 0;                       // tiles whose scores, whose sums have been issued
-            // scores of tile s_count, in the ring from unit 5 * s_count on
-            const auto scores = [&]() -> bool {
-                const uint32_t b = s_count & 1, d = tmem + b * C::kTmemS;
-                if (!bounded_wait(bar(sm.s_empty[b]), ((s_count >> 1) & 1) ^ 1, ctl, status, 3, s_count)) return false;
-                tc_fence_after();
-                for (int u = 0; u < kTileUnits; ++u) {
-                    const uint32_t unit = s_count * kTileUnits + u, at = unit % C::kUnits;
-                    if (!bounded_wait(bar(sm.full[at]), (unit / C::kUnits) & 1, ctl, status, 2, unit)) return false;
-                    const uint64_t da = umma_desc_k_major_sw128(units_at + at * kUnitBytes);
-                    const uint64_t db = umma_desc_k_major_sw128(q_at + u * C::kQChunk);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {                              // 32 bytes of K a step
-                        if (u < 4) tc_mma_f8(d, da + 2 * k, db + 2 * k, idesc_s, (u | k) != 0);
-                        else tc_mma_bf16(d + 2 * R, da + 2 * k, db + 2 * k, idesc_r, k != 0);
-                    }
-                    if (u == 4) {
-                        tc_commit(bar(sm.empty[at]));
-                        tc_commit(bar(sm.s_full[b]));
-                    }
-                }
-                ++s_count;
-                return true;
-            };
-            const auto sums = [&](bool fresh) -> bool {
-                const uint32_t b = p_count & 1;
-                if (!bounded_wait(bar(sm.p_full[b]), (p_count >> 1) & 1, ctl, status, 11, p_count)) return false;
-                tc_fence_after();
-                for (int u = 0; u < 4; ++u) {
-                    const uint32_t at = (p_count * kTileUnits + u) % C::kUnits;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)                                // 32 tokens a step
-                        tc_mma_f8(tmem + C::kTmemO + u * 2 * R, umma_desc_mn_major<128>(units_at + at * kUnitBytes + k * 32 * 128),
-                                  umma_desc_mn_major<2 * R>(p_at + b * C::kPBytes + k * 32 * 2 * R), idesc_o, !fresh || k != 0);
-                    tc_commit(bar(sm.empty[at]));
-                }
-                tc_commit(bar(sm.p_empty[b]));
-                ++p_count;
-                return true;
-            };
-            bool ok = true;
-            do {
-                ok = bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item);
-                ok = ok && scores();
-                for (int t = 0; t < w.n && ok; ++t) {
-                    if (t + 1 < w.n) ok = scores();
-                    // (the first sums of an item overwrite those of the item before it)
-                    if (ok && t == 0) ok = bounded_wait(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, 12, item);
-                    ok = ok && sums(t == 0);
-                }
-                ++item;
-            } while (ok && w.next(c, q));
-        }
-        __syncwarp();
     } else if (warp >= kFirstSoftmaxWarp) {
         // ------------------------------------------------------------ softmax
         const int sw = warp - kFirstSoftmaxWarp, half = sw >> 2, quarter = sw & 3;
         const int token = quarter * 32 + lane;                                 // of the tile: this thread's TMEM lane
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float dither = static_cast<float>((token * 79) & 127) * 0x1p-16f - 0x1.fcp-11f;   // evenly over (-2^-10, 2^-10), half a step either side
-        uint32_t tile_count = 0, item = 0;
+        uint32_t tile_count = 0;
         bool ok = true;                                                        // the same in all lanes of a warp
         const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t counter) -> bool {
             return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, counter));
         };
-        do {
-            const uint32_t par = item & 1;
-            // -------- the block's rows: a warp to every eighth row
-            for (int r = sw; r < R; r += kSoftmaxWarps) {
-                int tok = w.block << q.block_shift, head = w.head_block * R + r;
-                if (q.head_blocks == 1) {
-                    tok += r / q.heads;
-                    head = r % q.heads;
-                }
-                const bool valid = head < q.heads && tok < w.s.queries && (q.head_blocks > 1 || r < q.heads << q.block_shift);
-                uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                uint32_t pair = 0;
-                if (valid) {
-                    const int64_t row = w.s.first + tok;
+        // The rows of a block, a warp to every eighth: from memory ...
+        constexpr int kMine = R / kSoftmaxWarps;
+        uint4 qv[kMine][2];
+        uint32_t qr[kMine];
+        const auto fetch = [&]() {
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                const int place = place_of(q, w, R, sw + j * kSoftmaxWarps);
+                qv[j][0] = qv[j][1] = make_uint4(0, 0, 0, 0);
+                qr[j] = 0;
+                if (place >= 0) {
+                    const int64_t row = place / q.heads;
+                    const int head = place % q.heads;
                     const uint4* src = reinterpret_cast<const uint4*>(q.latent + row * q.latent_token + head * q.latent_head);
-                    v[0] = src[lane * 2], v[1] = src[lane * 2 + 1];
-                    pair = reinterpret_cast<const uint32_t*>(q.rope + row * q.rope_token + head * q.rope_head)[lane];
+                    qv[j][0] = src[lane * 2], qv[j][1] = src[lane * 2 + 1];
+                    qr[j] = reinterpret_cast<const uint32_t*>(q.rope + row * q.rope_token + head * q.rope_head)[lane];
                 }
+            }
+        };
+        // ... to shared memory, as operands of the first product
+        const auto stage = [&](uint32_t par) {
+            const int base = w.s.len - w.s.queries;
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                const int r = sw + j * kSoftmaxWarps;
                 float x[16], top = 0.0f;
                 bool finite = true;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t word = reinterpret_cast<const uint32_t*>(v)[i];
+                    const uint32_t word = reinterpret_cast<const uint32_t*>(qv[j])[i];
                     x[2 * i] = bf16_bits_to_float(word & 0xFFFFu);
                     x[2 * i + 1] = __uint_as_float(word & 0xFFFF0000u);
                 }
@@ -530,7 +571,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     top = fmaxf(top, fabsf(x[i]));
                     finite = finite && fabsf(x[i]) < INFINITY;
                 }
-                float re = bf16_bits_to_float(pair & 0xFFFFu), im = __uint_as_float(pair & 0xFFFF0000u);
+                const float re = bf16_bits_to_float(qr[j] & 0xFFFFu), im = __uint_as_float(qr[j] & 0xFFFF0000u);
                 finite = __all_sync(0xffffffffu, finite && fabsf(re) < INFINITY && fabsf(im) < INFINITY);
                 // (the rotated half is held divided by the same scale, in bf16: the scale is kept from being too small for that)
                 top = fmaxf(fmaxf(top, fmaxf(fabsf(re), fabsf(im)) * 0x1p-40f), 0x1p-100f);
@@ -553,21 +594,27 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 *reinterpret_cast<uint32_t*>(qs + 4 * C::kQChunk + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) =
                     finite ? pack_bf16x2(re * inv, im * inv) : 0u;
                 if (lane == 0) {
-                    const int base = w.s.len - w.s.queries;
-                    sm.place[par][r] = valid ? (w.s.first + tok) * q.heads + head : -1;
-                    sm.factor[par][r] = !valid ? 0.0f : finite ? s * q.scale * kLog2e : __uint_as_float(0x7FC00000u);
-                    sm.limit[par][r] = q.tree ? base - 1 : base + tok;
-                    sm.tree[par][r] = q.tree && valid ? q.tree[w.s.first + tok] : 0;
+                    const int place = place_of(q, w, R, r), query = place < 0 ? 0 : place / q.heads;
+                    sm.place[par][r] = place;
+                    sm.factor[par][r] = place < 0 ? 0.0f : finite ? s * q.scale * kLog2e : __uint_as_float(0x7FC00000u);
+                    sm.limit[par][r] = q.tree ? base - 1 : base + query - w.s.first;
+                    sm.tree[par][r] = q.tree && place >= 0 ? q.tree[query] : 0;
                 }
             }
             fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(sm.q_full));
+        };
+        fetch();
+        stage(0);
+        for (uint32_t item = 0;; ++item) {
+            const uint32_t par = item & 1;
             ok = barrier_all<32 * kSoftmaxWarps>(3, ok);                       // factors and limits of all rows
             if (!ok) break;
-            if (lane == 0) mbar_arrive(bar(sm.q_full));
-
-            float l[N], m = -INFINITY;                                         // m: of row own_row<N>()
+            // d = y - mv is the weight's exponent; nothing has been seen yet: mv far below every score
+            float l[N], mv[N], m = kNothing;                                   // m: mv of row own_row<N>()
 #pragma unroll
-            for (int i = 0; i < N; ++i) l[i] = 0.0f;
+            for (int i = 0; i < N; ++i) l[i] = 0.0f, mv[i] = kNothing;
             const int base = w.s.len - w.s.queries;                            // position of the first query's token
             for (int t = 0; t < w.n; ++t, ++tile_count) {
                 const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
@@ -609,10 +656,11 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         if (!present || !seen) y[i] = -INFINITY;
                     }
                 }
-                float mv[N];
-                bool moved;
-                float old = m;
-                {
+                // -------- a new maximum where some weight would pass 2^8: rare after the first tiles, so that the others only ask whether there is one
+                bool over = false;
+#pragma unroll
+                for (int i = 0; i < N; ++i) over = over || y[i] - mv[i] > kTop + kSlack;
+                if (!barrier_all<128>(1 + half, ok && !over)) {
                     float v[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) v[i] = y[i];
@@ -623,31 +671,30 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     float all = sm.top[b][half][0][own_row<N>()];
 #pragma unroll
                     for (int i = 1; i < 4; ++i) all = fmaxf(all, sm.top[b][half][i][own_row<N>()]);
-                    moved = all > m + kSlack || (m == -INFINITY && all > m);
-                    if (moved) m = all;
-                    broadcast_rows<N>(sm.row[sw], m == -INFINITY ? 0.0f : m - kTop, mv);
-                }
-                // -------- sums so far take the new maximum
-                if (t > 0 && __any_sync(0xffffffffu, moved && old != -INFINITY)) {
-                    float f[N];
-                    broadcast_rows<N>(sm.row2[sw], moved ? ex2(old - m) : 1.0f, f);
+                    const float old = m;
+                    if (all - m > kTop + kSlack) m = all - kTop;
+                    broadcast_rows<N>(sm.row[sw], m, mv);
+                    if (t > 0) {                                               // sums so far take it
+                        float f[N];
+                        broadcast_rows<N>(sm.row2[sw], ex2(old - m), f);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) l[i] *= f[i];
-                    const uint32_t before = tile_count - 1;
-                    ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
-                    tc_fence_after();
-                    if (ok) {
+                        for (int i = 0; i < N; ++i) l[i] *= f[i];
+                        const uint32_t before = tile_count - 1;
+                        ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
+                        tc_fence_after();
+                        if (ok) {
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {                          // hi and lo of four times 128 dimensions
-                            uint32_t o[N];
-                            const uint32_t at = tmem + lanes + C::kTmemO + u * R + half * N;
-                            tc_ld<N>(at, o);
-                            tc_wait_ld();
+                            for (int u = 0; u < 8; ++u) {                      // hi and lo of four times 128 dimensions
+                                uint32_t o[N];
+                                const uint32_t at = tmem + lanes + C::kTmemO + u * R + half * N;
+                                tc_ld<N>(at, o);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < N; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[i]);
-                            tc_st<N>(at, o);
+                                for (int i = 0; i < N; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[i]);
+                                tc_st<N>(at, o);
+                            }
+                            tc_wait_st();
                         }
-                        tc_wait_st();
                     }
                 }
                 // -------- weights: hi and lo, to shared memory
@@ -695,34 +742,41 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     if (lane == 0) mbar_arrive(bar(sm.p_full[b]));
                 }
             }
-            // -------- the item's result
-            float sum;
-            {
-                sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
-                if (lane % (32 / N) == 0) sm.sum[half][quarter][own_row<N>()] = sum;
-                ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
-                if (!ok) break;
-                sum = (sm.sum[half][0][own_row<N>()] + sm.sum[half][1][own_row<N>()]) + (sm.sum[half][2][own_row<N>()] + sm.sum[half][3][own_row<N>()]);
-            }
+            // -------- the item's result; the next item's queries on their way meanwhile
+            const Walk done = w;
+            const bool more = w.next(c, q);
+            if (more) fetch();
+            float sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
+            if (lane % (32 / N) == 0) sm.sum[half][quarter][own_row<N>()] = sum;
+            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
+            if (!ok) break;
+            sum = (sm.sum[half][0][own_row<N>()] + sm.sum[half][1][own_row<N>()]) + (sm.sum[half][2][own_row<N>()] + sm.sum[half][3][own_row<N>()]);
             float inv[N];
             broadcast_rows<N>(sm.row[sw], sum == 0.0f ? 0.0f : 1.0f / sum, inv);
+            if (more) stage(par ^ 1);                                          // (all scores of this item have been read)
+            const bool begins = done.tile == 0, ends = done.tile + done.n == done.tiles, whole = begins && ends;
+            const int part = 2 * blockIdx.x + (begins ? 1 : 0);
+            const float lse2 = sum == 0.0f ? -INFINITY : m + __log2f(sum);
+            if (quarter == 0 && lane % (32 / N) == 0) {
+                const int r = half * N + own_row<N>(), to = sm.place[par][r];
+                if (!whole) q.partial_lse[static_cast<int64_t>(part) * R + r] = lse2;
+                else if (q.lse && to >= 0) q.lse[to] = lse2 * kLn2;
+            }
+            if (threadIdx.x == 32 * kFirstSoftmaxWarp && begins && !ends) {
+                const int64_t end = first + (share - done.left) - done.n + done.tiles;      // of the block's tiles, in the list
+                q.cut[blockIdx.x] = make_int4(done.seq, done.block, done.head_block, static_cast<int>((end * min(total, static_cast<int64_t>(gridDim.x)) - 1) / total));
+            }
+            // four rows that this lane writes: 8 bytes each, of four dimensions that it gets from its neighbours
+            int to[N / 4];
+            {
+                const int* const place = sm.place[par] + half * N + (lane & 1) * (N / 2) + ((lane >> 1) & 1) * (N / 4);
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) to[i] = place[i];
+            }
             const uint32_t last = tile_count - 1;
             ok = wait(sm.p_empty[last & 1], (last >> 1) & 1, 12, last);
             tc_fence_after();
-            const bool begins = w.tile == 0, ends = w.tile + w.n == w.tiles, whole = begins && ends;
-            const int part = 2 * blockIdx.x + (begins ? 1 : 0);
             if (ok) {
-                const float lse2 = sum == 0.0f ? -INFINITY : m - kTop + __log2f(sum);
-                if (quarter == 0 && lane % (32 / N) == 0 && !whole) q.partial_lse[static_cast<int64_t>(part) * R + half * N + own_row<N>()] = lse2;
-                if (threadIdx.x == 32 * kFirstSoftmaxWarp && begins && !ends) {
-                    const int64_t end = first + (share - w.left) - w.n + w.tiles;          // of the block's tiles, in the list
-                    q.cut[blockIdx.x] = make_int4(w.seq, w.block, w.head_block, static_cast<int>((end * min(total, static_cast<int64_t>(gridDim.x)) - 1) / total));
-                }
-                const int* const place = sm.place[par] + half * N;
-                if (whole && q.lse && quarter == 0 && lane % (32 / N) == 0) {
-                    const int to = place[own_row<N>()];
-                    if (to >= 0) q.lse[to] = lse2 * kLn2;
-                }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint32_t hi[N], lo[N];
@@ -730,24 +784,37 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     tc_ld<N>(at, hi);
                     tc_ld<N>(at + R, lo);
                     tc_wait_ld();
-                    const int dim = u * 128 + token;
+                    if (!whole) {
+                        float* const dst = q.partial + (static_cast<int64_t>(part) * R + half * N) * kLatent + u * 128 + token;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float o = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
-                        if (whole) {
-                            const int to = place[i];
-                            if (to >= 0) q.out[static_cast<int64_t>(to) * kLatent + dim] = __float2bfloat16_rn(o);
-                        } else {
-                            q.partial[(static_cast<int64_t>(part) * R + half * N + i) * kLatent + dim] = o;
-                        }
+                        for (int i = 0; i < N; ++i) dst[i * kLatent] = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
+                        continue;
+                    }
+                    float o[N];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) o[i] = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
+                    uint32_t two[N / 2];
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) {                          // the other lane of a pair has the next dimension
+                        const bool odd = lane & 1;
+                        const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i] : o[i + N / 2], 1);
+                        two[i] = odd ? pack_bf16x2(got, o[i + N / 2]) : pack_bf16x2(o[i], got);
+                    }
+#pragma unroll
+                    for (int i = 0; i < N / 4; ++i) {
+                        const bool up = lane & 2;
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? two[i] : two[i + N / 4], 2);
+                        if (to[i] >= 0)
+                            *reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(to[i]) * kLatent + u * 128 + (token & ~3)) =
+                                up ? make_uint2(got, two[i + N / 4]) : make_uint2(two[i], got);
                     }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.o_empty));
-            ++item;
-        } while (w.next(c, q));
+            if (!more) break;
+        }
     }
 
     // ---------------------------------------------------------------- teardown
