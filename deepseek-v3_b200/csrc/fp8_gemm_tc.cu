@@ -829,6 +829,29 @@ int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int b
     return DSV3_OK;
 }
 
+// [rows, K] bytes, row-major, rows a multiple of 8 and K of 128; box = all chunks of 128 bytes of box_rows rows, in shared memory as groups of
+// eight rows: [box_rows / 8][K / 128][8][128], 128-byte swizzle, zero fill outside.
+int make_tmap_groups(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) {
+        set_last_error("cuTensorMapEncodeTiled is not available from the driver");
+        return DSV3_ERR_CUDA;
+    }
+    const cuuint64_t dims[4] = {kChunk, 8, static_cast<cuuint64_t>(K / kChunk), static_cast<cuuint64_t>(rows / 8)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(K), kChunk, static_cast<cuuint64_t>(8 * K)};
+    const cuuint32_t box[4] = {kChunk, 8, static_cast<cuuint32_t>(K / kChunk), static_cast<cuuint32_t>(box_rows / 8)};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled (groups of rows) failed with CUresult %d (rows=%lld K=%lld box_rows=%d)", static_cast<int>(r),
+                       static_cast<long long>(rows), static_cast<long long>(K), box_rows);
+        return DSV3_ERR_CUDA;
+    }
+    return DSV3_OK;
+}
+
 // Result matrix [M, N] bf16, row-major; box = 64 columns (128 bytes) x box_rows rows, 128-byte swizzle.
 int make_tmap_out(CUtensorMap* map, void* base, int64_t M, int64_t N, int box_rows) {
     EncodeTiledFn fn = encode_fn();

@@ -26,15 +26,21 @@
 namespace dsv3 {
 
 int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows);
+int make_tmap_groups(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows);
 
 namespace {
 
 constexpr int kTokens = 128;              // of a tile: MMA M of the first product, K of the second
-constexpr int kUnitBytes = kTokens * 128; // 128 bytes of each of a tile's tokens: a quarter of the latents, or the rotated values
-constexpr int kTileUnits = 5;
+// A tile is loaded and given back in two units of 64 tokens.  Its latents lie as [16 groups of eight tokens][4 chunks of 128 dimensions][8 tokens][128 bytes],
+// swizzled over 128 bytes: one copy brings a page's share of a unit, all four chunks of it (a copy per chunk and page: 450 cycles a chunk to issue, more
+// than a tile's share of HBM takes), and both MMAs find a chunk's groups 4096 bytes apart.
+constexpr int kUnitTokens = 64, kTileSlots = 2;
+constexpr int kLatentBytes = kTokens * kLatent, kRopeBytes = kTokens * 2 * kRope, kTileBytes = kLatentBytes + kRopeBytes;
+constexpr int kGroupBytes = 8 * kLatent;
 constexpr int kSoftmaxWarps = 8, kFirstSoftmaxWarp = 4;
 constexpr int kAttnThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
 constexpr int kScaleSlots = 4;
+constexpr int kFewParts = 8;              // of a block that several CTAs worked on
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // The running maximum moves when a score exceeds it by more than kSlack, and stands for 2^kTop: the largest weight is 2^8.
 constexpr float kSlack = 1.0f, kTop = 7.0f;
@@ -53,14 +59,14 @@ struct Queries {
     float* lse;
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
+    int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
     float* partial;                       // [2 * grid][R, 512]
     float* partial_lse;                   // [2 * grid][R]
-    int4* cut;                            // [grid]: the item that begins in a CTA and ends in a later one
+    int4* cut;                            // [2 * grid]: the item that begins in a CTA and ends in a later one
 };
 
 template <int R>
 struct Cfg {
-    static constexpr int kUnits = R == 16 ? 12 : 10;
     static constexpr int kQChunk = 2 * R * 128;                 // hi and lo rows of 128 latents
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
@@ -81,7 +87,7 @@ struct Small {                                                  // shared memory
     float top[2][2][4][R / 2];                                  // [tile parity][half][warp][row]
     float sum[2][4][R / 2];
     float row[kSoftmaxWarps][R / 2], row2[kSoftmaxWarps][R / 2];
-    uint64_t full[Cfg<R>::kUnits], empty[Cfg<R>::kUnits];
+    uint64_t full[2 * kTileSlots], empty[2 * kTileSlots];
     uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
     Control ctl;
     int64_t warp_sum[kAttnThreads / 32];
@@ -91,7 +97,7 @@ struct Small {                                                  // shared memory
 
 template <int R>
 constexpr int smem_bytes() {
-    return 1024 + Cfg<R>::kUnits * kUnitBytes + Cfg<R>::kQBytes + 2 * Cfg<R>::kPBytes + static_cast<int>(sizeof(Small<R>));
+    return 1024 + kTileSlots * kTileBytes + Cfg<R>::kQBytes + 2 * Cfg<R>::kPBytes + static_cast<int>(sizeof(Small<R>));
 }
 static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
 
@@ -126,6 +132,12 @@ __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t* r) {
                      : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// All chunks of groups of eight rows from `group` on, to shared memory as [group][chunk][8][128]
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int group, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst), "l"(tmap), "r"(0),
+                 "r"(group), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
@@ -136,16 +148,16 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Operand descriptor of a transposed (MN-major) tile with rows of kWidth bytes, one row per step of K, swizzled over kWidth bytes: groups of eight rows are
-// 8 * kWidth bytes apart.  The tile is one swizzle atom wide, so that the offset between atoms is not used.
-template <int kWidth>
-__device__ __forceinline__ uint64_t umma_desc_mn_major(uint32_t smem_addr) {
+// Operand descriptor of a tile whose rows of kWidth bytes are swizzled over that width, groups of eight rows kGroup bytes apart: rows are rows of the
+// matrix (K-major), or steps of K (transposed, MN-major).  The operand is one swizzle atom wide, so that the offset between atoms is not used.
+template <int kWidth, int kGroup>
+__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr) {
     static_assert(kWidth == 32 || kWidth == 64 || kWidth == 128, "swizzle width");
     constexpr uint64_t layout = kWidth == 128 ? 2 : kWidth == 64 ? 4 : 6;
     uint64_t d = 0;
     d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(8 * kWidth >> 4) << 16;
-    d |= static_cast<uint64_t>(8 * kWidth >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(kGroup >> 4) << 32;
     d |= static_cast<uint64_t>(1) << 46;
     d |= layout << 61;
     return d;
@@ -220,9 +232,9 @@ struct Walk {
         }
         offset -= tiles_before(q, s, lo, blocks) * q.head_blocks;
         block = lo;
-        const int t = block_tiles(q, s, lo);
-        head_block = static_cast<int>(offset / t);
-        tile = static_cast<int>(offset - static_cast<int64_t>(head_block) * t);
+        const uint32_t t = block_tiles(q, s, lo), rest = static_cast<uint32_t>(offset);    // less than the tiles of one block of tokens
+        head_block = static_cast<int>(rest / t);
+        tile = static_cast<int>(rest - head_block * t);
         left = share;
         settle(q);
     }
@@ -242,10 +254,27 @@ struct Walk {
     }
 };
 
+// The list cut in equal shares: the first `more` of them have one tile more.  No share is empty before the last that is not.
+struct Shares {
+    int64_t size_less, more;
+    int ctas;
+    __device__ int64_t first(int64_t c) const { return size_less * min(c, static_cast<int64_t>(ctas)) + min(c, more); }
+    __device__ int64_t size(int64_t c) const { return c < ctas ? size_less + (c < more ? 1 : 0) : 0; }
+    __device__ int owner(int64_t tile) const {
+        const int64_t large = more * (size_less + 1);
+        return static_cast<int>(tile < large ? tile / (size_less + 1) : more + (tile - large) / size_less);
+    }
+};
+__device__ __forceinline__ Shares shares_of(int64_t total, int ctas) {
+    if (total < ctas) return {1, 0, static_cast<int>(total)};
+    const int64_t each = (total >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas)) : total / ctas;
+    return {each, total - each * ctas, ctas};
+}
+
 // Row r of an item's block: query * heads + head, or -1 where it is none.
 __device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) {
-    int token = w.block << q.block_shift, head = w.head_block * rows + r;
-    if (q.head_blocks == 1) {
+    int token = w.block << q.block_shift, head = (w.head_block + static_cast<int>(blockIdx.x) % q.group) * rows + r;
+    if (q.heads <= rows) {
         if (r >= q.heads << q.block_shift) return -1;
         token += r / q.heads;
         head = r % q.heads;
@@ -255,7 +284,7 @@ __device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int row
 
 // All threads: this CTA's share [*first, *first + share) of the list, and where in which sequence it starts.
 template <typename Sm>
-__device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, int64_t* total_out, int64_t* first_out) {
+__device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, Shares* shares_out, int64_t* first_out) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Seq x;
     const auto mine = [&](int s) -> int64_t {
@@ -289,10 +318,10 @@ __device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, in
         scan(mine(s0 + threadIdx.x), &sum);
         total += sum;
     }
-    // (no CTA between two that work on the same block is without a tile)
-    const int64_t ctas = min(total, static_cast<int64_t>(gridDim.x)), at_cta = min(static_cast<int64_t>(blockIdx.x), ctas);
-    const int64_t first = ctas ? total * at_cta / ctas : 0, share = at_cta < ctas ? total * (at_cta + 1) / ctas - first : 0;
-    *total_out = total;
+    const Shares sh = shares_of(total, gridDim.x / q.group);
+    const int64_t at_cta = blockIdx.x / q.group;
+    const int64_t first = sh.first(at_cta), share = sh.size(at_cta);
+    *shares_out = sh;
     *first_out = first;
     if (share == 0) return 0;
     int64_t at = 0;
@@ -356,8 +385,8 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     constexpr int N = C::kRows;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* const units = smem;
-    uint8_t* const qs = units + C::kUnits * kUnitBytes;
+    uint8_t* const tiles = smem;
+    uint8_t* const qs = tiles + kTileSlots * kTileBytes;
     uint8_t* const ps = qs + C::kQBytes;
     Small<R>& sm = *reinterpret_cast<Small<R>*>(ps + 2 * C::kPBytes);
     Control* const ctl = &sm.ctl;
@@ -366,7 +395,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 
     griddep_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::kUnits; ++i) {
+        for (int i = 0; i < 2 * kTileSlots; ++i) {
             mbar_init(bar(sm.full[i]), 1);
             mbar_init(bar(sm.empty[i]), 1);
         }
@@ -387,13 +416,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         tma_prefetch_desc(&map_rope);
     }
     griddep_wait();
-    int64_t total, first;
-    const int64_t share = find_share(c, q, sm, &total, &first);     // (its barriers also publish what was set up above)
+    Shares shares;
+    int64_t first;
+    const int64_t share = find_share(c, q, sm, &shares, &first);     // (its barriers also publish what was set up above)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
-    if (threadIdx.x == 32 * kFirstSoftmaxWarp && q.cut) q.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 32 * kFirstSoftmaxWarp && q.cut) q.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
 
     Walk w;
     if (share > 0) w.begin(q, sm.start, sm.start_offset, share);
@@ -403,14 +433,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     } else if (warp == 0) {
         // ------------------------------------------------------------ loads.  The lanes look up a tile's pages together, one tile ahead; one lane issues, with
         // coordinates that the warp has in common: copies issued by the lanes of several pages cost 490 cycles a unit.
-        const int rows = min(1 << c.page_shift, kTokens), boxes_max = kTokens / rows;
+        const int rows = min(1 << c.page_shift, kUnitTokens), unit_boxes = kUnitTokens / rows;
         const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
-        uint32_t unit = 0, slot = 0, turn = 1, tile_count = 0;
+        uint32_t tile_count = 0;
         bool ok = true;
         // the slot where this lane's box of a tile begins; absent: -1, behind the sequence's end: -2
         const auto look_up = [&](const Walk& at, int t) -> int {
             const int64_t p0 = static_cast<int64_t>(at.tile + t) * kTokens + lane * rows;
-            return lane < boxes_max && p0 < at.s.len ? slot_of(c, at.seq, static_cast<uint32_t>(p0)) : -2;
+            return lane < 2 * unit_boxes && p0 < at.s.len ? slot_of(c, at.seq, static_cast<uint32_t>(p0)) : -2;
         };
         int mine = look_up(w, 0);
         bool more = true;
@@ -424,76 +454,76 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     more = w.next(c, q);
                     if (more) mine = look_up(w, 0);
                 }
-                const int boxes = __popc(__ballot_sync(0xffffffffu, at > -2)), present = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                const uint32_t used = __ballot_sync(0xffffffffu, at > -2), present = __ballot_sync(0xffffffffu, at >= 0);
                 float* const scales = sm.scales[tile_count & (kScaleSlots - 1)];
-                for (int u = 0; u < kTileUnits; ++u, ++unit) {
-                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), turn, ctl, status, 1, unit));
+                const uint32_t tile_at = smem_u32(tiles) + (tile_count & 1) * kTileBytes;
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t slot = 2 * (tile_count & 1) + h, full = bar(sm.full[slot]);
+                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), ((tile_count >> 1) & 1) ^ 1, ctl, status, 1, tile_count));
                     if (!ok) break;
-                    if (u == 0 && boxes != present) {                          // an absent page: its tokens have no scale
-                        if (at == -1)
+                    const uint32_t of_unit = ((1u << unit_boxes) - 1u) << (h * unit_boxes);
+                    const int boxes = __popc(used & of_unit);
+                    if ((used & ~present & of_unit) != 0) {                    // an absent page: its tokens have no scale
+                        if (at == -1 && lane / unit_boxes == h)
                             for (int i = 0; i < rows; ++i) scales[lane * rows + i] = 0.0f;
                         __syncwarp();
                     }
-                    const uint32_t full = bar(sm.full[slot]), dst = smem_u32(units) + slot * kUnitBytes;
-                    if (elect_one()) mbar_arrive_expect_tx(full, boxes * rows * 128 + (u == 0 ? present * rows * 4 : 0));
-                    for (int i = 0; i < boxes; ++i) {
+                    if (elect_one()) mbar_arrive_expect_tx(full, boxes * rows * (kLatent + 2 * kRope) + __popc(present & of_unit) * rows * 4);
+                    for (int i = h * unit_boxes; i < h * unit_boxes + boxes; ++i) {
                         const int from = __shfl_sync(0xffffffffu, at, i);
                         const int y = from >= 0 ? from : static_cast<int>(outside);
                         if (elect_one()) {
-                            if (u < 4) tma_load_2d(dst + i * rows * 128, &map_latent, u * 128, y, full);
-                            else tma_load_2d(dst + i * rows * 128, &map_rope, 0, y, full);
-                            if (u == 0 && from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
+                            tma_load_4d(tile_at + i * rows * kLatent, &map_latent, y >> 3, full);
+                            tma_load_2d(tile_at + kLatentBytes + i * rows * 2 * kRope, &map_rope, 0, y, full);
+                            if (from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
                         }
                         __syncwarp();
                     }
-                    if (++slot == C::kUnits) slot = 0, turn ^= 1;
                 }
             }
             more = more && ok;
         }
         // none of the commits onto empty[] may be in flight when the CTA leaves its shared memory to another
-        for (uint32_t u = unit > C::kUnits ? unit - C::kUnits : 0u; ok && u < unit; ++u)
-            ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[u % C::kUnits]), (u / C::kUnits) & 1, ctl, status, 1, u));
+        for (uint32_t t = tile_count > 2 ? tile_count - 2 : 0u; ok && t < tile_count; ++t)
+            for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[2 * (t & 1) + h]), (t >> 1) & 1, ctl, status, 1, t));
     } else if (warp == 1) {
         // ------------------------------------------------------------ scores.  The warp stays converged and elects a lane for the MMAs alone: addresses and
         // descriptors then stay in uniform registers.  The sums have an issuer of their own: in one thread, a tile whose weights are there waits behind
         // the next tile's loads, which wait for the room that its sums make.
         constexpr uint32_t idesc_s = umma_idesc_e4m3_f32(kTokens, 2 * R), idesc_r = idesc_bf16(kTokens, R);
-        const uint32_t units_at = smem_u32(units), q_at = smem_u32(qs);
-        uint32_t slot = 0, turn = 0, count = 0, item = 0;                      // ring position and its parity, tiles, items
+        const uint32_t q_at = smem_u32(qs);
+        uint32_t count = 0, item = 0;                                          // tiles, items
         bool ok = true;
         do {
             ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item));
             for (int t = 0; t < w.n && ok; ++t, ++count) {
-                const uint32_t b = count & 1, d = tmem + b * C::kTmemS;
-                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.s_empty[b]), ((count >> 1) & 1) ^ 1, ctl, status, 3, count));
-                for (int u = 0; u < kTileUnits && ok; ++u) {
-                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.full[slot]), turn, ctl, status, 2, count));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t da = umma_desc_k_major_sw128(units_at + slot * kUnitBytes), db = umma_desc_k_major_sw128(q_at + u * C::kQChunk);
-                    if (elect_one()) {
+                const uint32_t b = count & 1, phase = (count >> 1) & 1, d = tmem + b * C::kTmemS, at = smem_u32(tiles) + b * kTileBytes;
+                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.s_empty[b]), phase ^ 1, ctl, status, 3, count));
+                for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.full[2 * b + h]), phase, ctl, status, 2, count));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t da = umma_desc<128, kGroupBytes>(at), db = umma_desc<128, 1024>(q_at);
+                const uint64_t ra = umma_desc<128, 1024>(at + kLatentBytes), rb = umma_desc<128, 1024>(q_at + 4 * C::kQChunk);
+                if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {                          // 32 bytes of K a step
-                            if (u < 4) tc_mma_f8(d, da + 2 * k, db + 2 * k, idesc_s, (u | k) != 0);
-                            else tc_mma_bf16(d + 2 * R, da + 2 * k, db + 2 * k, idesc_r, k != 0);
-                        }
-                        if (u == 4) {
-                            tc_commit(bar(sm.empty[slot]));
-                            tc_commit(bar(sm.s_full[b]));
-                        }
+                    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)                            // 32 bytes of K a step
+                            tc_mma_f8(d, da + (u * 1024 >> 4) + 2 * k, db + (u * C::kQChunk >> 4) + 2 * k, idesc_s, (u | k) != 0);
                     }
-                    __syncwarp();
-                    if (++slot == C::kUnits) slot = 0, turn ^= 1;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma_bf16(d + 2 * R, ra + 2 * k, rb + 2 * k, idesc_r, k != 0);
+                    tc_commit(bar(sm.s_full[b]));
                 }
+                __syncwarp();
             }
             ++item;
         } while (ok && w.next(c, q));
     } else if (warp == 2) {
         // ------------------------------------------------------------ sums
         constexpr uint32_t idesc_o = umma_idesc_e4m3_f32(kTokens, 2 * R) | kIdescTransposed;
-        const uint32_t units_at = smem_u32(units), p_at = smem_u32(ps);
-        uint32_t slot = 0, count = 0, item = 0;
+        const uint32_t p_at = smem_u32(ps);
+        uint32_t count = 0, item = 0;
         bool ok = true;
         do {
             for (int t = 0; t < w.n && ok; ++t, ++count) {
@@ -503,22 +533,18 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 if (ok && t == 0) ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, 12, item));
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t db = umma_desc_mn_major<2 * R>(p_at + b * C::kPBytes);
+                const uint64_t da = umma_desc<128, kGroupBytes>(smem_u32(tiles) + b * kTileBytes), db = umma_desc<2 * R, 16 * R>(p_at + b * C::kPBytes);
+                if (elect_one()) {
 #pragma unroll
-                for (int u = 0; u < kTileUnits; ++u) {
-                    if (u < 4) {
-                        const uint64_t da = umma_desc_mn_major<128>(units_at + slot * kUnitBytes);
-                        if (elect_one()) {
+                    for (int k = 0; k < 4; ++k) {                              // 32 tokens a step
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)                        // 32 tokens a step
-                                tc_mma_f8(tmem + C::kTmemO + u * 2 * R, da + (k * 32 * 128 >> 4), db + (k * 32 * 2 * R >> 4), idesc_o, (t | k) != 0);
-                            tc_commit(bar(sm.empty[slot]));
-                            if (u == 3) tc_commit(bar(sm.p_empty[b]));
-                        }
-                        __syncwarp();
+                        for (int u = 0; u < 4; ++u)
+                            tc_mma_f8(tmem + C::kTmemO + u * 2 * R, da + ((k * 4 * kGroupBytes + u * 1024) >> 4), db + (k * 32 * 2 * R >> 4), idesc_o, (t | k) != 0);
+                        if (k & 1) tc_commit(bar(sm.empty[2 * b + (k >> 1)]));
                     }
-                    if (++slot == C::kUnits) slot = 0;
+                    tc_commit(bar(sm.p_empty[b]));
                 }
+                __syncwarp();
             }
             ++item;
         } while (ok && w.next(c, q));
@@ -618,9 +644,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             const int base = w.s.len - w.s.queries;                            // position of the first query's token
             for (int t = 0; t < w.n; ++t, ++tile_count) {
                 const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
-                const uint32_t unit = tile_count * kTileUnits;
                 const int p = (w.tile + t) * kTokens + token;
-                ok = ok && wait(sm.full[unit % C::kUnits], (unit / C::kUnits) & 1, 2, unit);
+                // (room for the weights, and the tokens' scales: both there before the scores are)
+                if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, 12, tile_count);
+                ok = ok && wait(sm.full[2 * b + (quarter >> 1)], phase, 2, tile_count);
                 const float sc = sm.scales[tile_count & (kScaleSlots - 1)][token];
                 ok = ok && wait(sm.s_full[b], phase, 4, tile_count);
                 tc_fence_after();
@@ -698,7 +725,6 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     }
                 }
                 // -------- weights: hi and lo, to shared memory
-                if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, 12, tile_count);
                 if (ok) {
                     const float inv = present ? power_reciprocal(sc) : 0.0f;
                     uint32_t hi[N / 4], lo[N / 4];
@@ -724,17 +750,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         *reinterpret_cast<uint2*>(row + ((1 ^ turn) << 4) + half * 8) = make_uint2(lo[0], lo[1]);
                     }
                     // Behind the sequence's end lie other sequences' bytes, or none at all; no weight, but 0 x NaN is not 0.
-                    if (__any_sync(0xffffffffu, p >= w.s.len)) {
+                    if (p >= w.s.len) {
+                        uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + half * 2048;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t mine = unit + half * 2 + u, at = mine % C::kUnits;
-                            ok = ok && wait(sm.full[at], (mine / C::kUnits) & 1, 2, mine);
-                            if (ok && p >= w.s.len) {
-                                uint4* const v = reinterpret_cast<uint4*>(units + at * kUnitBytes + token * 128);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
-                            }
-                        }
+                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     tc_fence_before();
                     fence_proxy_async_shared();
@@ -762,9 +781,13 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 if (!whole) q.partial_lse[static_cast<int64_t>(part) * R + r] = lse2;
                 else if (q.lse && to >= 0) q.lse[to] = lse2 * kLn2;
             }
-            if (threadIdx.x == 32 * kFirstSoftmaxWarp && begins && !ends) {
-                const int64_t end = first + (share - done.left) - done.n + done.tiles;      // of the block's tiles, in the list
-                q.cut[blockIdx.x] = make_int4(done.seq, done.block, done.head_block, static_cast<int>((end * min(total, static_cast<int64_t>(gridDim.x)) - 1) / total));
+            if (threadIdx.x == 32 * kFirstSoftmaxWarp && !ends) {                // (one item of a CTA at most)
+                const int64_t start = first + (share - done.left) - done.n - done.tile;     // of the block's tiles, in the list
+                const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + done.tiles - 1) - begun + 1;
+                if (begins || parts > kFewParts) {
+                    q.cut[2 * blockIdx.x] = make_int4(parts, done.block, done.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
+                    q.cut[2 * blockIdx.x + 1] = make_int4(done.s.len, done.s.queries, done.s.first, 0);
+                }
             }
             // four rows that this lane writes: 8 bytes each, of four dimensions that it gets from its neighbours
             int to[N / 4];
@@ -833,28 +856,34 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
-// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  A block of threads to kCombineRows rows of a cut block, which is
-// named by the CTA that it begins in.
-constexpr int kCombineThreads = 256, kCombineRows = 2;
+// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  A row of thread blocks to every CTA of the kernel before: where a block of
+// query heads is in few parts, the row of the CTA that it begins in joins them, 128 threads to a query head; where it is in many, the rows of all
+// CTAs but its last share the query heads, and a thread block splits a head's parts among its four teams.
+constexpr int kCombineThreads = 512, kTeams = kCombineThreads / 128;
 template <int R>
-__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const LatentCache c, const Queries q) {
+__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Queries q) {
+    __shared__ float4 sums[kTeams][128];
+    __shared__ float weights[kTeams];
     griddep_launch_dependents();
     griddep_wait();
-    const int4 cut = q.cut[blockIdx.x];
+    const int4 cut = q.cut[2 * blockIdx.x];
     if (cut.x < 0) return;
-    const int r = blockIdx.y * kCombineRows + threadIdx.x / 128;
-    const Seq s = load_seq(c, q, cut.x);
-    int tok = cut.y << q.block_shift, head = cut.z * R + r;
-    if (q.head_blocks == 1) {
-        tok += r / q.heads;
-        head = r % q.heads;
-    }
-    if (head >= q.heads || tok >= s.queries || (q.head_blocks == 1 && r >= q.heads << q.block_shift)) return;
-    const int parts = cut.w - static_cast<int>(blockIdx.x) + 1;
-    const auto part = [&](int i) { return static_cast<int64_t>(2 * (static_cast<int>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * R + r; };
-    float top = -INFINITY;
+    const int4 seq = q.cut[2 * blockIdx.x + 1];
+    Walk w;
+    w.block = cut.y, w.head_block = cut.z;
+    w.s = {seq.x, seq.y, seq.z};
+    const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
+    const bool few = parts <= kFewParts;
+    const int r = few ? blockIdx.y * kTeams + team : cut.w * (R / kTeams) + blockIdx.y;
+    if (r >= R) return;
+    const int place = place_of(q, w, R, r);
+    if (place < 0) return;                                                     // (a whole team, or, with many parts, the whole block)
+    const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
+    const auto part = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R + r; };
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     bool nan = false;
-    for (int i = threadIdx.x & 31; i < parts; i += 32) {
+    for (int i = lane; i < parts; i += 32) {
         const float v = q.partial_lse[part(i)];
         nan = nan || isnan(v);
         top = fmaxf(top, v);
@@ -863,26 +892,35 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const L
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     nan = __any_sync(0xffffffffu, nan);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
+#pragma unroll 8
+    for (int i = few ? 0 : team; i < parts; i += few ? 1 : kTeams) {
         const float f = ex2(q.partial_lse[part(i)] - ref);
-        const float4 v = reinterpret_cast<const float4*>(q.partial + part(i) * kLatent)[threadIdx.x & 127];
+        const float4 v = reinterpret_cast<const float4*>(q.partial + part(i) * kLatent)[at];
         sum += f;
         acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
     }
+    if (!few) {
+        sums[team][at] = acc;
+        if (at == 0) weights[team] = sum;
+        __syncthreads();
+        if (team != 0) return;
+#pragma unroll
+        for (int i = 1; i < kTeams; ++i) {
+            const float4 v = sums[i][at];
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            sum += weights[i];
+        }
+    }
     const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t to = (static_cast<int64_t>(s.first) + tok) * q.heads + head;
-    reinterpret_cast<uint2*>(q.out + to * kLatent)[threadIdx.x & 127] =
+    reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(place) * kLatent)[at] =
         make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (q.lse && (threadIdx.x & 127) == 0) q.lse[to] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+    if (q.lse && at == 0) q.lse[place] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
 // Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
 int block_rows(int64_t tokens, int heads, int n_seqs) { return (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32; }
 
-size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + sizeof(int4)); }
+size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
 
 template <int R>
 int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool cut, unsigned int* status,
@@ -891,7 +929,7 @@ int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const
     DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
     if (cut)
-        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / kCombineRows), dim3(kCombineThreads), 0, stream, c, q));
+        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / kTeams), dim3(kCombineThreads), 0, stream, q));
     return DSV3_OK;
 }
 
@@ -946,21 +984,23 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     unsigned int* const status = status_device_ptr();
     if (!status) return DSV3_ERR_CUDA;
     const int64_t slots = static_cast<int64_t>(c.n_pages) << c.page_shift;
-    const int box = c.page_shift < 7 ? 1 << c.page_shift : kTokens;
+    const int box = c.page_shift < 6 ? 1 << c.page_shift : kUnitTokens;
     CUtensorMap map_latent, map_rope;
-    if (const int rc = make_tmap(&map_latent, c.latent, slots, kLatent, box); rc != DSV3_OK) return rc;
+    if (const int rc = make_tmap_groups(&map_latent, c.latent, slots, kLatent, box); rc != DSV3_OK) return rc;
     if (const int rc = make_tmap(&map_rope, c.rope, slots, 2 * kRope, box); rc != DSV3_OK) return rc;
     // tokens to a block: a power of two, so that the tiles of a causal sequence can be counted without adding them up
     int shift = 0;
     while ((heads << (shift + 1)) <= rows) ++shift;
+    // the blocks of a token's heads see the same tiles: side by side in as many CTAs, unless those are not there
+    const int head_blocks = (heads + rows - 1) / rows, group = 2 * head_blocks <= grid ? head_blocks : 1;
     float* const partial = static_cast<float*>(workspace);
     float* const partial_lse = cut ? partial + static_cast<size_t>(grid) * 2 * rows * kLatent : nullptr;
     int4* const list = cut ? reinterpret_cast<int4*>(partial_lse + static_cast<size_t>(grid) * 2 * rows) : nullptr;
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       (heads + rows - 1) / rows, shift, partial, partial_lse, list};
-    return rows == 16 ? launch<16>(c, q, map_latent, map_rope, grid, cut, status, st) : launch<32>(c, q, map_latent, map_rope, grid, cut, status, st);
+                       head_blocks / group, shift, group, partial, partial_lse, list};
+    return rows == 16 ? launch<16>(c, q, map_latent, map_rope, grid / group * group, cut, status, st) : launch<32>(c, q, map_latent, map_rope, grid / group * group, cut, status, st);
 }
 
 }  // extern "C"
