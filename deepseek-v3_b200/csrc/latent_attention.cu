@@ -9,8 +9,8 @@
 // hi = e4m3(q), lo = e4m3(q - hi) is the query itself (scaled by a power of two per row, and down to 2^-18 of the row's largest value); a weight 2^(y - m) is off by
 // at most 2^-8 of itself, what rounding it to bf16 would cost.  Two e4m3 products take the time of one in bf16, and half the operand bytes.
 //   The token's scale is a factor of its scores and, taken into the exponent as log2 s, of its weight in the second product.
-//   Rounding of small weights: lo is stored times 16, so that its grid is 2^-13 of a scale on which the row's largest weight lies in [2^7, 2^8); what is
-// below half of that would round to zero, and thousands of tokens that each weigh 2^-21 of one first token do matter.  So a fixed offset
+//   Rounding of small weights: lo is stored times 16, so that its grid is 2^-13 on a scale where the row's largest weight is 2^5 or more; what is
+// below half of that would round to zero, and thousands of tokens that each weigh 2^-19 of one first token do matter.  So a fixed offset
 // per token, evenly spread over a step of the grid, is added before rounding: sums of small weights stay what they are.
 //
 // The tokens are the rows of both MMAs (128 of them) and the query heads the columns: with 16 query heads (one decoding sequence on one rank of
@@ -40,10 +40,12 @@ constexpr int kGroupBytes = 8 * kLatent;
 constexpr int kSoftmaxWarps = 8, kFirstSoftmaxWarp = 4;
 constexpr int kAttnThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
 constexpr int kScaleSlots = 4;
+constexpr int kAhead = 4, kBoxSlots = 4;  // tiles whose pages are looked up before they are loaded; of which the pages are kept
 constexpr int kFewParts = 8;              // of a block that several CTAs worked on
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-// The running maximum moves when a score exceeds it by more than kSlack, and stands for 2^kTop: the largest weight is 2^8.
-constexpr float kSlack = 1.0f, kTop = 7.0f;
+// The maximum that weights are relative to moves when a weight would pass 2^(kTop + kSlack), and then stands for 2^kTop.  e4m3 ends at 448; a wide slack costs two of
+// the bits below (see the grid of small weights above) and spares nearly all passes over the sums so far.
+constexpr float kTop = 5.0f, kSlack = 3.75f;
 constexpr float kNothing = -3.0e38f;      // below every finite score, and no infinity: -inf less this is -inf
 constexpr float kLoScale = 16.0f;         // the largest remainder is 2^-4 of 2^8
 
@@ -76,30 +78,6 @@ struct Cfg {
     static constexpr int kTmemCols = R == 16 ? 256 : 512;
     static_assert(kTmemO + 8 * R <= kTmemCols, "TMEM");
 };
-
-template <int R>
-struct Small {                                                  // shared memory beside the operand tiles
-    float scales[kScaleSlots][kTokens];
-    float factor[2][R];                                         // k[r] by item parity
-    int64_t tree[2][R];
-    int place[2][R];                                            // query * heads + head, -1 for a row that is none
-    int limit[2][R];                                            // last position that a row sees (a tree: of those before the queries)
-    float top[2][2][4][R / 2];                                  // [tile parity][half][warp][row]
-    float sum[2][4][R / 2];
-    float row[kSoftmaxWarps][R / 2], row2[kSoftmaxWarps][R / 2];
-    uint64_t full[2 * kTileSlots], empty[2 * kTileSlots];
-    uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
-    Control ctl;
-    int64_t warp_sum[kAttnThreads / 32];
-    int64_t start_offset;
-    int4 start;                                                 // sequence, its cached tokens, queries, first query
-};
-
-template <int R>
-constexpr int smem_bytes() {
-    return 1024 + kTileSlots * kTileBytes + Cfg<R>::kQBytes + 2 * Cfg<R>::kPBytes + static_cast<int>(sizeof(Small<R>));
-}
-static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
 
 // ---------------------------------------------------------------- PTX
 __device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -168,8 +146,8 @@ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f
 // ---------------------------------------------------------------- who works on what
 // The work is a list of tiles: for every sequence, block of its query heads and 128 cached tokens that some row of the block sees one (at least one
 // per block, which writes the zeros of rows that see nothing).  A CTA takes an equal, contiguous share of the list, whatever the lengths are; a block's
-// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  Every role walks the
-// list by itself.
+// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  One warp walks the
+// list and leaves what the others need in shared memory.
 struct Seq {
     int len, queries, first;              // cached tokens, queries, index of the first query
 };
@@ -192,39 +170,40 @@ __device__ __forceinline__ int block_tiles(const Queries& q, const Seq& s, int b
     return tiles_of(s.len - s.queries + min((block + 1) << q.block_shift, s.queries));
 }
 // sum over j = 1 .. x of max(1, ceil(j / m)); x <= 0: what is to be subtracted for j = x + 1 .. 0
-__device__ __forceinline__ int64_t ramp(int64_t x, int shift) {
+__device__ __forceinline__ int64_t ramp(int x, int shift) {
     if (x <= 0) return x;
-    const int64_t m = 1ll << shift, n = x >> shift;
-    return m * (n * (n + 1) / 2) + (x - (n << shift)) * (n + 1);
+    const uint32_t n = x >> shift, rest = x - (n << shift);
+    return ((static_cast<uint64_t>(n) * (n + 1) / 2) << shift) + static_cast<uint64_t>(rest) * (n + 1);
 }
 // Tiles of a sequence's first n blocks of tokens (of one block of heads).  Block i sees base + (i + 1) 2^b tokens (the last one: all); with m = 128 / 2^b that
 // is ceil((u + i + 1) / m) tiles, where u = ceil(base / 2^b).
-__device__ __forceinline__ int64_t tiles_before(const Queries& q, const Seq& s, int n, int blocks) {
+__device__ __forceinline__ int tiles_before(const Queries& q, const Seq& s, int n, int blocks) {
     if (n == 0) return 0;
-    if (q.tree) return static_cast<int64_t>(n) * tiles_of(s.len);
-    const int64_t u = (static_cast<int64_t>(s.len) - s.queries + (1 << q.block_shift) - 1) >> q.block_shift;
+    if (q.tree || blocks == 1) return n * tiles_of(s.len);
+    const int u = (s.len - s.queries + (1 << q.block_shift) - 1) >> q.block_shift;
     const int shift = 7 - q.block_shift;
     const int whole = n == blocks ? n - 1 : n;
-    return ramp(u + whole, shift) - ramp(u, shift) + (n == blocks ? tiles_of(s.len) : 0);
+    return static_cast<int>(ramp(u + whole, shift) - ramp(u, shift)) + (n == blocks ? tiles_of(s.len) : 0);
 }
 
 struct Walk {
     Seq s;
     int seq, block, head_block;
     int tile, n, tiles;                   // first tile of the item, how many, how many the whole block has
-    int64_t left;                         // of the CTA's share, behind this item
+    int left;                             // of the CTA's share, behind this item
 
     __device__ void settle(const Queries& q) {
         tiles = block_tiles(q, s, block);
-        n = static_cast<int>(min(static_cast<int64_t>(tiles - tile), left));
+        n = min(tiles - tile, left);
         left -= n;
     }
     // the share starts at tile `offset` of sequence `sq`
-    __device__ void begin(const Queries& q, const int4& start, int64_t offset, int64_t share) {
-        seq = start.x;
-        s = {start.y, start.z, start.w};
+    __device__ __forceinline__ void begin(const Queries& q, int sq, const Seq& x, int offset, int share) {
+        seq = sq;
+        s = x;
         const int blocks = blocks_of(q, s);
         int lo = 0, hi = blocks;          // largest block whose tiles begin at or before the offset
+#pragma unroll 1
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (tiles_before(q, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
@@ -232,13 +211,13 @@ struct Walk {
         }
         offset -= tiles_before(q, s, lo, blocks) * q.head_blocks;
         block = lo;
-        const uint32_t t = block_tiles(q, s, lo), rest = static_cast<uint32_t>(offset);    // less than the tiles of one block of tokens
-        head_block = static_cast<int>(rest / t);
-        tile = static_cast<int>(rest - head_block * t);
+        const int t = block_tiles(q, s, lo);
+        head_block = q.head_blocks > 1 ? offset / t : 0;
+        tile = offset - head_block * t;
         left = share;
         settle(q);
     }
-    __device__ bool next(const LatentCache& c, const Queries& q) {
+    __device__ __forceinline__ bool next(const LatentCache& c, const Queries& q) {
         if (left == 0) return false;
         tile = 0;
         if (++head_block == q.head_blocks) {
@@ -256,18 +235,17 @@ struct Walk {
 
 // The list cut in equal shares: the first `more` of them have one tile more.  No share is empty before the last that is not.
 struct Shares {
-    int64_t size_less, more;
-    int ctas;
-    __device__ int64_t first(int64_t c) const { return size_less * min(c, static_cast<int64_t>(ctas)) + min(c, more); }
-    __device__ int64_t size(int64_t c) const { return c < ctas ? size_less + (c < more ? 1 : 0) : 0; }
-    __device__ int owner(int64_t tile) const {
-        const int64_t large = more * (size_less + 1);
-        return static_cast<int>(tile < large ? tile / (size_less + 1) : more + (tile - large) / size_less);
+    int size_less, more, ctas;
+    __device__ int first(int c) const { return size_less * min(c, ctas) + min(c, more); }
+    __device__ int size(int c) const { return c < ctas ? size_less + (c < more ? 1 : 0) : 0; }
+    __device__ int owner(int tile) const {
+        const int large = more * (size_less + 1);
+        return tile < large ? tile / (size_less + 1) : more + (tile - large) / size_less;
     }
 };
-__device__ __forceinline__ Shares shares_of(int64_t total, int ctas) {
-    if (total < ctas) return {1, 0, static_cast<int>(total)};
-    const int64_t each = (total >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas)) : total / ctas;
+__device__ __forceinline__ Shares shares_of(int total, int ctas) {
+    if (total < ctas) return {1, 0, total};
+    const int each = static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas);
     return {each, total - each * ctas, ctas};
 }
 
@@ -282,63 +260,93 @@ __device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int row
     return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
 }
 
-// All threads: this CTA's share [*first, *first + share) of the list, and where in which sequence it starts.
+// What the other warps need of a step of the walk.
+struct Item {
+    int len, base;                        // the sequence's cached tokens, position of its first query's token
+    int tile, n;                          // first tile, how many
+    bool begins, ends, last;              // of the block; the CTA's last item
+};
+constexpr int kItemSlots = 4;
+
+template <int R>
+struct Small {                                                  // shared memory beside the operand tiles
+    alignas(128) float scales[kScaleSlots][kTokens];
+    alignas(16) float factor[2][R];                                         // k[r] by item parity
+    int64_t tree[kItemSlots][R];
+    int limit[kItemSlots][R];                                   // last position that a row sees (a tree: of those before the queries)
+    int place[kItemSlots][R];                                   // query * heads + head, -1 for a row that is none
+    Item item[kItemSlots];
+    uint32_t listed, finished;                                  // items that are written down, whose results have been read
+    float top[2][2][4][R / 2];                                  // [tile parity][half][warp][row]
+    float sum[2][4][R / 2];
+    alignas(16) float row[kSoftmaxWarps][R / 2];                // (read four at a time, as the factors are)
+    alignas(16) float row2[kSoftmaxWarps][R / 2];
+    uint64_t full[2 * kTileSlots], empty[2 * kTileSlots];
+    uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
+    Control ctl;
+    int boxes[kBoxSlots][kTokens / 16];
+    uint32_t looked_up, taken;                                  // tiles whose boxes are written, have been read
+    int warp_sum[kAttnThreads / 32];
+    Walk walk;                                                  // the first item
+    Shares shares;
+};
+
+template <int R>
+constexpr int smem_bytes() {
+    return 1024 + kTileSlots * kTileBytes + Cfg<R>::kQBytes + 2 * Cfg<R>::kPBytes + static_cast<int>(sizeof(Small<R>));
+}
+static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
+
+// All threads: this CTA's share of the list, and its first item (sm.walk).
 template <typename Sm>
-__device__ int64_t find_share(const LatentCache& c, const Queries& q, Sm& sm, Shares* shares_out, int64_t* first_out) {
+__device__ __forceinline__ void find_share(const LatentCache& c, const Queries& q, Sm& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Seq x;
-    const auto mine = [&](int s) -> int64_t {
-        if (s >= c.n_seqs) return 0;
-        x = load_seq(c, q, s);
-        const int b = blocks_of(q, x);
-        return tiles_before(q, x, b, b) * q.head_blocks;
-    };
-    const int64_t kept = mine(threadIdx.x);
-    const auto scan = [&](int64_t v, int64_t* sum) -> int64_t {       // tiles of the threads before this one; *sum: of all
-        int64_t run = v;
+    const bool once = c.n_seqs <= kAttnThreads;
+    int total = 0;
+    // a thread to a sequence; with more sequences than threads once for the total and once more for the place of the share's start
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        int at = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < c.n_seqs; s0 += kAttnThreads) {
+            const int seq = s0 + static_cast<int>(threadIdx.x);
+            Seq x = {0, 0, 0};
+            int mine = 0;
+            if (seq < c.n_seqs) {
+                x = load_seq(c, q, seq);
+                const int b = blocks_of(q, x);
+                mine = tiles_before(q, x, b, b) * q.head_blocks;
+            }
+            int run = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += u;
+            }
+            __syncthreads();
+            if (lane == 31) sm.warp_sum[warp] = run;
+            __syncthreads();
+            int before = at + run - mine;
+#pragma unroll
+            for (int w = 0; w < kAttnThreads / 32; ++w) {
+                const int v = sm.warp_sum[w];
+                if (w < warp) before += v;
+                at += v;
+            }
+            if (pass == 0 && !once) continue;
+            if (once) total = at;
+            const Shares sh = shares_of(total, gridDim.x / q.group);
+            const int group = blockIdx.x / q.group, first = sh.first(group), share = sh.size(group);
+            if (share > 0 && before <= first && first < before + mine) {
+                Walk w;
+                w.begin(q, seq, x, first - before, share);
+                sm.walk = w;
+            }
+            if (threadIdx.x == 0) sm.shares = sh;
         }
-        __syncthreads();
-        if (lane == 31) sm.warp_sum[warp] = run;
-        __syncthreads();
-        int64_t before = run - v, all = 0;
-        for (int w = 0; w < kAttnThreads / 32; ++w) {
-            if (w < warp) before += sm.warp_sum[w];
-            all += sm.warp_sum[w];
-        }
-        *sum = all;
-        return before;
-    };
-    int64_t total, sum;
-    const int64_t kept_before = scan(kept, &total);
-    for (int s0 = kAttnThreads; s0 < c.n_seqs; s0 += kAttnThreads) {
-        scan(mine(s0 + threadIdx.x), &sum);
-        total += sum;
+        if (once) break;
+        total = at;
     }
-    const Shares sh = shares_of(total, gridDim.x / q.group);
-    const int64_t at_cta = blockIdx.x / q.group;
-    const int64_t first = sh.first(at_cta), share = sh.size(at_cta);
-    *shares_out = sh;
-    *first_out = first;
-    if (share == 0) return 0;
-    int64_t at = 0;
-    for (int s0 = 0; s0 < c.n_seqs && at <= first; s0 += kAttnThreads) {
-        const int64_t v = s0 || c.n_seqs > kAttnThreads ? mine(s0 + threadIdx.x) : kept;
-        int64_t before = kept_before;
-        sum = 0;
-        if (s0 || c.n_seqs > kAttnThreads) before = scan(v, &sum) + at;
-        if (before <= first && first < before + v) {
-            sm.start = make_int4(s0 + threadIdx.x, x.len, x.queries, x.first);
-            sm.start_offset = first - before;
-        }
-        at += sum;
-        if (c.n_seqs <= kAttnThreads) break;
-    }
-    __syncthreads();
-    return share;
 }
 
 // ---------------------------------------------------------------- reductions over a tile's tokens
@@ -372,6 +380,29 @@ __device__ __forceinline__ void broadcast_rows(float* to, float own, float (&v)[
     for (int i = 0; i < N; i += 4) {
         const float4 f = *reinterpret_cast<const float4*>(to + i);
         v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+}
+
+// Waits until another warp's counter in shared memory has reached `want`, as bounded_wait does for a barrier.
+__device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, Control* ctl, unsigned int* status) {
+    uint64_t t0 = 0;
+    for (uint32_t spins = 0;; ++spins) {
+        if (*static_cast<const volatile uint32_t*>(counter) >= want) {
+            __threadfence_block();
+            return true;
+        }
+        __nanosleep(20);
+        if (spins >= 4096u && (spins & 255u) == 0u) {
+            if (ctl->abort_flag) return false;
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) {
+                t0 = now;
+            } else if (now - t0 > kWaitLimitNs) {
+                ctl->abort_flag = 1;
+                if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.x;
+                return false;
+            }
+        }
     }
 }
 
@@ -409,6 +440,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         mbar_init(bar(sm.o_empty), kSoftmaxWarps);
         mbar_fence_init();
         ctl->abort_flag = 0;
+        sm.looked_up = sm.taken = sm.listed = sm.finished = 0;
     }
     if (warp == 1) tc_alloc(smem_u32(&ctl->tmem_base), C::kTmemCols);
     if (warp == 0) {
@@ -416,87 +448,127 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         tma_prefetch_desc(&map_rope);
     }
     griddep_wait();
-    Shares shares;
-    int64_t first;
-    const int64_t share = find_share(c, q, sm, &shares, &first);     // (its barriers also publish what was set up above)
+    find_share(c, q, sm);                 // (its barriers also publish what was set up above)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
-    if (threadIdx.x == 32 * kFirstSoftmaxWarp && q.cut) q.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 32 * 3 && q.cut) q.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
 
-    Walk w;
-    if (share > 0) w.begin(q, sm.start, sm.start_offset, share);
+    const Shares shares = sm.shares;
+    const int first = shares.first(blockIdx.x / q.group), share = shares.size(blockIdx.x / q.group);
+    const auto listed = [&](uint32_t item) -> bool { return __all_sync(0xffffffffu, follow(&sm.listed, item + 1, ctl, status)); };
 
     if (share == 0) {
         // nothing to do
     } else if (warp == 0) {
-        // ------------------------------------------------------------ loads.  The lanes look up a tile's pages together, one tile ahead; one lane issues, with
-        // coordinates that the warp has in common: copies issued by the lanes of several pages cost 490 cycles a unit.
+        // ------------------------------------------------------------ loads.  One lane issues, with coordinates that the warp has in common.
         const int rows = min(1 << c.page_shift, kUnitTokens), unit_boxes = kUnitTokens / rows;
         const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
         uint32_t tile_count = 0;
         bool ok = true;
-        // the slot where this lane's box of a tile begins; absent: -1, behind the sequence's end: -2
-        const auto look_up = [&](const Walk& at, int t) -> int {
-            const int64_t p0 = static_cast<int64_t>(at.tile + t) * kTokens + lane * rows;
-            return lane < 2 * unit_boxes && p0 < at.s.len ? slot_of(c, at.seq, static_cast<uint32_t>(p0)) : -2;
-        };
-        int mine = look_up(w, 0);
-        bool more = true;
-        while (more) {
-            const int n = w.n;
-            for (int t = 0; t < n && ok; ++t, ++tile_count) {
-                const int at = mine;
-                if (t + 1 < n) {
-                    mine = look_up(w, t + 1);
-                } else {
-                    more = w.next(c, q);
-                    if (more) mine = look_up(w, 0);
+        for (; ok && tile_count < static_cast<uint32_t>(share); ++tile_count) {
+            ok = __all_sync(0xffffffffu, follow(&sm.looked_up, tile_count + 1, ctl, status));
+            const int at = lane < 2 * unit_boxes ? sm.boxes[tile_count & (kBoxSlots - 1)][lane] : -2;
+            __syncwarp();
+            if (lane == 0) *static_cast<volatile uint32_t*>(&sm.taken) = tile_count + 1;
+            const uint32_t used = __ballot_sync(0xffffffffu, at > -2), present = __ballot_sync(0xffffffffu, at >= 0);
+            float* const scales = sm.scales[tile_count & (kScaleSlots - 1)];
+            const uint32_t tile_at = smem_u32(tiles) + (tile_count & 1) * kTileBytes;
+            for (int h = 0; h < 2 && ok; ++h) {
+                const uint32_t slot = 2 * (tile_count & 1) + h, full = bar(sm.full[slot]);
+                const uint32_t of_unit = ((1u << unit_boxes) - 1u) << (h * unit_boxes);
+                const int boxes = __popc(used & of_unit), bytes = boxes * rows * (kLatent + 2 * kRope) + __popc(present & of_unit) * rows * 4;
+                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), ((tile_count >> 1) & 1) ^ 1, ctl, status, 1, tile_count));
+                if (!ok) break;
+                if ((used & ~present & of_unit) != 0) {                        // an absent page: its tokens have no scale
+                    if (at == -1 && lane / unit_boxes == h)
+                        for (int i = 0; i < rows; ++i) scales[lane * rows + i] = 0.0f;
+                    __syncwarp();
                 }
-                const uint32_t used = __ballot_sync(0xffffffffu, at > -2), present = __ballot_sync(0xffffffffu, at >= 0);
-                float* const scales = sm.scales[tile_count & (kScaleSlots - 1)];
-                const uint32_t tile_at = smem_u32(tiles) + (tile_count & 1) * kTileBytes;
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t slot = 2 * (tile_count & 1) + h, full = bar(sm.full[slot]);
-                    ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), ((tile_count >> 1) & 1) ^ 1, ctl, status, 1, tile_count));
-                    if (!ok) break;
-                    const uint32_t of_unit = ((1u << unit_boxes) - 1u) << (h * unit_boxes);
-                    const int boxes = __popc(used & of_unit);
-                    if ((used & ~present & of_unit) != 0) {                    // an absent page: its tokens have no scale
-                        if (at == -1 && lane / unit_boxes == h)
-                            for (int i = 0; i < rows; ++i) scales[lane * rows + i] = 0.0f;
-                        __syncwarp();
+                if (elect_one()) mbar_arrive_expect_tx(full, bytes);
+                for (int i = h * unit_boxes; i < h * unit_boxes + boxes; ++i) {
+                    const int from = __shfl_sync(0xffffffffu, at, i);
+                    const int y = from >= 0 ? from : static_cast<int>(outside);
+                    if (elect_one()) {
+                        tma_load_4d(tile_at + i * rows * kLatent, &map_latent, y >> 3, full);
+                        tma_load_2d(tile_at + kLatentBytes + i * rows * 2 * kRope, &map_rope, 0, y, full);
+                        if (from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
                     }
-                    if (elect_one()) mbar_arrive_expect_tx(full, boxes * rows * (kLatent + 2 * kRope) + __popc(present & of_unit) * rows * 4);
-                    for (int i = h * unit_boxes; i < h * unit_boxes + boxes; ++i) {
-                        const int from = __shfl_sync(0xffffffffu, at, i);
-                        const int y = from >= 0 ? from : static_cast<int>(outside);
-                        if (elect_one()) {
-                            tma_load_4d(tile_at + i * rows * kLatent, &map_latent, y >> 3, full);
-                            tma_load_2d(tile_at + kLatentBytes + i * rows * 2 * kRope, &map_rope, 0, y, full);
-                            if (from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
-                        }
-                        __syncwarp();
-                    }
+                    __syncwarp();
                 }
             }
-            more = more && ok;
         }
         // none of the commits onto empty[] may be in flight when the CTA leaves its shared memory to another
         for (uint32_t t = tile_count > 2 ? tile_count - 2 : 0u; ok && t < tile_count; ++t)
             for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[2 * (t & 1) + h]), (t >> 1) & 1, ctl, status, 1, t));
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ the walk: items and their rows, and pages some tiles ahead of the loads.  (To bring the
+        // pages to L2 as well, one to six tiles ahead, only gave HBM more to do: 64 sequences of up to 8192 tokens with 16 heads 56 us without, 58 to 68 with.)
+        Walk w = sm.walk;
+        const int rows = min(1 << c.page_shift, kUnitTokens), boxes = kTokens / rows;
+        uint32_t tile_count = 0, item = 0;
+        bool ok = true;
+        do {
+            // -------- a lane to a row of the block
+            const uint32_t at_item = item & (kItemSlots - 1);
+            const int place = lane < R ? place_of(q, w, R, lane) : -1, query = place < 0 ? 0 : place / q.heads, head = place - query * q.heads;
+            const int64_t word = q.tree && place >= 0 ? q.tree[query] : 0;
+            if (item > 0 && place >= 0) {                                      // its query will be read when the item before is done
+                const char* const lat = reinterpret_cast<const char*>(q.latent + query * q.latent_token + head * q.latent_head);
+#pragma unroll
+                for (int i = 0; i < 2 * kLatent; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(lat + i));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q.rope + query * q.rope_token + head * q.rope_head));
+            }
+            if (item >= kItemSlots) ok = __all_sync(0xffffffffu, follow(&sm.finished, item + 1 - kItemSlots, ctl, status));
+            if (!ok) break;
+            const int base = w.s.len - w.s.queries;
+            const bool begins = w.tile == 0, ends = w.tile + w.n == w.tiles;
+            if (lane < R) {
+                sm.place[at_item][lane] = place;
+                sm.limit[at_item][lane] = q.tree ? base - 1 : base + query - w.s.first;
+                sm.tree[at_item][lane] = word;
+            }
+            if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, w.left == 0};
+            __threadfence_block();
+            __syncwarp();
+            if (lane == 0) *static_cast<volatile uint32_t*>(&sm.listed) = item + 1;
+            for (int t = 0; t < w.n && ok; ++t, ++tile_count) {
+                // the slot where this lane's box begins; absent: -1, behind the sequence's end: -2
+                const int64_t p0 = static_cast<int64_t>(w.tile + t) * kTokens + lane * rows;
+                const int at = lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
+                if (tile_count >= kAhead) ok = __all_sync(0xffffffffu, follow(&sm.taken, tile_count + 1 - kAhead, ctl, status));
+                if (lane < boxes) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
+                __threadfence_block();
+                __syncwarp();
+                if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
+            }
+            if (lane == 0 && !ends) {                                          // (one item of a CTA at most)
+                const int start = first + (share - w.left) - w.n - w.tile;     // of the block's tiles, in the list
+                const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + w.tiles - 1) - begun + 1;
+                if (begins || parts > kFewParts) {
+                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
+                    q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
+                }
+            }
+            __syncwarp();
+            ++item;
+        } while (ok && w.next(c, q));
     } else if (warp == 1) {
         // ------------------------------------------------------------ scores.  The warp stays converged and elects a lane for the MMAs alone: addresses and
         // descriptors then stay in uniform registers.  The sums have an issuer of their own: in one thread, a tile whose weights are there waits behind
         // the next tile's loads, which wait for the room that its sums make.
         constexpr uint32_t idesc_s = umma_idesc_e4m3_f32(kTokens, 2 * R), idesc_r = idesc_bf16(kTokens, R);
         const uint32_t q_at = smem_u32(qs);
-        uint32_t count = 0, item = 0;                                          // tiles, items
-        bool ok = true;
-        do {
+        uint32_t count = 0;                                                    // of tiles
+        bool ok = true, last = false;
+        for (uint32_t item = 0; ok && !last; ++item) {
+            ok = listed(item);
+            if (!ok) break;
+            const int n = sm.item[item & (kItemSlots - 1)].n;
+            last = sm.item[item & (kItemSlots - 1)].last;
             ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item));
-            for (int t = 0; t < w.n && ok; ++t, ++count) {
+            for (int t = 0; t < n && ok; ++t, ++count) {
                 const uint32_t b = count & 1, phase = (count >> 1) & 1, d = tmem + b * C::kTmemS, at = smem_u32(tiles) + b * kTileBytes;
                 ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.s_empty[b]), phase ^ 1, ctl, status, 3, count));
                 for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.full[2 * b + h]), phase, ctl, status, 2, count));
@@ -517,16 +589,19 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 }
                 __syncwarp();
             }
-            ++item;
-        } while (ok && w.next(c, q));
+        }
     } else if (warp == 2) {
         // ------------------------------------------------------------ sums
         constexpr uint32_t idesc_o = umma_idesc_e4m3_f32(kTokens, 2 * R) | kIdescTransposed;
         const uint32_t p_at = smem_u32(ps);
-        uint32_t count = 0, item = 0;
-        bool ok = true;
-        do {
-            for (int t = 0; t < w.n && ok; ++t, ++count) {
+        uint32_t count = 0;
+        bool ok = true, last = false;
+        for (uint32_t item = 0; ok && !last; ++item) {
+            ok = listed(item);
+            if (!ok) break;
+            const int n = sm.item[item & (kItemSlots - 1)].n;
+            last = sm.item[item & (kItemSlots - 1)].last;
+            for (int t = 0; t < n && ok; ++t, ++count) {
                 const uint32_t b = count & 1;
                 ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.p_full[b]), (count >> 1) & 1, ctl, status, 11, count));
                 // (an item's first sums overwrite those of the item before it)
@@ -546,8 +621,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 }
                 __syncwarp();
             }
-            ++item;
-        } while (ok && w.next(c, q));
+        }
     } else if (warp >= kFirstSoftmaxWarp) {
         // ------------------------------------------------------------ softmax
         const int sw = warp - kFirstSoftmaxWarp, half = sw >> 2, quarter = sw & 3;
@@ -559,55 +633,50 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t counter) -> bool {
             return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, counter));
         };
-        // The rows of a block, a warp to every eighth: from memory ...
+        // The rows of a block, a warp to every eighth of them: all on their way from memory before the first is brought to shared memory, as an operand of
+        // the first product.  (This is a single warp's chain of dependent instructions; where the rows lie has been worked out before.)
         constexpr int kMine = R / kSoftmaxWarps;
         uint4 qv[kMine][2];
         uint32_t qr[kMine];
-        const auto fetch = [&]() {
+        const auto fetch = [&](uint32_t at_item) {
+            const int place = lane < kMine ? sm.place[at_item][sw + lane * kSoftmaxWarps] : -1;
+            const int row = place < 0 ? 0 : place / q.heads, head = place - row * q.heads;
+            const int64_t lat = row * q.latent_token + head * q.latent_head, rot = row * q.rope_token + head * q.rope_head;
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
-                const int place = place_of(q, w, R, sw + j * kSoftmaxWarps);
                 qv[j][0] = qv[j][1] = make_uint4(0, 0, 0, 0);
                 qr[j] = 0;
-                if (place >= 0) {
-                    const int64_t row = place / q.heads;
-                    const int head = place % q.heads;
-                    const uint4* src = reinterpret_cast<const uint4*>(q.latent + row * q.latent_token + head * q.latent_head);
+                const uint4* src = reinterpret_cast<const uint4*>(q.latent + __shfl_sync(0xffffffffu, lat, j));
+                const uint32_t* from = reinterpret_cast<const uint32_t*>(q.rope + __shfl_sync(0xffffffffu, rot, j));
+                if (__shfl_sync(0xffffffffu, place, j) >= 0) {
                     qv[j][0] = src[lane * 2], qv[j][1] = src[lane * 2 + 1];
-                    qr[j] = reinterpret_cast<const uint32_t*>(q.rope + row * q.rope_token + head * q.rope_head)[lane];
+                    qr[j] = from[lane];
                 }
             }
         };
-        // ... to shared memory, as operands of the first product
         const auto stage = [&](uint32_t par) {
-            const int base = w.s.len - w.s.queries;
+            float own = 1.0f;                                                  // scale of this lane's row
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
                 const int r = sw + j * kSoftmaxWarps;
-                float x[16], top = 0.0f;
-                bool finite = true;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t word = reinterpret_cast<const uint32_t*>(qv[j])[i];
-                    x[2 * i] = bf16_bits_to_float(word & 0xFFFFu);
-                    x[2 * i + 1] = __uint_as_float(word & 0xFFFF0000u);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    top = fmaxf(top, fabsf(x[i]));
-                    finite = finite && fabsf(x[i]) < INFINITY;
-                }
+                const uint32_t* const x2 = reinterpret_cast<const uint32_t*>(qv[j]);
                 const float re = bf16_bits_to_float(qr[j] & 0xFFFFu), im = __uint_as_float(qr[j] & 0xFFFF0000u);
-                finite = __all_sync(0xffffffffu, finite && fabsf(re) < INFINITY && fabsf(im) < INFINITY);
-                // (the rotated half is held divided by the same scale, in bf16: the scale is kept from being too small for that)
-                top = fmaxf(fmaxf(top, fmaxf(fabsf(re), fabsf(im)) * 0x1p-40f), 0x1p-100f);
+                // largest size: of two values at a time, as whole numbers; NaN and infinities come out on top
+                uint32_t top2 = 0;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float s = finite ? power_scale(top) : 1.0f, inv = finite ? power_reciprocal(s) : 0.0f;
+                for (int i = 0; i < 8; ++i) top2 = __vmaxu2(top2, x2[i] & 0x7FFF7FFFu);
+                uint32_t top1 = max(max(top2 & 0xFFFFu, top2 >> 16), 0u), rot1 = max(qr[j] & 0x7FFFu, (qr[j] >> 16) & 0x7FFFu);
+                top1 = __reduce_max_sync(0xffffffffu, top1);
+                rot1 = __reduce_max_sync(0xffffffffu, rot1);
+                const bool finite = max(top1, rot1) < 0x7F80u;
+                // (the rotated half is held divided by the same scale, in bf16: the scale is kept from being too small for that)
+                const float top = fmaxf(fmaxf(bf16_bits_to_float(top1), bf16_bits_to_float(rot1) * 0x1p-40f), 0x1p-100f);
+                const float s = finite ? power_scale(top) : __uint_as_float(0x7FC00000u), inv = finite ? power_reciprocal(s) : 0.0f;
+                if (lane == j) own = s;
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float a = finite ? x[2 * i] * inv : 0.0f, b = finite ? x[2 * i + 1] * inv : 0.0f;
+                    const float a = finite ? bf16_bits_to_float(x2[i] & 0xFFFFu) * inv : 0.0f, b = finite ? __uint_as_float(x2[i] & 0xFFFF0000u) * inv : 0.0f;
                     const uint16_t h = cvt_e4m3x2(a, b);
                     const float2 f = e4m3x2_to_float2(h);
                     const uint16_t l = cvt_e4m3x2(a - f.x, b - f.y);
@@ -619,29 +688,27 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 *reinterpret_cast<uint4*>(chunk + (R + r) * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 *reinterpret_cast<uint32_t*>(qs + 4 * C::kQChunk + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) =
                     finite ? pack_bf16x2(re * inv, im * inv) : 0u;
-                if (lane == 0) {
-                    const int place = place_of(q, w, R, r), query = place < 0 ? 0 : place / q.heads;
-                    sm.place[par][r] = place;
-                    sm.factor[par][r] = place < 0 ? 0.0f : finite ? s * q.scale * kLog2e : __uint_as_float(0x7FC00000u);
-                    sm.limit[par][r] = q.tree ? base - 1 : base + query - w.s.first;
-                    sm.tree[par][r] = q.tree && place >= 0 ? q.tree[query] : 0;
-                }
             }
+            if (lane < kMine) sm.factor[par][sw + lane * kSoftmaxWarps] = own * q.scale * kLog2e;
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.q_full));
         };
-        fetch();
-        stage(0);
+        ok = listed(0);
+        if (ok) {
+            fetch(0);
+            stage(0);
+        }
         for (uint32_t item = 0;; ++item) {
-            const uint32_t par = item & 1;
-            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);                       // factors and limits of all rows
+            const uint32_t par = item & 1, at_item = item & (kItemSlots - 1);
+            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);                       // the factors of all rows; the item before is done with
             if (!ok) break;
+            if (threadIdx.x == 32 * kFirstSoftmaxWarp) *static_cast<volatile uint32_t*>(&sm.finished) = item;
+            const Item w = sm.item[at_item];
             // d = y - mv is the weight's exponent; nothing has been seen yet: mv far below every score
             float l[N], mv[N], m = kNothing;                                   // m: mv of row own_row<N>()
 #pragma unroll
             for (int i = 0; i < N; ++i) l[i] = 0.0f, mv[i] = kNothing;
-            const int base = w.s.len - w.s.queries;                            // position of the first query's token
             for (int t = 0; t < w.n; ++t, ++tile_count) {
                 const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
                 const int p = (w.tile + t) * kTokens + token;
@@ -673,13 +740,13 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                             y[i + j] = fmaf((__uint_as_float(hi[i + j]) + __uint_as_float(lo[i + j])) + __uint_as_float(ro[i + j]), sc * g[j], e);
                     }
                 }
-                const bool present = p < w.s.len && sc != 0.0f;
-                if (!__all_sync(0xffffffffu, present && p < base)) {
+                const bool present = p < w.len && sc != 0.0f;
+                if (!__all_sync(0xffffffffu, present && p < w.base)) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
                         const int r = half * N + i;
-                        bool seen = p <= sm.limit[par][r];
-                        if (q.tree) seen = seen || (p >= base && p - base < 64 && ((sm.tree[par][r] >> (p - base)) & 1));
+                        bool seen = p <= sm.limit[at_item][r];
+                        if (q.tree) seen = seen || (p >= w.base && p - w.base < 64 && ((sm.tree[at_item][r] >> (p - w.base)) & 1));
                         if (!present || !seen) y[i] = -INFINITY;
                     }
                 }
@@ -710,7 +777,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
                         tc_fence_after();
                         if (ok) {
-#pragma unroll
+#pragma unroll 2
                             for (int u = 0; u < 8; ++u) {                      // hi and lo of four times 128 dimensions
                                 uint32_t o[N];
                                 const uint32_t at = tmem + lanes + C::kTmemO + u * R + half * N;
@@ -750,7 +817,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         *reinterpret_cast<uint2*>(row + ((1 ^ turn) << 4) + half * 8) = make_uint2(lo[0], lo[1]);
                     }
                     // Behind the sequence's end lie other sequences' bytes, or none at all; no weight, but 0 x NaN is not 0.
-                    if (p >= w.s.len) {
+                    if (p >= w.len) {
                         uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + half * 2048;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -762,9 +829,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 }
             }
             // -------- the item's result; the next item's queries on their way meanwhile
-            const Walk done = w;
-            const bool more = w.next(c, q);
-            if (more) fetch();
+            if (!w.last) {
+                ok = ok && listed(item + 1);
+                if (ok) fetch((item + 1) & (kItemSlots - 1));
+            }
             float sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
             if (lane % (32 / N) == 0) sm.sum[half][quarter][own_row<N>()] = sum;
             ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
@@ -772,27 +840,19 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             sum = (sm.sum[half][0][own_row<N>()] + sm.sum[half][1][own_row<N>()]) + (sm.sum[half][2][own_row<N>()] + sm.sum[half][3][own_row<N>()]);
             float inv[N];
             broadcast_rows<N>(sm.row[sw], sum == 0.0f ? 0.0f : 1.0f / sum, inv);
-            if (more) stage(par ^ 1);                                          // (all scores of this item have been read)
-            const bool begins = done.tile == 0, ends = done.tile + done.n == done.tiles, whole = begins && ends;
-            const int part = 2 * blockIdx.x + (begins ? 1 : 0);
+            if (!w.last) stage(par ^ 1);                                         // (all scores of this item have been read)
+            const bool whole = w.begins && w.ends;
+            const int part = 2 * blockIdx.x + (w.begins ? 1 : 0);
             const float lse2 = sum == 0.0f ? -INFINITY : m + __log2f(sum);
             if (quarter == 0 && lane % (32 / N) == 0) {
-                const int r = half * N + own_row<N>(), to = sm.place[par][r];
+                const int r = half * N + own_row<N>(), to = sm.place[at_item][r];
                 if (!whole) q.partial_lse[static_cast<int64_t>(part) * R + r] = lse2;
                 else if (q.lse && to >= 0) q.lse[to] = lse2 * kLn2;
-            }
-            if (threadIdx.x == 32 * kFirstSoftmaxWarp && !ends) {                // (one item of a CTA at most)
-                const int64_t start = first + (share - done.left) - done.n - done.tile;     // of the block's tiles, in the list
-                const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + done.tiles - 1) - begun + 1;
-                if (begins || parts > kFewParts) {
-                    q.cut[2 * blockIdx.x] = make_int4(parts, done.block, done.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
-                    q.cut[2 * blockIdx.x + 1] = make_int4(done.s.len, done.s.queries, done.s.first, 0);
-                }
             }
             // four rows that this lane writes: 8 bytes each, of four dimensions that it gets from its neighbours
             int to[N / 4];
             {
-                const int* const place = sm.place[par] + half * N + (lane & 1) * (N / 2) + ((lane >> 1) & 1) * (N / 4);
+                const int* const place = sm.place[at_item] + half * N + (lane & 1) * (N / 2) + ((lane >> 1) & 1) * (N / 4);
 #pragma unroll
                 for (int i = 0; i < N / 4; ++i) to[i] = place[i];
             }
@@ -836,7 +896,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.o_empty));
-            if (!more) break;
+            if (w.last) break;
         }
     }
 
@@ -975,7 +1035,13 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
         return DSV3_ERR_UNSUPPORTED;
     }
     const int grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
-    const bool cut = (static_cast<int64_t>(c.pages_width) << c.page_shift) > kTokens;
+    const int64_t longest = static_cast<int64_t>(c.pages_width) << c.page_shift;
+    if (tokens * ((heads + rows - 1) / rows) > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1)) {   // (the kernel counts tiles in 32 bits)
+        set_last_error("latent_attention: %lld queries of %d heads over up to %lld tokens are too much work for a call", static_cast<long long>(tokens), heads,
+                       static_cast<long long>(longest));
+        return DSV3_ERR_UNSUPPORTED;
+    }
+    const bool cut = longest > kTokens;
     if (cut && (!workspace || workspace_bytes < partial_bytes(rows, grid) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
         set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, grid));
         return DSV3_ERR_WORKSPACE;
