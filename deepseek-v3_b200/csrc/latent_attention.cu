@@ -66,10 +66,11 @@ struct Queries {
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
-    int grid;                             // CTAs
+    int grid, most_cut;                   // CTAs; blocks that may be cut
     float* partial;                       // [2 * grid][2][512][R / 2]: results of blocks that are cut
     float* partial_lse;                   // [2 * grid][R]
-    int* tickets;                         // [2 levels][grid][2], zero between calls
+    int* tickets;                         // [2 levels][grid][2], zero between calls; or null: latent_join_kernel joins them
+    int4* cut;                            // [2 * grid]: for it, the block that begins in a CTA and ends in a later one
 };
 
 template <int R>
@@ -151,7 +152,7 @@ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f
 // ---------------------------------------------------------------- who works on what
 // The work is a list of tiles: for every sequence, block of its query heads and 128 cached tokens that some row of the block sees one (at least one
 // per block, which writes the zeros of rows that see nothing).  A CTA takes an equal, contiguous share of the list, whatever the lengths are; a block's
-// tiles in one CTA are an item, and a block that is cut leaves partial results, which the last CTA to finish one joins.  One warp walks the
+// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  One warp walks the
 // list and leaves what the others need in shared memory.
 struct Seq {
     int len, queries, first;              // cached tokens, queries, index of the first query
@@ -255,8 +256,8 @@ __device__ __forceinline__ Shares shares_of(int total, int ctas) {
 }
 
 // Row r of an item's block: query * heads + head, or -1 where it is none.
-__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) {
-    int token = w.block << q.block_shift, head = (w.head_block + static_cast<int>(blockIdx.x) % q.group) * rows + r;
+__device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int rows, int r, int cta) {
+    int token = w.block << q.block_shift, head = (w.head_block + cta % q.group) * rows + r;
     if (q.heads <= rows) {
         if (r >= q.heads << q.block_shift) return -1;
         token += r / q.heads;
@@ -264,6 +265,7 @@ __device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int row
     }
     return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
 }
+__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) { return place_at(q, w, rows, r, static_cast<int>(blockIdx.x)); }
 
 // What the other warps need of a step of the walk.
 struct Item {
@@ -545,6 +547,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
+    if (threadIdx.x == 32 * 3 && q.cut) q.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
 
     const Shares shares = sm.shares;
     const int first = shares.first(blockIdx.x / q.group), share = shares.size(blockIdx.x / q.group);
@@ -626,6 +629,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 const int begun = shares.owner(start);
                 part = static_cast<int>(blockIdx.x) / q.group - begun;
                 parts = shares.owner(start + w.tiles - 1) - begun + 1;
+                if (lane == 0 && q.cut && begins) {                                        // (one item of a CTA at most)
+                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, 0);
+                    q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
+                }
             }
             if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, w.left == 0, part, parts};
             __threadfence_block();
@@ -910,7 +917,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     if (p >= w.len) {
                         uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + half * 2048;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     tc_fence_before();
                     fence_proxy_async_shared();
@@ -986,9 +993,9 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.o_empty));
-            if (!whole) {
+            if (!whole && q.tickets) {
                 // -------- The last CTA to have its part of a block done joins the parts, in their order: up to kFewParts at a time, then the results of those.
-                // (A kernel of its own for this, behind this one, cost 3 to 20 us a call.)
+                // (With most sequences cut, a kernel of its own costs 4 to 11 us a call.)
                 const int begun = static_cast<int>(blockIdx.x) - w.part * q.group, t0 = threadIdx.x - 32 * kFirstSoftmaxWarp;
                 int from = w.part & ~(kFewParts - 1), step = 1, count = min(kFewParts, w.parts - from);
                 for (int level = 0; level < 2; ++level) {
@@ -1027,12 +1034,89 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
+// Where few blocks are worked on by many CTAs, their parts are joined by a kernel of its own, which has all SMs for it: kJoinSlices thread blocks for each block that
+// was cut, one to 16 dimensions of half of the rows.  Its threads are as many teams as there are, which share the parts.
+constexpr int kJoinThreads = 512, kJoinDims = 16, kJoinSlices = 2 * kLatent / kJoinDims;
+template <int R>
+__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const Queries q) {
+    constexpr int N = R / 2, kQuads = N / 4, kTeamThreads = kJoinDims * kQuads, kTeams = kJoinThreads / kTeamThreads;
+    constexpr int kTeam = kJoinThreads / N < 32 ? kJoinThreads / N : 32, kMost = (160 + kTeam - 1) / kTeam;      // threads to a row's weights; parts to a thread
+    constexpr int kEach = (160 + kTeams - 1) / kTeams;                         // parts to a team
+    extern __shared__ float4 shared4[];
+    float* const weights = reinterpret_cast<float*>(shared4);                  // [parts][N], which add up to one
+    __shared__ float4 sums[kTeams][kTeamThreads];
+    __shared__ int place[N];
+    __shared__ int found[kJoinThreads / 32 + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = blockIdx.y & 1, slice = blockIdx.y >> 1;
+    griddep_launch_dependents();
+    griddep_wait();
+    // the CTA that this thread block's block begins in: the blockIdx.x-th of those that one begins in and does not end
+    const int4 mine = static_cast<int>(threadIdx.x) < q.grid ? q.cut[2 * threadIdx.x] : make_int4(-1, 0, 0, 0);
+    const int4 sequence = static_cast<int>(threadIdx.x) < q.grid ? q.cut[2 * threadIdx.x + 1] : make_int4(0, 0, 0, 0);
+    const uint32_t these = __ballot_sync(0xffffffffu, mine.x > 0);
+    if (lane == 0) found[warp] = __popc(these);
+    __syncthreads();
+    int rank = __popc(these & ((1u << lane) - 1u)), all = 0;
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+        if (w < warp) rank += found[w];
+        all += found[w];
+    }
+    if (static_cast<int>(blockIdx.x) >= all) return;
+    __shared__ int4 cut, seq;
+    __shared__ int begun;
+    if (mine.x > 0 && rank == static_cast<int>(blockIdx.x)) cut = mine, seq = sequence, begun = threadIdx.x;
+    __syncthreads();
+    const int parts = cut.x, cta = begun;
+    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)); };
+    // results first: they take longest
+    const int team = threadIdx.x / kTeamThreads, t = threadIdx.x % kTeamThreads, quad = t % kQuads, dim = slice * kJoinDims + t / kQuads;
+    float4 v[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        v[j] = team + j * kTeams < parts ? reinterpret_cast<const float4*>(q.partial + ((slot(team + j * kTeams) * 2 + half) * kLatent + dim) * N)[quad]
+                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (threadIdx.x < kTeam * N) {
+        const int r = threadIdx.x / kTeam, k = threadIdx.x % kTeam;
+        float f[kMost], lse2;
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) f[j] = k + j * kTeam < parts ? q.partial_lse[slot(k + j * kTeam) * R + half * N + r] : -INFINITY;
+        const float inv = join_weights<kTeam>(f, &lse2);
+#pragma unroll
+        for (int j = 0; j < kMost; ++j)
+            if (k + j * kTeam < parts) weights[(k + j * kTeam) * N + r] = f[j] * inv;
+        if (k == 0) {
+            Walk w;
+            w.block = cut.y, w.head_block = cut.z;
+            w.s = {seq.x, seq.y, seq.z};
+            place[r] = place_at(q, w, R, half * N + r, cta);
+            if (q.lse && place[r] >= 0 && slice == 0) q.lse[place[r]] = lse2 * kLn2;
+        }
+    }
+    __syncthreads();
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        if (team + j * kTeams >= parts) break;
+        const float4 f = *reinterpret_cast<const float4*>(weights + (team + j * kTeams) * N + quad * 4);
+        acc.x = fmaf(f.x, v[j].x, acc.x), acc.y = fmaf(f.y, v[j].y, acc.y), acc.z = fmaf(f.z, v[j].z, acc.z), acc.w = fmaf(f.w, v[j].w, acc.w);
+    }
+    sums[team][t] = acc;
+    __syncthreads();
+    if (threadIdx.x >= kTeamThreads) return;
+#pragma unroll
+    for (int i = 1; i < kTeams; ++i) {
+        const float4 x = sums[i][t];
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    }
+    store_quad<kQuads>(q, acc, place + quad * 4, dim);
+}
+
 // How a call is laid out.
 struct Layout {
     int rows;                             // of a block of query heads: 16 where a sequence has no more (on average: the numbers of queries are device memory), else 32
-    int head_blocks, block_shift, group, grid;
-    bool cut;                             // whether blocks can be
-    size_t partial, partial_lse, bytes;                                  // offsets in the workspace, whose header holds the tickets, and its size
+    int head_blocks, block_shift, group, grid, most_cut;
+    bool cut, tickets;                    // whether blocks can be cut; whether the kernel itself joins them
+    size_t partial, partial_lse, list, bytes;                                  // offsets in the workspace, whose header holds the tickets, and its size
 };
 Layout layout_of(int64_t tokens, int heads, int n_seqs, int64_t longest) {
     Layout l = {};
@@ -1046,10 +1130,16 @@ Layout layout_of(int64_t tokens, int heads, int n_seqs, int64_t longest) {
     l.grid = sms / l.group * l.group;
     l.cut = longest > kTokens;            // (a block of one tile is never cut)
     if (!l.cut) return l;
+    // With at least a quarter as many blocks as shares a block is in a few parts, as long as lengths are alike, and the last CTA to finish one joins them.  With
+    // fewer, a kernel of its own.
+    const int64_t sequences = tokens < n_seqs ? tokens : n_seqs, blocks = l.head_blocks / l.group * (tokens >> l.block_shift > sequences ? tokens >> l.block_shift : sequences);
+    l.tickets = 4 * blocks >= l.grid / l.group;
     static_assert(kMaxJoin * kFewParts * 4 * sizeof(int) <= DSV3_WORKSPACE_HEADER_BYTES, "tickets");
+    l.most_cut = static_cast<int>(std::min<int64_t>(l.grid, l.head_blocks * (n_seqs + (tokens >> l.block_shift))));
     l.partial = DSV3_WORKSPACE_HEADER_BYTES;
     l.partial_lse = l.partial + static_cast<size_t>(l.grid) * 2 * l.rows * kLatent * sizeof(float);
-    l.bytes = l.partial_lse + static_cast<size_t>(l.grid) * 2 * l.rows * sizeof(float);
+    l.list = l.partial_lse + static_cast<size_t>(l.grid) * 2 * l.rows * sizeof(float);
+    l.bytes = l.list + static_cast<size_t>(l.grid) * 2 * sizeof(int4);
     return l;
 }
 
@@ -1064,6 +1154,8 @@ int launch(const LatentCache& c, const Queries& q, const CUtensorMap& map_latent
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(q.grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    if (q.cut)
+        DSV3_CUDA_TRY(launch_dependent(latent_join_kernel<R>, dim3(q.most_cut, kJoinSlices), dim3(kJoinThreads), q.grid * (R / 2) * sizeof(float), stream, q));
     return DSV3_OK;
 }
 
@@ -1131,8 +1223,9 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       l.head_blocks / l.group, l.block_shift, l.group, l.grid, l.cut ? reinterpret_cast<float*>(ws + l.partial) : nullptr,
-                       l.cut ? reinterpret_cast<float*>(ws + l.partial_lse) : nullptr, l.cut ? reinterpret_cast<int*>(ws) : nullptr};
+                       l.head_blocks / l.group, l.block_shift, l.group, l.grid, l.most_cut, l.cut ? reinterpret_cast<float*>(ws + l.partial) : nullptr,
+                       l.cut ? reinterpret_cast<float*>(ws + l.partial_lse) : nullptr, l.tickets ? reinterpret_cast<int*>(ws) : nullptr,
+                       l.cut && !l.tickets ? reinterpret_cast<int4*>(ws + l.list) : nullptr};
     return l.rows == 16 ? launch<16>(c, q, map_latent, map_rope, status, st) : launch<32>(c, q, map_latent, map_rope, status, st);
 }
 
