@@ -20,7 +20,6 @@
 // (MN-major) in the second, from the same bytes.
 #include <cuda.h>
 
-#include <algorithm>
 #include <atomic>
 
 #include "latent_cache.cuh"
@@ -66,7 +65,7 @@ struct Queries {
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
-    int grid, most_cut;                   // CTAs; blocks that may be cut
+    int grid;
     float* partial;                       // [2 * grid][2][512][R / 2]: results of blocks that are cut
     float* partial_lse;                   // [2 * grid][R]
     int* tickets;                         // [2 levels][grid][2], zero between calls; or null: latent_join_kernel joins them
@@ -256,8 +255,8 @@ __device__ __forceinline__ Shares shares_of(int total, int ctas) {
 }
 
 // Row r of an item's block: query * heads + head, or -1 where it is none.
-__device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int rows, int r, int cta) {
-    int token = w.block << q.block_shift, head = (w.head_block + cta % q.group) * rows + r;
+__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) {
+    int token = w.block << q.block_shift, head = (w.head_block + static_cast<int>(blockIdx.x) % q.group) * rows + r;
     if (q.heads <= rows) {
         if (r >= q.heads << q.block_shift) return -1;
         token += r / q.heads;
@@ -265,7 +264,6 @@ __device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int row
     }
     return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
 }
-__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) { return place_at(q, w, rows, r, static_cast<int>(blockIdx.x)); }
 
 // What the other warps need of a step of the walk.
 struct Item {
@@ -415,87 +413,89 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
     }
 }
 
-// ---------------------------------------------------------------- joining the parts of a block: out = sum_p 2^(lse_p - lse) out_p
-// The weights of a row's parts from their logarithms, by a team of kTeam threads (neighbours in a warp), kEach parts to a thread: v[j] becomes part
-// k + j * kTeam's weight.  Returns the reciprocal of their sum; *lse2: its logarithm with the largest's.
-template <int kTeam, int kEach>
-__device__ __forceinline__ float join_weights(float (&v)[kEach], float* lse2) {
-    float top = -INFINITY, sum = 0.0f;
-    bool nan = false;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) top = fmaxf(top, v[j]), nan = nan || isnan(v[j]);
-#pragma unroll
-    for (int o = kTeam / 2; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        nan = (__shfl_xor_sync(0xffffffffu, nan ? 1 : 0, o) != 0) || nan;
-    }
-    const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) sum += v[j] = ex2(v[j] - ref);
-#pragma unroll
-    for (int o = kTeam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    *lse2 = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? -INFINITY : top + __log2f(sum);
-    return nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
-}
-// Four rows of a dimension in every lane, kQuads lanes to a dimension: to four dimensions of a row, in bf16.  place: of the lane's four rows.
-template <int kQuads>
-__device__ __forceinline__ void store_quad(const Queries& q, const float4& a, const int* place, int dim) {
-    const int lane = threadIdx.x & 31;
-    const bool b0 = lane & kQuads, b1 = lane & (2 * kQuads);                   // of the dimension's number
-    const float x = __shfl_xor_sync(0xffffffffu, b0 ? a.x : a.z, kQuads), y = __shfl_xor_sync(0xffffffffu, b0 ? a.y : a.w, kQuads);
-    const uint32_t p0 = b0 ? pack_bf16x2(x, a.z) : pack_bf16x2(a.x, x), p1 = b0 ? pack_bf16x2(y, a.w) : pack_bf16x2(a.y, y);   // rows 2 b0, 2 b0 + 1
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, b1 ? p0 : p1, 2 * kQuads);
-    const int to = place[(b0 ? 2 : 0) + (b1 ? 1 : 0)];
-    if (to >= 0) *reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(to) * kLatent + (dim & ~3)) = b1 ? make_uint2(got, p1) : make_uint2(p0, got);
-}
-
-// All softmax warps: parts of a block, those of the CTAs cta, cta + step, ...; the first is one in which a block begins (`begins`) or goes on.  To the rows'
-// places in the result, or, without them, to where the first part's result was.
+// All softmax warps: results of parts of a block, out = sum_p 2^(lse_p - lse) out_p.  The parts are those of the CTAs cta, cta + step, ...; the first is
+// one in which a block begins (`begins`) or goes on.  To the rows' places in the result, or, without them, to where the first part's result was.
 template <int R>
 __device__ __forceinline__ void join_parts(const Queries& q, float* scratch, int t, int cta, bool begins, int step, int count, const int* place) {
     constexpr int N = R / 2, kThreads = 32 * kSoftmaxWarps, kTeam = kThreads / R, kEach = (kMaxJoin + kTeam - 1) / kTeam;
-    float* const weights = scratch;                                            // [kMaxJoin][R], which add up to one
-    static_assert(kMaxJoin * R * 4 <= 2 * Cfg<R>::kPBytes, "scratch");
+    float* const weights = scratch;                                            // [kMaxJoin][R]
+    float* const total = scratch + kMaxJoin * R;                               // [R]
+    static_assert((kMaxJoin + 1) * R * 4 <= 2 * Cfg<R>::kPBytes, "scratch");
     const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * step) + (i == 0 && begins ? 1 : 0)); };
     {
+        // a team of threads to a row
         const int r = t / kTeam, k = t % kTeam;
-        float v[kEach], lse2;
+        float v[kEach], top = -INFINITY, sum = 0.0f;
+        bool nan = false;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) v[j] = k + j * kTeam < count ? __ldcg(q.partial_lse + slot(k + j * kTeam) * R + r) : -INFINITY;
-        const float inv = join_weights<kTeam>(v, &lse2);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            if (k + j * kTeam < count) weights[(k + j * kTeam) * R + r] = v[j] * inv;
+        for (int j = 0; j < kEach; ++j) top = fmaxf(top, v[j]), nan = nan || isnan(v[j]);
+#pragma unroll
+        for (int o = kTeam / 2; o > 0; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            nan = (__shfl_xor_sync(0xffffffffu, nan ? 1 : 0, o) != 0) || nan;
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const float f = ex2(v[j] - ref);
+            if (k + j * kTeam < count) weights[(k + j * kTeam) * R + r] = f, sum += f;
+        }
+#pragma unroll
+        for (int o = kTeam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (k == 0) {
+            total[r] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float lse2 = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? -INFINITY : top + __log2f(sum);
             if (!place) __stcg(q.partial_lse + slot(0) * R + r, lse2);         // (read above, by this team alone)
             else if (q.lse && place[r] >= 0) q.lse[place[r]] = lse2 * kLn2;
         }
     }
     asm volatile("bar.sync 3, %0;" ::"n"(kThreads) : "memory");
-    // Neighbouring threads read neighbouring rows, then neighbouring dimensions.  kAtOnce loads of a part under way together, and two parts'.
-    constexpr int kQuads = N / 4, kDims = kThreads / kQuads, kAtOnce = 4;      // dimensions at a time
-    const int quad = t % kQuads, dim0 = t / kQuads;
+    // Some sums at a time: all of a few parts' loads are under way together.
+    constexpr int kDims = 32 / N;                                              // 2 or 4 sums of N rows at a time
+    constexpr int kSteps = 2 * kLatent / kThreads / kDims;
 #pragma unroll 1
-    for (int s0 = 0; s0 < 2 * kLatent / kDims; s0 += kAtOnce) {
-        const int half = s0 / (kLatent / kDims), row = half * N + quad * 4;
-        const int64_t at = static_cast<int64_t>(half) * kLatent + (s0 % (kLatent / kDims)) * kDims + dim0;
-        float4 acc[kAtOnce];
+    for (int step_of = 0; step_of < kSteps; ++step_of) {
+        float acc[kDims][N];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[d][i] = 0.0f;
+        const auto at = [&](int d) { return step_of * kDims + d; };            // bit 0: which half of the rows; above: which dimensions
+#pragma unroll 2
         for (int p = 0; p < count; ++p) {
-            float4 v[kAtOnce];
+            float4 v[kDims][N / 4];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(q.partial + (slot(p) * 2 * kLatent + at + i * kDims) * N) + quad);
-            const float4 f = *reinterpret_cast<const float4*>(weights + p * R + row);
+            for (int d = 0; d < kDims; ++d)
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i)
-                acc[i].x = fmaf(f.x, v[i].x, acc[i].x), acc[i].y = fmaf(f.y, v[i].y, acc[i].y), acc[i].z = fmaf(f.z, v[i].z, acc[i].z), acc[i].w = fmaf(f.w, v[i].w, acc[i].w);
+                for (int i = 0; i < N / 4; ++i)
+                    v[d][i] = __ldcg(reinterpret_cast<const float4*>(q.partial + ((slot(p) * 2 + (at(d) & 1)) * kLatent + (at(d) >> 1) * kThreads + t) * N) + i);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(weights + p * R + (at(d) & 1) * N + i), x = v[d][i / 4];
+                    acc[d][i] = fmaf(f.x, x.x, acc[d][i]), acc[d][i + 1] = fmaf(f.y, x.y, acc[d][i + 1]), acc[d][i + 2] = fmaf(f.z, x.z, acc[d][i + 2]),
+                    acc[d][i + 3] = fmaf(f.w, x.w, acc[d][i + 3]);
+                }
         }
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            if (place) store_quad<kQuads>(q, acc[i], place + row, static_cast<int>(at % kLatent) + i * kDims);
-            else __stcg(reinterpret_cast<float4*>(q.partial + (slot(0) * 2 * kLatent + at + i * kDims) * N) + quad, acc[i]);
+        for (int d = 0; d < kDims; ++d) {
+            const int half = at(d) & 1, dim = (at(d) >> 1) * kThreads + t;
+            if (place) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int to = place[half * N + i];
+                    if (to >= 0) q.out[static_cast<int64_t>(to) * kLatent + dim] = __float2bfloat16_rn(acc[d][i] * total[half * N + i]);
+                }
+            } else {
+                float4* const to = reinterpret_cast<float4*>(q.partial + ((slot(0) * 2 + half) * kLatent + dim) * N);
+#pragma unroll
+                for (int i = 0; i < N; i += 4)
+                    __stcg(to + i / 4, make_float4(acc[d][i] * total[half * N + i], acc[d][i + 1] * total[half * N + i + 1], acc[d][i + 2] * total[half * N + i + 2],
+                                                   acc[d][i + 3] * total[half * N + i + 3]));
+            }
         }
     }
 }
@@ -629,8 +629,8 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 const int begun = shares.owner(start);
                 part = static_cast<int>(blockIdx.x) / q.group - begun;
                 parts = shares.owner(start + w.tiles - 1) - begun + 1;
-                if (lane == 0 && q.cut && begins) {                                        // (one item of a CTA at most)
-                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, 0);
+                if (lane == 0 && q.cut && !ends && (begins || parts > kFewParts)) {        // (one item of a CTA at most)
+                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, part);
                     q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
                 }
             }
@@ -1034,87 +1034,115 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
-// Where few blocks are worked on by many CTAs, their parts are joined by a kernel of its own, which has all SMs for it: kJoinSlices thread blocks for each block that
-// was cut, one to 16 dimensions of half of the rows.  Its threads are as many teams as there are, which share the parts.
-constexpr int kJoinThreads = 512, kJoinDims = 16, kJoinSlices = 2 * kLatent / kJoinDims;
+// Where few blocks are worked on by many CTAs, their parts are joined by a kernel of its own, which has all SMs for it.  Thread blocks to every CTA of the kernel
+// before, each for half of the rows and a part of the dimensions, a thread to a dimension: a block of query heads in few parts is joined by the thread blocks of the CTA that it
+// begins in; one in many parts by those of eight CTAs, 16 threads to a dimension, each for a sixteenth of the parts.
+constexpr int kJoinThreads = 256, kJoinTeams = 16, kJoinSlices = kLatent * kJoinTeams / kJoinThreads / 8;
 template <int R>
 __global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const Queries q) {
-    constexpr int N = R / 2, kQuads = N / 4, kTeamThreads = kJoinDims * kQuads, kTeams = kJoinThreads / kTeamThreads;
-    constexpr int kTeam = kJoinThreads / N < 32 ? kJoinThreads / N : 32, kMost = (160 + kTeam - 1) / kTeam;      // threads to a row's weights; parts to a thread
-    constexpr int kEach = (160 + kTeams - 1) / kTeams;                         // parts to a team
+    constexpr int N = R / 2, kTeam = kJoinThreads / N;
     extern __shared__ float4 shared4[];
-    float* const weights = reinterpret_cast<float*>(shared4);                  // [parts][N], which add up to one
-    __shared__ float4 sums[kTeams][kTeamThreads];
+    float* const weights = reinterpret_cast<float*>(shared4);                  // [parts][N]
+    __shared__ float4 sums[kJoinThreads];
+    __shared__ float total[N];
     __shared__ int place[N];
-    __shared__ int found[kJoinThreads / 32 + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = blockIdx.y & 1, slice = blockIdx.y >> 1;
     griddep_launch_dependents();
     griddep_wait();
-    // the CTA that this thread block's block begins in: the blockIdx.x-th of those that one begins in and does not end
-    const int4 mine = static_cast<int>(threadIdx.x) < q.grid ? q.cut[2 * threadIdx.x] : make_int4(-1, 0, 0, 0);
-    const int4 sequence = static_cast<int>(threadIdx.x) < q.grid ? q.cut[2 * threadIdx.x + 1] : make_int4(0, 0, 0, 0);
-    const uint32_t these = __ballot_sync(0xffffffffu, mine.x > 0);
-    if (lane == 0) found[warp] = __popc(these);
-    __syncthreads();
-    int rank = __popc(these & ((1u << lane) - 1u)), all = 0;
-    for (int w = 0; w < kJoinThreads / 32; ++w) {
-        if (w < warp) rank += found[w];
-        all += found[w];
-    }
-    if (static_cast<int>(blockIdx.x) >= all) return;
-    __shared__ int4 cut, seq;
-    __shared__ int begun;
-    if (mine.x > 0 && rank == static_cast<int>(blockIdx.x)) cut = mine, seq = sequence, begun = threadIdx.x;
-    __syncthreads();
-    const int parts = cut.x, cta = begun;
+    const int4 cut = q.cut[2 * blockIdx.x], seq = q.cut[2 * blockIdx.x + 1];
+    if (cut.x < 0) return;
+    const int parts = cut.x, half = blockIdx.y & 1, slice = blockIdx.y >> 1;
+    const bool few = parts <= kFewParts;
+    if (!few && cut.w >= 8) return;
+    const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
     const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)); };
-    // results first: they take longest
-    const int team = threadIdx.x / kTeamThreads, t = threadIdx.x % kTeamThreads, quad = t % kQuads, dim = slice * kJoinDims + t / kQuads;
-    float4 v[kEach];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < parts * N; i += kJoinThreads) weights[i] = q.partial_lse[slot(i / N) * R + half * N + i % N];
+    if (threadIdx.x < N) {
+        Walk w;
+        w.block = cut.y, w.head_block = cut.z;
+        w.s = {seq.x, seq.y, seq.z};
+        place[threadIdx.x] = place_of(q, w, R, half * N + threadIdx.x);
+    }
+    __syncthreads();
+    {
+        const int r = threadIdx.x / kTeam, t = threadIdx.x % kTeam;
+        float top = -INFINITY, sum = 0.0f;
+        bool nan = false;
+        for (int i = t; i < parts; i += kTeam) top = fmaxf(top, weights[i * N + r]), nan = nan || isnan(weights[i * N + r]);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-        v[j] = team + j * kTeams < parts ? reinterpret_cast<const float4*>(q.partial + ((slot(team + j * kTeams) * 2 + half) * kLatent + dim) * N)[quad]
-                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (threadIdx.x < kTeam * N) {
-        const int r = threadIdx.x / kTeam, k = threadIdx.x % kTeam;
-        float f[kMost], lse2;
+        for (int o = kTeam / 2; o > 0; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            nan = (__shfl_xor_sync(0xffffffffu, nan ? 1 : 0, o) != 0) || nan;
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int i = t; i < parts; i += kTeam) {
+            const float f = ex2(weights[i * N + r] - ref);
+            weights[i * N + r] = f;
+            sum += f;
+        }
 #pragma unroll
-        for (int j = 0; j < kMost; ++j) f[j] = k + j * kTeam < parts ? q.partial_lse[slot(k + j * kTeam) * R + half * N + r] : -INFINITY;
-        const float inv = join_weights<kTeam>(f, &lse2);
-#pragma unroll
-        for (int j = 0; j < kMost; ++j)
-            if (k + j * kTeam < parts) weights[(k + j * kTeam) * N + r] = f[j] * inv;
-        if (k == 0) {
-            Walk w;
-            w.block = cut.y, w.head_block = cut.z;
-            w.s = {seq.x, seq.y, seq.z};
-            place[r] = place_at(q, w, R, half * N + r, cta);
-            if (q.lse && place[r] >= 0 && slice == 0) q.lse[place[r]] = lse2 * kLn2;
+        for (int o = kTeam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (t == 0) {
+            total[r] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+            if (q.lse && place[r] >= 0 && slice == 0 && cut.w == 0)
+                q.lse[place[r]] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
         }
     }
     __syncthreads();
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (few && slice >= kLatent / kJoinThreads) return;
+    const int threads = few ? 1 : kJoinTeams, dims = kJoinThreads / threads;   // to a dimension; dimensions of this thread block
+    const int dim = (few ? slice * dims : (slice * 8 + cut.w) * dims) + static_cast<int>(threadIdx.x) % dims, team = static_cast<int>(threadIdx.x) / dims;
+    float4 acc[N / 4];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        if (team + j * kTeams >= parts) break;
-        const float4 f = *reinterpret_cast<const float4*>(weights + (team + j * kTeams) * N + quad * 4);
-        acc.x = fmaf(f.x, v[j].x, acc.x), acc.y = fmaf(f.y, v[j].y, acc.y), acc.z = fmaf(f.z, v[j].z, acc.z), acc.w = fmaf(f.w, v[j].w, acc.w);
-    }
-    sums[team][t] = acc;
-    __syncthreads();
-    if (threadIdx.x >= kTeamThreads) return;
+    for (int i = 0; i < N / 4; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = few ? 0 : team; p0 < parts; p0 += 4 * threads) {
+        float4 v[4][N / 4];
 #pragma unroll
-    for (int i = 1; i < kTeams; ++i) {
-        const float4 x = sums[i][t];
-        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i)
+                v[j][i] = p0 + j * threads < parts
+                              ? reinterpret_cast<const float4*>(q.partial + ((slot(p0 + j * threads) * 2 + half) * kLatent + dim) * N)[i]
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (p0 + j * threads >= parts) break;
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const float4 f = reinterpret_cast<const float4*>(weights + (p0 + j * threads) * N)[i];
+                acc[i].x = fmaf(f.x, v[j][i].x, acc[i].x), acc[i].y = fmaf(f.y, v[j][i].y, acc[i].y), acc[i].z = fmaf(f.z, v[j][i].z, acc[i].z),
+                acc[i].w = fmaf(f.w, v[j][i].w, acc[i].w);
+            }
+        }
     }
-    store_quad<kQuads>(q, acc, place + quad * 4, dim);
+    if (few) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float4 a = acc[i / 4];
+            const float v = i % 4 == 0 ? a.x : i % 4 == 1 ? a.y : i % 4 == 2 ? a.z : a.w;
+            if (place[i] >= 0) q.out[static_cast<int64_t>(place[i]) * kLatent + dim] = __float2bfloat16_rn(v * total[i]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        __syncthreads();
+        sums[threadIdx.x] = acc[i];
+        __syncthreads();
+        if (team < 4) {                                                        // a team to a row
+            float v = 0.0f;
+#pragma unroll
+            for (int t = 0; t < kJoinTeams; ++t) v += reinterpret_cast<const float*>(&sums[t * dims + threadIdx.x % dims])[team];
+            const int r = 4 * i + team;
+            if (place[r] >= 0) q.out[static_cast<int64_t>(place[r]) * kLatent + dim] = __float2bfloat16_rn(v * total[r]);
+        }
+    }
 }
 
 // How a call is laid out.
 struct Layout {
     int rows;                             // of a block of query heads: 16 where a sequence has no more (on average: the numbers of queries are device memory), else 32
-    int head_blocks, block_shift, group, grid, most_cut;
+    int head_blocks, block_shift, group, grid;
     bool cut, tickets;                    // whether blocks can be cut; whether the kernel itself joins them
     size_t partial, partial_lse, list, bytes;                                  // offsets in the workspace, whose header holds the tickets, and its size
 };
@@ -1124,7 +1152,7 @@ Layout layout_of(int64_t tokens, int heads, int n_seqs, int64_t longest) {
     l.head_blocks = (heads + l.rows - 1) / l.rows;
     // tokens to a block: a power of two, so that the tiles of a causal sequence can be counted without adding them up
     while ((heads << (l.block_shift + 1)) <= l.rows) ++l.block_shift;
-    const int sms = std::min(num_sms(), kMaxJoin * kFewParts);
+    const int sms = num_sms();
     // the blocks of a token's heads see the same tiles: side by side in as many CTAs, unless those are not there
     l.group = 2 * l.head_blocks <= sms ? l.head_blocks : 1;
     l.grid = sms / l.group * l.group;
@@ -1133,9 +1161,7 @@ Layout layout_of(int64_t tokens, int heads, int n_seqs, int64_t longest) {
     // With at least a quarter as many blocks as shares a block is in a few parts, as long as lengths are alike, and the last CTA to finish one joins them.  With
     // fewer, a kernel of its own.
     const int64_t sequences = tokens < n_seqs ? tokens : n_seqs, blocks = l.head_blocks / l.group * (tokens >> l.block_shift > sequences ? tokens >> l.block_shift : sequences);
-    l.tickets = 4 * blocks >= l.grid / l.group;
-    static_assert(kMaxJoin * kFewParts * 4 * sizeof(int) <= DSV3_WORKSPACE_HEADER_BYTES, "tickets");
-    l.most_cut = static_cast<int>(std::min<int64_t>(l.grid, l.head_blocks * (n_seqs + (tokens >> l.block_shift))));
+    l.tickets = 4 * blocks >= l.grid / l.group && l.grid / l.group <= kMaxJoin * kFewParts && l.grid * 4 * sizeof(int) <= DSV3_WORKSPACE_HEADER_BYTES;
     l.partial = DSV3_WORKSPACE_HEADER_BYTES;
     l.partial_lse = l.partial + static_cast<size_t>(l.grid) * 2 * l.rows * kLatent * sizeof(float);
     l.list = l.partial_lse + static_cast<size_t>(l.grid) * 2 * l.rows * sizeof(float);
@@ -1155,7 +1181,7 @@ int launch(const LatentCache& c, const Queries& q, const CUtensorMap& map_latent
     }
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(q.grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
     if (q.cut)
-        DSV3_CUDA_TRY(launch_dependent(latent_join_kernel<R>, dim3(q.most_cut, kJoinSlices), dim3(kJoinThreads), q.grid * (R / 2) * sizeof(float), stream, q));
+        DSV3_CUDA_TRY(launch_dependent(latent_join_kernel<R>, dim3(q.grid, 2 * kJoinSlices), dim3(kJoinThreads), q.grid * (R / 2) * sizeof(float), stream, q));
     return DSV3_OK;
 }
 
@@ -1223,7 +1249,7 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       l.head_blocks / l.group, l.block_shift, l.group, l.grid, l.most_cut, l.cut ? reinterpret_cast<float*>(ws + l.partial) : nullptr,
+                       l.head_blocks / l.group, l.block_shift, l.group, l.grid, l.cut ? reinterpret_cast<float*>(ws + l.partial) : nullptr,
                        l.cut ? reinterpret_cast<float*>(ws + l.partial_lse) : nullptr, l.tickets ? reinterpret_cast<int*>(ws) : nullptr,
                        l.cut && !l.tickets ? reinterpret_cast<int4*>(ws + l.list) : nullptr};
     return l.rows == 16 ? launch<16>(c, q, map_latent, map_rope, status, st) : launch<32>(c, q, map_latent, map_rope, status, st);
