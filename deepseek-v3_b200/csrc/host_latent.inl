@@ -166,14 +166,14 @@ PyObject* py_latent_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         sizes.pop_back();
         if (with_lse) lse = new_cuda(sizes, at::kFloat, dev);
         const size_t need = dsv3_latent_attention_workspace_bytes(l.tokens, static_cast<int>(l.heads), p.c.n_seqs, p.c.pages_width * p.c.page_size);
-        const at::Tensor ws = need ? workspace(dev, need) : at::Tensor();
-        const size_t ws_bytes = need ? static_cast<size_t>(ws.numel()) : 0;
+        // (given back after the launches: torch hands the memory out again in the stream's order)
+        const at::Tensor ws = need ? new_cuda({static_cast<int64_t>(need)}, at::kByte, dev) : at::Tensor();
         void *op = out.data_ptr(), *wp = need ? ws.data_ptr() : nullptr;
         float* sp = with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
         const void *qlp = ql.const_data_ptr(), *qrp = qr.const_data_ptr();
         call_library(dev, [&](dsv3_stream_t st) {
             return dsv3_latent_attention(&p.c, qlp, l.token_stride, l.head_stride, qrp, r.token_stride, r.head_stride, l.tokens, static_cast<int>(l.heads), lp,
-                                         cup, tp, static_cast<float>(scale), op, sp, wp, ws_bytes, st);
+                                         cup, tp, static_cast<float>(scale), op, sp, wp, need, st);
         });
         return with_lse ? wrap_pair(std::move(out), std::move(lse)) : wrap(std::move(out));
     });

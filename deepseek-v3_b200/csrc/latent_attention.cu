@@ -20,8 +20,6 @@
 // (MN-major) in the second, from the same bytes.
 #include <cuda.h>
 
-#include <atomic>
-
 #include "latent_cache.cuh"
 #include "tc_wait.cuh"
 
@@ -44,7 +42,6 @@ constexpr int kAttnThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
 constexpr int kScaleSlots = 4;
 constexpr int kAhead = 4, kBoxSlots = 4;  // tiles whose pages are looked up before they are loaded; of which the pages are kept
 constexpr int kFewParts = 8;              // of a block that several CTAs worked on
-constexpr int kMaxJoin = 20;              // results that are joined at a time: a group of kFewParts, or as many groups as a grid has
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // The maximum that weights are relative to moves when a weight would pass 2^(kTop + kSlack), and then stands for 2^kTop.  e4m3 ends at 448; a wide slack costs two of
 // the bits below (see the grid of small weights above) and spares nearly all passes over the sums so far.
@@ -65,11 +62,9 @@ struct Queries {
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
-    int grid;
-    float* partial;                       // [2 * grid][2][512][R / 2]: results of blocks that are cut
+    float* partial;                       // [2 * grid][R, 512]
     float* partial_lse;                   // [2 * grid][R]
-    int* tickets;                         // [2 levels][grid][2], zero between calls; or null: latent_join_kernel joins them
-    int4* cut;                            // [2 * grid]: for it, the block that begins in a CTA and ends in a later one
+    int4* cut;                            // [2 * grid]: the item that begins in a CTA and ends in a later one
 };
 
 template <int R>
@@ -270,7 +265,6 @@ struct Item {
     int len, base;                        // the sequence's cached tokens, position of its first query's token
     int tile, n;                          // first tile, how many
     bool begins, ends, last;              // of the block; the CTA's last item
-    int part, parts;                      // a block that is cut: which of how many
 };
 constexpr int kItemSlots = 4;
 
@@ -292,7 +286,6 @@ struct Small {                                                  // shared memory
     Control ctl;
     int boxes[kBoxSlots][kTokens / 16];
     uint32_t looked_up, taken;                                  // tiles whose boxes are written, have been read
-    int ticket;
     int warp_sum[kAttnThreads / 32];
     Walk walk;                                                  // the first item
     Shares shares;
@@ -408,93 +401,6 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
                 ctl->abort_flag = 1;
                 if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.x;
                 return false;
-            }
-        }
-    }
-}
-
-// All softmax warps: results of parts of a block, out = sum_p 2^(lse_p - lse) out_p.  The parts are those of the CTAs cta, cta + step, ...; the first is
-// one in which a block begins (`begins`) or goes on.  To the rows' places in the result, or, without them, to where the first part's result was.
-template <int R>
-__device__ __forceinline__ void join_parts(const Queries& q, float* scratch, int t, int cta, bool begins, int step, int count, const int* place) {
-    constexpr int N = R / 2, kThreads = 32 * kSoftmaxWarps, kTeam = kThreads / R, kEach = (kMaxJoin + kTeam - 1) / kTeam;
-    float* const weights = scratch;                                            // [kMaxJoin][R]
-    float* const total = scratch + kMaxJoin * R;                               // [R]
-    static_assert((kMaxJoin + 1) * R * 4 <= 2 * Cfg<R>::kPBytes, "scratch");
-    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * step) + (i == 0 && begins ? 1 : 0)); };
-    {
-        // a team of threads to a row
-        const int r = t / kTeam, k = t % kTeam;
-        float v[kEach], top = -INFINITY, sum = 0.0f;
-        bool nan = false;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) v[j] = k + j * kTeam < count ? __ldcg(q.partial_lse + slot(k + j * kTeam) * R + r) : -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) top = fmaxf(top, v[j]), nan = nan || isnan(v[j]);
-#pragma unroll
-        for (int o = kTeam / 2; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            nan = (__shfl_xor_sync(0xffffffffu, nan ? 1 : 0, o) != 0) || nan;
-        }
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const float f = ex2(v[j] - ref);
-            if (k + j * kTeam < count) weights[(k + j * kTeam) * R + r] = f, sum += f;
-        }
-#pragma unroll
-        for (int o = kTeam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (k == 0) {
-            total[r] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float lse2 = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? -INFINITY : top + __log2f(sum);
-            if (!place) __stcg(q.partial_lse + slot(0) * R + r, lse2);         // (read above, by this team alone)
-            else if (q.lse && place[r] >= 0) q.lse[place[r]] = lse2 * kLn2;
-        }
-    }
-    asm volatile("bar.sync 3, %0;" ::"n"(kThreads) : "memory");
-    // Some sums at a time: all of a few parts' loads are under way together.
-    constexpr int kDims = 32 / N;                                              // 2 or 4 sums of N rows at a time
-    constexpr int kSteps = 2 * kLatent / kThreads / kDims;
-#pragma unroll 1
-    for (int step_of = 0; step_of < kSteps; ++step_of) {
-        float acc[kDims][N];
-#pragma unroll
-        for (int d = 0; d < kDims; ++d)
-#pragma unroll
-            for (int i = 0; i < N; ++i) acc[d][i] = 0.0f;
-        const auto at = [&](int d) { return step_of * kDims + d; };            // bit 0: which half of the rows; above: which dimensions
-#pragma unroll 2
-        for (int p = 0; p < count; ++p) {
-            float4 v[kDims][N / 4];
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int i = 0; i < N / 4; ++i)
-                    v[d][i] = __ldcg(reinterpret_cast<const float4*>(q.partial + ((slot(p) * 2 + (at(d) & 1)) * kLatent + (at(d) >> 1) * kThreads + t) * N) + i);
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int i = 0; i < N; i += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(weights + p * R + (at(d) & 1) * N + i), x = v[d][i / 4];
-                    acc[d][i] = fmaf(f.x, x.x, acc[d][i]), acc[d][i + 1] = fmaf(f.y, x.y, acc[d][i + 1]), acc[d][i + 2] = fmaf(f.z, x.z, acc[d][i + 2]),
-                    acc[d][i + 3] = fmaf(f.w, x.w, acc[d][i + 3]);
-                }
-        }
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-            const int half = at(d) & 1, dim = (at(d) >> 1) * kThreads + t;
-            if (place) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int to = place[half * N + i];
-                    if (to >= 0) q.out[static_cast<int64_t>(to) * kLatent + dim] = __float2bfloat16_rn(acc[d][i] * total[half * N + i]);
-                }
-            } else {
-                float4* const to = reinterpret_cast<float4*>(q.partial + ((slot(0) * 2 + half) * kLatent + dim) * N);
-#pragma unroll
-                for (int i = 0; i < N; i += 4)
-                    __stcg(to + i / 4, make_float4(acc[d][i] * total[half * N + i], acc[d][i + 1] * total[half * N + i + 1], acc[d][i + 2] * total[half * N + i + 2],
-                                                   acc[d][i + 3] * total[half * N + i + 3]));
             }
         }
     }
@@ -623,18 +529,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 sm.limit[at_item][lane] = q.tree ? base - 1 : base + query - w.s.first;
                 sm.tree[at_item][lane] = word;
             }
-            int part = 0, parts = 1;
-            if (!begins || !ends) {
-                const int start = first + (share - w.left) - w.n - w.tile;     // of the block's tiles, in the list
-                const int begun = shares.owner(start);
-                part = static_cast<int>(blockIdx.x) / q.group - begun;
-                parts = shares.owner(start + w.tiles - 1) - begun + 1;
-                if (lane == 0 && q.cut && !ends && (begins || parts > kFewParts)) {        // (one item of a CTA at most)
-                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, part);
-                    q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
-                }
-            }
-            if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, w.left == 0, part, parts};
+            if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, w.left == 0};
             __threadfence_block();
             __syncwarp();
             if (lane == 0) *static_cast<volatile uint32_t*>(&sm.listed) = item + 1;
@@ -647,6 +542,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 __threadfence_block();
                 __syncwarp();
                 if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
+            }
+            if (lane == 0 && !ends) {                                          // (one item of a CTA at most)
+                const int start = first + (share - w.left) - w.n - w.tile;     // of the block's tiles, in the list
+                const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + w.tiles - 1) - begun + 1;
+                if (begins || parts > kFewParts) {
+                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
+                    q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
+                }
             }
             __syncwarp();
             ++item;
@@ -964,15 +867,15 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     tc_ld<N>(at, hi);
                     tc_ld<N>(at + R, lo);
                     tc_wait_ld();
+                    if (!whole) {
+                        float* const dst = q.partial + (static_cast<int64_t>(part) * R + half * N) * kLatent + u * 128 + token;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dst[i * kLatent] = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
+                        continue;
+                    }
                     float o[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) o[i] = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
-                    if (!whole) {                                              // a dimension's rows side by side, as this thread has them
-                        float4* const dst = reinterpret_cast<float4*>(q.partial + ((static_cast<int64_t>(part) * 2 + half) * kLatent + u * 128 + token) * N);
-#pragma unroll
-                        for (int i = 0; i < N; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        continue;
-                    }
                     uint32_t two[N / 2];
 #pragma unroll
                     for (int i = 0; i < N / 2; ++i) {                          // the other lane of a pair has the next dimension
@@ -993,27 +896,6 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.o_empty));
-            if (!whole && q.tickets) {
-                // -------- The last CTA to have its part of a block done joins the parts, in their order: up to kFewParts at a time, then the results of those.
-                // (With most sequences cut, a kernel of its own costs 4 to 11 us a call.)
-                const int begun = static_cast<int>(blockIdx.x) - w.part * q.group, t0 = threadIdx.x - 32 * kFirstSoftmaxWarp;
-                int from = w.part & ~(kFewParts - 1), step = 1, count = min(kFewParts, w.parts - from);
-                for (int level = 0; level < 2; ++level) {
-                    __threadfence();
-                    ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
-                    if (!ok) break;
-                    int* const ticket = q.tickets + 2 * (level * q.grid + begun + from * q.group) + (from == 0 ? 1 : 0);
-                    if (t0 == 0) sm.ticket = atomicAdd(ticket, 1);
-                    ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
-                    if (!ok || sm.ticket != count - 1) break;
-                    if (t0 == 0) *ticket = 0;                                  // as the next call expects it
-                    __threadfence();
-                    const bool all = level == 1 || w.parts <= kFewParts;
-                    join_parts<R>(q, reinterpret_cast<float*>(ps), t0, begun + from * q.group, from == 0, step * q.group, count, all ? sm.place[at_item] : nullptr);
-                    if (all) break;
-                    from = 0, step = kFewParts, count = (w.parts + kFewParts - 1) / kFewParts;
-                }
-            }
             if (w.last) break;
         }
     }
@@ -1034,154 +916,80 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
-// Where few blocks are worked on by many CTAs, their parts are joined by a kernel of its own, which has all SMs for it.  Thread blocks to every CTA of the kernel
-// before, each for half of the rows and a part of the dimensions, a thread to a dimension: a block of query heads in few parts is joined by the thread blocks of the CTA that it
-// begins in; one in many parts by those of eight CTAs, 16 threads to a dimension, each for a sixteenth of the parts.
-constexpr int kJoinThreads = 256, kJoinTeams = 16, kJoinSlices = kLatent * kJoinTeams / kJoinThreads / 8;
+// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  A row of thread blocks to every CTA of the kernel before: where a block of
+// query heads is in few parts, the row of the CTA that it begins in joins them, 128 threads to a query head; where it is in many, the rows of all
+// CTAs but its last share the query heads, and a thread block splits a head's parts among its four teams.
+constexpr int kCombineThreads = 512, kTeams = kCombineThreads / 128;
 template <int R>
-__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const Queries q) {
-    constexpr int N = R / 2, kTeam = kJoinThreads / N;
-    extern __shared__ float4 shared4[];
-    float* const weights = reinterpret_cast<float*>(shared4);                  // [parts][N]
-    __shared__ float4 sums[kJoinThreads];
-    __shared__ float total[N];
-    __shared__ int place[N];
+__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Queries q) {
+    __shared__ float4 sums[kTeams][128];
+    __shared__ float weights[kTeams];
     griddep_launch_dependents();
     griddep_wait();
-    const int4 cut = q.cut[2 * blockIdx.x], seq = q.cut[2 * blockIdx.x + 1];
+    const int4 cut = q.cut[2 * blockIdx.x];
     if (cut.x < 0) return;
-    const int parts = cut.x, half = blockIdx.y & 1, slice = blockIdx.y >> 1;
+    const int4 seq = q.cut[2 * blockIdx.x + 1];
+    Walk w;
+    w.block = cut.y, w.head_block = cut.z;
+    w.s = {seq.x, seq.y, seq.z};
+    const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
     const bool few = parts <= kFewParts;
-    if (!few && cut.w >= 8) return;
+    const int r = few ? blockIdx.y * kTeams + team : cut.w * (R / kTeams) + blockIdx.y;
+    if (r >= R) return;
+    const int place = place_of(q, w, R, r);
+    if (place < 0) return;                                                     // (a whole team, or, with many parts, the whole block)
     const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
-    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)); };
-#pragma unroll 4
-    for (int i = threadIdx.x; i < parts * N; i += kJoinThreads) weights[i] = q.partial_lse[slot(i / N) * R + half * N + i % N];
-    if (threadIdx.x < N) {
-        Walk w;
-        w.block = cut.y, w.head_block = cut.z;
-        w.s = {seq.x, seq.y, seq.z};
-        place[threadIdx.x] = place_of(q, w, R, half * N + threadIdx.x);
-    }
-    __syncthreads();
-    {
-        const int r = threadIdx.x / kTeam, t = threadIdx.x % kTeam;
-        float top = -INFINITY, sum = 0.0f;
-        bool nan = false;
-        for (int i = t; i < parts; i += kTeam) top = fmaxf(top, weights[i * N + r]), nan = nan || isnan(weights[i * N + r]);
-#pragma unroll
-        for (int o = kTeam / 2; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            nan = (__shfl_xor_sync(0xffffffffu, nan ? 1 : 0, o) != 0) || nan;
-        }
-        const float ref = top == -INFINITY ? 0.0f : top;
-        for (int i = t; i < parts; i += kTeam) {
-            const float f = ex2(weights[i * N + r] - ref);
-            weights[i * N + r] = f;
-            sum += f;
-        }
-#pragma unroll
-        for (int o = kTeam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (t == 0) {
-            total[r] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (q.lse && place[r] >= 0 && slice == 0 && cut.w == 0)
-                q.lse[place[r]] = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
-        }
-    }
-    __syncthreads();
-    if (few && slice >= kLatent / kJoinThreads) return;
-    const int threads = few ? 1 : kJoinTeams, dims = kJoinThreads / threads;   // to a dimension; dimensions of this thread block
-    const int dim = (few ? slice * dims : (slice * 8 + cut.w) * dims) + static_cast<int>(threadIdx.x) % dims, team = static_cast<int>(threadIdx.x) / dims;
-    float4 acc[N / 4];
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p0 = few ? 0 : team; p0 < parts; p0 += 4 * threads) {
-        float4 v[4][N / 4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i)
-                v[j][i] = p0 + j * threads < parts
-                              ? reinterpret_cast<const float4*>(q.partial + ((slot(p0 + j * threads) * 2 + half) * kLatent + dim) * N)[i]
-                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (p0 + j * threads >= parts) break;
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const float4 f = reinterpret_cast<const float4*>(weights + (p0 + j * threads) * N)[i];
-                acc[i].x = fmaf(f.x, v[j][i].x, acc[i].x), acc[i].y = fmaf(f.y, v[j][i].y, acc[i].y), acc[i].z = fmaf(f.z, v[j][i].z, acc[i].z),
-                acc[i].w = fmaf(f.w, v[j][i].w, acc[i].w);
-            }
-        }
-    }
-    if (few) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float4 a = acc[i / 4];
-            const float v = i % 4 == 0 ? a.x : i % 4 == 1 ? a.y : i % 4 == 2 ? a.z : a.w;
-            if (place[i] >= 0) q.out[static_cast<int64_t>(place[i]) * kLatent + dim] = __float2bfloat16_rn(v * total[i]);
-        }
-        return;
+    const auto part = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R + r; };
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    bool nan = false;
+    for (int i = lane; i < parts; i += 32) {
+        const float v = q.partial_lse[part(i)];
+        nan = nan || isnan(v);
+        top = fmaxf(top, v);
     }
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    nan = __any_sync(0xffffffffu, nan);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 8
+    for (int i = few ? 0 : team; i < parts; i += few ? 1 : kTeams) {
+        const float f = ex2(q.partial_lse[part(i)] - ref);
+        const float4 v = reinterpret_cast<const float4*>(q.partial + part(i) * kLatent)[at];
+        sum += f;
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+    if (!few) {
+        sums[team][at] = acc;
+        if (at == 0) weights[team] = sum;
         __syncthreads();
-        sums[threadIdx.x] = acc[i];
-        __syncthreads();
-        if (team < 4) {                                                        // a team to a row
-            float v = 0.0f;
+        if (team != 0) return;
 #pragma unroll
-            for (int t = 0; t < kJoinTeams; ++t) v += reinterpret_cast<const float*>(&sums[t * dims + threadIdx.x % dims])[team];
-            const int r = 4 * i + team;
-            if (place[r] >= 0) q.out[static_cast<int64_t>(place[r]) * kLatent + dim] = __float2bfloat16_rn(v * total[r]);
+        for (int i = 1; i < kTeams; ++i) {
+            const float4 v = sums[i][at];
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            sum += weights[i];
         }
     }
+    const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+    reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(place) * kLatent)[at] =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (q.lse && at == 0) q.lse[place] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
-// How a call is laid out.
-struct Layout {
-    int rows;                             // of a block of query heads: 16 where a sequence has no more (on average: the numbers of queries are device memory), else 32
-    int head_blocks, block_shift, group, grid;
-    bool cut, tickets;                    // whether blocks can be cut; whether the kernel itself joins them
-    size_t partial, partial_lse, list, bytes;                                  // offsets in the workspace, whose header holds the tickets, and its size
-};
-Layout layout_of(int64_t tokens, int heads, int n_seqs, int64_t longest) {
-    Layout l = {};
-    l.rows = (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32;
-    l.head_blocks = (heads + l.rows - 1) / l.rows;
-    // tokens to a block: a power of two, so that the tiles of a causal sequence can be counted without adding them up
-    while ((heads << (l.block_shift + 1)) <= l.rows) ++l.block_shift;
-    const int sms = num_sms();
-    // the blocks of a token's heads see the same tiles: side by side in as many CTAs, unless those are not there
-    l.group = 2 * l.head_blocks <= sms ? l.head_blocks : 1;
-    l.grid = sms / l.group * l.group;
-    l.cut = longest > kTokens;            // (a block of one tile is never cut)
-    if (!l.cut) return l;
-    // With at least a quarter as many blocks as shares a block is in a few parts, as long as lengths are alike, and the last CTA to finish one joins them.  With
-    // fewer, a kernel of its own.
-    const int64_t sequences = tokens < n_seqs ? tokens : n_seqs, blocks = l.head_blocks / l.group * (tokens >> l.block_shift > sequences ? tokens >> l.block_shift : sequences);
-    l.tickets = 4 * blocks >= l.grid / l.group && l.grid / l.group <= kMaxJoin * kFewParts && l.grid * 4 * sizeof(int) <= DSV3_WORKSPACE_HEADER_BYTES;
-    l.partial = DSV3_WORKSPACE_HEADER_BYTES;
-    l.partial_lse = l.partial + static_cast<size_t>(l.grid) * 2 * l.rows * kLatent * sizeof(float);
-    l.list = l.partial_lse + static_cast<size_t>(l.grid) * 2 * l.rows * sizeof(float);
-    l.bytes = l.list + static_cast<size_t>(l.grid) * 2 * sizeof(int4);
-    return l;
-}
+// Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
+int block_rows(int64_t tokens, int heads, int n_seqs) { return (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32; }
+
+size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
 
 template <int R>
-int launch(const LatentCache& c, const Queries& q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, unsigned int* status, cudaStream_t stream) {
+int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool cut, unsigned int* status,
+           cudaStream_t stream) {
     const auto kern = latent_attention_kernel<R>;
-    static std::atomic<uint64_t> prepared{0};                                  // devices
-    int device = 0;
-    DSV3_CUDA_TRY(cudaGetDevice(&device));
-    if (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1)) {
-        DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
-        if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
-    }
-    DSV3_CUDA_TRY(launch_dependent(kern, dim3(q.grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
-    if (q.cut)
-        DSV3_CUDA_TRY(launch_dependent(latent_join_kernel<R>, dim3(q.grid, 2 * kJoinSlices), dim3(kJoinThreads), q.grid * (R / 2) * sizeof(float), stream, q));
+    DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
+    DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    if (cut)
+        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / kTeams), dim3(kCombineThreads), 0, stream, q));
     return DSV3_OK;
 }
 
@@ -1193,8 +1001,8 @@ using namespace dsv3;
 extern "C" {
 
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest) {
-    if (tokens <= 0 || heads <= 0 || heads > 1024 || n_seqs <= 0 || longest < 0 || tokens > 0x7FFFFFFFll / heads) return 0;
-    return layout_of(tokens, heads, n_seqs, longest).bytes;
+    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || longest <= kTokens) return 0;      // (a block of one tile is never cut)
+    return partial_bytes(block_rows(tokens, heads, n_seqs), num_sms());
 }
 
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
@@ -1226,15 +1034,16 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
         set_last_error("latent_attention: takes at most 1024 heads and 2^31 query heads");
         return DSV3_ERR_UNSUPPORTED;
     }
+    const int grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
     const int64_t longest = static_cast<int64_t>(c.pages_width) << c.page_shift;
-    const Layout l = layout_of(tokens, heads, c.n_seqs, longest);
-    if (tokens * l.head_blocks > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1)) {      // (the kernels count tiles in 32 bits)
+    if (tokens * ((heads + rows - 1) / rows) > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1)) {   // (the kernel counts tiles in 32 bits)
         set_last_error("latent_attention: %lld queries of %d heads over up to %lld tokens are too much work for a call", static_cast<long long>(tokens), heads,
                        static_cast<long long>(longest));
         return DSV3_ERR_UNSUPPORTED;
     }
-    if (l.bytes && (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
-        set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", l.bytes);
+    const bool cut = longest > kTokens;
+    if (cut && (!workspace || workspace_bytes < partial_bytes(rows, grid) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
+        set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, grid));
         return DSV3_ERR_WORKSPACE;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1245,14 +1054,19 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     CUtensorMap map_latent, map_rope;
     if (const int rc = make_tmap_groups(&map_latent, c.latent, slots, kLatent, box); rc != DSV3_OK) return rc;
     if (const int rc = make_tmap(&map_rope, c.rope, slots, 2 * kRope, box); rc != DSV3_OK) return rc;
-    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    // tokens to a block: a power of two, so that the tiles of a causal sequence can be counted without adding them up
+    int shift = 0;
+    while ((heads << (shift + 1)) <= rows) ++shift;
+    // the blocks of a token's heads see the same tiles: side by side in as many CTAs, unless those are not there
+    const int head_blocks = (heads + rows - 1) / rows, group = 2 * head_blocks <= grid ? head_blocks : 1;
+    float* const partial = static_cast<float*>(workspace);
+    float* const partial_lse = cut ? partial + static_cast<size_t>(grid) * 2 * rows * kLatent : nullptr;
+    int4* const list = cut ? reinterpret_cast<int4*>(partial_lse + static_cast<size_t>(grid) * 2 * rows) : nullptr;
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       l.head_blocks / l.group, l.block_shift, l.group, l.grid, l.cut ? reinterpret_cast<float*>(ws + l.partial) : nullptr,
-                       l.cut ? reinterpret_cast<float*>(ws + l.partial_lse) : nullptr, l.tickets ? reinterpret_cast<int*>(ws) : nullptr,
-                       l.cut && !l.tickets ? reinterpret_cast<int4*>(ws + l.list) : nullptr};
-    return l.rows == 16 ? launch<16>(c, q, map_latent, map_rope, status, st) : launch<32>(c, q, map_latent, map_rope, status, st);
+                       head_blocks / group, shift, group, partial, partial_lse, list};
+    return rows == 16 ? launch<16>(c, q, map_latent, map_rope, grid / group * group, cut, status, st) : launch<32>(c, q, map_latent, map_rope, grid / group * group, cut, status, st);
 }
 
 }  // extern "C"

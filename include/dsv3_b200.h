@@ -383,8 +383,7 @@ int dsv3_latent_keep(const dsv3_latent_cache_t* cache, const int32_t* first, con
  *              queries' own tokens are still the last ones of their sequence; a query sees all before them, and of them those whose bit is
  *              set (bit j: the j-th; from the 64th on none is seen).
  *   out      : bf16 [tokens, heads, 512], lse : fp32 [tokens, heads].  A query that sees nothing: zeros, and -inf.
- * workspace: dsv3_latent_attention_workspace_bytes() bytes under the rules of dsv3_fp8_gemm's (zeroed header, 256-byte aligned, not shared by
- * overlapping calls); longest: what a row of pages can hold, pages_width * page_size.  It may be null when the size query returns 0.
+ * workspace: dsv3_latent_attention_workspace_bytes() bytes, 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
  */
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest);
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
