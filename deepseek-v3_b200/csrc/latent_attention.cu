@@ -20,6 +20,8 @@
 // (MN-major) in the second, from the same bytes.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "latent_cache.cuh"
 #include "tc_wait.cuh"
 
@@ -250,8 +252,8 @@ __device__ __forceinline__ Shares shares_of(int total, int ctas) {
 }
 
 // Row r of an item's block: query * heads + head, or -1 where it is none.
-__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) {
-    int token = w.block << q.block_shift, head = (w.head_block + static_cast<int>(blockIdx.x) % q.group) * rows + r;
+__device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int rows, int r, int cta) {
+    int token = w.block << q.block_shift, head = (w.head_block + cta % q.group) * rows + r;
     if (q.heads <= rows) {
         if (r >= q.heads << q.block_shift) return -1;
         token += r / q.heads;
@@ -259,6 +261,7 @@ __device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int row
     }
     return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
 }
+__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) { return place_at(q, w, rows, r, static_cast<int>(blockIdx.x)); }
 
 // What the other warps need of a step of the walk.
 struct Item {
@@ -820,7 +823,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     if (p >= w.len) {
                         uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + half * 2048;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     tc_fence_before();
                     fence_proxy_async_shared();
@@ -916,35 +919,78 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
-// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  A row of thread blocks to every CTA of the kernel before: where a block of
-// query heads is in few parts, the row of the CTA that it begins in joins them, 128 threads to a query head; where it is in many, the rows of all
-// CTAs but its last share the query heads, and a thread block splits a head's parts among its four teams.
-constexpr int kCombineThreads = 512, kTeams = kCombineThreads / 128;
+// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  Thread blocks to every CTA of the kernel before, a team of 128 threads
+// to kTeamRows rows: where a block of query heads is in few parts, those of the CTA that it begins in join them; where it is in many, those of
+// all CTAs but its last take a row each, and their teams share its parts.  (The last CTA of a block joining its parts, in the kernel before, took longer:
+// 64 sequences of up to 8192 tokens with 16 heads 50.3 us instead of 48.3, one of 131072 with four drafts 70 instead of 50.)
+constexpr int kCombineThreads = 512, kTeams = kCombineThreads / 128, kTeamRows = 2;
 template <int R>
 __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Queries q) {
+    constexpr int kRows = kTeamRows, kBlocks = R / (kTeams * kRows);
     __shared__ float4 sums[kTeams][128];
     __shared__ float weights[kTeams];
     griddep_launch_dependents();
     griddep_wait();
-    const int4 cut = q.cut[2 * blockIdx.x];
+    const int4 cut = q.cut[2 * blockIdx.x], seq = q.cut[2 * blockIdx.x + 1];
     if (cut.x < 0) return;
-    const int4 seq = q.cut[2 * blockIdx.x + 1];
     Walk w;
     w.block = cut.y, w.head_block = cut.z;
     w.s = {seq.x, seq.y, seq.z};
     const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
-    const bool few = parts <= kFewParts;
-    const int r = few ? blockIdx.y * kTeams + team : cut.w * (R / kTeams) + blockIdx.y;
-    if (r >= R) return;
-    const int place = place_of(q, w, R, r);
-    if (place < 0) return;                                                     // (a whole team, or, with many parts, the whole block)
     const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
-    const auto part = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R + r; };
+    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R; };
+    const auto store = [&](int place, const float4& acc, float top, float sum, bool nan) {
+        const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+        reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(place) * kLatent)[at] =
+            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        if (q.lse && at == 0) q.lse[place] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+    };
+    if (parts <= kFewParts) {
+        const int r0 = (blockIdx.y * kTeams + team) * kRows;
+        float4 acc[kRows];
+        float top[kRows], sum[kRows];
+        bool nan[kRows];
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), top[j] = -INFINITY, sum[j] = 0.0f, nan[j] = false;
+        // a running maximum again, so that a part's logarithm and result are loaded together, two parts at a time
+        for (int i = 0; i < parts; i += 2) {
+            float f[2][kRows];
+            float4 v[2][kRows];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    f[k][j] = i + k < parts ? q.partial_lse[slot(i + k) + r0 + j] : -INFINITY;
+                    v[k][j] = i + k < parts ? reinterpret_cast<const float4*>(q.partial + (slot(i + k) + r0 + j) * kLatent)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) {
+                const float m = fmaxf(top[j], fmaxf(f[0][j], f[1][j])), ref = m == -INFINITY ? 0.0f : m;
+                const float old = ex2(top[j] - ref), a = ex2(f[0][j] - ref), b = ex2(f[1][j] - ref);
+                nan[j] = nan[j] || isnan(f[0][j]) || isnan(f[1][j]);
+                top[j] = m;
+                sum[j] = fmaf(sum[j], old, a + b);
+                acc[j].x = fmaf(acc[j].x, old, fmaf(a, v[0][j].x, b * v[1][j].x)), acc[j].y = fmaf(acc[j].y, old, fmaf(a, v[0][j].y, b * v[1][j].y));
+                acc[j].z = fmaf(acc[j].z, old, fmaf(a, v[0][j].z, b * v[1][j].z)), acc[j].w = fmaf(acc[j].w, old, fmaf(a, v[0][j].w, b * v[1][j].w));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const int place = place_at(q, w, R, r0 + j, cta);
+            if (place >= 0) store(place, acc[j], top[j], sum[j], nan[j]);
+        }
+        return;
+    }
+    const int r = cut.w * kBlocks + blockIdx.y;
+    static_assert(kFewParts * kBlocks >= R, "a row to each");
+    if (r >= R) return;
+    const int place = place_at(q, w, R, r, cta);
+    if (place < 0) return;                                                     // (the whole thread block)
     float top = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     bool nan = false;
     for (int i = lane; i < parts; i += 32) {
-        const float v = q.partial_lse[part(i)];
+        const float v = q.partial_lse[slot(i) + r];
         nan = nan || isnan(v);
         top = fmaxf(top, v);
     }
@@ -953,28 +999,23 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
     nan = __any_sync(0xffffffffu, nan);
     const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll 8
-    for (int i = few ? 0 : team; i < parts; i += few ? 1 : kTeams) {
-        const float f = ex2(q.partial_lse[part(i)] - ref);
-        const float4 v = reinterpret_cast<const float4*>(q.partial + part(i) * kLatent)[at];
+    for (int i = team; i < parts; i += kTeams) {
+        const float f = ex2(q.partial_lse[slot(i) + r] - ref);
+        const float4 v = reinterpret_cast<const float4*>(q.partial + (slot(i) + r) * kLatent)[at];
         sum += f;
         acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
     }
-    if (!few) {
-        sums[team][at] = acc;
-        if (at == 0) weights[team] = sum;
-        __syncthreads();
-        if (team != 0) return;
+    sums[team][at] = acc;
+    if (at == 0) weights[team] = sum;
+    __syncthreads();
+    if (team != 0) return;
 #pragma unroll
-        for (int i = 1; i < kTeams; ++i) {
-            const float4 v = sums[i][at];
-            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-            sum += weights[i];
-        }
+    for (int i = 1; i < kTeams; ++i) {
+        const float4 v = sums[i][at];
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        sum += weights[i];
     }
-    const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
-    reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(place) * kLatent)[at] =
-        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (q.lse && at == 0) q.lse[place] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+    store(place, acc, top, sum, nan);
 }
 
 // Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
@@ -986,10 +1027,16 @@ template <int R>
 int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool cut, unsigned int* status,
            cudaStream_t stream) {
     const auto kern = latent_attention_kernel<R>;
-    DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
+    static std::atomic<uint64_t> prepared{0};                                  // devices
+    int device = 0;
+    DSV3_CUDA_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1)) {
+        DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
+        if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
     if (cut)
-        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / kTeams), dim3(kCombineThreads), 0, stream, q));
+        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / (kTeams * kTeamRows)), dim3(kCombineThreads), 0, stream, q));
     return DSV3_OK;
 }
 

@@ -240,6 +240,19 @@ def test_many_sequences():
     _compare(_queries(g, 333, 4), cache, table, lens, [1] * 333, packed=False)
 
 
+@pytest.mark.parametrize("heads, drafts", [(16, 1), (16, 2), (128, 1)])
+def test_one_long_among_many(heads, drafts):
+    """A block cut among nearly all SMs, whose parts are joined in two steps, among others in few parts and whole ones."""
+    lens = [100] * 40 + [16000] + [300, 129, 1] * 10
+    g, cache, table = _setup(17 + heads + drafts, lens, 64)
+    counts = [drafts if n > 1 else 1 for n in lens]
+    q = _queries(g, sum(counts), heads)
+    first = _compare(q, cache, table, lens, counts)
+    for _ in range(3):                                                     # whichever CTA comes last
+        again = U.dsv3().latent_attention(*q, cache, table, U.i32(lens), SCALE, cu_seqlens_q=U.offsets(counts), return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_long_sequence():
     lens, counts = [20011, 3], [2, 1]
     g, cache, table = _setup(15, lens, 128)
