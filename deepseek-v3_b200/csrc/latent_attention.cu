@@ -39,8 +39,7 @@ constexpr int kTokens = 128;              // of a tile: MMA M of the first produ
 constexpr int kUnitTokens = 64, kTileSlots = 2;
 constexpr int kLatentBytes = kTokens * kLatent, kRopeBytes = kTokens * 2 * kRope, kTileBytes = kLatentBytes + kRopeBytes;
 constexpr int kGroupBytes = 8 * kLatent;
-constexpr int kSoftmaxWarps = 8, kFirstSoftmaxWarp = 4;
-constexpr int kAttnThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
+constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kScaleSlots = 4;
 constexpr int kAhead = 4, kBoxSlots = 4;  // tiles whose pages are looked up before they are loaded; of which the pages are kept
 constexpr int kFewParts = 8;              // of a block that several CTAs worked on
@@ -74,7 +73,10 @@ struct Cfg {
     static constexpr int kQChunk = 2 * R * 128;                 // hi and lo rows of 128 latents
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
-    static constexpr int kRows = R / 2;                         // of a softmax warp
+    // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  (Sixteen rows to a thread took longer, and nothing but the tile's own chain of
+    // steps bounds it with 32 rows: 0x1us.)
+    static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
+    static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
     static constexpr int kTmemO = 2 * kTmemS;
     static constexpr int kTmemCols = R == 16 ? 256 : 512;
@@ -280,16 +282,16 @@ struct Small {                                                  // shared memory
     int place[kItemSlots][R];                                   // query * heads + head, -1 for a row that is none
     Item item[kItemSlots];
     uint32_t listed, finished;                                  // items that are written down, whose results have been read
-    float top[2][2][4][R / 2];                                  // [tile parity][half][warp][row]
-    float sum[2][4][R / 2];
-    alignas(16) float row[kSoftmaxWarps][R / 2];                // (read four at a time, as the factors are)
-    alignas(16) float row2[kSoftmaxWarps][R / 2];
+    float top[2][Cfg<R>::kParts][4][Cfg<R>::kRows];             // [tile parity][part of the rows][warp][row]
+    float sum[Cfg<R>::kParts][4][Cfg<R>::kRows];
+    alignas(16) float row[Cfg<R>::kSoftmaxWarps][Cfg<R>::kRows];                // (read four at a time, as the factors are)
+    alignas(16) float row2[Cfg<R>::kSoftmaxWarps][Cfg<R>::kRows];
     uint64_t full[2 * kTileSlots], empty[2 * kTileSlots];
     uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
     Control ctl;
     int boxes[kBoxSlots][kTokens / 16];
     uint32_t looked_up, taken;                                  // tiles whose boxes are written, have been read
-    int warp_sum[kAttnThreads / 32];
+    int warp_sum[Cfg<R>::kThreads / 32];
     Walk walk;                                                  // the first item
     Shares shares;
 };
@@ -301,17 +303,17 @@ constexpr int smem_bytes() {
 static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
 
 // All threads: this CTA's share of the list, and its first item (sm.walk).
-template <typename Sm>
+template <int R, typename Sm>
 __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& q, Sm& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool once = c.n_seqs <= kAttnThreads;
+    const bool once = c.n_seqs <= Cfg<R>::kThreads;
     int total = 0;
     // a thread to a sequence; with more sequences than threads once for the total and once more for the place of the share's start
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         int at = 0;
 #pragma unroll 1
-        for (int s0 = 0; s0 < c.n_seqs; s0 += kAttnThreads) {
+        for (int s0 = 0; s0 < c.n_seqs; s0 += Cfg<R>::kThreads) {
             const int seq = s0 + static_cast<int>(threadIdx.x);
             Seq x = {0, 0, 0};
             int mine = 0;
@@ -331,7 +333,7 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
             __syncthreads();
             int before = at + run - mine;
 #pragma unroll
-            for (int w = 0; w < kAttnThreads / 32; ++w) {
+            for (int w = 0; w < Cfg<R>::kThreads / 32; ++w) {
                 const int v = sm.warp_sum[w];
                 if (w < warp) before += v;
                 at += v;
@@ -410,13 +412,14 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
 }
 
 // ---------------------------------------------------------------- the kernel
-// Warp 0 loads, warp 1 issues the MMAs, warps 4 to 11 do the softmax: four of them (one per quarter of the 128 TMEM lanes, a lane a token) for each half of the rows.
+// Warp 0 loads, warps 1 and 2 issue the MMAs, warp 3 walks the list, the others do the softmax: four of them (one per quarter of the 128 TMEM lanes, a lane a token)
+// for every eight rows.
 template <int R>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(Cfg<R>::kThreads, 1)
 latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __grid_constant__ CUtensorMap map_rope, const LatentCache c, const Queries q,
                         unsigned int* status) {
     using C = Cfg<R>;
-    constexpr int N = C::kRows;
+    constexpr int N = C::kRows, kSoftmaxWarps = C::kSoftmaxWarps;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles = smem;
@@ -451,7 +454,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         tma_prefetch_desc(&map_rope);
     }
     griddep_wait();
-    find_share(c, q, sm);                 // (its barriers also publish what was set up above)
+    find_share<R>(c, q, sm);                 // (its barriers also publish what was set up above)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -627,7 +630,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         }
     } else if (warp >= kFirstSoftmaxWarp) {
         // ------------------------------------------------------------ softmax
-        const int sw = warp - kFirstSoftmaxWarp, half = sw >> 2, quarter = sw & 3;
+        const int sw = warp - kFirstSoftmaxWarp, part_of = sw >> 2, quarter = sw & 3;
         const int token = quarter * 32 + lane;                                 // of the tile: this thread's TMEM lane
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float dither = static_cast<float>((token * 79) & 127) * 0x1p-16f - 0x1.fcp-11f;   // evenly over (-2^-10, 2^-10), half a step either side
@@ -704,7 +707,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         }
         for (uint32_t item = 0;; ++item) {
             const uint32_t par = item & 1, at_item = item & (kItemSlots - 1);
-            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);                       // the factors of all rows; the item before is done with
+            ok = barrier_all<32 * kSoftmaxWarps>(1, ok);                       // the factors of all rows; the item before is done with
             if (!ok) break;
             if (threadIdx.x == 32 * kFirstSoftmaxWarp) *static_cast<volatile uint32_t*>(&sm.finished) = item;
             const Item w = sm.item[at_item];
@@ -724,7 +727,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 float y[N];
                 {
                     uint32_t hi[N], lo[N], ro[N];
-                    const uint32_t at = tmem + lanes + b * C::kTmemS + half * N;
+                    const uint32_t at = tmem + lanes + b * C::kTmemS + part_of * N;
                     tc_ld<N>(at, hi);
                     tc_ld<N>(at + R, lo);
                     tc_ld<N>(at + 2 * R, ro);
@@ -733,7 +736,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(sm.s_empty[b]));
                     const float e = static_cast<float>(static_cast<int>(__float_as_uint(sc) >> 23) - 127);     // log2 of a power of two
-                    const float4* const k = reinterpret_cast<const float4*>(sm.factor[par] + half * N);
+                    const float4* const k = reinterpret_cast<const float4*>(sm.factor[par] + part_of * N);
 #pragma unroll
                     for (int i = 0; i < N; i += 4) {
                         const float4 f = k[i / 4];
@@ -747,7 +750,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 if (!__all_sync(0xffffffffu, present && p < w.base)) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
-                        const int r = half * N + i;
+                        const int r = part_of * N + i;
                         bool seen = p <= sm.limit[at_item][r];
                         if (q.tree) seen = seen || (p >= w.base && p - w.base < 64 && ((sm.tree[at_item][r] >> (p - w.base)) & 1));
                         if (!present || !seen) y[i] = -INFINITY;
@@ -757,17 +760,17 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 bool over = false;
 #pragma unroll
                 for (int i = 0; i < N; ++i) over = over || y[i] - mv[i] > kTop + kSlack;
-                if (!barrier_all<128>(1 + half, ok && !over)) {
+                if (!barrier_all<128>(2 + part_of, ok && !over)) {
                     float v[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) v[i] = y[i];
                     const float top = reduce_rows<N>(v, [](float a, float b2) { return fmaxf(a, b2); });
-                    if (lane % (32 / N) == 0) sm.top[b][half][quarter][own_row<N>()] = top;
-                    ok = barrier_all<128>(1 + half, ok);
+                    if (lane % (32 / N) == 0) sm.top[b][part_of][quarter][own_row<N>()] = top;
+                    ok = barrier_all<128>(2 + part_of, ok);
                     if (!ok) break;
-                    float all = sm.top[b][half][0][own_row<N>()];
+                    float all = sm.top[b][part_of][0][own_row<N>()];
 #pragma unroll
-                    for (int i = 1; i < 4; ++i) all = fmaxf(all, sm.top[b][half][i][own_row<N>()]);
+                    for (int i = 1; i < 4; ++i) all = fmaxf(all, sm.top[b][part_of][i][own_row<N>()]);
                     const float old = m;
                     if (all - m > kTop + kSlack) m = all - kTop;
                     broadcast_rows<N>(sm.row[sw], m, mv);
@@ -783,7 +786,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 #pragma unroll 2
                             for (int u = 0; u < 8; ++u) {                      // hi and lo of four times 128 dimensions
                                 uint32_t o[N];
-                                const uint32_t at = tmem + lanes + C::kTmemO + u * R + half * N;
+                                const uint32_t at = tmem + lanes + C::kTmemO + u * R + part_of * N;
                                 tc_ld<N>(at, o);
                                 tc_wait_ld();
 #pragma unroll
@@ -810,20 +813,15 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         else hi[i / 4] |= static_cast<uint32_t>(h) << 16, lo[i / 4] |= static_cast<uint32_t>(g) << 16;
                     }
                     uint8_t* const row = ps + b * C::kPBytes + token * 2 * R;
-                    if constexpr (R == 32) {                                   // four 16-byte places a token: hi of either half, lo of either half
-                        const int turn = (token >> 1) & 3;
-                        *reinterpret_cast<uint4*>(row + ((half ^ turn) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(row + (((2 + half) ^ turn) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    } else {                                                   // two: hi, lo
-                        const int turn = (token >> 2) & 1;
-                        *reinterpret_cast<uint2*>(row + (turn << 4) + half * 8) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(row + ((1 ^ turn) << 4) + half * 8) = make_uint2(lo[0], lo[1]);
-                    }
+                    // (16-byte places of a token's row: hi of sixteen rows each, then lo; swizzled over the row's 2 R bytes)
+                    const int turn = R == 32 ? (token >> 1) & 3 : (token >> 2) & 1, place16 = part_of >> 1;
+                    *reinterpret_cast<uint2*>(row + ((place16 ^ turn) << 4) + (part_of & 1) * 8) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(row + (((R / 16 + place16) ^ turn) << 4) + (part_of & 1) * 8) = make_uint2(lo[0], lo[1]);
                     // Behind the sequence's end lie other sequences' bytes, or none at all; no weight, but 0 x NaN is not 0.
                     if (p >= w.len) {
-                        uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + half * 2048;
+                        uint8_t* const v = tiles + b * kTileBytes + (token >> 3) * kGroupBytes + (token & 7) * 128 + part_of * (4 / C::kParts) * 1024;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < 32 / C::kParts; ++i) *reinterpret_cast<uint4*>(v + (i >> 3) * 1024 + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     tc_fence_before();
                     fence_proxy_async_shared();
@@ -837,10 +835,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 if (ok) fetch((item + 1) & (kItemSlots - 1));
             }
             float sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
-            if (lane % (32 / N) == 0) sm.sum[half][quarter][own_row<N>()] = sum;
-            ok = barrier_all<32 * kSoftmaxWarps>(3, ok);
+            if (lane % (32 / N) == 0) sm.sum[part_of][quarter][own_row<N>()] = sum;
+            ok = barrier_all<32 * kSoftmaxWarps>(1, ok);
             if (!ok) break;
-            sum = (sm.sum[half][0][own_row<N>()] + sm.sum[half][1][own_row<N>()]) + (sm.sum[half][2][own_row<N>()] + sm.sum[half][3][own_row<N>()]);
+            sum = (sm.sum[part_of][0][own_row<N>()] + sm.sum[part_of][1][own_row<N>()]) + (sm.sum[part_of][2][own_row<N>()] + sm.sum[part_of][3][own_row<N>()]);
             float inv[N];
             broadcast_rows<N>(sm.row[sw], sum == 0.0f ? 0.0f : 1.0f / sum, inv);
             if (!w.last) stage(par ^ 1);                                         // (all scores of this item have been read)
@@ -848,14 +846,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             const int part = 2 * blockIdx.x + (w.begins ? 1 : 0);
             const float lse2 = sum == 0.0f ? -INFINITY : m + __log2f(sum);
             if (quarter == 0 && lane % (32 / N) == 0) {
-                const int r = half * N + own_row<N>(), to = sm.place[at_item][r];
+                const int r = part_of * N + own_row<N>(), to = sm.place[at_item][r];
                 if (!whole) q.partial_lse[static_cast<int64_t>(part) * R + r] = lse2;
                 else if (q.lse && to >= 0) q.lse[to] = lse2 * kLn2;
             }
             // four rows that this lane writes: 8 bytes each, of four dimensions that it gets from its neighbours
             int to[N / 4];
             {
-                const int* const place = sm.place[at_item] + half * N + (lane & 1) * (N / 2) + ((lane >> 1) & 1) * (N / 4);
+                const int* const place = sm.place[at_item] + part_of * N + (lane & 1) * (N / 2) + ((lane >> 1) & 1) * (N / 4);
 #pragma unroll
                 for (int i = 0; i < N / 4; ++i) to[i] = place[i];
             }
@@ -866,12 +864,12 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint32_t hi[N], lo[N];
-                    const uint32_t at = tmem + lanes + C::kTmemO + u * 2 * R + half * N;
+                    const uint32_t at = tmem + lanes + C::kTmemO + u * 2 * R + part_of * N;
                     tc_ld<N>(at, hi);
                     tc_ld<N>(at + R, lo);
                     tc_wait_ld();
                     if (!whole) {
-                        float* const dst = q.partial + (static_cast<int64_t>(part) * R + half * N) * kLatent + u * 128 + token;
+                        float* const dst = q.partial + (static_cast<int64_t>(part) * R + part_of * N) * kLatent + u * 128 + token;
 #pragma unroll
                         for (int i = 0; i < N; ++i) dst[i * kLatent] = fmaf(__uint_as_float(lo[i]), 1.0f / kLoScale, __uint_as_float(hi[i])) * inv[i];
                         continue;
@@ -1034,7 +1032,7 @@ int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const
         DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(kAttnThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(Cfg<R>::kThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
     if (cut)
         DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / (kTeams * kTeamRows)), dim3(kCombineThreads), 0, stream, q));
     return DSV3_OK;
