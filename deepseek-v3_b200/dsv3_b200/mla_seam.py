@@ -1,0 +1,91 @@
+"""Seam above the latent cache: a replacement for ``MLA.forward`` of the reference's ``model.py``.
+
+``MLA.forward`` (model.py:446-497, ``attn_impl = "absorb"``) normalises, rotates and stores the new tokens in bf16 buffers and then runs two score
+einsums, a softmax and a weighted-sum einsum over the whole prefix.  The replacement keeps the projections, the absorbed products with ``wkv_b`` and the
+arguments, and does the rest with the operators of ``latent.py``: one launch stores the new tokens in the 8-bit cache, ``latent_attention`` reads it.
+
+    import model, dsv3_b200
+    dsv3_b200.install_mla(model)        # model.MLA.forward = mla_forward
+
+A module's cache is made on its first call, of the size of its bf16 buffers; ``mla_cache(module)`` gives it with its block table, for
+``latent_cache_keep`` and ``latent_cache_read``.  Drafted tokens: with a tree of them, ``mask`` is the int64 ``[batch, tokens]`` of
+``latent_attention``'s ``tree_mask`` and ``freqs_cis`` has a row per node, that of its depth.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .latent import LATENT_DIM, ROPE_DIM, LatentCache, allocate_latent_cache, latent_attention, latent_cache_write
+from .ops import weight_dequant
+
+PAGE = 64
+
+
+class MlaCache(NamedTuple):
+    pool: LatentCache
+    block_table: torch.Tensor       # int32 [max_batch, pages of a sequence]: sequence b has pages b * pages ... in order
+    first_page_slot: int            # slots of a sequence: b * first_page_slot + position
+    max_len: int
+
+
+def mla_cache(module) -> MlaCache:
+    """The 8-bit cache of an MLA module, made on first use after its bf16 buffers (model.py:439-444)."""
+    cache = module.__dict__.get("_dsv3_latent")
+    if cache is None:
+        buffer = module.kv_cache if hasattr(module, "kv_cache") else module.k_cache
+        batch, length = buffer.shape[:2]
+        pages = -(-length // PAGE)
+        table = torch.arange(batch * pages, dtype=torch.int32, device=buffer.device).view(batch, pages)
+        cache = MlaCache(allocate_latent_cache(batch * pages, PAGE, buffer.device), table, pages * PAGE, length)
+        module.__dict__["_dsv3_latent"] = cache
+    return cache
+
+
+def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
+    """Neighbouring values of the last dimension as a complex number, times their angle's (model.py:378-393)."""
+    z = torch.view_as_complex(x.float().view(*x.shape[:-1], -1, 2)) * freqs_cis.view(1, x.size(1), 1, -1)
+    return torch.view_as_real(z).flatten(3).to(x.dtype)
+
+
+def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
+    """``MLA.forward`` on the 8-bit latent cache.  ``mask``: None for one token, the reference's causal mask (any floating tensor is taken for it), or
+    int64 words of a tree of drafted tokens."""
+    bsz, seqlen, _ = x.shape
+    rope = self.qk_rope_head_dim
+    if self.kv_lora_rank != LATENT_DIM or rope != ROPE_DIM:
+        raise NotImplementedError(f"the latent cache holds {LATENT_DIM} + {ROPE_DIM} values a token (kv_lora_rank {self.kv_lora_rank}, qk_rope_head_dim {rope})")
+    tree = mask if mask is not None and not mask.is_floating_point() else None
+    if mask is None and seqlen > 1:
+        raise NotImplementedError("several tokens without a mask would see one another both ways; latent_attention is causal")
+    cache = mla_cache(self)
+    end_pos = start_pos + seqlen
+    if bsz > cache.block_table.size(0) or end_pos > cache.max_len:
+        raise ValueError(f"{bsz} sequences of {end_pos} tokens do not fit a cache of {cache.block_table.size(0)} of {cache.max_len}")
+
+    q = self.wq(x) if self.q_lora_rank == 0 else self.wq_b(self.q_norm(self.wq_a(x)))
+    q = q.view(bsz, seqlen, self.n_local_heads, -1)
+    q_nope, q_rope = torch.split(q, [self.qk_nope_head_dim, rope], dim=-1)
+    kv = self.wkv_a(x)
+    step = torch.arange(seqlen, device=x.device)
+    slots = (torch.arange(bsz, device=x.device) * cache.first_page_slot + start_pos)[:, None] + step
+    latent_cache_write(cache.pool, kv, self.kv_norm.weight, freqs_cis, step.repeat(bsz), slots, self.kv_norm.eps)
+
+    weight = self.wkv_b.weight
+    scale = getattr(self.wkv_b, "scale", None)
+    if scale is not None:
+        weight = weight_dequant(weight, scale, block_size)
+    weight = weight.view(self.n_local_heads, -1, LATENT_DIM)
+    q_latent = torch.einsum("bshd,hdc->bshc", q_nope, weight[:, :self.qk_nope_head_dim])
+    lens = torch.full((bsz,), end_pos, dtype=torch.int32, device=x.device)
+    out = latent_attention(q_latent, _rotate(q_rope, freqs_cis), cache.pool, cache.block_table[:bsz, :-(-end_pos // PAGE)], lens, self.softmax_scale, tree_mask=tree)
+    return self.wo(torch.einsum("bshc,hdc->bshd", out, weight[:, -self.v_head_dim:]).flatten(2))
+
+
+def install_mla(model_module) -> None:
+    """Point ``model_module.MLA.forward`` at ``mla_forward``; ``model_module.block_size`` is read at call time, as in the reference."""
+    def forward(self, x, start_pos, freqs_cis, mask):
+        return mla_forward(self, x, start_pos, freqs_cis, mask, block_size=getattr(model_module, "block_size", 128))
+    forward.__doc__ = mla_forward.__doc__
+    model_module.MLA.forward = forward
