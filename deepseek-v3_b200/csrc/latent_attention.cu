@@ -18,6 +18,13 @@
 //   S^T [128 tokens, hi | lo]  = C [128, 512] Q^T,  S_rope^T [128, R] = K [128, 64] Q_rope^T (bf16),  O^T [4 x 128 dims, hi | lo] += C^T P^T
 // hi and lo stand side by side as columns, which reads C once for both.  C is the MMA's A operand in both products, K-major in the first and transposed
 // (MN-major) in the second, from the same bytes.
+//
+// What bounds it (B200; a call and its join):
+//   16 rows (a decoding sequence on one rank of eight): HBM.  A tile is 82 KB and 148 CTAs read 6.3 TB/s while they go; 64 sequences of up to 8192 tokens, 196 MB,
+//   take 47 us, of which 28 are that.  The rest is a start (8 us: the work list, the queries and the first tile come from memory one after another), an end (1 us) and the join.
+//   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3300: the
+//   products of a tile wait for its weights, those for its scores, and two tiles are all that fits, so that one's softmax hides only half of the other's products.
+//   128 heads of 32 sequences of 8192 tokens 115 us, a chunk of 515 tokens 113 (44 to 45 at the rate of library bf16 products).
 #include <cuda.h>
 
 #include <atomic>
@@ -73,8 +80,9 @@ struct Cfg {
     static constexpr int kQChunk = 2 * R * 128;                 // hi and lo rows of 128 latents
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
-    // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  (Sixteen rows to a thread took longer, and nothing but the tile's own chain of
-    // steps bounds it with 32 rows: 0x1us.)
+    // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  With 32 rows the softmax is part of the chain that a tile waits for; eight warps of 16 rows to a
+    // thread took 90 us instead of 78 for 128 sequences of 1024 tokens and 128 heads, 81 instead of 74 for trees of 24 drafts, 53 instead of 47 for one
+    // sequence of 131072 tokens.
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
@@ -184,7 +192,7 @@ __device__ __forceinline__ int64_t ramp(int x, int shift) {
 __device__ __forceinline__ int tiles_before(const Queries& q, const Seq& s, int n, int blocks) {
     if (n == 0) return 0;
     if (q.tree || blocks == 1) return n * tiles_of(s.len);
-    const int u = (s.len - s.queries + (1 << q.block_shift) - 1) >> q.block_shift;
+    const int u = static_cast<int>((static_cast<int64_t>(s.len) - s.queries + (1 << q.block_shift) - 1) >> q.block_shift);
     const int shift = 7 - q.block_shift;
     const int whole = n == blocks ? n - 1 : n;
     return static_cast<int>(ramp(u + whole, shift) - ramp(u, shift)) + (n == blocks ? tiles_of(s.len) : 0);
@@ -228,8 +236,10 @@ struct Walk {
             head_block = 0;
             if (++block >= blocks_of(q, s)) {
                 block = 0;
-                do s = load_seq(c, q, ++seq);
-                while (s.queries == 0);
+                do {
+                    if (++seq >= c.n_seqs) return false;                       // (offsets that decrease can count more tiles than 32 bits hold)
+                    s = load_seq(c, q, seq);
+                } while (s.queries == 0);
             }
         }
         settle(q);
@@ -272,6 +282,7 @@ struct Item {
     bool begins, ends, last;              // of the block; the CTA's last item
 };
 constexpr int kItemSlots = 4;
+constexpr uint64_t kItemLimitNs = 100 * kWaitLimitNs;   // the walk waits for whole items, and one has up to 2^24 tiles of 2 us
 
 template <int R>
 struct Small {                                                  // shared memory beside the operand tiles
@@ -389,7 +400,7 @@ __device__ __forceinline__ void broadcast_rows(float* to, float own, float (&v)[
 }
 
 // Waits until another warp's counter in shared memory has reached `want`, as bounded_wait does for a barrier.
-__device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, Control* ctl, unsigned int* status) {
+__device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, Control* ctl, unsigned int* status, uint64_t limit_ns = kWaitLimitNs) {
     uint64_t t0 = 0;
     for (uint32_t spins = 0;; ++spins) {
         if (*static_cast<const volatile uint32_t*>(counter) >= want) {
@@ -402,7 +413,7 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
             const uint64_t now = global_timer_ns();
             if (t0 == 0) {
                 t0 = now;
-            } else if (now - t0 > kWaitLimitNs) {
+            } else if (now - t0 > limit_ns) {
                 ctl->abort_flag = 1;
                 if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.x;
                 return false;
@@ -526,7 +537,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 for (int i = 0; i < 2 * kLatent; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(lat + i));
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(q.rope + query * q.rope_token + head * q.rope_head));
             }
-            if (item >= kItemSlots) ok = __all_sync(0xffffffffu, follow(&sm.finished, item + 1 - kItemSlots, ctl, status));
+            if (item >= kItemSlots) ok = __all_sync(0xffffffffu, follow(&sm.finished, item + 1 - kItemSlots, ctl, status, kItemLimitNs));
             if (!ok) break;
             const int base = w.s.len - w.s.queries;
             const bool begins = w.tile == 0, ends = w.tile + w.n == w.tiles;

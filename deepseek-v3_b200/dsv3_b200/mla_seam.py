@@ -7,7 +7,7 @@ arguments, and does the rest with the operators of ``latent.py``: one launch sto
     import model, dsv3_b200
     dsv3_b200.install_mla(model)        # model.MLA.forward = mla_forward
 
-A module's cache is made on its first call, of the size of its bf16 buffers; ``mla_cache(module)`` gives it with its block table, for
+A module's cache is made on its first call (not in a captured graph), of the size of its bf16 buffers; ``mla_cache(module)`` gives it with its block table, for
 ``latent_cache_keep`` and ``latent_cache_read``.  Drafted tokens: with a tree of them, ``mask`` is the int64 ``[batch, tokens]`` of
 ``latent_attention``'s ``tree_mask`` and ``freqs_cis`` has a row per node, that of its depth.
 """
@@ -34,6 +34,8 @@ def mla_cache(module) -> MlaCache:
     """The 8-bit cache of an MLA module, made on first use after its bf16 buffers (model.py:439-444)."""
     cache = module.__dict__.get("_dsv3_latent")
     if cache is None:
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an MLA module's cache is made on its first call, which cannot be a captured one: every replay would clear it")
         buffer = module.kv_cache if hasattr(module, "kv_cache") else module.k_cache
         batch, length = buffer.shape[:2]
         pages = -(-length // PAGE)

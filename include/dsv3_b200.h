@@ -320,10 +320,10 @@ int dsv3_few_down(const void* table2, int n, const void* route, const void* h, i
  *   rope   : bf16 [64]    the rotated key divided by `scale`
  *   scale  : fp32         s, the least power of two with max(amax, 1e-4) <= 448 s, amax being the largest |latent|
  * (e4m3 has its own exponent: a finer grid of scales would gain at most one bit at the bottom of the range, and a power of two costs
- * the rotated values nothing).  A token with a value that is not finite has zero bytes and scale NaN: a query that sees it becomes NaN, one that does
+ * the rotated values nothing; attention takes the scale as its exponent, so that it has to be a power of two, or NaN).  A token with a value that is not finite has zero bytes and scale NaN: a query that sees it becomes NaN, one that does
  * not is not touched by it.
  * Tokens lie in pages of a pool: latent [n_pages, page_size, 512], rope [n_pages, page_size, 64], scale [n_pages, page_size], contiguous, latent and rope
- * 16-byte aligned; page_size is a power of two from 16 on; n_pages * page_size < 2^31.  A token's slot is page * page_size + its place in the page.
+ * 16-byte aligned (attention: scale too); page_size is a power of two from 16 on; n_pages * page_size < 2^31, and so is pages_width * page_size.  A token's slot is page * page_size + its place in the page.
  * pages: int32 [n_seqs, pages_width], rows pages_stride apart: the pages of a sequence in order of position.  Entries behind a sequence's last
  * token are not read; one that names no page of the pool makes its tokens absent (attention does not see them, read returns zeros, keep does not move them).
  */
@@ -343,7 +343,7 @@ typedef struct dsv3_latent_cache {
 /*
  * New tokens -- `kv, k_pe = split(wkv_a(x))`, kv_norm, apply_rotary_emb and the two stores of model.py:469-471, 484-485 in one launch.
  *   kv        : bf16 [tokens, 576] with rows kv_stride apart (a multiple of 8; 16-byte aligned): 512 latent values, then 64 to rotate
- *   weight    : [512] of the norm, bf16 or fp32 (weight_fp32); latent = kv / sqrt(mean(kv^2) + eps) * weight, in fp32
+ *   weight    : [512] of the norm, bf16 or fp32 (weight_fp32), 16-byte aligned; latent = kv / sqrt(mean(kv^2) + eps) * weight, in fp32
  *   freqs     : complex64 [n_positions, 32], cos + i sin of every angle; pair j of a token's rotated values is multiplied by freqs[position, j]
  *   positions : int64 [tokens]; a token whose position the table does not hold is stored as one that is not finite
  *   slots     : int64 [tokens], all different; a token whose slot lies outside the pool is not stored
@@ -383,7 +383,8 @@ int dsv3_latent_keep(const dsv3_latent_cache_t* cache, const int32_t* first, con
  *              queries' own tokens are still the last ones of their sequence; a query sees all before them, and of them those whose bit is
  *              set (bit j: the j-th; from the 64th on none is seen).
  *   out      : bf16 [tokens, heads, 512], lse : fp32 [tokens, heads].  A query that sees nothing: zeros, and -inf.
- * workspace: dsv3_latent_attention_workspace_bytes() bytes, 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
+ * Refused: a pool without pages; query blocks times tiles of 128 positions, with every row of pages full, that reach 2^31.
+ * workspace: dsv3_latent_attention_workspace_bytes() bytes (longest: pages_width * page_size), 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
  */
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest);
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,

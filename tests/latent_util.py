@@ -75,7 +75,11 @@ def attention(q_latent, q_rope, cache, table, lens, counts, scale, tree=None):
     """out, lse and a bound of what rounding may make of out, per element, for packed queries.
 
     The bound: a result in bf16 is off by half a step, 2^-8 of it.  A weight enters the second product with 8 significant bits, off by 2^-8 of
-    itself, or, where it is small, by half of 2^-13 of a scale on which the running maximum is at least 2^6 (2^-20 of the largest weight).  A score is a sum of 576
+    itself, or, where it is small, by at most a step of 2^-13 (half of one from rounding, half from the offset before it) on a scale where the largest
+    weight is at least 2^5.  The token of that weight has a latent above 224 as stored, no token one above 448: a step on any token is at most
+    2^-13 * 448 / (2^5 * 224) = 2^-17 of `top`, the largest product of a weight and its token's largest latent.  n of them add up to n of that at most; the offsets
+    are even over a step, which makes an error's mean zero, and then a sum of n > 64 is above 16 sqrt(n) 2^-18 with a chance of 2 exp(-32) (Hoeffding, on
+    errors between -2^-17 and 2^-17: 2 exp(-2 (16 sqrt(n) 2^-18)^2 / (n (2^-16)^2))).  A score is a sum of 576
     products in fp32, off by 576 * 2^-24 of the sum of their sizes, and its error is the weight's relative one; as much again comes from the exponent's
     argument, which has 24 bits of at most the largest score.  A weight's error e comes twice, in the sum and in its divisor; 2^-14 stands for
     the exponential, the sums and the division."""
@@ -110,7 +114,8 @@ def attention(q_latent, q_rope, cache, table, lens, counts, scale, tree=None):
             spread_of = w @ cs.abs()
             # small weights: a weight enters times its token's scale, so what counts is the largest product of the two
             top = (w * cs.abs().amax(-1)).amax(-1, keepdim=True)
-            bounds.append(2.0 ** -8 * o.abs() + (2.0 ** -8 + 2 * e) * spread_of + int(seen.sum()) * 2.0 ** -20 * 448 / 256 * top)
+            many = int(seen.sum())
+            bounds.append(2.0 ** -8 * o.abs() + (2.0 ** -8 + 2 * e) * spread_of + min(many * 2.0 ** -17, 16 * many ** 0.5 * 2.0 ** -18) * top)
             outs.append(o)
             lses.append(lse)
     shape = (0, q_latent.shape[1])

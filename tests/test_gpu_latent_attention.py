@@ -240,6 +240,46 @@ def test_many_sequences():
     _compare(_queries(g, 333, 4), cache, table, lens, [1] * 333, packed=False)
 
 
+@pytest.mark.parametrize("heads, drafts", [(5, 1), (12, 3), (40, 1)])
+def test_more_sequences_than_threads(heads, drafts):
+    """1400 sequences: the list of tiles is added up in several rounds.  One is long, some have no queries."""
+    lens = [(i * 37) % 140 + 3 for i in range(1400)]
+    lens[901] = 5000
+    counts = [0 if i % 11 == 5 else drafts for i in range(1400)]
+    g, cache, table = _setup(19 + heads, lens, 16)
+    _compare(_queries(g, sum(counts), heads), cache, table, lens, counts)
+
+
+def test_slots_whose_bytes_pass_32_bits():
+    """A pool of 8.4 million tokens, of which one sequence uses pages at both ends: offsets in bytes pass 2^32."""
+    d = U.dsv3()
+    n_pages, page, n = 131200, 64, 300
+    g = torch.Generator(device="cuda").manual_seed(20)
+    small = U.make_cache(g, 5, page)
+    cache = d.LatentCache(*(torch.empty(n_pages, *t.shape[1:], dtype=t.dtype, device="cuda") for t in small))
+    names = [n_pages - 1, 0, n_pages - 40, 131071, 131072]
+    assert names[3] * page * 512 < 1 << 32 <= names[4] * page * 512
+    for big, few in zip(cache, small):
+        for i, name in enumerate(names):
+            big[name] = few[i]
+    table, few = U.i32([names]), U.i32([list(range(5))])
+    q = _queries(g, 2, 16)
+    out = d.latent_attention(*q, cache, table, U.i32([n]), SCALE, return_lse=True)
+    want = d.latent_attention(*q, small, few, U.i32([n]), SCALE, return_lse=True)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    for a, b in zip(d.latent_cache_read(cache, table, U.offsets([n]), n), d.latent_cache_read(small, few, U.offsets([n]), n)):
+        assert torch.equal(a, b)
+    kv = torch.randn(2, 576, generator=g, device="cuda", dtype=torch.float32).bfloat16()
+    f, w = torch.ones(4, 32, dtype=torch.complex64, device="cuda"), torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    for c, slots in ((cache, [n_pages * page - 1, 131072 * page + 5]), (small, [63, 4 * page + 5])):
+        d.latent_cache_write(c, kv, w, f, torch.arange(2, device="cuda"), torch.tensor(slots, device="cuda"))
+    d.latent_cache_keep(cache, table, U.i32([60]), U.i32([[3, 200]]), U.i32([2]))
+    d.latent_cache_keep(small, few, U.i32([60]), U.i32([[3, 200]]), U.i32([2]))
+    for big, few_of in zip(cache, small):
+        for i, name in enumerate(names):
+            assert torch.equal(big[name].view(torch.uint8), few_of[i].view(torch.uint8))
+
+
 @pytest.mark.parametrize("heads, drafts", [(16, 1), (16, 2), (128, 1)])
 def test_one_long_among_many(heads, drafts):
     """A block cut among nearly all SMs, whose parts are joined in two steps, among others in few parts and whole ones."""

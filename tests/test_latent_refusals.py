@@ -30,12 +30,12 @@ def _lib():
     return lib, _lib
 
 
-def _write(lib, cache, kv=16, stride=576, tokens=1, n_positions=8):
-    return lib.dsv3_latent_write(cache, kv, stride, 16, 0, 1e-6, 16, n_positions, 16, 16, tokens, None)
+def _write(lib, cache, kv=16, stride=576, tokens=1, n_positions=8, weight=16, freqs=16):
+    return lib.dsv3_latent_write(cache, kv, stride, weight, 0, 1e-6, freqs, n_positions, 16, 16, tokens, None)
 
 
-def _attention(lib, cache, q=16, stride=512, tokens=2, heads=1, out=16, cu=None):
-    return lib.dsv3_latent_attention(cache, q, stride, stride, q, 64, 64, tokens, heads, 16, cu, None, 1.0, out, None, None, 0, None)
+def _attention(lib, cache, q=16, stride=512, tokens=2, heads=1, out=16, cu=None, workspace=None, workspace_bytes=0):
+    return lib.dsv3_latent_attention(cache, q, stride, stride, q, 64, 64, tokens, heads, 16, cu, None, 1.0, out, None, workspace, workspace_bytes, None)
 
 
 @pytest.mark.parametrize("over, status", [
@@ -66,7 +66,12 @@ def test_calls_that_are_refused_and_calls_of_nothing():
     assert _write(lib, _cache(), kv=None) == names.ERR_INVALID_ARGUMENT
     assert _write(lib, _cache(), kv=24) == names.ERR_UNSUPPORTED
     assert _write(lib, _cache(), stride=580) == names.ERR_UNSUPPORTED
+    assert _write(lib, _cache(), weight=24) == names.ERR_UNSUPPORTED
+    assert _write(lib, _cache(), weight=None) == names.ERR_INVALID_ARGUMENT
+    assert _write(lib, _cache(), freqs=20) == names.ERR_UNSUPPORTED
+    assert _write(lib, _cache(), freqs=None) == names.ERR_INVALID_ARGUMENT
     assert _write(lib, _cache(), tokens=0) == names.OK
+    assert lib.dsv3_latent_read(_cache(), 16, 1 << 31, 16, 16, None) == names.ERR_UNSUPPORTED
     assert lib.dsv3_latent_read(_cache(), 16, -1, 16, 16, None) == names.ERR_INVALID_ARGUMENT
     assert lib.dsv3_latent_read(_cache(), None, 1, 16, 16, None) == names.ERR_INVALID_ARGUMENT
     assert lib.dsv3_latent_read(_cache(), 16, 1, 24, 16, None) == names.ERR_UNSUPPORTED
@@ -79,6 +84,16 @@ def test_calls_that_are_refused_and_calls_of_nothing():
     assert _attention(lib, _cache(), tokens=3) == names.ERR_INVALID_ARGUMENT            # do not divide among two sequences
     assert _attention(lib, _cache(), q=24) == names.ERR_UNSUPPORTED
     assert _attention(lib, _cache(), stride=516) == names.ERR_UNSUPPORTED
+    assert _attention(lib, _cache(), out=24) == names.ERR_UNSUPPORTED
+    assert _attention(lib, _cache(scale=4100)) == names.ERR_UNSUPPORTED
+    assert _attention(lib, _cache(n_pages=0)) == names.ERR_INVALID_ARGUMENT
+    assert _attention(lib, _cache(n_seqs=0)) == names.ERR_INVALID_ARGUMENT
+    assert _attention(lib, _cache(pages_width=1 << 20), tokens=1 << 14) == names.ERR_UNSUPPORTED         # 2^14 times 2^19 tiles
+    assert _attention(lib, _cache(pages_width=1 << 25)) == names.ERR_UNSUPPORTED
+    need = lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 4 * 64)
+    assert need > 0 and lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 128) == 0
+    for at, size in ((None, need), (1024, need - 1), (1040, need)):
+        assert _attention(lib, _cache(pages_width=4), workspace=at, workspace_bytes=size) == names.ERR_WORKSPACE
     assert _attention(lib, _cache(), heads=1025) == names.ERR_UNSUPPORTED
     assert _attention(lib, _cache(), tokens=0) == names.OK
     assert b"heads" in names.lib.dsv3_last_error()
@@ -134,3 +149,18 @@ def test_no_cpu_path():
         d.latent_cache_read(c, table, cu, 1)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         d.latent_cache_keep(c, table, cu[:2], table, cu[:2])
+
+
+def test_a_module_whose_cache_would_be_made_in_a_captured_graph(monkeypatch):
+    import types
+    import dsv3_b200 as d
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    module = types.SimpleNamespace(kv_cache=torch.zeros(2, 70, 512))
+    with pytest.raises(RuntimeError, match="captured"):
+        d.mla_cache(module)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    cache = d.mla_cache(module)
+    assert cache.block_table.tolist() == [[0, 1], [2, 3]] and cache.pool.scale.shape == (4, 64)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert d.mla_cache(module) is cache
