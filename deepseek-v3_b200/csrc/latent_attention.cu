@@ -22,9 +22,9 @@
 // What bounds it (B200; a call and its join):
 //   16 rows (a decoding sequence on one rank of eight): HBM.  A tile is 82 KB and 148 CTAs read 6.3 TB/s while they go; 64 sequences of up to 8192 tokens, 196 MB,
 //   take 47 us, of which 28 are that.  The rest is a start (8 us: the work list, the queries and the first tile come from memory one after another), an end (1 us) and the join.
-//   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3300: the
+//   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3100: the
 //   products of a tile wait for its weights, those for its scores, and two tiles are all that fits, so that one's softmax hides only half of the other's products.
-//   128 heads of 32 sequences of 8192 tokens 115 us, a chunk of 515 tokens 113 (44 to 45 at the rate of library bf16 products).
+//   128 heads of 32 sequences of 8192 tokens 110 us, a chunk of 515 tokens 109 (44 to 45 at the rate of library bf16 products).
 #include <cuda.h>
 
 #include <atomic>
@@ -42,7 +42,8 @@ namespace {
 constexpr int kTokens = 128;              // of a tile: MMA M of the first product, K of the second
 // A tile is loaded and given back in two units of 64 tokens.  Its latents lie as [16 groups of eight tokens][4 chunks of 128 dimensions][8 tokens][128 bytes],
 // swizzled over 128 bytes: one copy brings a page's share of a unit, all four chunks of it (a copy per chunk and page: 450 cycles a chunk to issue, more
-// than a tile's share of HBM takes), and both MMAs find a chunk's groups 4096 bytes apart.
+// than a tile's share of HBM takes), and both MMAs find a chunk's groups 4096 bytes apart.  (Four units of 32 tokens: 124 us instead of 110 for 128 heads of 32
+// sequences of 8192 tokens, every wait more than its earlier copy gains; two units of 256 dimensions, whose scores could begin alone: 114.)
 constexpr int kUnitTokens = 64, kTileSlots = 2;
 constexpr int kLatentBytes = kTokens * kLatent, kRopeBytes = kTokens * 2 * kRope, kTileBytes = kLatentBytes + kRopeBytes;
 constexpr int kGroupBytes = 8 * kLatent;
@@ -80,9 +81,9 @@ struct Cfg {
     static constexpr int kQChunk = 2 * R * 128;                 // hi and lo rows of 128 latents
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
-    // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  With 32 rows the softmax is part of the chain that a tile waits for; eight warps of 16 rows to a
-    // thread took 90 us instead of 78 for 128 sequences of 1024 tokens and 128 heads, 81 instead of 74 for trees of 24 drafts, 53 instead of 47 for one
-    // sequence of 131072 tokens.
+    // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  With 32 rows the softmax is part of the chain that a tile waits for: eight warps of 16 rows to a
+    // thread took 15 % longer for 128 sequences of 1024 tokens and 128 heads (75 us now), 9 % for 24 trees of 13 drafts (72), 13 % for one
+    // sequence of 131072 tokens (45).
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
@@ -135,6 +136,30 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Two values at a time: an instruction instead of two (the softmax's warps are short of issue slots with 32 rows: 110 us instead of 115 for 128 heads of 32
+// sequences of 8192 tokens).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
 
@@ -722,10 +747,11 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             if (!ok) break;
             if (threadIdx.x == 32 * kFirstSoftmaxWarp) *static_cast<volatile uint32_t*>(&sm.finished) = item;
             const Item w = sm.item[at_item];
-            // d = y - mv is the weight's exponent; nothing has been seen yet: mv far below every score
-            float l[N], mv[N], m = kNothing;                                   // m: mv of row own_row<N>()
+            // d = y + less is the weight's exponent, less the row's negated maximum; nothing has been seen yet: far below every score
+            float2 l[N / 2], less[N / 2];
+            float m = kNothing;                                                // of row own_row<N>()
 #pragma unroll
-            for (int i = 0; i < N; ++i) l[i] = 0.0f, mv[i] = kNothing;
+            for (int i = 0; i < N / 2; ++i) l[i] = make_float2(0.0f, 0.0f), less[i] = make_float2(-kNothing, -kNothing);
             for (int t = 0; t < w.n; ++t, ++tile_count) {
                 const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
                 const int p = (w.tile + t) * kTokens + token;
@@ -735,7 +761,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 const float sc = sm.scales[tile_count & (kScaleSlots - 1)][token];
                 ok = ok && wait(sm.s_full[b], phase, 4, tile_count);
                 tc_fence_after();
-                float y[N];
+                float2 y[N / 2];
                 {
                     uint32_t hi[N], lo[N], ro[N];
                     const uint32_t at = tmem + lanes + b * C::kTmemS + part_of * N;
@@ -748,13 +774,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     if (lane == 0) mbar_arrive(bar(sm.s_empty[b]));
                     const float e = static_cast<float>(static_cast<int>(__float_as_uint(sc) >> 23) - 127);     // log2 of a power of two
                     const float4* const k = reinterpret_cast<const float4*>(sm.factor[par] + part_of * N);
+                    const auto two = [](const uint32_t* v) { return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
 #pragma unroll
                     for (int i = 0; i < N; i += 4) {
                         const float4 f = k[i / 4];
-                        const float g[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            y[i + j] = fmaf((__uint_as_float(hi[i + j]) + __uint_as_float(lo[i + j])) + __uint_as_float(ro[i + j]), sc * g[j], e);
+                        for (int j = 0; j < 4; j += 2)
+                            y[(i + j) / 2] = fma2(add2(add2(two(hi + i + j), two(lo + i + j)), two(ro + i + j)),
+                                                  mul2(make_float2(sc, sc), j ? make_float2(f.z, f.w) : make_float2(f.x, f.y)), make_float2(e, e));
                     }
                 }
                 const bool present = p < w.len && sc != 0.0f;
@@ -764,17 +791,21 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         const int r = part_of * N + i;
                         bool seen = p <= sm.limit[at_item][r];
                         if (q.tree) seen = seen || (p >= w.base && p - w.base < 64 && ((sm.tree[at_item][r] >> (p - w.base)) & 1));
-                        if (!present || !seen) y[i] = -INFINITY;
+                        if (!present || !seen) (i & 1 ? y[i / 2].y : y[i / 2].x) = -INFINITY;
                     }
                 }
                 // -------- a new maximum where some weight would pass 2^8: rare after the first tiles, so that the others only ask whether there is one
-                bool over = false;
+                float2 d[N / 2];
+                float most = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < N; ++i) over = over || y[i] - mv[i] > kTop + kSlack;
-                if (!barrier_all<128>(2 + part_of, ok && !over)) {
-                    float v[N];
+                for (int i = 0; i < N / 2; ++i) {
+                    d[i] = add2(y[i], less[i]);
+                    most = fmaxf(most, fmaxf(d[i].x, d[i].y));
+                }
+                if (!barrier_all<128>(2 + part_of, ok && !(most > kTop + kSlack))) {
+                    float v[N], mv[N];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) v[i] = y[i];
+                    for (int i = 0; i < N; ++i) v[i] = i & 1 ? y[i / 2].y : y[i / 2].x;
                     const float top = reduce_rows<N>(v, [](float a, float b2) { return fmaxf(a, b2); });
                     if (lane % (32 / N) == 0) sm.top[b][part_of][quarter][own_row<N>()] = top;
                     ok = barrier_all<128>(2 + part_of, ok);
@@ -784,12 +815,17 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     for (int i = 1; i < 4; ++i) all = fmaxf(all, sm.top[b][part_of][i][own_row<N>()]);
                     const float old = m;
                     if (all - m > kTop + kSlack) m = all - kTop;
-                    broadcast_rows<N>(sm.row[sw], m, mv);
+                    broadcast_rows<N>(sm.row[sw], -m, mv);
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) {
+                        less[i] = make_float2(mv[2 * i], mv[2 * i + 1]);
+                        d[i] = add2(y[i], less[i]);
+                    }
                     if (t > 0) {                                               // sums so far take it
                         float f[N];
                         broadcast_rows<N>(sm.row2[sw], ex2(old - m), f);
 #pragma unroll
-                        for (int i = 0; i < N; ++i) l[i] *= f[i];
+                        for (int i = 0; i < N / 2; ++i) l[i] = mul2(l[i], make_float2(f[2 * i], f[2 * i + 1]));
                         const uint32_t before = tile_count - 1;
                         ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
                         tc_fence_after();
@@ -814,12 +850,13 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     uint32_t hi[N / 4], lo[N / 4];
 #pragma unroll
                     for (int i = 0; i < N; i += 2) {
-                        const float a = ex2(y[i] - mv[i]), d = ex2(y[i + 1] - mv[i + 1]);
-                        l[i] = fmaf(a, inv, l[i]);
-                        l[i + 1] = fmaf(d, inv, l[i + 1]);
-                        const uint16_t h = cvt_e4m3x2(a, d);
-                        const float2 f = e4m3x2_to_float2(h);
-                        const uint16_t g = cvt_e4m3x2(fmaf(a - f.x, kLoScale, a > 0.0f ? dither : 0.0f), fmaf(d - f.y, kLoScale, d > 0.0f ? dither : 0.0f));
+                        const float2 a = make_float2(ex2(d[i / 2].x), ex2(d[i / 2].y));
+                        l[i / 2] = fma2(a, make_float2(inv, inv), l[i / 2]);
+                        const uint16_t h = cvt_e4m3x2(a.x, a.y);
+                        // (the offset alone rounds to zero: no weight stays none)
+                        const float2 rest = fma2(e4m3x2_to_float2(h), make_float2(-1.0f, -1.0f), a);
+                        const float2 scaled = fma2(rest, make_float2(kLoScale, kLoScale), make_float2(dither, dither));
+                        const uint16_t g = cvt_e4m3x2(scaled.x, scaled.y);
                         if ((i & 2) == 0) hi[i / 4] = h, lo[i / 4] = g;
                         else hi[i / 4] |= static_cast<uint32_t>(h) << 16, lo[i / 4] |= static_cast<uint32_t>(g) << 16;
                     }
@@ -845,7 +882,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 ok = ok && listed(item + 1);
                 if (ok) fetch((item + 1) & (kItemSlots - 1));
             }
-            float sum = reduce_rows<N>(l, [](float a, float b2) { return a + b2; });
+            float of_row[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) of_row[i] = i & 1 ? l[i / 2].y : l[i / 2].x;
+            float sum = reduce_rows<N>(of_row, [](float a, float b2) { return a + b2; });
             if (lane % (32 / N) == 0) sm.sum[part_of][quarter][own_row<N>()] = sum;
             ok = barrier_all<32 * kSoftmaxWarps>(1, ok);
             if (!ok) break;
