@@ -70,6 +70,7 @@ struct Queries {
     float* lse;
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
+    bool whole;                           // blocks are not cut (unless the kernel looks whether to cut them)
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
     float* partial;                       // [2 * grid][R, 512]
     float* partial_lse;                   // [2 * grid][R]
@@ -183,8 +184,16 @@ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f
 // ---------------------------------------------------------------- who works on what
 // The work is a list of tiles: for every sequence, block of its query heads and 128 cached tokens that some row of the block sees one (at least one
 // per block, which writes the zeros of rows that see nothing).  A CTA takes an equal, contiguous share of the list, whatever the lengths are; a block's
-// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  One warp walks the
+// tiles in one CTA are an item, and a block that is cut leaves partial results which latent_combine_kernel joins.  Where there are no more blocks than CTAs and
+// cutting them would save little, a block is one entry of the list and stays whole.  One warp walks the
 // list and leaves what the others need in shared memory.
+// Whether to cut: an SM's longest block against its equal share of all tiles (0.8 to 1.7 us each), against the ends of more items and the join.
+//   Where no row of pages holds more than kSmallTiles tiles the host decides, by the rows' length, and launches no join for whole blocks.  Heads, sequences x tokens:
+//   16, 1 x 137 9.1 us, cut 11.2; 16, 60 x 384 11.3, 17.4; 16, 140 x 1024 24.4, 29.3; 128, 24 x 1024 21.6, 29.5; beyond the line 16, 1 x 1024 15.5, 13.1.
+//   Elsewhere the kernel looks at the lengths (which takes a kernel of its own: 0.5 us more for those that have no use for it).  Rows of pages 50 times as long:
+//   16, 60 x 384 13.2 us, cut 17.5; 16, 140 x 4096 67, 73; 128, 36 x 2048 39, 43; beyond the line 128, 8 x 768 19.7, 18.0.
+constexpr int kSmallTiles = 8, kSmallSaved = 5, kSaved = 4;
+constexpr int kBlockBits = 8;             // of a word that counts tiles and blocks
 struct Seq {
     int len, queries, first;              // cached tokens, queries, index of the first query
 };
@@ -222,20 +231,24 @@ __device__ __forceinline__ int tiles_before(const Queries& q, const Seq& s, int 
     const int whole = n == blocks ? n - 1 : n;
     return static_cast<int>(ramp(u + whole, shift) - ramp(u, shift)) + (n == blocks ? tiles_of(s.len) : 0);
 }
+// ... of the list of work
+__device__ __forceinline__ int entries_before(const Queries& q, bool whole, const Seq& s, int n, int blocks) { return whole ? n : tiles_before(q, s, n, blocks); }
 
 struct Walk {
+    bool whole;                           // blocks are entries of the list, not their tiles
     Seq s;
     int seq, block, head_block;
     int tile, n, tiles;                   // first tile of the item, how many, how many the whole block has
-    int left;                             // of the CTA's share, behind this item
+    int left;                             // entries of the CTA's share, behind this item
 
     __device__ void settle(const Queries& q) {
         tiles = block_tiles(q, s, block);
-        n = min(tiles - tile, left);
-        left -= n;
+        n = whole ? tiles : min(tiles - tile, left);
+        left -= whole ? 1 : n;
     }
-    // the share starts at tile `offset` of sequence `sq`
-    __device__ __forceinline__ void begin(const Queries& q, int sq, const Seq& x, int offset, int share) {
+    // the share starts at entry `offset` of sequence `sq`
+    __device__ __forceinline__ void begin(const Queries& q, bool whole_blocks, int sq, const Seq& x, int offset, int share) {
+        whole = whole_blocks;
         seq = sq;
         s = x;
         const int blocks = blocks_of(q, s);
@@ -243,12 +256,12 @@ struct Walk {
 #pragma unroll 1
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (tiles_before(q, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
+            if (entries_before(q, whole, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
             else hi = mid;
         }
-        offset -= tiles_before(q, s, lo, blocks) * q.head_blocks;
+        offset -= entries_before(q, whole, s, lo, blocks) * q.head_blocks;
         block = lo;
-        const int t = block_tiles(q, s, lo);
+        const int t = whole ? 1 : block_tiles(q, s, lo);
         head_block = q.head_blocks > 1 ? offset / t : 0;
         tile = offset - head_block * t;
         left = share;
@@ -325,9 +338,9 @@ struct Small {                                                  // shared memory
     uint64_t full[2 * kTileSlots], empty[2 * kTileSlots];
     uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], q_full, o_empty;
     Control ctl;
-    int boxes[kBoxSlots][kTokens / 16];
+    int boxes[kBoxSlots][kTokens / 16 + 1];                     // and whether the tile is the CTA's last
     uint32_t looked_up, taken;                                  // tiles whose boxes are written, have been read
-    int warp_sum[Cfg<R>::kThreads / 32];
+    int2 warp_sum[Cfg<R>::kThreads / 32];
     Walk walk;                                                  // the first item
     Shares shares;
 };
@@ -339,7 +352,7 @@ constexpr int smem_bytes() {
 static_assert(smem_bytes<16>() <= 232448 && smem_bytes<32>() <= 232448, "shared memory of a CTA");
 
 // All threads: this CTA's share of the list, and its first item (sm.walk).
-template <int R, typename Sm>
+template <int R, bool kLooks, typename Sm>
 __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& q, Sm& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool once = c.n_seqs <= Cfg<R>::kThreads;
@@ -352,12 +365,17 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
         for (int s0 = 0; s0 < c.n_seqs; s0 += Cfg<R>::kThreads) {
             const int seq = s0 + static_cast<int>(threadIdx.x);
             Seq x = {0, 0, 0};
-            int mine = 0;
+            int mine = 0, most = 0;                                            // tiles, or tiles and blocks, or blocks; tiles of the longest block
             if (seq < c.n_seqs) {
                 x = load_seq(c, q, seq);
                 const int b = blocks_of(q, x);
-                mine = tiles_before(q, x, b, b) * q.head_blocks;
+                mine = entries_before(q, !kLooks && q.whole, x, b, b) * q.head_blocks;
+                if (kLooks) {
+                    mine = mine << kBlockBits | b * q.head_blocks;
+                    most = b == 0 ? 0 : tiles_of(x.len);
+                }
             }
+            if (kLooks) most = __reduce_max_sync(0xffffffffu, most);
             int run = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -365,22 +383,31 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
                 if (lane >= o) run += u;
             }
             __syncthreads();
-            if (lane == 31) sm.warp_sum[warp] = run;
+            if (lane == 31) sm.warp_sum[warp] = make_int2(run, most);
             __syncthreads();
             int before = at + run - mine;
 #pragma unroll
             for (int w = 0; w < Cfg<R>::kThreads / 32; ++w) {
-                const int v = sm.warp_sum[w];
-                if (w < warp) before += v;
-                at += v;
+                const int2 v = sm.warp_sum[w];
+                if (w < warp) before += v.x;
+                at += v.x;
+                most = max(most, v.y);
             }
             if (pass == 0 && !once) continue;
             if (once) total = at;
+            bool whole = q.whole;
+            if (kLooks) {                                             // (a single round; all blocks fit their bits)
+                constexpr int mask = (1 << kBlockBits) - 1;
+                whole = (most - kSaved) * static_cast<int>(gridDim.x / q.group) <= total >> kBlockBits;
+                total = whole ? total & mask : total >> kBlockBits;
+                before = whole ? before & mask : before >> kBlockBits;
+                mine = whole ? mine & mask : mine >> kBlockBits;
+            }
             const Shares sh = shares_of(total, gridDim.x / q.group);
             const int group = blockIdx.x / q.group, first = sh.first(group), share = sh.size(group);
             if (share > 0 && before <= first && first < before + mine) {
                 Walk w;
-                w.begin(q, seq, x, first - before, share);
+                w.begin(q, whole, seq, x, first - before, share);
                 sm.walk = w;
             }
             if (threadIdx.x == 0) sm.shares = sh;
@@ -450,7 +477,7 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
 // ---------------------------------------------------------------- the kernel
 // Warp 0 loads, warps 1 and 2 issue the MMAs, warp 3 walks the list, the others do the softmax: four of them (one per quarter of the 128 TMEM lanes, a lane a token)
 // for every eight rows.
-template <int R>
+template <int R, bool kLooks>
 __global__ void __launch_bounds__(Cfg<R>::kThreads, 1)
 latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __grid_constant__ CUtensorMap map_rope, const LatentCache c, const Queries q,
                         unsigned int* status) {
@@ -490,7 +517,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         tma_prefetch_desc(&map_rope);
     }
     griddep_wait();
-    find_share<R>(c, q, sm);                 // (its barriers also publish what was set up above)
+    find_share<R, kLooks>(c, q, sm);                 // (its barriers also publish what was set up above)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -509,9 +536,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
         uint32_t tile_count = 0;
         bool ok = true;
-        for (; ok && tile_count < static_cast<uint32_t>(share); ++tile_count) {
+        for (bool last = false; ok && !last; ++tile_count) {
             ok = __all_sync(0xffffffffu, follow(&sm.looked_up, tile_count + 1, ctl, status));
-            const int at = lane < 2 * unit_boxes ? sm.boxes[tile_count & (kBoxSlots - 1)][lane] : -2;
+            const int word = lane <= kTokens / 16 ? sm.boxes[tile_count & (kBoxSlots - 1)][lane] : -2, at = lane < 2 * unit_boxes ? word : -2;
+            last = __shfl_sync(0xffffffffu, word, kTokens / 16) != 0;
             __syncwarp();
             if (lane == 0) *static_cast<volatile uint32_t*>(&sm.taken) = tile_count + 1;
             const uint32_t used = __ballot_sync(0xffffffffu, at > -2), present = __ballot_sync(0xffffffffu, at >= 0);
@@ -578,9 +606,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             for (int t = 0; t < w.n && ok; ++t, ++tile_count) {
                 // the slot where this lane's box begins; absent: -1, behind the sequence's end: -2
                 const int64_t p0 = static_cast<int64_t>(w.tile + t) * kTokens + lane * rows;
-                const int at = lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
+                int at = lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
+                if (lane == kTokens / 16) at = w.left == 0 && t == w.n - 1;
                 if (tile_count >= kAhead) ok = __all_sync(0xffffffffu, follow(&sm.taken, tile_count + 1 - kAhead, ctl, status));
-                if (lane < boxes) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
+                if (lane <= kTokens / 16) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
                 __threadfence_block();
                 __syncwarp();
                 if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
@@ -1070,12 +1099,23 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
 // Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
 int block_rows(int64_t tokens, int heads, int n_seqs) { return (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32; }
 
+enum Cut : int { kCut, kLook, kWhole };
+Cut cut_mode(int64_t tokens, int heads, int n_seqs, int64_t longest, int grid) {
+    if (longest <= kTokens) return kWhole;
+    const int rows = block_rows(tokens, heads, n_seqs);
+    const int64_t blocks = tokens * ((heads + rows - 1) / rows), most = (longest + kTokens - 1) / kTokens;
+    if (blocks > grid) return kCut;
+    if (most <= kSmallTiles && most * (grid - blocks) <= static_cast<int64_t>(kSmallSaved) * grid) return kWhole;
+    // (what the kernel adds up in one round and one word)
+    return n_seqs <= Cfg<16>::kThreads && grid < 1 << kBlockBits && blocks * most < 1 << (31 - kBlockBits) ? kLook : kCut;
+}
+
 size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
 
-template <int R>
-int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool cut, unsigned int* status,
+template <int R, bool kLooks>
+int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, unsigned int* status,
            cudaStream_t stream) {
-    const auto kern = latent_attention_kernel<R>;
+    const auto kern = latent_attention_kernel<R, kLooks>;
     static std::atomic<uint64_t> prepared{0};                                  // devices
     int device = 0;
     DSV3_CUDA_TRY(cudaGetDevice(&device));
@@ -1084,7 +1124,7 @@ int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(Cfg<R>::kThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
-    if (cut)
+    if (!q.whole)
         DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / (kTeams * kTeamRows)), dim3(kCombineThreads), 0, stream, q));
     return DSV3_OK;
 }
@@ -1097,7 +1137,7 @@ using namespace dsv3;
 extern "C" {
 
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest) {
-    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || longest <= kTokens) return 0;      // (a block of one tile is never cut)
+    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || cut_mode(tokens, heads, n_seqs, longest, num_sms()) == kWhole) return 0;
     return partial_bytes(block_rows(tokens, heads, n_seqs), num_sms());
 }
 
@@ -1137,7 +1177,8 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
                        static_cast<long long>(longest));
         return DSV3_ERR_UNSUPPORTED;
     }
-    const bool cut = longest > kTokens;
+    const Cut mode = cut_mode(tokens, heads, c.n_seqs, longest, grid);
+    const bool cut = mode != kWhole;
     if (cut && (!workspace || workspace_bytes < partial_bytes(rows, grid) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
         set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, grid));
         return DSV3_ERR_WORKSPACE;
@@ -1161,8 +1202,9 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       head_blocks / group, shift, group, partial, partial_lse, list};
-    return rows == 16 ? launch<16>(c, q, map_latent, map_rope, grid / group * group, cut, status, st) : launch<32>(c, q, map_latent, map_rope, grid / group * group, cut, status, st);
+                       head_blocks / group, shift, mode == kWhole, group, partial, partial_lse, list};
+    const auto go = rows == 16 ? (mode == kLook ? launch<16, true> : launch<16, false>) : mode == kLook ? launch<32, true> : launch<32, false>;
+    return go(c, q, map_latent, map_rope, grid / group * group, status, st);
 }
 
 }  // extern "C"

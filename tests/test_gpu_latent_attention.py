@@ -250,6 +250,27 @@ def test_more_sequences_than_threads(heads, drafts):
     _compare(_queries(g, sum(counts), heads), cache, table, lens, counts)
 
 
+@pytest.mark.parametrize("lens, heads, drafts", [([1100] * 140, 16, 1), ([1300] + [200] * 120, 8, 1), ([700, 650, 1100] * 12, 128, 1), ([620] * 9, 16, 15), ([4000, 3999], 16, 70)])
+def test_blocks_left_whole_and_blocks_cut(lens, heads, drafts):
+    """About as many blocks as SMs, equal and not, and far more: cut among CTAs or one to each, by what their lengths say."""
+    g, cache, table = _setup(23 + heads, lens, 64)
+    q = _queries(g, drafts * len(lens), heads)
+    _compare(q, cache, table, lens, [drafts] * len(lens))
+
+
+def test_a_wide_table_is_the_narrow_one():
+    """Short sequences in a table for 40 times their length: whole blocks either way, and the same bits."""
+    d = U.dsv3()
+    lens = [300, 20, 129, 384]
+    g, cache, table = _setup(22, lens, 16)
+    q = _queries(g, 4, 16)
+    wide = torch.full((4, 1000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    narrow = _compare(q, cache, table, lens, [1] * 4)
+    out = d.latent_attention(*q, cache, wide, U.i32(lens), SCALE, return_lse=True)
+    assert torch.equal(out[0], narrow[0]) and torch.equal(out[1], narrow[1])
+
+
 def test_slots_whose_bytes_pass_32_bits():
     """A pool of 8.4 million tokens, of which one sequence uses pages at both ends: offsets in bytes pass 2^32."""
     d = U.dsv3()

@@ -90,10 +90,10 @@ def test_calls_that_are_refused_and_calls_of_nothing():
     assert _attention(lib, _cache(n_seqs=0)) == names.ERR_INVALID_ARGUMENT
     assert _attention(lib, _cache(pages_width=1 << 20), tokens=1 << 14) == names.ERR_UNSUPPORTED         # 2^14 times 2^19 tiles
     assert _attention(lib, _cache(pages_width=1 << 25)) == names.ERR_UNSUPPORTED
-    need = lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 4 * 64)
-    assert need > 0 and lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 128) == 0
+    need = lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 64 * 64)
+    assert need > 0 and lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 128) == 0     # (one tile: nothing to cut)
     for at, size in ((None, need), (1024, need - 1), (1040, need)):
-        assert _attention(lib, _cache(pages_width=4), workspace=at, workspace_bytes=size) == names.ERR_WORKSPACE
+        assert _attention(lib, _cache(pages_width=64), workspace=at, workspace_bytes=size) == names.ERR_WORKSPACE
     assert _attention(lib, _cache(), heads=1025) == names.ERR_UNSUPPORTED
     assert _attention(lib, _cache(), tokens=0) == names.OK
     assert b"heads" in names.lib.dsv3_last_error()
