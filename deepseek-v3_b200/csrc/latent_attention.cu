@@ -87,6 +87,7 @@ struct Cfg {
     // sequence of 131072 tokens (45).
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
+    static constexpr int kItemCost = 2;
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
     static constexpr int kTmemO = 2 * kTmemS;
     static constexpr int kTmemCols = R == 16 ? 256 : 512;
@@ -232,44 +233,51 @@ __device__ __forceinline__ int tiles_before(const Queries& q, const Seq& s, int 
     return static_cast<int>(ramp(u + whole, shift) - ramp(u, shift)) + (n == blocks ? tiles_of(s.len) : 0);
 }
 // ... of the list of work
-__device__ __forceinline__ int entries_before(const Queries& q, bool whole, const Seq& s, int n, int blocks) { return whole ? n : tiles_before(q, s, n, blocks); }
+template <int R>
+__device__ __forceinline__ int entries_before(const Queries& q, bool whole, const Seq& s, int n, int blocks) {
+    return whole ? n : tiles_before(q, s, n, blocks) + n * Cfg<R>::kItemCost;
+}
 
+template <int R>
 struct Walk {
-    bool whole;                           // blocks are entries of the list, not their tiles
+    bool whole, more;                     // blocks are entries of the list, not their tiles; the CTA's share has more of them
     Seq s;
     int seq, block, head_block;
     int tile, n, tiles;                   // first tile of the item, how many, how many the whole block has
-    int left;                             // entries of the CTA's share, behind this item
+    int share, at;                        // entries of the CTA; the first tile's place in the list, from the share's start on
 
     __device__ void settle(const Queries& q) {
         tiles = block_tiles(q, s, block);
-        n = whole ? tiles : min(tiles - tile, left);
-        left -= whole ? 1 : n;
+        tile = max(0, -at);
+        n = min(whole ? 1 : tiles, share - at) - tile;
+        if (whole) tile = 0, n = tiles;
+        more = next_at() < share;
     }
-    // the share starts at entry `offset` of sequence `sq`
-    __device__ __forceinline__ void begin(const Queries& q, bool whole_blocks, int sq, const Seq& x, int offset, int share) {
+    __device__ int next_at() const { return at + (whole ? 1 : tiles + Cfg<R>::kItemCost); }
+    // the share starts at entry `offset` of sequence `sq`.  (No tiles: nothing but what a block takes beside them.)
+    __device__ __forceinline__ void begin(const Queries& q, bool whole_blocks, int sq, const Seq& x, int offset, int entries) {
         whole = whole_blocks;
         seq = sq;
         s = x;
         const int blocks = blocks_of(q, s);
-        int lo = 0, hi = blocks;          // largest block whose tiles begin at or before the offset
+        int lo = 0, hi = blocks;          // largest block whose entries begin at or before the offset
 #pragma unroll 1
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (entries_before(q, whole, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
+            if (entries_before<R>(q, whole, s, mid, blocks) * q.head_blocks <= offset) lo = mid;
             else hi = mid;
         }
-        offset -= entries_before(q, whole, s, lo, blocks) * q.head_blocks;
+        offset -= entries_before<R>(q, whole, s, lo, blocks) * q.head_blocks;
         block = lo;
-        const int t = whole ? 1 : block_tiles(q, s, lo);
+        const int t = whole ? 1 : block_tiles(q, s, lo) + Cfg<R>::kItemCost;
         head_block = q.head_blocks > 1 ? offset / t : 0;
-        tile = offset - head_block * t;
-        left = share;
+        share = entries;
+        at = (whole ? 0 : Cfg<R>::kItemCost) - (offset - head_block * t);
         settle(q);
     }
     __device__ __forceinline__ bool next(const LatentCache& c, const Queries& q) {
-        if (left == 0) return false;
-        tile = 0;
+        if (!more) return false;
+        at = next_at();
         if (++head_block == q.head_blocks) {
             head_block = 0;
             if (++block >= blocks_of(q, s)) {
@@ -302,7 +310,9 @@ __device__ __forceinline__ Shares shares_of(int total, int ctas) {
 }
 
 // Row r of an item's block: query * heads + head, or -1 where it is none.
-__device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int rows, int r, int cta) {
+template <int R>
+__device__ __forceinline__ int place_at(const Queries& q, const Walk<R>& w, int r, int cta) {
+    constexpr int rows = R;
     int token = w.block << q.block_shift, head = (w.head_block + cta % q.group) * rows + r;
     if (q.heads <= rows) {
         if (r >= q.heads << q.block_shift) return -1;
@@ -311,7 +321,8 @@ __device__ __forceinline__ int place_at(const Queries& q, const Walk& w, int row
     }
     return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
 }
-__device__ __forceinline__ int place_of(const Queries& q, const Walk& w, int rows, int r) { return place_at(q, w, rows, r, static_cast<int>(blockIdx.x)); }
+template <int R>
+__device__ __forceinline__ int place_of(const Queries& q, const Walk<R>& w, int r) { return place_at(q, w, r, static_cast<int>(blockIdx.x)); }
 
 // What the other warps need of a step of the walk.
 struct Item {
@@ -341,7 +352,7 @@ struct Small {                                                  // shared memory
     int boxes[kBoxSlots][kTokens / 16 + 1];                     // and whether the tile is the CTA's last
     uint32_t looked_up, taken;                                  // tiles whose boxes are written, have been read
     int2 warp_sum[Cfg<R>::kThreads / 32];
-    Walk walk;                                                  // the first item
+    Walk<R> walk;                                               // the first item
     Shares shares;
 };
 
@@ -369,9 +380,10 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
             if (seq < c.n_seqs) {
                 x = load_seq(c, q, seq);
                 const int b = blocks_of(q, x);
-                mine = entries_before(q, !kLooks && q.whole, x, b, b) * q.head_blocks;
-                if (kLooks) {
-                    mine = mine << kBlockBits | b * q.head_blocks;
+                if (!kLooks) {
+                    mine = entries_before<R>(q, q.whole, x, b, b) * q.head_blocks;
+                } else {
+                    mine = tiles_before(q, x, b, b) * q.head_blocks << kBlockBits | b * q.head_blocks;
                     most = b == 0 ? 0 : tiles_of(x.len);
                 }
             }
@@ -399,14 +411,13 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
             if (kLooks) {                                             // (a single round; all blocks fit their bits)
                 constexpr int mask = (1 << kBlockBits) - 1;
                 whole = (most - kSaved) * static_cast<int>(gridDim.x / q.group) <= total >> kBlockBits;
-                total = whole ? total & mask : total >> kBlockBits;
-                before = whole ? before & mask : before >> kBlockBits;
-                mine = whole ? mine & mask : mine >> kBlockBits;
+                const auto entries = [&](int x) { return whole ? x & mask : (x >> kBlockBits) + (x & mask) * Cfg<R>::kItemCost; };
+                total = entries(total), before = entries(before), mine = entries(mine);
             }
             const Shares sh = shares_of(total, gridDim.x / q.group);
             const int group = blockIdx.x / q.group, first = sh.first(group), share = sh.size(group);
             if (share > 0 && before <= first && first < before + mine) {
-                Walk w;
+                Walk<R> w;
                 w.begin(q, whole, seq, x, first - before, share);
                 sm.walk = w;
             }
@@ -528,7 +539,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     const int first = shares.first(blockIdx.x / q.group), share = shares.size(blockIdx.x / q.group);
     const auto listed = [&](uint32_t item) -> bool { return __all_sync(0xffffffffu, follow(&sm.listed, item + 1, ctl, status)); };
 
-    if (share == 0) {
+    if (share == 0 || sm.walk.n <= 0) {
         // nothing to do
     } else if (warp == 0) {
         // ------------------------------------------------------------ loads.  One lane issues, with coordinates that the warp has in common.
@@ -575,14 +586,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     } else if (warp == 3) {
         // ------------------------------------------------------------ the walk: items and their rows, and pages some tiles ahead of the loads.  (To bring the
         // pages to L2 as well, one to six tiles ahead, only gave HBM more to do: 64 sequences of up to 8192 tokens with 16 heads 56 us without, 58 to 68 with.)
-        Walk w = sm.walk;
+        Walk<R> w = sm.walk;
         const int rows = min(1 << c.page_shift, kUnitTokens), boxes = kTokens / rows;
         uint32_t tile_count = 0, item = 0;
         bool ok = true;
         do {
             // -------- a lane to a row of the block
             const uint32_t at_item = item & (kItemSlots - 1);
-            const int place = lane < R ? place_of(q, w, R, lane) : -1, query = place < 0 ? 0 : place / q.heads, head = place - query * q.heads;
+            const int place = lane < R ? place_of(q, w, lane) : -1, query = place < 0 ? 0 : place / q.heads, head = place - query * q.heads;
             const int64_t word = q.tree && place >= 0 ? q.tree[query] : 0;
             if (item > 0 && place >= 0) {                                      // its query will be read when the item before is done
                 const char* const lat = reinterpret_cast<const char*>(q.latent + query * q.latent_token + head * q.latent_head);
@@ -599,7 +610,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 sm.limit[at_item][lane] = q.tree ? base - 1 : base + query - w.s.first;
                 sm.tree[at_item][lane] = word;
             }
-            if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, w.left == 0};
+            if (lane == 0) sm.item[at_item] = {w.s.len, base, w.tile, w.n, begins, ends, !w.more};
             __threadfence_block();
             __syncwarp();
             if (lane == 0) *static_cast<volatile uint32_t*>(&sm.listed) = item + 1;
@@ -607,7 +618,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 // the slot where this lane's box begins; absent: -1, behind the sequence's end: -2
                 const int64_t p0 = static_cast<int64_t>(w.tile + t) * kTokens + lane * rows;
                 int at = lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
-                if (lane == kTokens / 16) at = w.left == 0 && t == w.n - 1;
+                if (lane == kTokens / 16) at = !w.more && t == w.n - 1;
                 if (tile_count >= kAhead) ok = __all_sync(0xffffffffu, follow(&sm.taken, tile_count + 1 - kAhead, ctl, status));
                 if (lane <= kTokens / 16) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
                 __threadfence_block();
@@ -615,7 +626,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
             }
             if (lane == 0 && !ends) {                                          // (one item of a CTA at most)
-                const int start = first + (share - w.left) - w.n - w.tile;     // of the block's tiles, in the list
+                const int start = first + w.at;                                // of the block's tiles, in the list
                 const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + w.tiles - 1) - begun + 1;
                 if (begins || parts > kFewParts) {
                     q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
@@ -1011,9 +1022,9 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
     griddep_wait();
     const int4 cut = q.cut[2 * blockIdx.x], seq = q.cut[2 * blockIdx.x + 1];
     if (cut.x < 0) return;
-    Walk w;
+    Walk<R> w;
     w.block = cut.y, w.head_block = cut.z;
-    w.s = {seq.x, seq.y, seq.z};
+    w.s = Seq{seq.x, seq.y, seq.z};
     const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
     const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
     const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R; };
@@ -1054,7 +1065,7 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
         }
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
-            const int place = place_at(q, w, R, r0 + j, cta);
+            const int place = place_at(q, w, r0 + j, cta);
             if (place >= 0) store(place, acc[j], top[j], sum[j], nan[j]);
         }
         return;
@@ -1062,7 +1073,7 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
     const int r = cut.w * kBlocks + blockIdx.y;
     static_assert(kFewParts * kBlocks >= R, "a row to each");
     if (r >= R) return;
-    const int place = place_at(q, w, R, r, cta);
+    const int place = place_at(q, w, r, cta);
     if (place < 0) return;                                                     // (the whole thread block)
     float top = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1172,7 +1183,7 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     }
     const int grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
     const int64_t longest = static_cast<int64_t>(c.pages_width) << c.page_shift;
-    if (tokens * ((heads + rows - 1) / rows) > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1)) {   // (the kernel counts tiles in 32 bits)
+    if (tokens * ((heads + rows - 1) / rows) > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1 + Cfg<32>::kItemCost)) {   // (the kernel counts tiles in 32 bits)
         set_last_error("latent_attention: %lld queries of %d heads over up to %lld tokens are too much work for a call", static_cast<long long>(tokens), heads,
                        static_cast<long long>(longest));
         return DSV3_ERR_UNSUPPORTED;
