@@ -1008,14 +1008,20 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     }
 }
 
-// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  Thread blocks to every CTA of the kernel before, a team of 128 threads
-// to kTeamRows rows: where a block of query heads is in few parts, those of the CTA that it begins in join them; where it is in many, those of
-// all CTAs but its last take a row each, and their teams share its parts.  (The last CTA of a block joining its parts, in the kernel before, took longer:
-// 64 sequences of up to 8192 tokens with 16 heads 50.3 us instead of 48.3, one of 131072 with four drafts 70 instead of 50.)
-constexpr int kCombineThreads = 512, kTeams = kCombineThreads / 128, kTeamRows = 2;
-template <int R>
-__global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Queries q) {
-    constexpr int kRows = kTeamRows, kBlocks = R / (kTeams * kRows);
+// The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  Thread blocks to every CTA of the kernel before, of teams of 128
+// threads: where a block of query heads is in few parts, those of the CTA that it begins in join them, a team to a row; where it is in many, those of
+// all CTAs but its last take a row each, and their teams share its parts.
+//   It costs a launch, 1 to 4 us, and reads up to 19 MB that were just written, 4 us.  Where parts are few on average small blocks with a row to a team: 64 sequences of up to
+// 8192 tokens with 16 heads 45.2 us, 512 threads and two rows 46.7; where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
+// thread blocks that have nothing to do).  The last CTA of a block joining its parts, in the kernel before, took 2 us longer for the first and 20 for the second.
+template <bool kMany>
+struct Join {
+    static constexpr int kThreads = kMany ? 512 : 256, kTeams = kThreads / 128, kRows = kMany ? 2 : 1, kMinBlocks = kMany ? 2 : 6, kUnroll = kMany ? 8 : 2;
+};
+template <int R, bool kMany>
+__global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks) latent_combine_kernel(const Queries q) {
+    using J = Join<kMany>;
+    constexpr int kTeams = J::kTeams;
     __shared__ float4 sums[kTeams][128];
     __shared__ float weights[kTeams];
     griddep_launch_dependents();
@@ -1027,7 +1033,16 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
     w.s = Seq{seq.x, seq.y, seq.z};
     const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
     const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
-    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R; };
+    const auto slot = [&](int i, int r) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R + r; };
+    const auto part = [&](int i, int r) { return reinterpret_cast<const float4*>(q.partial + slot(i, r) * kLatent)[at]; };
+    const auto add = [](float4& acc, float f, const float4& v) {
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    };
+    const auto warp_max = [](float v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    };
     const auto store = [&](int place, const float4& acc, float top, float sum, bool nan) {
         const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
         reinterpret_cast<uint2*>(q.out + static_cast<int64_t>(place) * kLatent)[at] =
@@ -1035,64 +1050,52 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
         if (q.lse && at == 0) q.lse[place] = nan ? inv : sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
     };
     if (parts <= kFewParts) {
-        const int r0 = (blockIdx.y * kTeams + team) * kRows;
-        float4 acc[kRows];
-        float top[kRows], sum[kRows];
-        bool nan[kRows];
+        static_assert(kFewParts <= 32, "a lane to a part");
 #pragma unroll
-        for (int j = 0; j < kRows; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), top[j] = -INFINITY, sum[j] = 0.0f, nan[j] = false;
-        // a running maximum again, so that a part's logarithm and result are loaded together, two parts at a time
-        for (int i = 0; i < parts; i += 2) {
-            float f[2][kRows];
-            float4 v[2][kRows];
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int j = 0; j < kRows; ++j) {
-                    f[k][j] = i + k < parts ? q.partial_lse[slot(i + k) + r0 + j] : -INFINITY;
-                    v[k][j] = i + k < parts ? reinterpret_cast<const float4*>(q.partial + (slot(i + k) + r0 + j) * kLatent)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-#pragma unroll
-            for (int j = 0; j < kRows; ++j) {
-                const float m = fmaxf(top[j], fmaxf(f[0][j], f[1][j])), ref = m == -INFINITY ? 0.0f : m;
-                const float old = ex2(top[j] - ref), a = ex2(f[0][j] - ref), b = ex2(f[1][j] - ref);
-                nan[j] = nan[j] || isnan(f[0][j]) || isnan(f[1][j]);
-                top[j] = m;
-                sum[j] = fmaf(sum[j], old, a + b);
-                acc[j].x = fmaf(acc[j].x, old, fmaf(a, v[0][j].x, b * v[1][j].x)), acc[j].y = fmaf(acc[j].y, old, fmaf(a, v[0][j].y, b * v[1][j].y));
-                acc[j].z = fmaf(acc[j].z, old, fmaf(a, v[0][j].z, b * v[1][j].z)), acc[j].w = fmaf(acc[j].w, old, fmaf(a, v[0][j].w, b * v[1][j].w));
+        for (int j = 0; j < J::kRows; ++j) {
+            const int r = (static_cast<int>(blockIdx.y) * J::kRows + j) * kTeams + team;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 v = part(0, r), next = part(1, r);                          // (there are two at least)
+            const float mine = lane < parts ? q.partial_lse[slot(lane, r)] : -INFINITY;
+            const bool nan = __any_sync(0xffffffffu, isnan(mine));
+            const float top = warp_max(mine), f = ex2(mine - (top == -INFINITY ? 0.0f : top));
+            float sum = 0.0f;
+#pragma unroll 1
+            for (int i = 0;; ++i) {
+                const float a = __shfl_sync(0xffffffffu, f, i);
+                sum += a;
+                add(acc, a, v);
+                if (i == parts - 1) break;
+                v = next;
+                if (i < parts - 2) next = part(i + 2, r);
             }
-        }
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-            const int place = place_at(q, w, r0 + j, cta);
-            if (place >= 0) store(place, acc[j], top[j], sum[j], nan[j]);
+            const int place = place_at(q, w, r, cta);
+            if (place >= 0) store(place, acc, top, sum, nan);
         }
         return;
     }
-    const int r = cut.w * kBlocks + blockIdx.y;
-    static_assert(kFewParts * kBlocks >= R, "a row to each");
-    if (r >= R) return;
+    const int r = cut.w + static_cast<int>(blockIdx.y) * (parts - 1);
+    static_assert(kFewParts * (R / (kTeams * J::kRows)) >= R, "a row to each");
+    if (cut.w == parts - 1 || r >= R) return;
     const int place = place_at(q, w, r, cta);
     if (place < 0) return;                                                     // (the whole thread block)
     float top = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     bool nan = false;
     for (int i = lane; i < parts; i += 32) {
-        const float v = q.partial_lse[slot(i) + r];
+        const float v = q.partial_lse[slot(i, r)];
         nan = nan || isnan(v);
         top = fmaxf(top, v);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = warp_max(top);
     nan = __any_sync(0xffffffffu, nan);
     const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
+#pragma unroll J::kUnroll
     for (int i = team; i < parts; i += kTeams) {
-        const float f = ex2(q.partial_lse[slot(i) + r] - ref);
-        const float4 v = reinterpret_cast<const float4*>(q.partial + (slot(i) + r) * kLatent)[at];
+        const float f = ex2(q.partial_lse[slot(i, r)] - ref);
+        const float4 v = part(i, r);
         sum += f;
-        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+        add(acc, f, v);
     }
     sums[team][at] = acc;
     if (at == 0) weights[team] = sum;
@@ -1100,8 +1103,7 @@ __global__ void __launch_bounds__(kCombineThreads) latent_combine_kernel(const Q
     if (team != 0) return;
 #pragma unroll
     for (int i = 1; i < kTeams; ++i) {
-        const float4 v = sums[i][at];
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        add(acc, 1.0f, sums[i][at]);
         sum += weights[i];
     }
     store(place, acc, top, sum, nan);
@@ -1124,7 +1126,7 @@ Cut cut_mode(int64_t tokens, int heads, int n_seqs, int64_t longest, int grid) {
 size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
 
 template <int R, bool kLooks>
-int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, unsigned int* status,
+int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool many, unsigned int* status,
            cudaStream_t stream) {
     const auto kern = latent_attention_kernel<R, kLooks>;
     static std::atomic<uint64_t> prepared{0};                                  // devices
@@ -1135,8 +1137,10 @@ int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(Cfg<R>::kThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    const auto join = [&](auto kern, int threads, int rows) { return launch_dependent(kern, dim3(grid, R / rows), dim3(threads), 0, stream, q); };
     if (!q.whole)
-        DSV3_CUDA_TRY(launch_dependent(latent_combine_kernel<R>, dim3(grid, R / (kTeams * kTeamRows)), dim3(kCombineThreads), 0, stream, q));
+        DSV3_CUDA_TRY(many ? join(latent_combine_kernel<R, true>, Join<true>::kThreads, Join<true>::kTeams * Join<true>::kRows)
+                           : join(latent_combine_kernel<R, false>, Join<false>::kThreads, Join<false>::kTeams * Join<false>::kRows));
     return DSV3_OK;
 }
 
@@ -1215,7 +1219,8 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
                        head_blocks / group, shift, mode == kWhole, group, partial, partial_lse, list};
     const auto go = rows == 16 ? (mode == kLook ? launch<16, true> : launch<16, false>) : mode == kLook ? launch<32, true> : launch<32, false>;
-    return go(c, q, map_latent, map_rope, grid / group * group, status, st);
+    const int64_t blocks = (tokens * heads + rows - 1) / rows;
+    return go(c, q, map_latent, map_rope, grid / group * group, 2 * kFewParts * blocks <= grid, status, st);
 }
 
 }  // extern "C"
