@@ -21,10 +21,11 @@
 //
 // What bounds it (B200; a call and its join):
 //   16 rows (a decoding sequence on one rank of eight): HBM.  A tile is 82 KB and 148 CTAs read 6.3 TB/s while they go; 64 sequences of up to 8192 tokens, 196 MB,
-//   take 47 us, of which 28 are that.  The rest is a start (8 us: the work list, the queries and the first tile come from memory one after another), an end (1 us) and the join.
+//   take 44 us, of which 28 are that.  The rest is a start (6 us: the work list, then the pages and the queries, then the first tile come from memory one after
+//   another, and the first tiles of all SMs at once), the ends of items (1 us each) and the join.
 //   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3100: the
 //   products of a tile wait for its weights, those for its scores, and two tiles are all that fits, so that one's softmax hides only half of the other's products.
-//   128 heads of 32 sequences of 8192 tokens 110 us, a chunk of 515 tokens 109 (44 to 45 at the rate of library bf16 products).
+//   128 heads of 32 sequences of 8192 tokens 109 us, a chunk of 515 tokens 107 (44 to 45 at the rate of library bf16 products).
 #include <cuda.h>
 
 #include <atomic>
@@ -87,6 +88,8 @@ struct Cfg {
     // sequence of 131072 tokens (45).
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
+    // What a block takes beside its tiles, in tiles, when work is shared out: its queries' way to shared memory, its result's way out (2.2 and 3 us, with 16 and 32 rows).
+    // 24 trees of 13 drafts 64.6 us, with 0 72.6, with 1 66.9, with 3 65.3; 64 sequences of up to 8192 tokens with 16 heads 46.3, 47.8, 47.0, 46.7.
     static constexpr int kItemCost = 2;
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
     static constexpr int kTmemO = 2 * kTmemS;
@@ -585,12 +588,32 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[2 * (t & 1) + h]), (t >> 1) & 1, ctl, status, 1, t));
     } else if (warp == 3) {
         // ------------------------------------------------------------ the walk: items and their rows, and pages some tiles ahead of the loads.  (To bring the
-        // pages to L2 as well, one to six tiles ahead, only gave HBM more to do: 64 sequences of up to 8192 tokens with 16 heads 56 us without, 58 to 68 with.)
+        // pages to L2 as well, one to six tiles ahead, only gave HBM more to do: 4 to 20 % longer for 64 sequences of up to 8192 tokens with 16 heads.)
         Walk<R> w = sm.walk;
         const int rows = min(1 << c.page_shift, kUnitTokens), boxes = kTokens / rows;
         uint32_t tile_count = 0, item = 0;
         bool ok = true;
+        // the slot where this lane's box of a tile begins; absent: -1, behind the sequence's end: -2
+        const auto look_up = [&](int t) -> int {
+            const int64_t p0 = static_cast<int64_t>(w.tile + t) * kTokens + lane * rows;
+            return lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
+        };
+        const auto publish = [&](int t, int at) {
+            if (lane == kTokens / 16) at = !w.more && t == w.n - 1;
+            if (tile_count >= kAhead) ok = __all_sync(0xffffffffu, follow(&sm.taken, tile_count + 1 - kAhead, ctl, status));
+            if (lane <= kTokens / 16) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
+            __threadfence_block();
+            __syncwarp();
+            if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
+            ++tile_count;
+        };
         do {
+            int t = 0, ahead = look_up(0);
+            if (item == 0) {                                                   // (the first loads wait for this, and for nothing else)
+                publish(0, ahead);
+                t = 1;
+                if (w.n > 1) ahead = look_up(1);
+            }
             // -------- a lane to a row of the block
             const uint32_t at_item = item & (kItemSlots - 1);
             const int place = lane < R ? place_of(q, w, lane) : -1, query = place < 0 ? 0 : place / q.heads, head = place - query * q.heads;
@@ -614,16 +637,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             __threadfence_block();
             __syncwarp();
             if (lane == 0) *static_cast<volatile uint32_t*>(&sm.listed) = item + 1;
-            for (int t = 0; t < w.n && ok; ++t, ++tile_count) {
-                // the slot where this lane's box begins; absent: -1, behind the sequence's end: -2
-                const int64_t p0 = static_cast<int64_t>(w.tile + t) * kTokens + lane * rows;
-                int at = lane < boxes && p0 < w.s.len ? slot_of(c, w.seq, static_cast<uint32_t>(p0)) : -2;
-                if (lane == kTokens / 16) at = !w.more && t == w.n - 1;
-                if (tile_count >= kAhead) ok = __all_sync(0xffffffffu, follow(&sm.taken, tile_count + 1 - kAhead, ctl, status));
-                if (lane <= kTokens / 16) sm.boxes[tile_count & (kBoxSlots - 1)][lane] = at;
-                __threadfence_block();
-                __syncwarp();
-                if (lane == 0) *static_cast<volatile uint32_t*>(&sm.looked_up) = tile_count + 1;
+            for (; t < w.n && ok; ++t) {
+                const int at = ahead;
+                if (t + 1 < w.n) ahead = look_up(t + 1);
+                publish(t, at);
             }
             if (lane == 0 && !ends) {                                          // (one item of a CTA at most)
                 const int start = first + w.at;                                // of the block's tiles, in the list
@@ -720,8 +737,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         constexpr int kMine = R / kSoftmaxWarps;
         uint4 qv[kMine][2];
         uint32_t qr[kMine];
-        const auto fetch = [&](uint32_t at_item) {
-            const int place = lane < kMine ? sm.place[at_item][sw + lane * kSoftmaxWarps] : -1;
+        const auto fetch = [&](int place) {                                    // of the lane's row, of the first kMine lanes
             const int row = place < 0 ? 0 : place / q.heads, head = place - row * q.heads;
             const int64_t lat = row * q.latent_token + head * q.latent_head, rot = row * q.rope_token + head * q.rope_head;
 #pragma unroll
@@ -776,11 +792,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.q_full));
         };
+        // (the first rows are worked out here, not waited for: with the first page looked up before the walk's list is written 7.8 us instead of 8.3 for one tile)
+        fetch(lane < kMine ? place_of(q, sm.walk, sw + lane * kSoftmaxWarps) : -1);
+        stage(0);
         ok = listed(0);
-        if (ok) {
-            fetch(0);
-            stage(0);
-        }
         for (uint32_t item = 0;; ++item) {
             const uint32_t par = item & 1, at_item = item & (kItemSlots - 1);
             ok = barrier_all<32 * kSoftmaxWarps>(1, ok);                       // the factors of all rows; the item before is done with
@@ -920,7 +935,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             // -------- the item's result; the next item's queries on their way meanwhile
             if (!w.last) {
                 ok = ok && listed(item + 1);
-                if (ok) fetch((item + 1) & (kItemSlots - 1));
+                if (ok) fetch(lane < kMine ? sm.place[(item + 1) & (kItemSlots - 1)][sw + lane * kSoftmaxWarps] : -1);
             }
             float of_row[N];
 #pragma unroll
@@ -1009,14 +1024,14 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 }
 
 // The results of blocks that several CTAs worked on: out = sum_p 2^(lse_p - lse) out_p.  Thread blocks to every CTA of the kernel before, of teams of 128
-// threads: where a block of query heads is in few parts, those of the CTA that it begins in join them, a team to a row; where it is in many, those of
+// threads: where a block of query heads is in few parts, those of the CTA that it begins in join them, a team to a row, with kAtOnce parts on their way; where it is in many, those of
 // all CTAs but its last take a row each, and their teams share its parts.
 //   It costs a launch, 1 to 4 us, and reads up to 19 MB that were just written, 4 us.  Where parts are few on average small blocks with a row to a team: 64 sequences of up to
 // 8192 tokens with 16 heads 45.2 us, 512 threads and two rows 46.7; where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
 // thread blocks that have nothing to do).  The last CTA of a block joining its parts, in the kernel before, took 2 us longer for the first and 20 for the second.
 template <bool kMany>
 struct Join {
-    static constexpr int kThreads = kMany ? 512 : 256, kTeams = kThreads / 128, kRows = kMany ? 2 : 1, kMinBlocks = kMany ? 2 : 6, kUnroll = kMany ? 8 : 2;
+    static constexpr int kThreads = kMany ? 512 : 256, kTeams = kThreads / 128, kRows = kMany ? 2 : 1, kMinBlocks = kMany ? 2 : 6, kUnroll = kMany ? 8 : 2, kAtOnce = kMany ? 8 : 2;
 };
 template <int R, bool kMany>
 __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks) latent_combine_kernel(const Queries q) {
@@ -1055,19 +1070,24 @@ __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks
         for (int j = 0; j < J::kRows; ++j) {
             const int r = (static_cast<int>(blockIdx.y) * J::kRows + j) * kTeams + team;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float4 v = part(0, r), next = part(1, r);                          // (there are two at least)
+            float4 v[J::kAtOnce];
+#pragma unroll
+            for (int k = 0; k < J::kAtOnce; ++k)
+                if (k < 2 || k < parts) v[k] = part(k, r);                     // (there are two at least)
             const float mine = lane < parts ? q.partial_lse[slot(lane, r)] : -INFINITY;
             const bool nan = __any_sync(0xffffffffu, isnan(mine));
             const float top = warp_max(mine), f = ex2(mine - (top == -INFINITY ? 0.0f : top));
             float sum = 0.0f;
 #pragma unroll 1
-            for (int i = 0;; ++i) {
-                const float a = __shfl_sync(0xffffffffu, f, i);
-                sum += a;
-                add(acc, a, v);
-                if (i == parts - 1) break;
-                v = next;
-                if (i < parts - 2) next = part(i + 2, r);
+            for (int i = 0; i < parts; i += J::kAtOnce) {
+#pragma unroll
+                for (int k = 0; k < J::kAtOnce; ++k) {
+                    if (i + k >= parts) break;
+                    const float a = __shfl_sync(0xffffffffu, f, i + k);
+                    sum += a;
+                    add(acc, a, v[k]);
+                    if (i + k + J::kAtOnce < parts) v[k] = part(i + k + J::kAtOnce, r);
+                }
             }
             const int place = place_at(q, w, r, cta);
             if (place >= 0) store(place, acc, top, sum, nan);
