@@ -524,6 +524,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         mbar_fence_init();
         ctl->abort_flag = 0;
         sm.looked_up = sm.taken = sm.listed = sm.finished = 0;
+        sm.walk.n = 0;
     }
     if (warp == 1) tc_alloc(smem_u32(&ctl->tmem_base), C::kTmemCols);
     if (warp == 0) {
@@ -1194,6 +1195,10 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     if (c.n_seqs == 0 || (!cu_seqlens_q && tokens % c.n_seqs != 0)) {
         set_last_error("latent_attention: %lld queries do not divide among %d sequences", static_cast<long long>(tokens), c.n_seqs);
         return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    if (tree_mask && !cu_seqlens_q && tokens / c.n_seqs > 64) {
+        set_last_error("latent_attention: %lld drafted tokens to a sequence, a tree's masks name 64", static_cast<long long>(tokens / c.n_seqs));
+        return DSV3_ERR_UNSUPPORTED;
     }
     const int64_t strides = q_latent_token_stride | q_latent_head_stride | q_rope_token_stride | q_rope_head_stride;
     if (strides % 8 != 0 || (reinterpret_cast<uintptr_t>(q_latent) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(out)) % 16 != 0 ||

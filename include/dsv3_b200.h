@@ -383,7 +383,7 @@ int dsv3_latent_keep(const dsv3_latent_cache_t* cache, const int32_t* first, con
  *              queries' own tokens are still the last ones of their sequence; a query sees all before them, and of them those whose bit is
  *              set (bit j: the j-th; from the 64th on none is seen).
  *   out      : bf16 [tokens, heads, 512], lse : fp32 [tokens, heads].  A query that sees nothing: zeros, and -inf.
- * Refused: a pool without pages; query blocks times tiles of 128 positions, with every row of pages full, that reach 2^31.
+ * Refused: a pool without pages; a tree of more than 64 queries to a sequence where that is seen (cu_seqlens_q null); query blocks times tiles of 128 positions, with every row of pages full, that reach 2^31.
  * workspace: dsv3_latent_attention_workspace_bytes() bytes (longest: pages_width * page_size), 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
  */
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest);

@@ -34,8 +34,8 @@ def _write(lib, cache, kv=16, stride=576, tokens=1, n_positions=8, weight=16, fr
     return lib.dsv3_latent_write(cache, kv, stride, weight, 0, 1e-6, freqs, n_positions, 16, 16, tokens, None)
 
 
-def _attention(lib, cache, q=16, stride=512, tokens=2, heads=1, out=16, cu=None, workspace=None, workspace_bytes=0):
-    return lib.dsv3_latent_attention(cache, q, stride, stride, q, 64, 64, tokens, heads, 16, cu, None, 1.0, out, None, workspace, workspace_bytes, None)
+def _attention(lib, cache, q=16, stride=512, tokens=2, heads=1, out=16, cu=None, workspace=None, workspace_bytes=0, tree=None):
+    return lib.dsv3_latent_attention(cache, q, stride, stride, q, 64, 64, tokens, heads, 16, cu, tree, 1.0, out, None, workspace, workspace_bytes, None)
 
 
 @pytest.mark.parametrize("over, status", [
@@ -88,6 +88,8 @@ def test_calls_that_are_refused_and_calls_of_nothing():
     assert _attention(lib, _cache(scale=4100)) == names.ERR_UNSUPPORTED
     assert _attention(lib, _cache(n_pages=0)) == names.ERR_INVALID_ARGUMENT
     assert _attention(lib, _cache(n_seqs=0)) == names.ERR_INVALID_ARGUMENT
+    assert _attention(lib, _cache(), tokens=130, tree=16) == names.ERR_UNSUPPORTED                        # 65 to a sequence
+    assert b"64" in names.lib.dsv3_last_error()
     assert _attention(lib, _cache(pages_width=1 << 20), tokens=1 << 14) == names.ERR_UNSUPPORTED         # 2^14 times 2^19 tiles
     assert _attention(lib, _cache(pages_width=1 << 25)) == names.ERR_UNSUPPORTED
     need = lib.dsv3_latent_attention_workspace_bytes(2, 1, 2, 64 * 64)
