@@ -71,6 +71,9 @@ struct Queries {
     float* lse;
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
+    // 2^16 / heads + 1, for a block of several tokens, and 2^32 / CTAs with a share of their own + 1: a division is some forty instructions that come from memory before
+    // they run, once each in a kernel of this length (one tile 7.9 us with them, 7.5 without)
+    uint32_t per_head, per_cta;
     bool whole;                           // blocks are not cut (unless the kernel looks whether to cut them)
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
     float* partial;                       // [2 * grid][R, 512]
@@ -306,26 +309,28 @@ struct Shares {
         return tile < large ? tile / (size_less + 1) : more + (tile - large) / size_less;
     }
 };
-__device__ __forceinline__ Shares shares_of(int total, int ctas) {
+__device__ __forceinline__ Shares shares_of(int total, int ctas, uint32_t per_cta) {
     if (total < ctas) return {1, 0, total};
-    const int each = static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas);
+    int each = static_cast<int>(__umulhi(static_cast<uint32_t>(total), per_cta));   // total / ctas, or one more
+    if (static_cast<uint32_t>(each) * static_cast<uint32_t>(ctas) > static_cast<uint32_t>(total)) --each;
     return {each, total - each * ctas, ctas};
 }
 
-// Row r of an item's block: query * heads + head, or -1 where it is none.
+// Row r of an item's block, in the CTA that is the `member`-th of those side by side; query -1 where it is none.
+struct Row {
+    int query, head;
+};
 template <int R>
-__device__ __forceinline__ int place_at(const Queries& q, const Walk<R>& w, int r, int cta) {
-    constexpr int rows = R;
-    int token = w.block << q.block_shift, head = (w.head_block + cta % q.group) * rows + r;
-    if (q.heads <= rows) {
-        if (r >= q.heads << q.block_shift) return -1;
-        token += r / q.heads;
-        head = r % q.heads;
+__device__ __forceinline__ Row row_of(const Queries& q, const Walk<R>& w, int r, int member) {
+    int token = w.block << q.block_shift, head = (w.head_block + member) * R + r;
+    if (q.heads <= R) {
+        if (r >= q.heads << q.block_shift) return {-1, 0};
+        const int t = static_cast<int>(r * q.per_head >> 16);                  // r / heads, below 32
+        token += t;
+        head = r - t * q.heads;
     }
-    return head < q.heads && token < w.s.queries ? (w.s.first + token) * q.heads + head : -1;
+    return {head < q.heads && token < w.s.queries ? w.s.first + token : -1, head};
 }
-template <int R>
-__device__ __forceinline__ int place_of(const Queries& q, const Walk<R>& w, int r) { return place_at(q, w, r, static_cast<int>(blockIdx.x)); }
 
 // What the other warps need of a step of the walk.
 struct Item {
@@ -343,6 +348,7 @@ struct Small {                                                  // shared memory
     int64_t tree[kItemSlots][R];
     int limit[kItemSlots][R];                                   // last position that a row sees (a tree: of those before the queries)
     int place[kItemSlots][R];                                   // query * heads + head, -1 for a row that is none
+    int query[kItemSlots][R];
     Item item[kItemSlots];
     uint32_t listed, finished;                                  // items that are written down, whose results have been read
     float top[2][Cfg<R>::kParts][4][Cfg<R>::kRows];             // [tile parity][part of the rows][warp][row]
@@ -413,12 +419,12 @@ __device__ __forceinline__ void find_share(const LatentCache& c, const Queries& 
             bool whole = q.whole;
             if (kLooks) {                                             // (a single round; all blocks fit their bits)
                 constexpr int mask = (1 << kBlockBits) - 1;
-                whole = (most - kSaved) * static_cast<int>(gridDim.x / q.group) <= total >> kBlockBits;
+                whole = (most - kSaved) * static_cast<int>(gridDim.y) <= total >> kBlockBits;
                 const auto entries = [&](int x) { return whole ? x & mask : (x >> kBlockBits) + (x & mask) * Cfg<R>::kItemCost; };
                 total = entries(total), before = entries(before), mine = entries(mine);
             }
-            const Shares sh = shares_of(total, gridDim.x / q.group);
-            const int group = blockIdx.x / q.group, first = sh.first(group), share = sh.size(group);
+            const Shares sh = shares_of(total, gridDim.y, q.per_cta);
+            const int first = sh.first(blockIdx.y), share = sh.size(blockIdx.y);
             if (share > 0 && before <= first && first < before + mine) {
                 Walk<R> w;
                 w.begin(q, whole, seq, x, first - before, share);
@@ -481,7 +487,7 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
                 t0 = now;
             } else if (now - t0 > limit_ns) {
                 ctl->abort_flag = 1;
-                if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.x;
+                if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.y * gridDim.x + blockIdx.x;
                 return false;
             }
         }
@@ -537,10 +543,11 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
-    if (threadIdx.x == 32 * 3 && q.cut) q.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 32 * 3 && q.cut) q.cut[2 * (blockIdx.y * gridDim.x + blockIdx.x)] = make_int4(-1, 0, 0, 0);
 
+    const int cta = static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x), member = static_cast<int>(blockIdx.x);    // (CTAs side by side have one share)
     const Shares shares = sm.shares;
-    const int first = shares.first(blockIdx.x / q.group), share = shares.size(blockIdx.x / q.group);
+    const int first = shares.first(blockIdx.y), share = shares.size(blockIdx.y);
     const auto listed = [&](uint32_t item) -> bool { return __all_sync(0xffffffffu, follow(&sm.listed, item + 1, ctl, status)); };
 
     if (share == 0 || sm.walk.n <= 0) {
@@ -617,7 +624,8 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             }
             // -------- a lane to a row of the block
             const uint32_t at_item = item & (kItemSlots - 1);
-            const int place = lane < R ? place_of(q, w, lane) : -1, query = place < 0 ? 0 : place / q.heads, head = place - query * q.heads;
+            const Row row = lane < R ? row_of(q, w, lane, member) : Row{-1, 0};
+            const int query = max(row.query, 0), head = row.head, place = row.query < 0 ? -1 : query * q.heads + head;
             const int64_t word = q.tree && place >= 0 ? q.tree[query] : 0;
             if (item > 0 && place >= 0) {                                      // its query will be read when the item before is done
                 const char* const lat = reinterpret_cast<const char*>(q.latent + query * q.latent_token + head * q.latent_head);
@@ -631,6 +639,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             const bool begins = w.tile == 0, ends = w.tile + w.n == w.tiles;
             if (lane < R) {
                 sm.place[at_item][lane] = place;
+                sm.query[at_item][lane] = query;
                 sm.limit[at_item][lane] = q.tree ? base - 1 : base + query - w.s.first;
                 sm.tree[at_item][lane] = word;
             }
@@ -645,10 +654,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             }
             if (lane == 0 && !ends) {                                          // (one item of a CTA at most)
                 const int start = first + w.at;                                // of the block's tiles, in the list
-                const int begun = begins ? static_cast<int>(blockIdx.x) / q.group : shares.owner(start), parts = shares.owner(start + w.tiles - 1) - begun + 1;
+                const int begun = begins ? static_cast<int>(blockIdx.y) : shares.owner(start), parts = shares.owner(start + w.tiles - 1) - begun + 1;
                 if (begins || parts > kFewParts) {
-                    q.cut[2 * blockIdx.x] = make_int4(parts, w.block, w.head_block, static_cast<int>(blockIdx.x) / q.group - begun);
-                    q.cut[2 * blockIdx.x + 1] = make_int4(w.s.len, w.s.queries, w.s.first, 0);
+                    q.cut[2 * cta] = make_int4(parts, w.block, w.head_block, static_cast<int>(blockIdx.y) - begun);
+                    q.cut[2 * cta + 1] = make_int4(member, w.s.queries, w.s.first, 0);
                 }
             }
             __syncwarp();
@@ -738,16 +747,16 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         constexpr int kMine = R / kSoftmaxWarps;
         uint4 qv[kMine][2];
         uint32_t qr[kMine];
-        const auto fetch = [&](int place) {                                    // of the lane's row, of the first kMine lanes
-            const int row = place < 0 ? 0 : place / q.heads, head = place - row * q.heads;
-            const int64_t lat = row * q.latent_token + head * q.latent_head, rot = row * q.rope_token + head * q.rope_head;
+        const auto fetch = [&](const Row& row) {                               // of the first kMine lanes
+            const int query = max(row.query, 0);
+            const int64_t lat = query * q.latent_token + row.head * q.latent_head, rot = query * q.rope_token + row.head * q.rope_head;
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
                 qv[j][0] = qv[j][1] = make_uint4(0, 0, 0, 0);
                 qr[j] = 0;
                 const uint4* src = reinterpret_cast<const uint4*>(q.latent + __shfl_sync(0xffffffffu, lat, j));
                 const uint32_t* from = reinterpret_cast<const uint32_t*>(q.rope + __shfl_sync(0xffffffffu, rot, j));
-                if (__shfl_sync(0xffffffffu, place, j) >= 0) {
+                if (__shfl_sync(0xffffffffu, row.query, j) >= 0) {
                     qv[j][0] = src[lane * 2], qv[j][1] = src[lane * 2 + 1];
                     qr[j] = from[lane];
                 }
@@ -794,7 +803,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             if (lane == 0) mbar_arrive(bar(sm.q_full));
         };
         // (the first rows are worked out here, not waited for: with the first page looked up before the walk's list is written 7.8 us instead of 8.3 for one tile)
-        fetch(lane < kMine ? place_of(q, sm.walk, sw + lane * kSoftmaxWarps) : -1);
+        fetch(lane < kMine ? row_of(q, sm.walk, sw + lane * kSoftmaxWarps, member) : Row{-1, 0});
         stage(0);
         ok = listed(0);
         for (uint32_t item = 0;; ++item) {
@@ -936,7 +945,13 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             // -------- the item's result; the next item's queries on their way meanwhile
             if (!w.last) {
                 ok = ok && listed(item + 1);
-                if (ok) fetch(lane < kMine ? sm.place[(item + 1) & (kItemSlots - 1)][sw + lane * kSoftmaxWarps] : -1);
+                Row row = {-1, 0};
+                if (ok && lane < kMine) {
+                    const uint32_t next = (item + 1) & (kItemSlots - 1);
+                    const int r = sw + lane * kSoftmaxWarps, query = sm.query[next][r], place = sm.place[next][r];
+                    if (place >= 0) row = {query, place - query * q.heads};
+                }
+                if (ok) fetch(row);
             }
             float of_row[N];
 #pragma unroll
@@ -950,7 +965,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             broadcast_rows<N>(sm.row[sw], sum == 0.0f ? 0.0f : 1.0f / sum, inv);
             if (!w.last) stage(par ^ 1);                                         // (all scores of this item have been read)
             const bool whole = w.begins && w.ends;
-            const int part = 2 * blockIdx.x + (w.begins ? 1 : 0);
+            const int part = 2 * cta + (w.begins ? 1 : 0);
             const float lse2 = sum == 0.0f ? -INFINITY : m + __log2f(sum);
             if (quarter == 0 && lane % (32 / N) == 0) {
                 const int r = part_of * N + own_row<N>(), to = sm.place[at_item][r];
@@ -1046,7 +1061,7 @@ __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks
     if (cut.x < 0) return;
     Walk<R> w;
     w.block = cut.y, w.head_block = cut.z;
-    w.s = Seq{seq.x, seq.y, seq.z};
+    w.s = Seq{0, seq.y, seq.z};
     const int parts = cut.x, team = threadIdx.x >> 7, lane = threadIdx.x & 31, at = threadIdx.x & 127;
     const int cta = static_cast<int>(blockIdx.x) - cut.w * q.group;            // that the block begins in
     const auto slot = [&](int i, int r) { return static_cast<int64_t>(2 * (cta + i * q.group) + (i == 0 ? 1 : 0)) * R + r; };
@@ -1090,7 +1105,8 @@ __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks
                     if (i + k + J::kAtOnce < parts) v[k] = part(i + k + J::kAtOnce, r);
                 }
             }
-            const int place = place_at(q, w, r, cta);
+            const Row row = row_of(q, w, r, seq.x);
+            const int place = row.query < 0 ? -1 : row.query * q.heads + row.head;
             if (place >= 0) store(place, acc, top, sum, nan);
         }
         return;
@@ -1098,7 +1114,8 @@ __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks
     const int r = cut.w + static_cast<int>(blockIdx.y) * (parts - 1);
     static_assert(kFewParts * (R / (kTeams * J::kRows)) >= R, "a row to each");
     if (cut.w == parts - 1 || r >= R) return;
-    const int place = place_at(q, w, r, cta);
+    const Row row = row_of(q, w, r, seq.x);
+    const int place = row.query < 0 ? -1 : row.query * q.heads + row.head;
     if (place < 0) return;                                                     // (the whole thread block)
     float top = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1157,7 +1174,7 @@ int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const
         DSV3_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<R>()));
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    DSV3_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(Cfg<R>::kThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
+    DSV3_CUDA_TRY(launch_dependent(kern, dim3(q.group, grid / q.group), dim3(Cfg<R>::kThreads), smem_bytes<R>(), stream, map_latent, map_rope, c, q, status));
     const auto join = [&](auto kern, int threads, int rows) { return launch_dependent(kern, dim3(grid, R / rows), dim3(threads), 0, stream, q); };
     if (!q.whole)
         DSV3_CUDA_TRY(many ? join(latent_combine_kernel<R, true>, Join<true>::kThreads, Join<true>::kTeams * Join<true>::kRows)
@@ -1242,7 +1259,7 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       head_blocks / group, shift, mode == kWhole, group, partial, partial_lse, list};
+                       head_blocks / group, shift, 65536u / heads + 1u, 0xFFFFFFFFu / (grid / group) + 1u, mode == kWhole, group, partial, partial_lse, list};
     const auto go = rows == 16 ? (mode == kLook ? launch<16, true> : launch<16, false>) : mode == kLook ? launch<32, true> : launch<32, false>;
     const int64_t blocks = (tokens * heads + rows - 1) / rows;
     return go(c, q, map_latent, map_rope, grid / group * group, 2 * kFewParts * blocks <= grid, status, st);
