@@ -21,11 +21,11 @@
 //
 // What bounds it (B200; a call and its join):
 //   16 rows (a decoding sequence on one rank of eight): HBM.  A tile is 82 KB and 148 CTAs read 6.3 TB/s while they go; 64 sequences of up to 8192 tokens, 196 MB,
-//   take 44 us, of which 28 are that.  The rest is a start (6 us: the work list, then the pages and the queries, then the first tile come from memory one after
+//   take 42 us, of which 28 are that.  The rest is a start (6 us: the work list, then the pages and the queries, then the first tile come from memory one after
 //   another, and the first tiles of all SMs at once), the ends of items (1 us each) and the join.
 //   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3100: the
 //   products of a tile wait for its weights, those for its scores, and two tiles are all that fits, so that one's softmax hides only half of the other's products.
-//   128 heads of 32 sequences of 8192 tokens 109 us, a chunk of 515 tokens 107 (44 to 45 at the rate of library bf16 products).
+//   128 heads of 32 sequences of 8192 tokens 109 us, a chunk of 515 tokens 106 (44 to 45 at the rate of library bf16 products).
 #include <cuda.h>
 
 #include <atomic>
@@ -74,6 +74,7 @@ struct Queries {
     // 2^16 / heads + 1, for a block of several tokens, and 2^32 / CTAs with a share of their own + 1: a division is some forty instructions that come from memory before
     // they run, once each in a kernel of this length (one tile 7.9 us with them, 7.5 without)
     uint32_t per_head, per_cta;
+    bool read_once;                       // a sequence's queries are one block
     bool whole;                           // blocks are not cut (unless the kernel looks whether to cut them)
     int group;                            // CTAs that take the blocks of a token's heads side by side, so that a tile is read from HBM once; or 1
     float* partial;                       // [2 * grid][R, 512]
@@ -132,14 +133,27 @@ __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // All chunks of groups of eight rows from `group` on, to shared memory as [group][chunk][8][128]
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int group, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(dst), "l"(tmap), "r"(0),
-                 "r"(group), "r"(bar)
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int group, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %2, %2, %3}], [%4], %5;" ::"r"(dst),
+                 "l"(tmap), "r"(0), "r"(group), "r"(bar), "l"(policy)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_rope(uint32_t dst, const void* tmap, int row, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(tmap),
+                 "r"(0), "r"(row), "r"(bar), "l"(policy)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
+}
+// How long lines stay in the L2: as others, or as the first to go.  Tiles that are read once go first, so that the next launch finds code, lengths and pages there: 64
+// sequences of up to 8192 tokens with 16 heads 42.0 us instead of 43.9; a chunk of 515 tokens, whose blocks read the same tiles one after another, 108.6 instead of 106.3.
+__device__ __forceinline__ uint64_t l2_policy(bool once) {
+    uint64_t p;
+    if (once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -555,6 +569,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
     } else if (warp == 0) {
         // ------------------------------------------------------------ loads.  One lane issues, with coordinates that the warp has in common.
         const int rows = min(1 << c.page_shift, kUnitTokens), unit_boxes = kUnitTokens / rows;
+        const uint64_t policy = l2_policy(q.read_once);
         const uint32_t outside = c.n_pages << c.page_shift;                    // a row that TMA fills with zeros
         uint32_t tile_count = 0;
         bool ok = true;
@@ -583,8 +598,8 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     const int from = __shfl_sync(0xffffffffu, at, i);
                     const int y = from >= 0 ? from : static_cast<int>(outside);
                     if (elect_one()) {
-                        tma_load_4d(tile_at + i * rows * kLatent, &map_latent, y >> 3, full);
-                        tma_load_2d(tile_at + kLatentBytes + i * rows * 2 * kRope, &map_rope, 0, y, full);
+                        tma_load_4d(tile_at + i * rows * kLatent, &map_latent, y >> 3, full, policy);
+                        tma_load_rope(tile_at + kLatentBytes + i * rows * 2 * kRope, &map_rope, y, full, policy);
                         if (from >= 0) bulk_load(smem_u32(scales + i * rows), c.scale + from, rows * 4, full);
                     }
                     __syncwarp();
@@ -1259,7 +1274,7 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
     const Queries q = {static_cast<const __nv_bfloat16*>(q_latent), static_cast<const __nv_bfloat16*>(q_rope), q_latent_token_stride, q_latent_head_stride,
                        q_rope_token_stride, q_rope_head_stride, static_cast<int>(tokens), heads, seq_lens, cu_seqlens_q,
                        cu_seqlens_q ? 0 : static_cast<int>(tokens / c.n_seqs), tree_mask, softmax_scale, static_cast<__nv_bfloat16*>(out), lse,
-                       head_blocks / group, shift, 65536u / heads + 1u, 0xFFFFFFFFu / (grid / group) + 1u, mode == kWhole, group, partial, partial_lse, list};
+                       head_blocks / group, shift, 65536u / heads + 1u, 0xFFFFFFFFu / (grid / group) + 1u, (tokens + c.n_seqs - 1) / c.n_seqs * heads <= rows, mode == kWhole, group, partial, partial_lse, list};
     const auto go = rows == 16 ? (mode == kLook ? launch<16, true> : launch<16, false>) : mode == kLook ? launch<32, true> : launch<32, false>;
     const int64_t blocks = (tokens * heads + rows - 1) / rows;
     return go(c, q, map_latent, map_rope, grid / group * group, 2 * kFewParts * blocks <= grid, status, st);
