@@ -210,10 +210,10 @@ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f
 // list and leaves what the others need in shared memory.
 // Whether to cut: an SM's longest block against its equal share of all tiles (0.8 to 1.7 us each), against the ends of more items and the join.
 //   Where no row of pages holds more than kSmallTiles tiles the host decides, by the rows' length, and launches no join for whole blocks.  Heads, sequences x tokens:
-//   16, 1 x 137 9.1 us, cut 11.2; 16, 60 x 384 11.3, 17.4; 16, 140 x 1024 24.4, 29.3; 128, 24 x 1024 21.6, 29.5; beyond the line 16, 1 x 1024 15.5, 13.1.
-//   Elsewhere the kernel looks at the lengths (which takes a kernel of its own: 0.5 us more for those that have no use for it).  Rows of pages 50 times as long:
-//   16, 60 x 384 13.2 us, cut 17.5; 16, 140 x 4096 67, 73; 128, 36 x 2048 39, 43; beyond the line 128, 8 x 768 19.7, 18.0.
-constexpr int kSmallTiles = 8, kSmallSaved = 5, kSaved = 4;
+//   16, 1 x 137 8.3 us, cut 11.2; 16, 60 x 384 11.6, 13.7; 16, 140 x 1024 22.5, 26.1; 128, 24 x 1024 21.5, 27.1; beyond the line 16, 1 x 640 11.9, 11.1; 1 x 1024 15.2, 11.5.
+//   Elsewhere the kernel looks at the lengths (which takes a kernel of its own: up to 0.5 us more for those that have no use for it).  Rows of pages longer than that:
+//   16, 140 x 4096 64.5 us, cut 68.4; 128, 36 x 2048 39.6, 42.9; beyond the line 16, 1 x 512 12.1, 11.1; 128, 8 x 768 19.8, 16.5.
+constexpr int kSmallTiles = 8, kSmallSaved = 4, kSaved = 3;
 constexpr int kBlockBits = 8;             // of a word that counts tiles and blocks
 struct Seq {
     int len, queries, first;              // cached tokens, queries, index of the first query
