@@ -25,7 +25,7 @@
 //   another, and the first tiles of all SMs at once), the ends of items (1 us each) and the join.
 //   32 rows: shared memory.  A tile's products and weights read and write about 310 KB of it, 2400 cycles at 128 bytes a cycle, and a tile takes 3100: the
 //   products of a tile wait for its weights, those for its scores, and two tiles are all that fits, so that one's softmax hides only half of the other's products.
-//   128 heads of 32 sequences of 8192 tokens 109 us, a chunk of 515 tokens 106 (44 to 45 at the rate of library bf16 products).
+//   128 heads of 32 sequences of 8192 tokens 109 us (122 at the 1 kW limit), a chunk of 515 tokens 105 (44 to 45 at the rate of library bf16 products).
 #include <cuda.h>
 
 #include <atomic>
