@@ -88,12 +88,12 @@ struct Cfg {
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
     // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  With 32 rows the softmax is part of the chain that a tile waits for: eight warps of 16 rows to a
-    // thread took 15 % longer for 128 sequences of 1024 tokens and 128 heads (75 us now), 9 % for 24 trees of 13 drafts (72), 13 % for one
+    // thread took 15 % longer for 128 sequences of 1024 tokens and 128 heads (74 us now), 9 % for 24 trees of 13 drafts (62), 13 % for one
     // sequence of 131072 tokens (45).
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
     // What a block takes beside its tiles, in tiles, when work is shared out: its queries' way to shared memory, its result's way out (2.2 and 3 us, with 16 and 32 rows).
-    // 24 trees of 13 drafts 64.6 us, with 0 72.6, with 1 66.9, with 3 65.3; 64 sequences of up to 8192 tokens with 16 heads 46.3, 47.8, 47.0, 46.7.
+    // When it was chosen: 24 trees of 13 drafts 64.6 us, with 0 72.6, with 1 66.9, with 3 65.3; 64 sequences of up to 8192 tokens with 16 heads 46.3, 47.8, 47.0, 46.7.
     static constexpr int kItemCost = 2;
     static constexpr int kTmemS = 3 * R;                        // columns: hi, lo, rotated
     static constexpr int kTmemO = 2 * kTmemS;
@@ -1058,7 +1058,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 // threads: where a block of query heads is in few parts, those of the CTA that it begins in join them, a team to a row, with kAtOnce parts on their way; where it is in many, those of
 // all CTAs but its last take a row each, and their teams share its parts.
 //   It costs a launch, 1 to 4 us, and reads up to 19 MB that were just written, 4 us.  Where parts are few on average small blocks with a row to a team: 64 sequences of up to
-// 8192 tokens with 16 heads 45.2 us, 512 threads and two rows 46.7; where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
+// 8192 tokens with 16 heads 45.2 us, 512 threads and two rows 46.7 (41.4 now); where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
 // thread blocks that have nothing to do).  The last CTA of a block joining its parts, in the kernel before, took 2 us longer for the first and 20 for the second.
 template <bool kMany>
 struct Join {
