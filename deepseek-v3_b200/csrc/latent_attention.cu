@@ -10,8 +10,10 @@
 // at most 2^-8 of itself, what rounding it to bf16 would cost.  Two e4m3 products take the time of one in bf16, and half the operand bytes.
 //   The token's scale is a factor of its scores and, taken into the exponent as log2 s, of its weight in the second product.
 //   Rounding of small weights: lo is stored times 16, so that its grid is 2^-13 on a scale where the row's largest weight is 2^5 or more; what is
-// below half of that would round to zero, and thousands of tokens that each weigh 2^-19 of one first token do matter.  So a fixed offset
-// per token, evenly spread over a step of the grid, is added before rounding: sums of small weights stay what they are.
+// below half of that would round to zero, and thousands of tokens that each weigh 2^-19 of one first token do matter.  So an offset
+// per token, evenly spread over a step of the grid, is added before rounding: sums of small weights stay what they are.  Within a tile the offsets are 128 evenly spaced
+// ones; which token has which, and where between two steps they begin, a hash of the tile's number says, so that the errors of tokens whose content
+// follows their position (one place of every tile, every so many tokens) have a mean of zero as well, and those of different tiles have nothing to do with one another.
 //
 // The tokens are the rows of both MMAs (128 of them) and the query heads the columns: with 16 query heads (one decoding sequence on one rank of
 // eight) nothing is padded, and a tile costs what its 128 x 32 bytes per step take to be read from shared memory.
@@ -473,6 +475,16 @@ __device__ __forceinline__ float reduce_rows(float (&v)[N], Op op) {
     return v[0];
 }
 
+// The offset of the small weights of a token at position p, evenly over [-2^-10, 2^-10], half a step of lo either side (either end alone rounds to zero, the even one): an odd multiple
+// of its place in the tile, and a shift; both by the tile.  (Multiplicative hashing; a shift by the golden ratio from tile to tile is less work, but every 127th
+// token then has nearly the same offset.  Offsets that were the same in every tile lost up to a quarter of what sixteen places of every tile held.)
+__device__ __forceinline__ float small_offset(uint32_t p) {
+    uint32_t h = p / kTokens * 0x9E3779B1u;
+    h = (h ^ h >> 16) * 0x85EBCA6Bu;
+    static_assert(kTokens == 128, "p times a multiple of 2^25 is its place in the tile times that");
+    return static_cast<float>(static_cast<int>(p * ((h & 0xFE000000u) | 0x02000000u) + (h << 7))) * 0x1p-41f;
+}
+
 template <int N>
 __device__ __forceinline__ void broadcast_rows(float* to, float own, float (&v)[N]) {     // `to`: N floats of this warp
     __syncwarp();
@@ -751,7 +763,6 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         const int sw = warp - kFirstSoftmaxWarp, part_of = sw >> 2, quarter = sw & 3;
         const int token = quarter * 32 + lane;                                 // of the tile: this thread's TMEM lane
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const float dither = static_cast<float>((token * 79) & 127) * 0x1p-16f - 0x1.fcp-11f;   // evenly over (-2^-10, 2^-10), half a step either side
         uint32_t tile_count = 0;
         bool ok = true;                                                        // the same in all lanes of a warp
         const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t counter) -> bool {
@@ -835,6 +846,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             for (int t = 0; t < w.n; ++t, ++tile_count) {
                 const uint32_t b = tile_count & 1, phase = (tile_count >> 1) & 1;
                 const int p = (w.tile + t) * kTokens + token;
+                const float offset = small_offset(p);
                 // (room for the weights, and the tokens' scales: both there before the scores are)
                 if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, 12, tile_count);
                 ok = ok && wait(sm.full[2 * b + (quarter >> 1)], phase, 2, tile_count);
@@ -935,7 +947,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         const uint16_t h = cvt_e4m3x2(a.x, a.y);
                         // (the offset alone rounds to zero: no weight stays none)
                         const float2 rest = fma2(e4m3x2_to_float2(h), make_float2(-1.0f, -1.0f), a);
-                        const float2 scaled = fma2(rest, make_float2(kLoScale, kLoScale), make_float2(dither, dither));
+                        const float2 scaled = fma2(rest, make_float2(kLoScale, kLoScale), make_float2(offset, offset));
                         const uint16_t g = cvt_e4m3x2(scaled.x, scaled.y);
                         if ((i & 2) == 0) hi[i / 4] = h, lo[i / 4] = g;
                         else hi[i / 4] |= static_cast<uint32_t>(h) << 16, lo[i / 4] |= static_cast<uint32_t>(g) << 16;
