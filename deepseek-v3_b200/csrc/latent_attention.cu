@@ -6,7 +6,7 @@
 //
 // Both products run on e4m3 operands as they lie in the cache: nothing is converted to 16 bits on the way, which would cost a conversion and a
 // trip through shared memory per cached value.  What is not 8 bits wide is split in two e4m3 values: a bf16 query has 8 significant bits, so that
-// hi = e4m3(q), lo = e4m3(q - hi) is the query itself (scaled by a power of two per row, and down to 2^-18 of the row's largest value); a weight 2^(y - m) is off by
+// hi = e4m3(q), lo = e4m3(16 (q - hi)) is the query itself (scaled by a power of two per row): values down to 2^-13 of the row's largest as they are, those below off by 2^-21 of it at most; a weight 2^(y - m) is off by
 // at most 2^-8 of itself, what rounding it to bf16 would cost.  Two e4m3 products take the time of one in bf16, and half the operand bytes.
 //   The token's scale is a factor of its scores and, taken into the exponent as log2 s, of its weight in the second product.
 //   Rounding of small weights: lo is stored times 16, so that its grid is 2^-13 on a scale where the row's largest weight is 2^5 or more; what is
@@ -59,7 +59,7 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 // the bits below (see the grid of small weights above) and spares nearly all passes over the sums so far.
 constexpr float kTop = 5.0f, kSlack = 3.75f;
 constexpr float kNothing = -3.0e38f;      // below every finite score, and no infinity: -inf less this is -inf
-constexpr float kLoScale = 16.0f;         // the largest remainder is 2^-4 of 2^8
+constexpr float kLoScale = 16.0f;         // of remainders, so that the grid below e4m3's smallest normal value is finer by as much; the largest is 2^-4 of 2^8
 
 struct Queries {
     const __nv_bfloat16 *latent, *rope;
@@ -813,7 +813,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                     const float a = finite ? bf16_bits_to_float(x2[i] & 0xFFFFu) * inv : 0.0f, b = finite ? __uint_as_float(x2[i] & 0xFFFF0000u) * inv : 0.0f;
                     const uint16_t h = cvt_e4m3x2(a, b);
                     const float2 f = e4m3x2_to_float2(h);
-                    const uint16_t l = cvt_e4m3x2(a - f.x, b - f.y);
+                    const uint16_t l = cvt_e4m3x2((a - f.x) * kLoScale, (b - f.y) * kLoScale);
                     if (i & 1) hi[i / 2] |= static_cast<uint32_t>(h) << 16, lo[i / 2] |= static_cast<uint32_t>(l) << 16;
                     else hi[i / 2] = h, lo[i / 2] = l;
                 }
@@ -872,7 +872,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                         const float4 f = k[i / 4];
 #pragma unroll
                         for (int j = 0; j < 4; j += 2)
-                            y[(i + j) / 2] = fma2(add2(add2(two(hi + i + j), two(lo + i + j)), two(ro + i + j)),
+                            y[(i + j) / 2] = fma2(add2(fma2(two(lo + i + j), make_float2(1.0f / kLoScale, 1.0f / kLoScale), two(hi + i + j)), two(ro + i + j)),
                                                   mul2(make_float2(sc, sc), j ? make_float2(f.z, f.w) : make_float2(f.x, f.y)), make_float2(e, e));
                     }
                 }
