@@ -13,6 +13,7 @@ A module's cache is made on its first call (not in a captured graph), of the siz
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -51,9 +52,17 @@ def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
     return torch.view_as_real(z).flatten(3).to(x.dtype)
 
 
+def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
+    """Whether an additive mask hides what lies behind each token and nothing else (Transformer.forward's, model.py:738-798; the lowest number of its type serves for -inf too)."""
+    rows, columns = mask.shape
+    row, column = torch.arange(rows, device=mask.device), torch.arange(columns, device=mask.device)
+    seen = column <= row[:, None] + (start_pos if columns > rows else 0)
+    return torch.where(seen, mask == 0, mask <= torch.finfo(mask.dtype).min).all()
+
+
 def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
-    """``MLA.forward`` on the 8-bit latent cache.  ``mask``: None for one token, the reference's causal mask (any floating tensor is taken for it), or
-    int64 words of a tree of drafted tokens."""
+    """``MLA.forward`` on the 8-bit latent cache.  ``mask``: None for one token, the reference's causal mask (of these tokens, or of all up to them), or
+    int64 words of a tree of drafted tokens.  Masks of other shapes are refused; a floating mask that is not the causal one makes the result NaN (nothing is read back)."""
     bsz, seqlen, _ = x.shape
     rope = self.qk_rope_head_dim
     if self.kv_lora_rank != LATENT_DIM or rope != ROPE_DIM:
@@ -61,8 +70,15 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
     tree = mask if mask is not None and not mask.is_floating_point() else None
     if mask is None and seqlen > 1:
         raise NotImplementedError("several tokens without a mask would see one another both ways; latent_attention is causal")
-    cache = mla_cache(self)
     end_pos = start_pos + seqlen
+    causal = None
+    if mask is not None and tree is None:
+        if mask.shape not in ((seqlen, seqlen), (seqlen, end_pos)):
+            raise NotImplementedError(f"attention is causal, or that of a tree: a mask of shape {tuple(mask.shape)} is neither's ({seqlen} tokens from position {start_pos})")
+        causal = _is_causal(mask, start_pos)
+        if not mask.is_cuda and not causal:
+            raise NotImplementedError("attention is causal, or that of a tree; this mask is neither's")
+    cache = mla_cache(self)
     if bsz > cache.block_table.size(0) or end_pos > cache.max_len:
         raise ValueError(f"{bsz} sequences of {end_pos} tokens do not fit a cache of {cache.block_table.size(0)} of {cache.max_len}")
 
@@ -80,8 +96,9 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
         weight = weight_dequant(weight, scale, block_size)
     weight = weight.view(self.n_local_heads, -1, LATENT_DIM)
     q_latent = torch.einsum("bshd,hdc->bshc", q_nope, weight[:, :self.qk_nope_head_dim])
+    q_angles = freqs_cis if causal is None else freqs_cis.masked_fill(~causal.to(x.device), math.nan)
     lens = torch.full((bsz,), end_pos, dtype=torch.int32, device=x.device)
-    out = latent_attention(q_latent, _rotate(q_rope, freqs_cis), cache.pool, cache.block_table[:bsz, :-(-end_pos // PAGE)], lens, self.softmax_scale, tree_mask=tree)
+    out = latent_attention(q_latent, _rotate(q_rope, q_angles), cache.pool, cache.block_table[:bsz, :-(-end_pos // PAGE)], lens, self.softmax_scale, tree_mask=tree)
     return self.wo(torch.einsum("bshc,hdc->bshd", out, weight[:, -self.v_head_dim:]).flatten(2))
 
 
