@@ -3,6 +3,8 @@
 ``MLA.forward`` (model.py:446-497, ``attn_impl = "absorb"``) normalises, rotates and stores the new tokens in bf16 buffers and then runs two score
 einsums, a softmax and a weighted-sum einsum over the whole prefix.  The replacement keeps the projections, the absorbed products with ``wkv_b`` and the
 arguments, and does the rest with the operators of ``latent.py``: one launch stores the new tokens in the 8-bit cache, ``latent_attention`` reads it.
+``kv_norm`` is part of that launch where calling it does nothing but the RMS norm of its ``weight`` and ``eps``; one with hooks, a forward of its own or another
+norm is called, and its bf16 result stored.
 
     import model, dsv3_b200
     dsv3_b200.install_mla(model)        # model.MLA.forward = mla_forward
@@ -14,10 +16,13 @@ A module's cache is made on its first call (not in a captured graph), of the siz
 from __future__ import annotations
 
 import math
+import types
 from typing import NamedTuple, Optional
 
 import torch
+from torch.nn.modules import module as _nn_module
 
+from ._lib import host
 from .latent import LATENT_DIM, ROPE_DIM, LatentCache, allocate_latent_cache, latent_attention, latent_cache_write
 from .ops import weight_dequant
 
@@ -50,6 +55,48 @@ def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
     """Neighbouring values of the last dimension as a complex number, times their angle's (model.py:378-393)."""
     z = torch.view_as_complex(x.float().view(*x.shape[:-1], -1, 2)) * freqs_cis.view(1, x.size(1), 1, -1)
     return torch.view_as_real(z).flatten(3).to(x.dtype)
+
+
+def _norms_as_rms_norm(forward) -> bool:
+    """Whether ``forward`` gives x / sqrt(mean(x^2) + eps) * weight of an object that has ``dim``, ``weight`` and ``eps`` (model.py:270-294)."""
+    x = torch.linspace(-3, 2, 2 * LATENT_DIM, dtype=torch.float32, device="cpu").view(2, LATENT_DIM).bfloat16()
+    weight = torch.linspace(0.5, 2, LATENT_DIM, dtype=torch.float32, device="cpu").bfloat16()
+    try:
+        with torch.no_grad():
+            for eps in (1e-6, 0.5):
+                want = x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + eps) * weight.float()
+                got = forward(types.SimpleNamespace(dim=LATENT_DIM, weight=weight, eps=eps), x)
+                # (bf16 twice at most, after the norm and after the weight)
+                if got.shape != want.shape or not bool(((got.float() - want).abs() <= 2.0 ** -7 * 1.01 * want.abs()).all()):
+                    return False
+    except Exception:                                      # (a forward that needs more than that, or a GPU)
+        return False
+    return True
+
+
+_known_norms = {}        # class -> (its forward, the forward's code, answer)
+
+
+def _is_rms_norm(norm) -> bool:
+    """Whether calling ``norm`` is the RMS norm of its ``weight`` and ``eps`` and nothing else, which ``latent_cache_write`` can do in its place: a module that nothing
+    intercepts, of a class whose forward gives that on a stand-in.  Kept with the class, its forward and that one's code, and found anew when one of them is another."""
+    if host.intercepted(norm) or _nn_module._global_forward_hooks or _nn_module._global_forward_pre_hooks:
+        return False
+    cls = type(norm)
+    forward = getattr(cls, "forward", None)
+    if forward is None or cls.__call__ is not torch.nn.Module.__call__:
+        return False
+    code = getattr(forward, "__code__", None)
+    known = _known_norms.get(cls)
+    if known is None or known[0] is not forward or known[1] is not code:
+        if len(_known_norms) >= 64:
+            _known_norms.clear()
+        known = _known_norms[cls] = forward, code, _norms_as_rms_norm(forward)
+    return known[2]
+
+
+# With this eps beside a mean of squares below 2^96, and this weight, the norm of latent_cache_write is x * 2^-60 * 2^60
+_NO_NORM_EPS, _NO_NORM_WEIGHT = 2.0 ** 120, 2.0 ** 60
 
 
 def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
@@ -88,7 +135,12 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
     kv = self.wkv_a(x)
     step = torch.arange(seqlen, device=x.device)
     slots = (torch.arange(bsz, device=x.device) * cache.first_page_slot + start_pos)[:, None] + step
-    latent_cache_write(cache.pool, kv, self.kv_norm.weight, freqs_cis, step.repeat(bsz), slots, self.kv_norm.eps)
+    norm = self.kv_norm
+    if _is_rms_norm(norm):
+        latent_cache_write(cache.pool, kv, norm.weight, freqs_cis, step.repeat(bsz), slots, norm.eps)
+    else:
+        kv = torch.cat([norm(kv[..., :LATENT_DIM]).to(kv.dtype), kv[..., LATENT_DIM:]], -1)
+        latent_cache_write(cache.pool, kv, kv.new_full((LATENT_DIM,), _NO_NORM_WEIGHT, dtype=torch.float32), freqs_cis, step.repeat(bsz), slots, _NO_NORM_EPS)
 
     weight = self.wkv_b.weight
     scale = getattr(self.wkv_b, "scale", None)
