@@ -11,13 +11,14 @@ norm is called, and its bf16 result stored.
 
 A module's cache is made on its first call (not in a captured graph), of the size of its bf16 buffers; ``mla_cache(module)`` gives it with its block table, for
 ``latent_cache_keep`` and ``latent_cache_read``.  Drafted tokens: with a tree of them, ``mask`` is the int64 ``[batch, tokens]`` of
-``latent_attention``'s ``tree_mask`` and ``freqs_cis`` has a row per node, that of its depth.
+``latent_attention``'s ``tree_mask`` and ``freqs_cis`` has a row per node, that of its depth.  Sequences of which different numbers of drafts were kept are of different
+lengths from then on: ``start_pos`` is then an integer tensor ``[batch]`` and ``freqs_cis`` ``[batch, tokens, 32]``.
 """
 from __future__ import annotations
 
 import math
 import types
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Union
 
 import torch
 from torch.nn.modules import module as _nn_module
@@ -53,7 +54,7 @@ def mla_cache(module) -> MlaCache:
 
 def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
     """Neighbouring values of the last dimension as a complex number, times their angle's (model.py:378-393)."""
-    z = torch.view_as_complex(x.float().view(*x.shape[:-1], -1, 2)) * freqs_cis.view(1, x.size(1), 1, -1)
+    z = torch.view_as_complex(x.float().view(*x.shape[:-1], -1, 2)) * freqs_cis.view(-1, x.size(1), 1, x.size(-1) // 2)
     return torch.view_as_real(z).flatten(3).to(x.dtype)
 
 
@@ -107,9 +108,11 @@ def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
     return torch.where(seen, mask == 0, mask <= torch.finfo(mask.dtype).min).all()
 
 
-def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
+def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
     """``MLA.forward`` on the 8-bit latent cache.  ``mask``: None for one token, the reference's causal mask (of these tokens, or of all up to them), or
-    int64 words of a tree of drafted tokens.  Masks of other shapes are refused; a floating mask that is not the causal one makes the result NaN (nothing is read back)."""
+    int64 words of a tree of drafted tokens.  Masks of other shapes are refused; a floating mask that is not the causal one makes the result NaN (nothing is read back).
+    ``start_pos``: one for all sequences, or an int32 or int64 tensor ``[batch]`` beside ``x``, which a captured step reads when it is replayed; a sequence whose tokens do not fit
+    its cache is then not stored, and its result NaN.  ``freqs_cis``: ``[tokens, 32]``, or ``[batch, tokens, 32]``."""
     bsz, seqlen, _ = x.shape
     rope = self.qk_rope_head_dim
     if self.kv_lora_rank != LATENT_DIM or rope != ROPE_DIM:
@@ -117,16 +120,20 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
     tree = mask if mask is not None and not mask.is_floating_point() else None
     if mask is None and seqlen > 1:
         raise NotImplementedError("several tokens without a mask would see one another both ways; latent_attention is causal")
-    end_pos = start_pos + seqlen
-    causal = None
+    starts = start_pos if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else None
+    if starts is not None and (starts.shape != (bsz,) or starts.dtype not in (torch.int32, torch.int64) or starts.device != x.device):
+        raise ValueError(f"start_pos must be an integer, or int32 or int64 [{bsz}] on {x.device}")
+    end_pos = seqlen if starts is not None else start_pos + seqlen
+    valid = None                                           # which sequences' results are to be had: bool [batch], or of all
     if mask is not None and tree is None:
         if mask.shape not in ((seqlen, seqlen), (seqlen, end_pos)):
-            raise NotImplementedError(f"attention is causal, or that of a tree: a mask of shape {tuple(mask.shape)} is neither's ({seqlen} tokens from position {start_pos})")
-        causal = _is_causal(mask, start_pos)
-        if not mask.is_cuda and not causal:
+            raise NotImplementedError(f"attention is causal, or that of a tree: a mask of shape {tuple(mask.shape)} is neither's ({seqlen} tokens up to position {end_pos})")
+        valid = _is_causal(mask, end_pos - seqlen)
+        if not mask.is_cuda and not valid:
             raise NotImplementedError("attention is causal, or that of a tree; this mask is neither's")
+        valid = valid.to(x.device)
     cache = mla_cache(self)
-    if bsz > cache.block_table.size(0) or end_pos > cache.max_len:
+    if bsz > cache.block_table.size(0) or end_pos > cache.max_len or end_pos < seqlen:
         raise ValueError(f"{bsz} sequences of {end_pos} tokens do not fit a cache of {cache.block_table.size(0)} of {cache.max_len}")
 
     q = self.wq(x) if self.q_lora_rank == 0 else self.wq_b(self.q_norm(self.wq_a(x)))
@@ -134,13 +141,24 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
     q_nope, q_rope = torch.split(q, [self.qk_nope_head_dim, rope], dim=-1)
     kv = self.wkv_a(x)
     step = torch.arange(seqlen, device=x.device)
-    slots = (torch.arange(bsz, device=x.device) * cache.first_page_slot + start_pos)[:, None] + step
+    slots = (torch.arange(bsz, device=x.device) * cache.first_page_slot)[:, None] + step
+    if starts is None:
+        table = cache.block_table[:bsz, :-(-end_pos // PAGE)]
+        lens = torch.full((bsz,), end_pos, dtype=torch.int32, device=x.device)
+        slots += start_pos
+    else:
+        fits = (starts >= 0) & (starts <= cache.max_len - seqlen)
+        valid = fits if valid is None else fits & valid
+        table = cache.block_table[:bsz]
+        lens = (torch.where(fits, starts, 0) + seqlen).int()
+        slots = torch.where(fits[:, None], slots + starts[:, None], -1)
+    positions = torch.arange(bsz * seqlen, device=x.device) if freqs_cis.dim() == 3 else step.repeat(bsz)
     norm = self.kv_norm
     if _is_rms_norm(norm):
-        latent_cache_write(cache.pool, kv, norm.weight, freqs_cis, step.repeat(bsz), slots, norm.eps)
+        latent_cache_write(cache.pool, kv, norm.weight, freqs_cis.reshape(-1, ROPE_DIM // 2), positions, slots, norm.eps)
     else:
         kv = torch.cat([norm(kv[..., :LATENT_DIM]).to(kv.dtype), kv[..., LATENT_DIM:]], -1)
-        latent_cache_write(cache.pool, kv, kv.new_full((LATENT_DIM,), _NO_NORM_WEIGHT, dtype=torch.float32), freqs_cis, step.repeat(bsz), slots, _NO_NORM_EPS)
+        latent_cache_write(cache.pool, kv, kv.new_full((LATENT_DIM,), _NO_NORM_WEIGHT, dtype=torch.float32), freqs_cis.reshape(-1, ROPE_DIM // 2), positions, slots, _NO_NORM_EPS)
 
     weight = self.wkv_b.weight
     scale = getattr(self.wkv_b, "scale", None)
@@ -148,9 +166,10 @@ def mla_forward(self, x: torch.Tensor, start_pos: int, freqs_cis: torch.Tensor, 
         weight = weight_dequant(weight, scale, block_size)
     weight = weight.view(self.n_local_heads, -1, LATENT_DIM)
     q_latent = torch.einsum("bshd,hdc->bshc", q_nope, weight[:, :self.qk_nope_head_dim])
-    q_angles = freqs_cis if causal is None else freqs_cis.masked_fill(~causal.to(x.device), math.nan)
-    lens = torch.full((bsz,), end_pos, dtype=torch.int32, device=x.device)
-    out = latent_attention(q_latent, _rotate(q_rope, q_angles), cache.pool, cache.block_table[:bsz, :-(-end_pos // PAGE)], lens, self.softmax_scale, tree_mask=tree)
+    angles = freqs_cis.reshape(-1, seqlen, ROPE_DIM // 2)
+    if valid is not None:
+        angles = torch.where(valid.view(-1, 1, 1), angles, math.nan)
+    out = latent_attention(q_latent, _rotate(q_rope, angles), cache.pool, table, lens, self.softmax_scale, tree_mask=tree)
     return self.wo(torch.einsum("bshc,hdc->bshd", out, weight[:, -self.v_head_dim:]).flatten(2))
 
 
