@@ -61,6 +61,7 @@ int num_sms_of_device(int* device) {
     return budget > 0 && budget < all ? budget : all;
 }
 int num_sms() { return num_sms_of_device(nullptr); }
+int device_sms() { return all_sms(); }
 bool sm_budget_set() {
     const int budget = g_sm_budget.load(std::memory_order_relaxed);
     return budget > 0 && budget < all_sms();

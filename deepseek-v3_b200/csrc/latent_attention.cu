@@ -1177,18 +1177,19 @@ __global__ void __launch_bounds__(Join<kMany>::kThreads, Join<kMany>::kMinBlocks
 // Rows of a block: 16 where a sequence has no more query heads than that (on average: the numbers of queries are device memory), else 32.
 int block_rows(int64_t tokens, int heads, int n_seqs) { return (tokens + n_seqs - 1) / n_seqs * heads <= 16 ? 16 : 32; }
 
+// (By the SMs of the device, as the workspace is sized, whatever budget of them is set: another thread may set it between the query for the size and the call.)
 enum Cut : int { kCut, kLook, kWhole };
-Cut cut_mode(int64_t tokens, int heads, int n_seqs, int64_t longest, int grid) {
+Cut cut_mode(int64_t tokens, int heads, int n_seqs, int64_t longest, int sms) {
     if (longest <= kTokens) return kWhole;
     const int rows = block_rows(tokens, heads, n_seqs);
     const int64_t blocks = tokens * ((heads + rows - 1) / rows), most = (longest + kTokens - 1) / kTokens;
-    if (blocks > grid) return kCut;
-    if (most <= kSmallTiles && most * (grid - blocks) <= static_cast<int64_t>(kSmallSaved) * grid) return kWhole;
+    if (blocks > sms) return kCut;
+    if (most <= kSmallTiles && most * (sms - blocks) <= static_cast<int64_t>(kSmallSaved) * sms) return kWhole;
     // (what the kernel adds up in one round and one word)
-    return n_seqs <= Cfg<16>::kThreads && grid < 1 << kBlockBits && blocks * most < 1 << (31 - kBlockBits) ? kLook : kCut;
+    return n_seqs <= Cfg<16>::kThreads && sms < 1 << kBlockBits && blocks * most < 1 << (31 - kBlockBits) ? kLook : kCut;
 }
 
-size_t partial_bytes(int rows, int grid) { return static_cast<size_t>(grid) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
+size_t partial_bytes(int rows, int sms) { return static_cast<size_t>(sms) * (2 * rows * (kLatent + 1) * sizeof(float) + 2 * sizeof(int4)); }
 
 template <int R, bool kLooks>
 int launch(const LatentCache& c, Queries q, const CUtensorMap& map_latent, const CUtensorMap& map_rope, int grid, bool many, unsigned int* status,
@@ -1217,8 +1218,9 @@ using namespace dsv3;
 extern "C" {
 
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest) {
-    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || cut_mode(tokens, heads, n_seqs, longest, num_sms()) == kWhole) return 0;
-    return partial_bytes(block_rows(tokens, heads, n_seqs), num_sms());
+    const int sms = device_sms();
+    if (tokens <= 0 || heads <= 0 || n_seqs <= 0 || cut_mode(tokens, heads, n_seqs, longest, sms) == kWhole) return 0;
+    return partial_bytes(block_rows(tokens, heads, n_seqs), sms);
 }
 
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
@@ -1254,17 +1256,17 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
         set_last_error("latent_attention: takes at most 1024 heads and 2^31 query heads");
         return DSV3_ERR_UNSUPPORTED;
     }
-    const int grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
+    const int sms = device_sms(), grid = num_sms(), rows = block_rows(tokens, heads, c.n_seqs);
     const int64_t longest = static_cast<int64_t>(c.pages_width) << c.page_shift;
     if (tokens * ((heads + rows - 1) / rows) > 0x7FFFFFFFll / ((longest + kTokens - 1) / kTokens + 1 + Cfg<32>::kItemCost)) {   // (the kernel counts tiles in 32 bits)
         set_last_error("latent_attention: %lld queries of %d heads over up to %lld tokens are too much work for a call", static_cast<long long>(tokens), heads,
                        static_cast<long long>(longest));
         return DSV3_ERR_UNSUPPORTED;
     }
-    const Cut mode = cut_mode(tokens, heads, c.n_seqs, longest, grid);
+    const Cut mode = cut_mode(tokens, heads, c.n_seqs, longest, sms);
     const bool cut = mode != kWhole;
-    if (cut && (!workspace || workspace_bytes < partial_bytes(rows, grid) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
-        set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, grid));
+    if (cut && (!workspace || workspace_bytes < partial_bytes(rows, sms) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
+        set_last_error("latent_attention: the workspace must be 256-byte aligned and hold %zu bytes", partial_bytes(rows, sms));
         return DSV3_ERR_WORKSPACE;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -153,7 +153,7 @@ def set_gemm_policy(kernel: int = KERNEL_AUTO, split_k: int = 0) -> None:
 
 
 def set_num_sms(n: int = 0) -> None:
-    """SMs the persistent GEMM kernels may occupy from now on (0 = all): leave a concurrent collective its SMs."""
+    """SMs the persistent GEMM kernels and latent attention may occupy from now on (0 = all): leave a concurrent collective its SMs."""
     _lib.check(lib.dsv3_set_num_sms(int(n)))
 
 

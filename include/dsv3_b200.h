@@ -158,7 +158,7 @@ int dsv3_fp8_gemm_static(const void* a, const float* a_s, const void* b, const f
 int dsv3_set_gemm_policy(int kernel, int split_k);
 
 /*
- * SMs the persistent tcgen05 GEMM kernels (and the plans that size split-K for them) may occupy; 0 = all
+ * SMs the persistent tcgen05 GEMM kernels (and the plans that size split-K for them) and latent attention may occupy; 0 = all
  * (default).  No counterpart in the reference.  For hosts that run a collective next to the GEMMs: a persistent
  * kernel that fills every SM keeps the collective's CTAs waiting until it ends, and the GEMM launched after that
  * finds SMs taken and runs a straggling round; leaving the collective its SMs (about as many as it has
@@ -385,6 +385,8 @@ int dsv3_latent_keep(const dsv3_latent_cache_t* cache, const int32_t* first, con
  *   out      : bf16 [tokens, heads, 512], lse : fp32 [tokens, heads].  A query that sees nothing: zeros, and -inf.
  * Refused: a pool without pages; a tree of more than 64 queries to a sequence where that is seen (cu_seqlens_q null); query blocks times tiles of 128 positions, with every row of pages full, that reach 2^31.
  * workspace: dsv3_latent_attention_workspace_bytes() bytes (longest: pages_width * page_size), 256-byte aligned, not shared by calls that can overlap; its contents do not matter.
+ * The size is that of exactly these arguments on the current device; dsv3_set_num_sms does not change it.  It does not grow with them (few long blocks are cut, many short ones are not;
+ * blocks have 16 or 32 rows): one buffer for all calls is that of tokens 1, heads 32, n_seqs 1, longest 2^30, the largest there is.
  */
 size_t dsv3_latent_attention_workspace_bytes(int64_t tokens, int heads, int n_seqs, int64_t longest);
 int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent, int64_t q_latent_token_stride, int64_t q_latent_head_stride,
