@@ -165,6 +165,8 @@ PyObject* py_latent_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         at::Tensor out = new_cuda(sizes, at::kBFloat16, dev), lse;
         sizes.pop_back();
         if (with_lse) lse = new_cuda(sizes, at::kFloat, dev);
+        c10::cuda::OptionalCUDAGuard guard;                                    // (the size is that of the current device)
+        if (dev.index() != c10::cuda::current_device()) guard.set_device(dev);
         const size_t need = dsv3_latent_attention_workspace_bytes(l.tokens, static_cast<int>(l.heads), p.c.n_seqs, p.c.pages_width * p.c.page_size);
         // (given back after the launches: torch hands the memory out again in the stream's order)
         const at::Tensor ws = need ? new_cuda({static_cast<int64_t>(need)}, at::kByte, dev) : at::Tensor();
