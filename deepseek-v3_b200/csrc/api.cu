@@ -330,7 +330,7 @@ int dsv3_check_device_status(dsv3_stream_t stream, uint32_t detail[4]) {
     const unsigned int zero[4] = {0, 0, 0, 0};
     DSV3_CUDA_TRY(cudaMemcpy(dptr, zero, sizeof(zero), cudaMemcpyHostToDevice));
     set_last_error("device wait gave up: kind=%u (1 smem-empty, 2 smem-full, 3 tmem-empty, 4 tmem-full, 7/8 scale table, "
-                   "9 self-test, 10 all-reduce peer signal, 11-13 latent attention) counter=%u cta=%u",
+                   "9 self-test, 10 all-reduce peer signal, 11-15 latent attention's weights, room for weights, queries, room for sums, lists) counter=%u cta=%u",
                    host[1], host[2], host[3]);
     return DSV3_ERR_DEVICE_TIMEOUT;
 }

@@ -1370,8 +1370,9 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* status, uint64_t limi
         mbar_fence_init();
     }
     __syncthreads();
+    if (blockIdx.x + 1 < gridDim.x || blockIdx.y + 1 < gridDim.y) return;      // (the last block of the grid, whose number the status words tell)
     bool ok = true;
-    if (threadIdx.x < 32) ok = __all_sync(0xffffffffu, bounded_wait_ns(smem_u32(&bar), 0, &ctl, status, 9, 0, limit_ns));
+    if (threadIdx.x < 32) ok = __all_sync(0xffffffffu, bounded_wait_ns<true>(smem_u32(&bar), 0, &ctl, status, 9, 0, limit_ns));
     if (barrier_all<256>(1, ok)) status[1] = 10;
 }
 
@@ -1380,7 +1381,7 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* status, uint64_t limi
 int launch_bounded_wait_selftest(uint64_t limit_ns, cudaStream_t stream) {
     unsigned int* status = status_device_ptr();
     if (!status) return DSV3_ERR_CUDA;
-    bounded_wait_selftest_kernel<<<1, 256, 0, stream>>>(status, limit_ns);
+    bounded_wait_selftest_kernel<<<dim3(2, 3), 256, 0, stream>>>(status, limit_ns);
     DSV3_CUDA_TRY(cudaGetLastError());
     return DSV3_OK;
 }

@@ -54,6 +54,8 @@ constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kScaleSlots = 4;
 constexpr int kAhead = 4, kBoxSlots = 4;  // tiles whose pages are looked up before they are loaded; of which the pages are kept
 constexpr int kFewParts = 8;              // of a block that several CTAs worked on
+// What a wait that gave up was for (kinds of dsv3_check_device_status)
+constexpr uint32_t kTileRoom = 1, kTile = 2, kScoresRoom = 3, kScores = 4, kWeights = 11, kWeightsRoom = 12, kQueriesStaged = 13, kSumsRoom = 14, kList = 15;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // The maximum that weights are relative to moves when a weight would pass 2^(kTop + kSlack), and then stands for 2^kTop.  e4m3 ends at 448; a wide slack costs two of
 // the bits below (see the grid of small weights above) and spares nearly all passes over the sums so far.
@@ -513,7 +515,7 @@ __device__ __forceinline__ bool follow(const uint32_t* counter, uint32_t want, C
                 t0 = now;
             } else if (now - t0 > limit_ns) {
                 ctl->abort_flag = 1;
-                if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = 11, status[2] = want, status[3] = blockIdx.y * gridDim.x + blockIdx.x;
+                if (atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = kList, status[2] = want, status[3] = blockIdx.y * gridDim.x + blockIdx.x;
                 return false;
             }
         }
@@ -598,7 +600,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 const uint32_t slot = 2 * (tile_count & 1) + h, full = bar(sm.full[slot]);
                 const uint32_t of_unit = ((1u << unit_boxes) - 1u) << (h * unit_boxes);
                 const int boxes = __popc(used & of_unit), bytes = boxes * rows * (kLatent + 2 * kRope) + __popc(present & of_unit) * rows * 4;
-                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[slot]), ((tile_count >> 1) & 1) ^ 1, ctl, status, 1, tile_count));
+                ok = __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.empty[slot]), ((tile_count >> 1) & 1) ^ 1, ctl, status, kTileRoom, tile_count));
                 if (!ok) break;
                 if ((used & ~present & of_unit) != 0) {                        // an absent page: its tokens have no scale
                     if (at == -1 && lane / unit_boxes == h)
@@ -620,7 +622,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         }
         // none of the commits onto empty[] may be in flight when the CTA leaves its shared memory to another
         for (uint32_t t = tile_count > 2 ? tile_count - 2 : 0u; ok && t < tile_count; ++t)
-            for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.empty[2 * (t & 1) + h]), (t >> 1) & 1, ctl, status, 1, t));
+            for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.empty[2 * (t & 1) + h]), (t >> 1) & 1, ctl, status, kTileRoom, t));
     } else if (warp == 3) {
         // ------------------------------------------------------------ the walk: items and their rows, and pages some tiles ahead of the loads.  (To bring the
         // pages to L2 as well, one to six tiles ahead, only gave HBM more to do: 4 to 20 % longer for 64 sequences of up to 8192 tokens with 16 heads.)
@@ -703,11 +705,11 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             if (!ok) break;
             const int n = sm.item[item & (kItemSlots - 1)].n;
             last = sm.item[item & (kItemSlots - 1)].last;
-            ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.q_full), item & 1, ctl, status, 13, item));
+            ok = __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.q_full), item & 1, ctl, status, kQueriesStaged, item));
             for (int t = 0; t < n && ok; ++t, ++count) {
                 const uint32_t b = count & 1, phase = (count >> 1) & 1, d = tmem + b * C::kTmemS, at = smem_u32(tiles) + b * kTileBytes;
-                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.s_empty[b]), phase ^ 1, ctl, status, 3, count));
-                for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait(bar(sm.full[2 * b + h]), phase, ctl, status, 2, count));
+                ok = __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.s_empty[b]), phase ^ 1, ctl, status, kScoresRoom, count));
+                for (int h = 0; h < 2; ++h) ok = ok && __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.full[2 * b + h]), phase, ctl, status, kTile, count));
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t da = umma_desc<128, kGroupBytes>(at), db = umma_desc<128, 1024>(q_at);
@@ -739,9 +741,9 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             last = sm.item[item & (kItemSlots - 1)].last;
             for (int t = 0; t < n && ok; ++t, ++count) {
                 const uint32_t b = count & 1;
-                ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.p_full[b]), (count >> 1) & 1, ctl, status, 11, count));
+                ok = __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.p_full[b]), (count >> 1) & 1, ctl, status, kWeights, count));
                 // (an item's first sums overwrite those of the item before it)
-                if (ok && t == 0) ok = __all_sync(0xffffffffu, bounded_wait(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, 12, item));
+                if (ok && t == 0) ok = __all_sync(0xffffffffu, bounded_wait<true>(bar(sm.o_empty), (item & 1) ^ 1, ctl, status, kSumsRoom, item));
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t da = umma_desc<128, kGroupBytes>(smem_u32(tiles) + b * kTileBytes), db = umma_desc<2 * R, 16 * R>(p_at + b * C::kPBytes);
@@ -766,7 +768,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
         uint32_t tile_count = 0;
         bool ok = true;                                                        // the same in all lanes of a warp
         const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t counter) -> bool {
-            return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, counter));
+            return __all_sync(0xffffffffu, bounded_wait<true>(bar(b), parity, ctl, status, what, counter));
         };
         // The rows of a block, a warp to every eighth of them: all on their way from memory before the first is brought to shared memory, as an operand of
         // the first product.  (This is a single warp's chain of dependent instructions; where the rows lie has been worked out before.)
@@ -848,10 +850,10 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 const int p = (w.tile + t) * kTokens + token;
                 const float offset = small_offset(p);
                 // (room for the weights, and the tokens' scales: both there before the scores are)
-                if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, 12, tile_count);
-                ok = ok && wait(sm.full[2 * b + (quarter >> 1)], phase, 2, tile_count);
+                if (tile_count >= 2) ok = ok && wait(sm.p_empty[b], phase ^ 1, kWeightsRoom, tile_count);
+                ok = ok && wait(sm.full[2 * b + (quarter >> 1)], phase, kTile, tile_count);
                 const float sc = sm.scales[tile_count & (kScaleSlots - 1)][token];
-                ok = ok && wait(sm.s_full[b], phase, 4, tile_count);
+                ok = ok && wait(sm.s_full[b], phase, kScores, tile_count);
                 tc_fence_after();
                 float2 y[N / 2];
                 {
@@ -919,7 +921,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 #pragma unroll
                         for (int i = 0; i < N / 2; ++i) l[i] = mul2(l[i], make_float2(f[2 * i], f[2 * i + 1]));
                         const uint32_t before = tile_count - 1;
-                        ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, 12, before);
+                        ok = wait(sm.p_empty[before & 1], (before >> 1) & 1, kWeightsRoom, before);
                         tc_fence_after();
                         if (ok) {
 #pragma unroll 2
@@ -1007,7 +1009,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
                 for (int i = 0; i < N / 4; ++i) to[i] = place[i];
             }
             const uint32_t last = tile_count - 1;
-            ok = wait(sm.p_empty[last & 1], (last >> 1) & 1, 12, last);
+            ok = wait(sm.p_empty[last & 1], (last >> 1) & 1, kWeightsRoom, last);
             tc_fence_after();
             if (ok) {
 #pragma unroll

@@ -21,6 +21,8 @@ struct Control {
 // the global timer is slow enough to throttle the pipeline if it sat on the fast path).  When the
 // budget (limit_ns) runs out the thread records what it was waiting for in the status words, raises
 // the CTA-wide abort flag and returns false; it never traps and never spins without a bound.
+// k2d: the grid has two dimensions.  (Not asked of grids of one, whose kernels are short of registers.)
+template <bool k2d = false>
 __device__ __forceinline__ bool bounded_wait_ns(uint32_t bar, uint32_t parity, Control* ctl, unsigned int* status,
                                                 uint32_t what, uint32_t g, uint64_t limit_ns) {
     uint64_t t0 = 0;
@@ -34,9 +36,9 @@ __device__ __forceinline__ bool bounded_wait_ns(uint32_t bar, uint32_t parity, C
             } else if (now - t0 > limit_ns) {
                 ctl->abort_flag = 1;
                 if (atomicCAS(&status[0], 0u, 1u) == 0u) {
-                    status[1] = what;        // 1 empty, 2 full, 3 tmem-empty, 4 tmem-full, 7-8 scale table, 9 self-test
+                    status[1] = what;        // 1 empty, 2 full, 3 tmem-empty, 4 tmem-full, 7-8 scale table, 9 self-test, 11-15 latent attention
                     status[2] = g;           // chunk / unit counter of the waiting role
-                    status[3] = blockIdx.x;
+                    status[3] = k2d ? blockIdx.y * gridDim.x + blockIdx.x : blockIdx.x;
                 }
                 return false;
             }
@@ -44,9 +46,10 @@ __device__ __forceinline__ bool bounded_wait_ns(uint32_t bar, uint32_t parity, C
     }
 }
 
+template <bool k2d = false>
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, Control* ctl, unsigned int* status,
                                              uint32_t what, uint32_t g) {
-    return bounded_wait_ns(bar, parity, ctl, status, what, g, kWaitLimitNs);
+    return bounded_wait_ns<k2d>(bar, parity, ctl, status, what, g, kWaitLimitNs);
 }
 
 // The same wait for loops that are short of registers (the promotion loop of the 256-wide kernel): bounded by a
