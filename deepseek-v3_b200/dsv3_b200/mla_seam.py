@@ -17,6 +17,7 @@ lengths from then on: ``start_pos`` is then an integer tensor ``[batch]`` and ``
 from __future__ import annotations
 
 import math
+import threading
 import types
 from typing import NamedTuple, Optional, Union
 
@@ -37,19 +38,32 @@ class MlaCache(NamedTuple):
     max_len: int
 
 
+_making = threading.Lock()
+
+
 def mla_cache(module) -> MlaCache:
-    """The 8-bit cache of an MLA module, made on first use after its bf16 buffers (model.py:439-444)."""
+    """The 8-bit cache of an MLA module, made on first use after its bf16 buffers (model.py:439-444); where those have moved to another device it goes after them."""
     cache = module.__dict__.get("_dsv3_latent")
-    if cache is None:
+    buffer = module.kv_cache if hasattr(module, "kv_cache") else module.k_cache
+    if cache is not None and cache.block_table.device == buffer.device:
+        return cache
+    with _making:                                          # (one thread makes it; the others find it made)
+        cache = module.__dict__.get("_dsv3_latent")
+        if cache is not None and cache.block_table.device == buffer.device:
+            return cache
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an MLA module's cache is made on its first call, which cannot be a captured one: every replay would clear it")
-        buffer = module.kv_cache if hasattr(module, "kv_cache") else module.k_cache
-        batch, length = buffer.shape[:2]
-        pages = -(-length // PAGE)
-        table = torch.arange(batch * pages, dtype=torch.int32, device=buffer.device).view(batch, pages)
-        cache = MlaCache(allocate_latent_cache(batch * pages, PAGE, buffer.device), table, pages * PAGE, length)
+        if cache is not None:
+            cache = cache._replace(pool=LatentCache(*(t.to(buffer.device) for t in cache.pool)), block_table=cache.block_table.to(buffer.device))
+        else:
+            batch, length = buffer.shape[:2]
+            pages = -(-length // PAGE)
+            table = torch.arange(batch * pages, dtype=torch.int32, device=buffer.device).view(batch, pages)
+            cache = MlaCache(allocate_latent_cache(batch * pages, PAGE, buffer.device), table, pages * PAGE, length)
+        if buffer.is_cuda:
+            torch.cuda.current_stream(buffer.device).synchronize()         # (the threads that find it may be on streams of their own)
         module.__dict__["_dsv3_latent"] = cache
-    return cache
+        return cache
 
 
 def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
