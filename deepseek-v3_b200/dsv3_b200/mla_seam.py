@@ -127,9 +127,9 @@ _NO_NORM_EPS, _NO_NORM_WEIGHT = 2.0 ** 120, 2.0 ** 60
 def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
     """Whether an additive mask hides what lies behind each token and nothing else (Transformer.forward's, model.py:738-798; the lowest number of its type serves for -inf too)."""
     rows, columns = mask.shape
-    row, column = torch.arange(rows, device=mask.device), torch.arange(columns, device=mask.device)
-    seen = column <= row[:, None] + (start_pos if columns > rows else 0)
-    return torch.where(seen, mask == 0, mask <= torch.finfo(mask.dtype).min).all()
+    low = torch.finfo(mask.dtype).min
+    causal = mask.new_full((rows, columns), low).triu_(1 + (start_pos if columns > rows else 0))
+    return (mask.clamp(min=low) == causal).all()           # (few launches: a short prompt is bound by the host)
 
 
 def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
