@@ -76,7 +76,7 @@ struct Queries {
     // a block of query heads: `head_blocks` of them to a token, or 2^block_shift tokens to a block
     int head_blocks, block_shift;
     // 2^16 / heads + 1, for a block of several tokens, and 2^32 / CTAs with a share of their own + 1: a division is some forty instructions that come from memory before
-    // they run, once each in a kernel of this length (one tile 7.9 us with them, 7.5 without)
+    // they run, once each in a kernel of this length (one tile took 0.4 us longer with them)
     uint32_t per_head, per_cta;
     bool read_once;                       // a sequence's queries are one block
     bool whole;                           // blocks are not cut (unless the kernel looks whether to cut them)
@@ -92,8 +92,8 @@ struct Cfg {
     static constexpr int kQBytes = 4 * kQChunk + R * 128;
     static constexpr int kPBytes = kTokens * 2 * R;
     // Softmax warps: four, a quarter of the tile's tokens each, to eight rows.  With 32 rows the softmax is part of the chain that a tile waits for: eight warps of 16 rows to a
-    // thread took 15 % longer for 128 sequences of 1024 tokens and 128 heads (74 us now), 9 % for 24 trees of 13 drafts (62), 13 % for one
-    // sequence of 131072 tokens (45).
+    // thread took 15 % longer for 128 sequences of 1024 tokens and 128 heads, 9 % for 24 trees of 13 drafts, 13 % for one
+    // sequence of 131072 tokens.
     static constexpr int kRows = 8, kParts = R / kRows, kSoftmaxWarps = 4 * kParts;
     static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
     // What a block takes beside its tiles, in tiles, when work is shared out: its queries' way to shared memory, its result's way out (2.2 and 3 us, with 16 and 32 rows).
@@ -152,7 +152,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 // How long lines stay in the L2: as others, or as the first to go.  Tiles that are read once go first, so that the next launch finds code, lengths and pages there: 64
-// sequences of up to 8192 tokens with 16 heads 42.0 us instead of 43.9; a chunk of 515 tokens, whose blocks read the same tiles one after another, 108.6 instead of 106.3.
+// sequences of up to 8192 tokens with 16 heads 41.8 us instead of 43.9, 140 of 4096 65.0 instead of 66.4; a chunk of 515 tokens, whose blocks read the same tiles one after another, 108.6 instead of
+// 106.3.  (By the rows of a sequence: whether sequences share pages only the table tells.  64 on one prefix of 8192 tokens 47.7 us either way, on one of 32768 156.5 instead of 151.6.)
 __device__ __forceinline__ uint64_t l2_policy(bool once) {
     uint64_t p;
     if (once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
@@ -165,7 +166,7 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Two values at a time: an instruction instead of two (the softmax's warps are short of issue slots with 32 rows: 110 us instead of 115 for 128 heads of 32
+// Two values at a time: an instruction instead of two (the softmax's warps are short of issue slots with 32 rows: 4 % longer without for 128 heads of 32
 // sequences of 8192 tokens).
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
@@ -214,9 +215,9 @@ constexpr uint32_t idesc_bf16(uint32_t m, uint32_t n) { return umma_idesc_e4m3_f
 // list and leaves what the others need in shared memory.
 // Whether to cut: an SM's longest block against its equal share of all tiles (0.8 to 1.7 us each), against the ends of more items and the join.
 //   Where no row of pages holds more than kSmallTiles tiles the host decides, by the rows' length, and launches no join for whole blocks.  Heads, sequences x tokens:
-//   16, 1 x 137 8.3 us, cut 11.2; 16, 60 x 384 11.6, 13.7; 16, 140 x 1024 22.5, 26.1; 128, 24 x 1024 21.5, 27.1; beyond the line 16, 1 x 640 11.9, 11.1; 1 x 1024 15.2, 11.5.
+//   16, 1 x 137 8.4 us, cut 11.0; 16, 60 x 384 11.7, 13.5; 16, 140 x 1024 22.5, 25.9; 128, 24 x 1024 21.4, 26.9; beyond the line 16, 1 x 640 11.8, 10.9; 1 x 1024 14.9, 11.3.
 //   Elsewhere the kernel looks at the lengths (which takes a kernel of its own: up to 0.5 us more for those that have no use for it).  Rows of pages longer than that:
-//   16, 140 x 4096 64.5 us, cut 68.4; 128, 36 x 2048 39.6, 42.9; beyond the line 16, 1 x 512 12.1, 11.1; 128, 8 x 768 19.8, 16.5.
+//   16, 140 x 4096 64.9 us, cut 69.1; 128, 36 x 2048 40.4, 43.4; beyond the line, when it was drawn, 16, 1 x 512 12.1, 11.1; 128, 8 x 768 19.8, 16.5.
 constexpr int kSmallTiles = 8, kSmallSaved = 4, kSaved = 3;
 constexpr int kBlockBits = 8;             // of a word that counts tiles and blocks
 struct Seq {
@@ -830,7 +831,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(sm.q_full));
         };
-        // (the first rows are worked out here, not waited for: with the first page looked up before the walk's list is written 7.8 us instead of 8.3 for one tile)
+        // (the first rows are worked out here, not waited for: with the first page looked up before the walk's list is written 0.5 us less for one tile)
         fetch(lane < kMine ? row_of(q, sm.walk, sw + lane * kSoftmaxWarps, member) : Row{-1, 0});
         stage(0);
         ok = listed(0);
@@ -1072,7 +1073,7 @@ latent_attention_kernel(const __grid_constant__ CUtensorMap map_latent, const __
 // threads: where a block of query heads is in few parts, those of the CTA that it begins in join them, a team to a row, with kAtOnce parts on their way; where it is in many, those of
 // all CTAs but its last take a row each, and their teams share its parts.
 //   It costs a launch, 1 to 4 us, and reads up to 19 MB that were just written, 4 us.  Where parts are few on average small blocks with a row to a team: 64 sequences of up to
-// 8192 tokens with 16 heads 45.2 us, 512 threads and two rows 46.7 (41.4 now); where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
+// 8192 tokens with 16 heads 45.2 us when it was chosen, 512 threads and two rows 46.7; where they are many the other way round: one of 131072 with four drafts 45.8, 53 (the
 // thread blocks that have nothing to do).  The last CTA of a block joining its parts, in the kernel before, took 2 us longer for the first and 20 for the second.
 template <bool kMany>
 struct Join {

@@ -37,7 +37,8 @@ __device__ __forceinline__ void load8(const float* p, float* x) {
 // A warp to a token, 8 latent values of either half and one pair to rotate per lane, so that a warp's loads and stores are whole lines.
 //   c = kv * rsqrt(mean(kv^2) + eps) * weight, s = power_scale(max(amax|c|, 1e-4)), stored: e4m3(c / s), bf16(rot(k) / s), s
 // Everything in fp32 and rounded once; dividing by a power of two is exact.  The norm's weight stays in registers over a warp's tokens.
-// B200, fp32 weight: 16001 tokens 9.1 us (3.6 TB/s), 4096 3.2, one 1.8; a token to a warp and its weights loaded one by one, 16 neighbours to a lane: 20.6 us at 16001.
+// B200, fp32 weight, launches behind one another: 16001 tokens 9.2 us where all comes from HBM (3.6 TB/s), 7.0 where the L2 holds it; 4096 from the L2 3.3, one 1.7.  A token to a warp
+// and its weights loaded one by one, 16 neighbours to a lane, took 2.2 times as long at 16001.
 template <typename W>
 __global__ void __launch_bounds__(kThreads, kWriteBlocks) latent_write_kernel(LatentCache c, const __nv_bfloat16* __restrict__ kv, int64_t kv_stride,
                                                                 const W* __restrict__ weight, float eps, const float2* __restrict__ freqs,
@@ -118,7 +119,7 @@ __device__ __forceinline__ uint2 scaled4(uint32_t w, float s) {
 }
 
 // A warp to kReadRows rows of the result, all under way together; loads and stores are whole lines (with 16 neighbouring values to a lane, whose stores are not,
-// 49.3 us instead of 44.3 for 148 thousand tokens; HBM bounds it, at 6.1 TB/s).  The block's first row is looked up among the sequences by all threads, the others from there on.
+// 11 % longer; 148 thousand tokens 44.4 us: HBM bounds it, at 6.1 TB/s).  The block's first row is looked up among the sequences by all threads, the others from there on.
 constexpr int kReadRows = 4;
 __global__ void __launch_bounds__(kThreads) latent_read_kernel(LatentCache c, const int32_t* __restrict__ cu, int64_t total,
                                                                __nv_bfloat16* __restrict__ latent, __nv_bfloat16* __restrict__ rope) {
