@@ -147,6 +147,8 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
     starts = start_pos if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else None
     if starts is not None and (starts.shape != (bsz,) or starts.dtype not in (torch.int32, torch.int64) or starts.device != x.device):
         raise ValueError(f"start_pos must be an integer, or int32 or int64 [{bsz}] on {x.device}")
+    if tuple(freqs_cis.shape) not in ((seqlen, rope // 2), (bsz, seqlen, rope // 2)):
+        raise ValueError(f"freqs_cis must be [{seqlen}, {rope // 2}] or [{bsz}, {seqlen}, {rope // 2}], not {list(freqs_cis.shape)}")
     end_pos = seqlen if starts is not None else start_pos + seqlen
     valid = None                                           # which sequences' results are to be had: bool [batch], or of all
     if mask is not None and tree is None:

@@ -108,3 +108,11 @@ def test_starts_that_are_refused():
             m(x, bad, f[:1], None)
     with pytest.raises(ValueError, match="do not fit"):
         m(x, -1, f[:1], None)
+
+
+@pytest.mark.parametrize("shape", [(8, 32), (2, 32), (3, 32), (1, 4, 32), (3, 4, 32), (2, 8, 32), (2, 4, 16), (4, 64), (2, 2, 4, 32)])
+def test_angles_of_other_shapes_are_refused(shape):
+    """Of two sequences of four tokens; eight rows would do for both, but the second sequence's are not the first's."""
+    m, x = _model(4, 0), _tokens(2, 4, 15)
+    with pytest.raises(ValueError, match="freqs_cis"):
+        m(x, 0, torch.ones(shape, dtype=torch.complex64, device="cuda"), _causal(4))
