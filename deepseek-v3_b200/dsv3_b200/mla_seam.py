@@ -82,8 +82,25 @@ def _rotate(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
     return torch.view_as_real(z).flatten(3).to(x.dtype)
 
 
+def _with_torch_alone(forward):
+    """``forward`` with nothing of its surroundings but torch's modules and functions, and no builtins: code of its own (a kernel that takes its argument for device memory, say) is not
+    run; or None."""
+    if type(forward) is not types.FunctionType or forward.__closure__:
+        return None
+
+    def of_torch(value):
+        name = value.__name__ if isinstance(value, types.ModuleType) else getattr(value, "__module__", None) if callable(value) else None
+        return isinstance(name, str) and name.split(".")[0] == "torch"
+
+    around = {name: forward.__globals__[name] for name in forward.__code__.co_names if of_torch(forward.__globals__.get(name))}
+    return types.FunctionType(forward.__code__, {"__builtins__": {}, **around}, forward.__name__, forward.__defaults__)
+
+
 def _norms_as_rms_norm(forward) -> bool:
     """Whether ``forward`` gives x / sqrt(mean(x^2) + eps) * weight of an object that has ``dim``, ``weight`` and ``eps`` (model.py:270-294)."""
+    forward = _with_torch_alone(forward)
+    if forward is None:
+        return False
     x = torch.linspace(-3, 2, 2 * LATENT_DIM, dtype=torch.float32, device="cpu").view(2, LATENT_DIM).bfloat16()
     weight = torch.linspace(0.5, 2, LATENT_DIM, dtype=torch.float32, device="cpu").bfloat16()
     try:

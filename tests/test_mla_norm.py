@@ -103,3 +103,41 @@ def test_random_numbers_stay_as_they_are():
     torch.manual_seed(3)
     assert _seam()._is_rms_norm(Norm())
     assert torch.equal(torch.rand(4), want)
+
+
+RAN = []
+
+
+def _kernel(x, weight, eps):
+    RAN.append(x)                                                           # (would take the host's memory for the device's)
+    return F.rms_norm(x, (x.size(-1),), weight, eps)
+
+
+class CodeOfItsOwn(Norm):
+    def forward(self, x):
+        return _kernel(x, self.weight, self.eps)
+
+
+class Imports(Norm):
+    def forward(self, x):
+        import test_mla_norm
+        return test_mla_norm._kernel(x, self.weight, self.eps)
+
+
+class Opens(Norm):
+    def forward(self, x):
+        RAN.append(open)
+        return F.rms_norm(x, (self.dim,), self.weight, self.eps)
+
+
+def _closed_over(kernel):
+    class Closed(Norm):
+        def forward(self, x):
+            return kernel(x, self.weight, self.eps)
+    return Closed
+
+
+@pytest.mark.parametrize("cls", [CodeOfItsOwn, Imports, Opens, _closed_over(_kernel)])
+def test_code_of_its_own_is_not_run(cls):
+    RAN.clear()
+    assert not _seam()._is_rms_norm(cls(512)) and not RAN
