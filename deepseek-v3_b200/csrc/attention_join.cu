@@ -1,0 +1,134 @@
+// The results of the same queries over several pieces of their keys, joined (see include/dsv3_b200.h).
+//
+//   lse = log sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
+//
+// HBM bounds it: every part is read once.  dim / 8 neighbouring threads to a row, eight values each, up to four parts on their way at once.
+#include <algorithm>
+
+#include "attention_join.cuh"
+
+namespace dsv3 {
+namespace {
+
+constexpr int kThreads = 256, kAtOnce = 4;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+struct Parts {
+    const void* out[kMaxJoinParts];
+    const float* lse[kMaxJoinParts];
+    int n;
+    int64_t rows;
+    FastDiv row_threads;
+    int block_rows;
+    __nv_bfloat16* to;
+    float* to_lse;
+    const int32_t* cu;        // or null; rows of tokens before cu[0], and from cu[n_seqs] on, are left as they are
+    int n_seqs, heads;
+};
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_bits_to_float(u[i] & 0xFFFFu), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+}
+__device__ __forceinline__ void load8(const float* p, float* v) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ Parts p) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const uint32_t slot = fast_div(threadIdx.x, p.row_threads), at = threadIdx.x - slot * p.row_threads.d;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * p.block_rows + slot;
+    if (static_cast<int>(slot) >= p.block_rows || row >= p.rows) return;
+    if (p.cu && (row < static_cast<int64_t>(p.cu[0]) * p.heads || row >= static_cast<int64_t>(p.cu[p.n_seqs]) * p.heads)) return;
+    const int64_t from = (row * p.row_threads.d + at) * 8;
+    float top = -INFINITY;
+    bool nan = false;
+    for (int i = 0; i < p.n; ++i) {
+        const float v = p.lse[i][row];
+        nan = nan || isnan(v);
+        top = fmaxf(top, v);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float acc[8] = {}, sum = 0.0f;
+    for (int i0 = 0; i0 < p.n; i0 += kAtOnce) {
+        float v[kAtOnce][8], w[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (i0 + k >= p.n) break;
+            w[k] = p.lse[i0 + k][row];
+            // (what a part that sees nothing left there does not matter)
+            if (w[k] != -INFINITY) load8(static_cast<const T*>(p.out[i0 + k]) + from, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (i0 + k >= p.n) break;
+            if (w[k] == -INFINITY) continue;
+            const float e = exp2f((w[k] - ref) * kLog2e);
+            sum += e;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] = fmaf(e, v[k][j], acc[j]);
+        }
+    }
+    const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] *= inv;
+    *reinterpret_cast<uint4*>(p.to + from) = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+    if (p.to_lse && at == 0) p.to_lse[row] = nan ? inv : sum == 0.0f ? -INFINITY : top + log2f(sum) * kLn2;
+}
+
+template <typename T>
+int launch(const void* const* outs, const float* const* lses, int n, int64_t rows, int dim, const int32_t* cu, int n_seqs, int heads, void* out, float* lse,
+           cudaStream_t stream) {
+    const int row_threads = dim / 8, block_rows = kThreads / row_threads;
+    Parts p = {};
+    for (int i = 0; i < n; ++i) p.out[i] = outs[i], p.lse[i] = lses[i];
+    p.n = n, p.rows = rows, p.row_threads = make_fast_div(row_threads), p.block_rows = block_rows;
+    p.to = static_cast<__nv_bfloat16*>(out), p.to_lse = lse;
+    p.cu = cu, p.n_seqs = n_seqs, p.heads = heads;
+    DSV3_CUDA_TRY(launch_dependent(attention_join_kernel<T>, dim3(static_cast<unsigned>((rows + block_rows - 1) / block_rows)), dim3(kThreads), 0, stream, p));
+    return DSV3_OK;
+}
+
+}  // namespace
+
+int join_partials(const float* partial, const float* partial_lse, int n, int64_t rows, int dim, const int32_t* cu, int n_seqs, int heads, void* out, float* lse,
+                  cudaStream_t stream) {
+    const void* outs[kMaxJoinParts];
+    const float* lses[kMaxJoinParts];
+    for (int i = 0; i < n; ++i) outs[i] = partial + static_cast<int64_t>(i) * rows * dim, lses[i] = partial_lse + static_cast<int64_t>(i) * rows;
+    return launch<float>(outs, lses, n, rows, dim, cu, n_seqs, heads, out, lse, stream);
+}
+
+}  // namespace dsv3
+
+using namespace dsv3;
+
+extern "C" int dsv3_attention_join(const void* const* outs, const float* const* lses, int parts, int64_t rows, int dim, void* out, float* lse,
+                                   dsv3_stream_t stream) {
+    if (parts < 1 || rows < 0 || dim < 0 || !outs || !lses) {
+        set_last_error("attention_join: no parts, or a negative size");
+        return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    if (parts > kMaxJoinParts || dim % 8 != 0 || dim > 8 * kThreads || rows > 0x7FFFFFFFll) {
+        set_last_error("attention_join: takes up to %d parts of less than 2^31 rows of a multiple of 8 values (up to %d), not %d of %lld of %d", kMaxJoinParts, 8 * kThreads,
+                       parts, static_cast<long long>(rows), dim);
+        return DSV3_ERR_UNSUPPORTED;
+    }
+    if (rows == 0 || dim == 0) return DSV3_OK;
+    for (int i = 0; i < parts; ++i) {
+        if (!outs[i] || !lses[i] || !out) {
+            set_last_error("attention_join: null pointer");
+            return DSV3_ERR_INVALID_ARGUMENT;
+        }
+        if (reinterpret_cast<uintptr_t>(outs[i]) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0) {
+            set_last_error("attention_join: parts and result must be 16-byte aligned");
+            return DSV3_ERR_UNSUPPORTED;
+        }
+    }
+    return launch<__nv_bfloat16>(outs, lses, parts, rows, dim, nullptr, 0, 0, out, lse, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,975 @@
+// Attention of a prompt's queries over keys and values that the latents were expanded to (see include/dsv3_b200.h).
+//
+//   x[r, p] = q_nope[r] . k_nope[p] + q_rope[r] . k_rope[p]          r: a query of one head, p: a key; k_rope is shared by the heads
+//   out[r]  = sum_p 2^(c x - m) v[p] / sum_p 2^(c x - m)             c: softmax_scale log2(e), m: a running reference of the row
+//
+// One pass over the keys.  A CTA works on 256 queries of a head as two halves of 128 (the M of an MMA), a lane of TMEM and a softmax thread to a query; keys
+// come in tiles of 128, which both halves use.  Scores (128 columns of TMEM) and sums (128 more) of either half fill TMEM: while one half's
+// weights are formed the tensor core works for the other.  Weights go back to TMEM in bf16, over the scores they come from, as the A operand of the second product: they
+// never see shared memory, which the first product's operands keep busy (96 KB a tile and half at 128 bytes a cycle, as long as its MMAs take).
+//   The reference m of a row moves only where a weight would pass 2^8, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
+// (2^-9), sums and statistics are fp32.
+//   Blocks of at most 128 queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
+// than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
+//
+// Keys and values behind a sequence's end belong to another one, or to nobody: what they score is replaced, and their values are cleared in shared memory before the MMA
+// that would multiply them by zero (0 * NaN).  The same warp looks at the tiles that some queries of a block see only in part for values that are not finite.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "attention_join.cuh"
+#include "tc_wait.cuh"
+
+namespace dsv3 {
+
+int make_tmap_heads(CUtensorMap* map, const void* base, int width, int64_t heads, int64_t rows, int64_t head_stride, int64_t row_stride, int box_rows);
+
+namespace {
+
+constexpr int kNope = DSV3_NOPE_DIM, kRope = DSV3_ROPE_DIM, kValue = DSV3_VALUE_DIM;
+constexpr int kHalf = 128, kBlock = 2 * kHalf;   // queries
+constexpr int kTile = 128;                       // keys
+// Operands lie as rows of 64 values (128 bytes, swizzled).  Keys and values come through a ring of slots of 16 KB: three to a tile of keys (64 dimensions of 128 keys
+// each), two to one of values (64 keys of 128 dimensions each): beside the queries there is room for eight, one and a half tiles of both.
+constexpr int kSlots = 8, kSlotBytes = 16384, kKeySlots = 3, kValueSlots = 2, kTileSlots = kKeySlots + kValueSlots;
+constexpr int kQueryBytes = kKeySlots * kSlotBytes;
+constexpr int kOperandBytes = kSlots * kSlotBytes + 2 * kQueryBytes;
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10, kThreads = 384;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+static_assert(kSoftmaxRegs * 256 + kOtherRegs * 128 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
+constexpr int kTmemScores = 0, kTmemSums = 2 * kTile, kTmemCols = 512;
+constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 2;
+constexpr int kLanes = 32;                       // sequences that are put in order of their length
+// What a wait that gave up was for (kinds of dsv3_check_device_status)
+constexpr uint32_t kRoom = 1, kTileThere = 2, kScoresThere = 4, kWeightsThere = 16, kSumsThere = 17, kQueriesThere = 18, kGuarded = 19, kItems = 20, kHalves = 21;
+constexpr uint64_t kItemLimitNs = 100 * kWaitLimitNs;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kSlack = 8.0f;
+
+struct Params {
+    int tokens, kv_tokens, heads, n_seqs;
+    const int32_t *cu_q, *cu_k;           // null: per_q, per_k each
+    int per_q, per_k;
+    bool causal;
+    float scale;                          // softmax_scale log2(e)
+    int head_group;
+    int splits;
+    bool dynamic;                         // CTAs take the place of those that have not started; else every gridDim.x-th item
+    __nv_bfloat16* out;
+    float* lse;
+    float *partial, *partial_lse;         // with splits: [splits, tokens, heads, 128] and without the last
+};
+
+// A block of queries of one head, and the tiles of keys that a CTA takes of it.
+struct Item {
+    int q0, rows;                         // first query, how many (0: nothing left)
+    int k0, len;                          // the sequence's first key, how many it has
+    int limit;                            // last key that the first query sees (a further query one more, if causal)
+    int head, split;
+    int tile, n;                          // first tile, how many
+    int n0, n1;                           // ... of which either half takes
+    bool alternate;                       // both halves have the same queries and every other tile
+    int edge;                             // tiles from this one on are not seen as a whole by all queries
+};
+
+struct Small {
+    uint64_t full[kSlots], empty[kSlots];
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], guarded[2], item_full[kItemSlots], item_empty[kItemSlots], halves_full, halves_done, taken;
+    Item item[kItemSlots];
+    int not_finite[kItemSlots];           // first key whose values are not finite, of those in tiles that are not seen as a whole
+    alignas(16) uint32_t answer[4];
+    float2 row[2][kHalf];                 // reference and sum of the halves' rows, where they are joined
+    Control ctl;
+};
+constexpr int kSmallBytes = 3072, kSmemBytes = kSmallBytes + kOperandBytes;
+static_assert(sizeof(Small) <= kSmallBytes && kSmemBytes <= 232448, "shared memory of a CTA");
+
+// ---------------------------------------------------------------- PTX
+__device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// ... with A in TMEM
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int x, int head, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x),
+                 "r"(head), "r"(row), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+// Takes the place of a CTA of the grid that has not started; the answer (16 bytes) says whose.
+__device__ __forceinline__ void try_cancel(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int cancelled_cta(uint32_t answer) {       // or -1: all have started
+    int x;
+    asm volatile(
+        "{\n"
+        ".reg .b128 h;\n"
+        ".reg .pred p;\n"
+        ".reg .b32 y, z, w;\n"
+        "ld.shared.b128 h, [%1];\n"
+        "mov.b32 %0, -1;\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n"
+        "}\n"
+        : "=r"(x)
+        : "r"(answer)
+        : "memory");
+    return x;
+}
+
+// 64 keys of 128 values as two blocks of [64 keys][64 values], 128-byte swizzle, K (the keys) the slow dimension: groups of eight keys are 1024 bytes apart, the
+// blocks 8192.
+__device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(8192 >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+// bf16 x bf16 -> fp32
+constexpr uint32_t kIdescScores = umma_idesc_e4m3_f32(kHalf, kTile) | (1u << 7) | (1u << 10);
+constexpr uint32_t kIdescSums = umma_idesc_e4m3_f32(kHalf, kValue) | (1u << 7) | (1u << 10) | (1u << 16);   // B transposed
+
+// ---------------------------------------------------------------- who works on what
+struct Seq {
+    int q0, queries, k0, keys;
+};
+// (offsets that lead out of the tensors are cut off)
+__device__ __forceinline__ Seq load_seq(const Params& p, int s) {
+    Seq r = {0, 0, 0, 0};
+    if (s >= p.n_seqs) return r;
+    int q1, k1;
+    if (p.cu_q) r.q0 = p.cu_q[s], q1 = p.cu_q[s + 1];
+    else r.q0 = s * p.per_q, q1 = r.q0 + p.per_q;
+    if (p.cu_k) r.k0 = p.cu_k[s], k1 = p.cu_k[s + 1];
+    else r.k0 = s * p.per_k, k1 = r.k0 + p.per_k;
+    r.q0 = max(0, min(r.q0, p.tokens));
+    r.k0 = max(0, min(r.k0, p.kv_tokens));
+    r.queries = max(0, min(q1, p.tokens) - r.q0);
+    r.keys = max(0, min(k1, p.kv_tokens) - r.k0);
+    return r;
+}
+__device__ __forceinline__ int blocks_of(int queries) { return (queries + kBlock - 1) / kBlock; }
+
+// The list of items: groups of heads, in those the blocks of queries, in those the heads of the group and the parts of the keys.  A group has so many heads that the CTAs
+// that work at one time share few heads' keys, which the L2 then holds.  Blocks with more keys come first (up to 32 sequences): an SM that is done
+// takes the next item of the list, and what is left for the end is short.
+struct List {
+    Seq mine;                             // this lane's sequence (up to 32)
+    int blocks, behind;                   // its blocks; steps of two tiles by which it is shorter than the longest
+    int total, last_step;                 // blocks in all; steps in which blocks come up
+    int chunk, before;                    // beyond 32 sequences: first of the 32 at hand, blocks before those
+    __device__ __forceinline__ void begin(const Params& p) {
+        const int lane = threadIdx.x & 31;
+        chunk = before = 0;
+        mine = load_seq(p, lane);
+        blocks = blocks_of(mine.queries);
+        const int tiles = blocks > 0 ? (mine.keys + kTile - 1) / kTile : 0;
+        behind = (__reduce_max_sync(0xffffffffu, tiles) - tiles) >> 1;
+        last_step = __reduce_max_sync(0xffffffffu, blocks > 0 ? behind + blocks : 0) - 1;
+        total = __reduce_add_sync(0xffffffffu, blocks);
+        for (int s = kLanes; s < p.n_seqs; s += kLanes) total += __reduce_add_sync(0xffffffffu, blocks_of(load_seq(p, s + lane).queries));
+    }
+    __device__ __forceinline__ int up_to(int step) const {           // blocks that come up in steps 0 .. step
+        return __reduce_add_sync(0xffffffffu, max(0, min(step - behind + 1, blocks)));
+    }
+    // Whole warp: item number `at`.
+    __device__ __forceinline__ Item find(const Params& p, uint32_t at) {
+        Item it = {};
+        if (at >= static_cast<uint32_t>(total) * p.heads * p.splits) return it;
+        const uint32_t unsplit = at / p.splits;
+        it.split = static_cast<int>(at - unsplit * p.splits);
+        const uint32_t group = unsplit / (static_cast<uint32_t>(total) * p.head_group), in_group = unsplit - group * (static_cast<uint32_t>(total) * p.head_group);
+        const uint32_t heads = min(p.head_group, p.heads - static_cast<int>(group) * p.head_group);
+        const int place = static_cast<int>(in_group / heads);
+        it.head = static_cast<int>(group * p.head_group + in_group - place * heads);
+        Seq s;
+        int block;
+        if (p.n_seqs <= kLanes) {
+            int lo = 0, hi = last_step;                              // first step that comes up to more than `place` blocks
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (up_to(mid) > place) hi = mid;
+                else lo = mid + 1;
+            }
+            const int nth = place - (lo > 0 ? up_to(lo - 1) : 0);
+            uint32_t there = __ballot_sync(0xffffffffu, lo >= behind && lo < behind + blocks);
+            for (int i = 0; i < nth; ++i) there &= there - 1;
+            const int from = __ffs(there) - 1;
+            block = __shfl_sync(0xffffffffu, blocks - 1 - (lo - behind), from);
+            s = {__shfl_sync(0xffffffffu, mine.q0, from), __shfl_sync(0xffffffffu, mine.queries, from), __shfl_sync(0xffffffffu, mine.k0, from),
+                 __shfl_sync(0xffffffffu, mine.keys, from)};
+        } else {
+            const int lane = threadIdx.x & 31;
+            if (place < before) {
+                chunk = before = 0;
+                mine = load_seq(p, lane);
+                blocks = blocks_of(mine.queries);
+            }
+            for (;;) {
+                const int here = __reduce_add_sync(0xffffffffu, blocks);
+                if (place < before + here || chunk + kLanes >= p.n_seqs) break;
+                before += here;
+                chunk += kLanes;
+                mine = load_seq(p, chunk + lane);
+                blocks = blocks_of(mine.queries);
+            }
+            int run = blocks;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += u;
+            }
+            const int from = __ffs(__ballot_sync(0xffffffffu, before + run > place)) - 1;
+            block = __shfl_sync(0xffffffffu, run - 1, from) - (place - before);
+            s = {__shfl_sync(0xffffffffu, mine.q0, from), __shfl_sync(0xffffffffu, mine.queries, from), __shfl_sync(0xffffffffu, mine.k0, from),
+                 __shfl_sync(0xffffffffu, mine.keys, from)};
+        }
+        const int first = block * kBlock;
+        it.q0 = s.q0 + first;
+        it.rows = min(kBlock, s.queries - first);
+        it.k0 = s.k0;
+        it.len = s.keys;
+        it.limit = p.causal ? s.keys - s.queries + first : s.keys - 1;
+        it.alternate = it.rows <= kHalf;
+        const auto tiles_of_row = [&](int row) { return max(0, min(it.limit + (p.causal ? row : 0), s.keys - 1) + kTile) / kTile; };
+        const int all = tiles_of_row(it.rows - 1);
+        it.tile = static_cast<int>(static_cast<int64_t>(all) * it.split / p.splits);
+        const int end = static_cast<int>(static_cast<int64_t>(all) * (it.split + 1) / p.splits);
+        it.n = end - it.tile;
+        if (it.alternate) {
+            it.n0 = (it.n + 1) >> 1;
+            it.n1 = it.n >> 1;
+        } else {
+            it.n0 = max(0, min(end, tiles_of_row(kHalf - 1)) - it.tile);
+            it.n1 = it.n;
+        }
+        it.edge = max(0, min(it.limit, s.keys - 1) + 1) / kTile;
+        return it;
+    }
+};
+
+// Slots of an item's tiles, from its first on, in the order in which the MMAs come to them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... where tiles alternate.
+__device__ __forceinline__ uint32_t key_slot(const Item& it, int t) { return it.alternate && t > 0 ? kTileSlots * t - kValueSlots : kTileSlots * t; }
+__device__ __forceinline__ uint32_t value_slot(const Item& it, int t) {
+    return it.alternate && t + 1 < it.n ? kTileSlots * (t + 1) + 1 : kTileSlots * t + kKeySlots;
+}
+
+// ---------------------------------------------------------------- the kernel
+__global__ void __launch_bounds__(kThreads, 1)
+expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qr, const __grid_constant__ CUtensorMap map_kn,
+                          const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ CUtensorMap map_v, const Params p, unsigned int* status) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Small& sm = *reinterpret_cast<Small*>(smem);
+    Control* const ctl = &sm.ctl;
+    const uint32_t ring = smem_u32(smem) + kSmallBytes, queries = ring + kSlots * kSlotBytes;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const auto bar = [](const uint64_t& b) { return smem_u32(&b); };
+
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(bar(sm.full[i]), 1);
+            mbar_init(bar(sm.empty[i]), 2);                          // the MMAs, and the warp that looks at values
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(sm.q_full[i]), 1);
+            mbar_init(bar(sm.q_empty[i]), 1);
+            mbar_init(bar(sm.s_full[i]), 1);
+            mbar_init(bar(sm.p_full[i]), kSoftmaxWarps / 2);
+            mbar_init(bar(sm.o_full[i]), 1);
+            mbar_init(bar(sm.guarded[i]), 1);
+        }
+        for (int i = 0; i < kItemSlots; ++i) {
+            mbar_init(bar(sm.item_full[i]), 1);
+            mbar_init(bar(sm.item_empty[i]), kItemReaders);
+        }
+        mbar_init(bar(sm.halves_full), kSoftmaxWarps);
+        mbar_init(bar(sm.halves_done), kSoftmaxWarps);
+        mbar_init(bar(sm.taken), 1);
+        mbar_fence_init();
+        ctl->abort_flag = (ring & 1023u) != 0 ? 1u : 0u;             // (dynamic shared memory begins at a multiple of 1024; swizzled tiles rely on it)
+        if (ctl->abort_flag && atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = kRoom, status[2] = 0xFFFFFFFFu, status[3] = blockIdx.x;
+    }
+    if (warp == kMmaWarp) tc_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+    if (warp == kLoadWarp && lane == 0) {
+        tma_prefetch_desc(&map_qn);
+        tma_prefetch_desc(&map_qr);
+        tma_prefetch_desc(&map_kn);
+        tma_prefetch_desc(&map_kr);
+        tma_prefetch_desc(&map_v);
+    }
+    griddep_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    const bool well = ctl->abort_flag == 0;
+    // Whole warp: the item in the next slot of the list's ring, or one without rows.
+    const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t count) -> bool {
+        return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, count));
+    };
+    const auto next_item = [&](uint32_t count, bool& ok) -> Item {
+        Item it = {};
+        ok = __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_full[count % kItemSlots]), (count / kItemSlots) & 1, ctl, status, kItems, count, kItemLimitNs));
+        if (ok) it = sm.item[count % kItemSlots];
+        return it;
+    };
+    const auto item_done = [&](uint32_t count) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(sm.item_empty[count % kItemSlots]));
+    };
+
+    // (in the branches of the roles themselves: behind a common point the compiler counts on the lesser of both numbers)
+    if (!well) {
+        // nothing is started
+    } else if (warp >= kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp) {
+            // ------------------------------------------------------------ the list, and the loads
+            List list;
+            list.begin(p);
+            uint32_t slot = 0, active = 0, taken = 0;                    // slots filled; items with tiles
+            bool ok = true;
+            int at = static_cast<int>(blockIdx.x);
+            const auto fill = [&](auto&& copy) {
+                const uint32_t s = slot % kSlots;
+                ok = ok && wait(sm.empty[s], ((slot / kSlots) & 1) ^ 1, kRoom, slot);
+                if (ok && elect_one()) {
+                    mbar_arrive_expect_tx(bar(sm.full[s]), kSlotBytes);
+                    copy(ring + s * kSlotBytes, bar(sm.full[s]));
+                }
+                __syncwarp();
+                ++slot;
+            };
+            for (uint32_t count = 0; ok; ++count) {
+                const Item it = at < 0 ? Item{} : list.find(p, static_cast<uint32_t>(at));
+                const uint32_t place = count % kItemSlots;
+                ok = __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_empty[place]), ((count / kItemSlots) & 1) ^ 1, ctl, status, kItems, count, kItemLimitNs));
+                if (!ok) break;
+                if (lane == 0) {
+                    sm.item[place] = it;
+                    sm.not_finite[place] = 0x7FFFFFFF;
+                    mbar_arrive(bar(sm.item_full[place]));
+                }
+                __syncwarp();
+                if (it.rows == 0) break;
+                const bool more = p.dynamic;
+                if (more && elect_one()) {
+                    mbar_arrive_expect_tx(bar(sm.taken), 16);
+                    try_cancel(smem_u32(sm.answer), bar(sm.taken));
+                }
+                __syncwarp();
+                if (it.n > 0) {
+                    const auto load_queries = [&](int h) {
+                        ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
+                        if (ok && elect_one()) {
+                            if (h == 1 && it.alternate) {
+                                mbar_arrive(bar(sm.q_full[h]));          // (both halves use the first one's)
+                            } else {
+                                const uint32_t to = queries + h * kQueryBytes;
+                                const int row = it.q0 + h * kHalf;
+                                mbar_arrive_expect_tx(bar(sm.q_full[h]), kQueryBytes);
+                                tma_load_3d(to, &map_qn, 0, it.head, row, bar(sm.q_full[h]));
+                                tma_load_3d(to + kSlotBytes, &map_qn, 64, it.head, row, bar(sm.q_full[h]));
+                                tma_load_3d(to + 2 * kSlotBytes, &map_qr, 0, it.head, row, bar(sm.q_full[h]));
+                            }
+                        }
+                        __syncwarp();
+                    };
+                    const auto load_keys = [&](int t) {
+                        const int row = it.k0 + (it.tile + t) * kTile;
+                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 0, it.head, row, full); });
+                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 64, it.head, row, full); });
+                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kr, 0, 0, row, full); });
+                    };
+                    const auto load_values = [&](int t) {
+#pragma unroll
+                        for (int i = 0; i < kValueSlots; ++i) {
+                            const int row = it.k0 + (it.tile + t) * kTile + i * 64;
+                            fill([&](uint32_t to, uint32_t full) {
+                                tma_load_3d(to, &map_v, 0, it.head, row, full);
+                                tma_load_3d(to + kSlotBytes / 2, &map_v, 64, it.head, row, full);
+                            });
+                        }
+                    };
+                    load_queries(0);
+                    load_keys(0);
+                    load_queries(1);
+                    if (it.alternate && it.n > 1) load_keys(1);
+                    for (int t = 0; t < it.n && ok; ++t) {
+                        load_values(t);
+                        const int ahead = t + (it.alternate ? 2 : 1);
+                        if (ahead < it.n && ok) load_keys(ahead);
+                    }
+                    ++active;
+                }
+                if (more) {
+                    // (waited for in any case: the answer may not arrive in the shared memory of another CTA)
+                    const bool there = wait(sm.taken, taken & 1, kItems, taken);
+                    ++taken;
+                    ok = ok && there;
+                    if (ok) {
+                        at = cancelled_cta(smem_u32(sm.answer));
+                        fence_proxy_async_shared();
+                        __syncwarp();
+                    }
+                } else {
+                    at = at > 0x7FFFFFFF - static_cast<int>(gridDim.x) ? -1 : at + static_cast<int>(gridDim.x);
+                }
+            }
+            // none of the arrivals on empty[] may be in flight when the CTA leaves its shared memory to another
+            for (uint32_t s = slot > kSlots ? slot - kSlots : 0u; ok && s < slot; ++s) ok = wait(sm.empty[s % kSlots], (s / kSlots) & 1, kRoom, s);
+            for (int h = 0; h < 2 && ok && active > 0; ++h) ok = wait(sm.q_empty[h], (active - 1) & 1, kQueriesThere, active);
+        } else if (warp == kMmaWarp) {
+            // ------------------------------------------------------------ the MMAs.  The warp stays converged and elects a lane for them alone.
+            uint32_t slot = 0, active = 0, edges = 0, scores0 = 0, scores1 = 0;
+            bool ok = true;
+            for (uint32_t count = 0; ok; ++count) {
+                const Item it = next_item(count, ok);
+                if (!ok || it.rows == 0) break;
+                item_done(count);
+                if (it.n == 0) continue;
+                const auto slot_at = [&](uint32_t i) { return (slot + i) % kSlots; };
+                const auto await = [&](uint32_t first, int n) {
+                    for (int i = 0; i < n; ++i) ok = ok && wait(sm.full[slot_at(first + i)], ((slot + first + i) / kSlots) & 1, kTileThere, slot + first + i);
+                };
+                // scores of tile t for half h; `done`: the tile's keys are not needed any more, `all`: nor the half's queries
+                const auto score = [&](int h, int t, bool done, bool all) {
+                    const uint32_t first = key_slot(it, t), d = tmem + kTmemScores + h * kTile, q = queries + (it.alternate ? 0 : h * kQueryBytes);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < kKeySlots; ++c) {
+                            const uint32_t s = slot_at(first + c);
+                            const uint64_t a = umma_desc_k_major_sw128(q + c * kSlotBytes), b = umma_desc_k_major_sw128(ring + s * kSlotBytes);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) tc_mma_bf16(d, a + 2 * k, b + 2 * k, kIdescScores, (c | k) != 0);
+                            if (done) tc_commit(bar(sm.empty[s]));
+                        }
+                        tc_commit(bar(sm.s_full[h]));
+                        if (all) tc_commit(bar(sm.q_empty[h]));
+                        if (all && it.alternate) tc_commit(bar(sm.q_empty[h ^ 1]));
+                    }
+                    __syncwarp();
+                };
+                const auto sum = [&](int h, int t, bool first, bool done, bool last) {
+                    const uint32_t at = value_slot(it, t), d = tmem + kTmemSums + h * kValue, a = tmem + kTmemScores + h * kTile;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < kValueSlots; ++i) {
+                            const uint32_t s = slot_at(at + i);
+                            const uint64_t b = umma_desc_values(ring + s * kSlotBytes);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) tc_mma_bf16_ts(d, a + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), kIdescSums, !first || (i | k) != 0);
+                            if (done) tc_commit(bar(sm.empty[s]));
+                        }
+                        if (last) tc_commit(bar(sm.o_full[h]));
+                    }
+                    __syncwarp();
+                };
+                const auto weights = [&](int h) {
+                    const uint32_t count = h == 0 ? scores0 : scores1;
+                    ok = ok && wait(sm.p_full[h], (count - 1) & 1, kWeightsThere, count);
+                };
+                const auto values = [&](int t) {                         // (once a tile)
+                    await(value_slot(it, t), kValueSlots);
+                    if (it.tile + t >= it.edge) {
+                        ok = ok && wait(sm.guarded[edges & 1], (edges >> 1) & 1, kGuarded, edges);
+                        ++edges;
+                    }
+                };
+                for (int h = 0; h < 2; ++h) ok = ok && wait(sm.q_full[h], active & 1, kQueriesThere, active);
+                if (it.alternate) {
+                    // half t & 1 takes tile t
+                    for (int t = 0; t < min(2, it.n) && ok; ++t) {
+                        await(key_slot(it, t), kKeySlots);
+                        if (!ok) break;
+                        tc_fence_after();
+                        score(t, t, true, t + 1 == it.n);
+                        t == 0 ? ++scores0 : ++scores1;
+                    }
+                    for (int t = 0; t < it.n && ok; ++t) {
+                        const int h = t & 1;
+                        weights(h);
+                        values(t);
+                        if (!ok) break;
+                        tc_fence_after();
+                        sum(h, t, t < 2, true, t + 2 >= it.n);
+                        if (t + 2 < it.n) {
+                            await(key_slot(it, t + 2), kKeySlots);
+                            if (!ok) break;
+                            tc_fence_after();
+                            score(h, t + 2, true, t + 3 == it.n);
+                            h == 0 ? ++scores0 : ++scores1;
+                        }
+                    }
+                } else {
+                    const int n0 = it.n0, n1 = it.n1;      // (n0 <= n1: the second half sees what the first one does)
+                    await(0, kKeySlots);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (n0 > 0) {
+                        score(0, 0, false, n0 == 1);
+                        ++scores0;
+                    } else if (elect_one()) {
+                        tc_commit(bar(sm.q_empty[0]));
+                    }
+                    score(1, 0, true, n1 == 1);
+                    ++scores1;
+                    for (int t = 0; t < n1 && ok; ++t) {
+                        const bool first_too = t < n0;
+                        if (first_too) weights(0);
+                        values(t);
+                        if (!ok) break;
+                        if (first_too) {
+                            tc_fence_after();
+                            sum(0, t, t == 0, false, t + 1 == n0);
+                        }
+                        if (t + 1 < n1) await(key_slot(it, t + 1), kKeySlots);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (t + 1 < n0) {
+                            score(0, t + 1, false, t + 2 == n0);
+                            ++scores0;
+                        }
+                        weights(1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        sum(1, t, t == 0, true, t + 1 == n1);
+                        if (t + 1 < n1) {
+                            score(1, t + 1, true, t + 2 == n1);
+                            ++scores1;
+                        }
+                    }
+                }
+                slot += kTileSlots * it.n;
+                ++active;
+            }
+        } else if (warp == kGuardWarp) {
+            // ------------------------------------------------------------ values that the MMA must not see.  The warp follows the ring slot by slot (a wait by parity is exact only
+            // for who has seen the phase before), and works on the tiles that are not seen as a whole by all queries.
+            uint8_t* const base = smem + kSmallBytes;
+            uint32_t slot = 0, edges = 0;
+            bool ok = true;
+            for (uint32_t count = 0; ok; ++count) {
+                const Item it = next_item(count, ok);
+                if (!ok || it.rows == 0) break;
+                const uint32_t end = slot + kTileSlots * it.n, start = slot;
+                int t = 0;                                               // tile whose values come next
+                while (slot < end && ok) {
+                    const bool is_value = t < it.n && slot - start >= value_slot(it, t);
+                    const int n = is_value ? kValueSlots : kKeySlots;
+                    const bool look = is_value && it.tile + t >= it.edge;
+                    for (int i = 0; i < n && ok; ++i, ++slot) {
+                        const uint32_t s = slot % kSlots;
+                        ok = wait(sm.full[s], (slot / kSlots) & 1, kTileThere, slot);
+                        if (!ok) break;
+                        if (look) {
+                            const int key0 = (it.tile + t) * kTile + i * 64;
+                            uint4* const at = reinterpret_cast<uint4*>(base + s * kSlotBytes);
+                            // 64 keys x 8 pieces of 16 bytes, twice; rows are keys, and a row's pieces stay in it
+                            __nv_bfloat162 seen = __floats2bfloat162_rn(0.0f, 0.0f);
+                            const __nv_bfloat162 zero = seen;
+#pragma unroll 8
+                            for (int j = 0; j < kSlotBytes / 512; ++j) {
+                                const int key = key0 + ((j * 32 + lane) >> 3 & 63);
+                                if (key >= it.len) {
+                                    at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                                } else {
+                                    const uint4 v = at[j * 32 + lane];
+                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) seen = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, seen);   // NaN stays
+                                }
+                            }
+                            if (__any_sync(0xffffffffu, __hisnan(seen.x) || __hisnan(seen.y))) {
+                                int bad = 0x7FFFFFFF;
+                                for (int j = 0; j < kSlotBytes / 512; ++j) {
+                                    const int key = key0 + ((j * 32 + lane) >> 3 & 63);
+                                    const uint4 v = at[j * 32 + lane];
+                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                    bool finite = true;
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) finite = finite && (w[e] & 0x7F80u) != 0x7F80u && (w[e] & 0x7F800000u) != 0x7F800000u;
+                                    if (!finite) {
+                                        bad = min(bad, key);
+                                        at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                                }
+                                bad = __reduce_min_sync(0xffffffffu, bad);
+                                if (lane == 0) *static_cast<volatile int*>(&sm.not_finite[count % kItemSlots]) = min(bad, sm.not_finite[count % kItemSlots]);
+                            }
+                            fence_proxy_async_shared();
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(sm.empty[s]));
+                    }
+                    if (look && ok) {
+                        if (lane == 0) mbar_arrive(bar(sm.guarded[edges & 1]));
+                        ++edges;
+                    }
+                    if (is_value) ++t;
+                }
+                item_done(count);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        // ------------------------------------------------------------ softmax: a thread to a query
+        const int h = warp >> 2, quarter = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, scores_at = tmem + lanes + kTmemScores + h * kTile;
+        const float c = p.scale;
+        uint32_t tiles = 0, sums = 0, joins = 0;
+        bool ok = true;
+        for (uint32_t count = 0; ok; ++count) {
+            const Item it = next_item(count, ok);
+            if (!ok || it.rows == 0) break;
+            const int n = h == 0 ? it.n0 : it.n1, row0 = (it.alternate ? 0 : h * kHalf) + quarter * 32, row = row0 + lane;
+            const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);           // key that the query sees last
+            const int last0 = min(it.limit + (p.causal ? row0 : 0), it.len - 1);         // ... of the warp's first one
+            float top = -INFINITY;
+            float2 sum2 = make_float2(0.0f, 0.0f);
+            for (int t = 0; t < n; ++t, ++tiles) {
+                const int key0 = (it.tile + (it.alternate ? 2 * t + h : t)) * kTile;
+                ok = wait(sm.s_full[h], tiles & 1, kScoresThere, tiles);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t x[kTile];
+#pragma unroll
+                for (int i = 0; i < kTile; i += 32) tc_ld_x32(scores_at + i, x + i);
+                tc_wait_ld();
+                if (key0 + kTile - 1 > last0) {
+                    const int visible = last - key0;                 // columns beyond are none of the query's
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i) x[i] = i > visible ? 0xFF800000u : x[i];
+                }
+                float m[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m[i] = fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 4]));
+#pragma unroll
+                for (int i = 8; i < kTile; i += 8) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(m[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + j + 4]));
+                }
+                const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                // a weight would pass 2^8 (or nothing was seen so far): the reference moves
+                const bool moves = most * c > top * c + kSlack || (top == -INFINITY && most > -INFINITY);
+                if (t == 0) {
+                    top = most;
+                } else if (__any_sync(0xffffffffu, moves)) {
+                    // (the scores' arrival says that the sums before them are complete)
+                    const float f = moves ? (top == -INFINITY ? 0.0f : ex2((top - most) * c)) : 1.0f;
+                    if (moves) top = most;
+                    sum2.x *= f, sum2.y *= f;
+#pragma unroll 1
+                    for (int i = 0; i < kValue; i += 32) {
+                        uint32_t o[32];
+                        const uint32_t at = tmem + lanes + kTmemSums + h * kValue + i;
+                        tc_ld_x32(at, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tc_st_x32(at, o);
+                    }
+                }
+                const float ref = top == -INFINITY ? 0.0f : -top * c;
+                const float2 c2 = make_float2(c, c), ref2 = make_float2(ref, ref);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = g * 64 + 2 * i;
+                        const float2 y = fma2(make_float2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, ref2);
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        sum2 = add2(sum2, e);
+                        w[i] = pack_bf16x2(e.x, e.y);
+                    }
+                    tc_st_x32(scores_at + g * 32, w);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sm.p_full[h]));
+            }
+            if (!ok) break;
+            float sum = sum2.x + sum2.y;
+            if (n > 0) {
+                ok = wait(sm.o_full[h], sums & 1, kSumsThere, sums);
+                ++sums;
+                if (!ok) break;
+                tc_fence_after();
+            }
+            // Where the halves have the same queries, each takes half of the columns of their common result.
+            const bool joins_halves = it.alternate && it.n > 1;
+            float f = 1.0f, other = 0.0f;                            // factors of the half's sums, and of the other one's
+            if (joins_halves) {
+                sm.row[h][quarter * 32 + lane] = make_float2(top, sum);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sm.halves_full));
+                ok = wait(sm.halves_full, joins & 1, kHalves, joins);
+                if (!ok) break;
+                tc_fence_after();
+                const float2 theirs = sm.row[h ^ 1][quarter * 32 + lane];
+                const float both = fmaxf(top, theirs.x), ref = both == -INFINITY ? 0.0f : both;
+                f = ex2((top - ref) * c);
+                other = ex2((theirs.x - ref) * c);
+                sum = sum * f + theirs.y * other;
+                top = both;
+            }
+            const bool nothing = sum == 0.0f;
+            const bool spoilt = last >= *static_cast<volatile int*>(&sm.not_finite[count % kItemSlots]);
+            const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / sum;
+            f *= inv, other *= inv;
+            const bool writes = row < it.rows && (h == 0 || !it.alternate || joins_halves);
+            const int64_t place = static_cast<int64_t>(it.q0 + row) * p.heads + it.head;
+            const int64_t part = static_cast<int64_t>(it.split) * p.tokens * p.heads + place;
+            const int first = joins_halves ? h * (kValue / 2) : 0, end = joins_halves ? first + kValue / 2 : kValue;
+            if (h == 0 || !it.alternate || joins_halves) {
+#pragma unroll 1
+                for (int i = first; i < end; i += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tc_ld_x32(tmem + lanes + kTmemSums + h * kValue + i, o);
+                        if (joins_halves) {
+                            uint32_t o2[32];
+                            tc_ld_x32(tmem + lanes + kTmemSums + (h ^ 1) * kValue + i, o2);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f + __uint_as_float(o2[j]) * other);
+                        } else {
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        }
+                    }
+                    if (nothing) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = spoilt ? 0x7FC00000u : 0u;
+                    }
+                    if (writes && p.partial) {
+                        uint4* const to = reinterpret_cast<uint4*>(p.partial + part * kValue + i);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) to[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    } else if (writes) {
+                        uint4* const to = reinterpret_cast<uint4*>(p.out + place * kValue + i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const auto two = [&](int k) { return pack_bf16x2(__uint_as_float(o[8 * j + 2 * k]), __uint_as_float(o[8 * j + 2 * k + 1])); };
+                            to[j] = make_uint4(two(0), two(1), two(2), two(3));
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (writes && (h == 0 || !it.alternate)) {
+                const float lse = nothing ? -INFINITY : (top * c + log2f(sum)) * kLn2;
+                if (p.partial) p.partial_lse[part] = lse;
+                else if (p.lse) p.lse[place] = lse;
+            }
+            if (joins_halves) {                                      // (the other half still reads this one's sums)
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sm.halves_done));
+                ok = wait(sm.halves_done, joins & 1, kHalves, joins);
+                ++joins;
+                if (!ok) break;
+            }
+            item_done(count);
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (ctl->abort_flag) {
+        // give copies and MMAs that were already issued time to land before shared memory and TMEM are released
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tc_dealloc(tmem, kTmemCols);
+    }
+}
+
+// How a call is cut up.  What is known on the host is how many queries, keys and sequences there are, not which sequence has how many.
+struct Plan {
+    int64_t blocks;                       // at most
+    int splits, head_group;
+};
+constexpr int kLeastTiles = 4;            // of a part
+Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, int sms) {
+    Plan pl;
+    const int64_t each = ragged ? 0 : tokens / n_seqs;
+    const int64_t seqs = std::min(n_seqs, tokens);                   // that have queries
+    pl.blocks = ragged ? (tokens - seqs) / kBlock + seqs : n_seqs * ((each + kBlock - 1) / kBlock);
+    const int64_t items = pl.blocks * heads, tiles = kv_tokens / n_seqs / kTile;
+    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxJoinParts, sms / items, tiles / kLeastTiles})));
+    pl.head_group = static_cast<int>(n_seqs > kLanes ? heads : std::min<int64_t>(heads, std::max<int64_t>(1, (2 * sms + pl.blocks - 1) / pl.blocks)));
+    return pl;
+}
+size_t partial_bytes(const Plan& pl, int64_t tokens, int64_t heads) {
+    return pl.splits > 1 ? static_cast<size_t>(pl.splits) * tokens * heads * (kValue + 1) * sizeof(float) : 0;
+}
+
+int prepare_kernel() {
+    static std::atomic<uint64_t> prepared{0};                        // devices
+    int device = 0;
+    DSV3_CUDA_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1)) {
+        DSV3_CUDA_TRY(cudaFuncSetAttribute(expanded_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        // (the warps that ask for more registers wait for those that the block does not have)
+        cudaFuncAttributes attr = {};
+        DSV3_CUDA_TRY(cudaFuncGetAttributes(&attr, expanded_attention_kernel));
+        if (attr.numRegs * kThreads < kSoftmaxRegs * 256 + kOtherRegs * 128) {
+            set_last_error("expanded_attention: built with %d registers a thread, too few to share out", attr.numRegs);
+            return DSV3_ERR_UNSUPPORTED;
+        }
+        if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
+    return DSV3_OK;
+}
+
+}  // namespace
+}  // namespace dsv3
+
+using namespace dsv3;
+
+extern "C" {
+
+size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged) {
+    if (tokens <= 0 || kv_tokens <= 0 || heads <= 0 || n_seqs <= 0) return 0;
+    return partial_bytes(plan_of(tokens, kv_tokens, heads, n_seqs, ragged != 0, device_sms()), tokens, heads);
+}
+
+int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace, size_t workspace_bytes, dsv3_stream_t stream) {
+    if (!a || a->tokens < 0 || a->kv_tokens < 0 || a->heads < 0 || a->n_seqs < 0) {
+        set_last_error("expanded_attention: no arguments, or a negative size");
+        return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    if (a->tokens == 0 || a->heads == 0) return DSV3_OK;
+    if (!a->q_nope || !a->q_rope || !a->out || (a->kv_tokens > 0 && (!a->k_nope || !a->k_rope || !a->v))) {
+        set_last_error("expanded_attention: null pointer");
+        return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    const bool ragged = a->cu_seqlens_q != nullptr;
+    if (a->n_seqs == 0 || (!ragged && a->tokens % a->n_seqs != 0) || (!a->cu_seqlens_k && a->kv_tokens % a->n_seqs != 0)) {
+        set_last_error("expanded_attention: %lld queries or %lld keys do not divide among %d sequences", static_cast<long long>(a->tokens),
+                       static_cast<long long>(a->kv_tokens), a->n_seqs);
+        return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    if (!(a->softmax_scale > 0.0f) || a->softmax_scale > 1e30f) {
+        set_last_error("expanded_attention: softmax_scale must be positive and finite");
+        return DSV3_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t strides = a->q_nope_token_stride | a->q_nope_head_stride | a->q_rope_token_stride | a->q_rope_head_stride | a->k_nope_token_stride |
+                            a->k_nope_head_stride | a->k_rope_token_stride | a->v_token_stride | a->v_head_stride;
+    const uintptr_t pointers = reinterpret_cast<uintptr_t>(a->q_nope) | reinterpret_cast<uintptr_t>(a->q_rope) | reinterpret_cast<uintptr_t>(a->out) |
+                               (a->kv_tokens > 0 ? reinterpret_cast<uintptr_t>(a->k_nope) | reinterpret_cast<uintptr_t>(a->k_rope) | reinterpret_cast<uintptr_t>(a->v) : 0);
+    if (strides % 8 != 0 || strides < 0 || pointers % 16 != 0) {
+        set_last_error("expanded_attention: rows of queries, keys, values and out must be 16-byte aligned, strides not negative");
+        return DSV3_ERR_UNSUPPORTED;
+    }
+    const int sms = device_sms();
+    const Plan pl = plan_of(a->tokens, std::max<int64_t>(1, a->kv_tokens), a->heads, a->n_seqs, ragged, sms);
+    if (a->heads > 1024 || a->tokens > 0x7FFFFF00ll || a->kv_tokens > 0x7FFFFF00ll || pl.blocks * a->heads * pl.splits > 0x7FFFFFFFll) {
+        set_last_error("expanded_attention: more than 1024 heads, or 2^31 queries, keys or blocks of queries");
+        return DSV3_ERR_UNSUPPORTED;
+    }
+    const size_t need = partial_bytes(pl, a->tokens, a->heads);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) {
+        set_last_error("expanded_attention: the workspace must be 16-byte aligned and hold %zu bytes", need);
+        return DSV3_ERR_WORKSPACE;
+    }
+    unsigned int* const status = status_device_ptr();
+    if (!status) return DSV3_ERR_CUDA;
+    if (const int rc = prepare_kernel(); rc != DSV3_OK) return rc;
+    CUtensorMap qn, qr, kn, kr, v;
+    // (without keys nothing is loaded; the maps then describe the queries)
+    const bool keys = a->kv_tokens > 0;
+    int rc;
+    if ((rc = make_tmap_heads(&qn, a->q_nope, kNope, a->heads, a->tokens, a->q_nope_head_stride, a->q_nope_token_stride, kHalf)) != DSV3_OK) return rc;
+    if ((rc = make_tmap_heads(&qr, a->q_rope, kRope, a->heads, a->tokens, a->q_rope_head_stride, a->q_rope_token_stride, kHalf)) != DSV3_OK) return rc;
+    if (!keys) {
+        kn = v = qn;
+        kr = qr;
+    } else {
+        if ((rc = make_tmap_heads(&kn, a->k_nope, kNope, a->heads, a->kv_tokens, a->k_nope_head_stride, a->k_nope_token_stride, kTile)) != DSV3_OK) return rc;
+        if ((rc = make_tmap_heads(&kr, a->k_rope, kRope, 1, a->kv_tokens, 0, a->k_rope_token_stride, kTile)) != DSV3_OK) return rc;
+        if ((rc = make_tmap_heads(&v, a->v, kValue, a->heads, a->kv_tokens, a->v_head_stride, a->v_token_stride, kTile / 2)) != DSV3_OK) return rc;
+    }
+    const int64_t items = pl.blocks * a->heads * pl.splits, rows = a->tokens * a->heads;
+    // A CTA takes the place of one that has not started, so that no SM waits while there is work; with a budget of SMs, whose rest is not to be touched, CTAs take turns
+    const bool dynamic = !sm_budget_set();
+    float* const partial = need ? static_cast<float*>(workspace) : nullptr;
+    Params p = {};
+    p.tokens = static_cast<int>(a->tokens), p.kv_tokens = static_cast<int>(a->kv_tokens), p.heads = a->heads, p.n_seqs = a->n_seqs;
+    p.cu_q = a->cu_seqlens_q, p.cu_k = a->cu_seqlens_k;
+    p.per_q = ragged ? 0 : static_cast<int>(a->tokens / a->n_seqs), p.per_k = a->cu_seqlens_k ? 0 : static_cast<int>(a->kv_tokens / a->n_seqs);
+    p.causal = a->causal != 0;
+    p.scale = a->softmax_scale * kLog2e;
+    p.head_group = pl.head_group, p.splits = pl.splits, p.dynamic = dynamic;
+    p.out = static_cast<__nv_bfloat16*>(a->out), p.lse = a->lse;
+    p.partial = partial, p.partial_lse = need ? partial + pl.splits * rows * kValue : nullptr;
+    const int64_t grid = dynamic ? items : std::min<int64_t>(items, num_sms());
+    DSV3_CUDA_TRY(launch_dependent(expanded_attention_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kSmemBytes, static_cast<cudaStream_t>(stream), qn, qr, kn,
+                                   kr, v, p, status));
+    if (!need) return DSV3_OK;
+    return join_partials(partial, p.partial_lse, pl.splits, rows, kValue, p.cu_q, a->n_seqs, a->heads, a->out, a->lse, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

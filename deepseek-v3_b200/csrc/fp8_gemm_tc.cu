@@ -852,6 +852,30 @@ int make_tmap_groups(CUtensorMap* map, const void* base, int64_t rows, int64_t K
     return DSV3_OK;
 }
 
+// [rows, heads, width] bf16 with any strides (in elements, multiples of 8) of rows and heads; box = 64 values (128 bytes) of one head x box_rows rows, 128-byte swizzle, zero
+// fill outside.
+int make_tmap_heads(CUtensorMap* map, const void* base, int width, int64_t heads, int64_t rows, int64_t head_stride, int64_t row_stride, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) {
+        set_last_error("cuTensorMapEncodeTiled is not available from the driver");
+        return DSV3_ERR_CUDA;
+    }
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    // (a dimension of one has no stride)
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? head_stride : width) * 2, static_cast<cuuint64_t>(rows > 1 ? row_stride : heads * width) * 2};
+    const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled (heads) failed with CUresult %d (rows=%lld heads=%lld width=%d strides=%lld,%lld)", static_cast<int>(r),
+                       static_cast<long long>(rows), static_cast<long long>(heads), width, static_cast<long long>(row_stride), static_cast<long long>(head_stride));
+        return DSV3_ERR_CUDA;
+    }
+    return DSV3_OK;
+}
+
 // Result matrix [M, N] bf16, row-major; box = 64 columns (128 bytes) x box_rows rows, 128-byte swizzle.
 int make_tmap_out(CUtensorMap* map, void* base, int64_t M, int64_t N, int box_rows) {
     EncodeTiledFn fn = encode_fn();

@@ -873,6 +873,7 @@ PyObject* py_drop_workspaces(PyObject*, PyObject*) {
 }
 
 #include "host_latent.inl"
+#include "host_expanded.inl"
 
 PyMethodDef methods[] = {
     {"set_error_class", py_set_error_class, METH_O, "class raised for a non-zero status: cls(status, message)"},
@@ -904,6 +905,12 @@ PyMethodDef methods[] = {
      "(latent, rope, scale, block_table, first, path, count)"},
     {"latent_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_latent_attention)), METH_FASTCALL,
      "(q_latent, q_rope, latent, rope, scale, block_table, seq_lens, softmax_scale, cu_seqlens_q, tree_mask, return_lse)"},
+    {"expanded_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_expanded_attention)), METH_FASTCALL,
+     "(q_nope, q_rope, k_nope, k_rope, v, softmax_scale, cu_seqlens_q, cu_seqlens_k, causal, return_lse)"},
+    {"attention_join", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_attention_join)), METH_FASTCALL, "(outs, lses, return_lse)"},
+    {"rotary_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_rotary_table)), METH_FASTCALL,
+     "(length, dim, theta, factor, original_length, beta_fast, beta_slow, start, device)"},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_rotary)), METH_FASTCALL, "(x, freqs, positions, half_layout, offset, inverse, out)"},
     {"set_stats", py_set_stats, METH_O, "dict whose counters linear() keeps"},
     {"forget", py_forget, METH_NOARGS, "drop the remembered quantisations"},
     {"drop_workspaces", py_drop_workspaces, METH_NOARGS, "give the split-K workspaces back"},

@@ -34,6 +34,7 @@ EXPORTS = (
     "dsv3_fp8_linear", "dsv3_swiglu_quant", "dsv3_selftest_bounded_wait", "dsv3_p2p_handle_bytes", "dsv3_p2p_create", "dsv3_p2p_connect", "dsv3_p2p_connect_local", "dsv3_p2p_base",
     "dsv3_allreduce_oneshot", "dsv3_allreduce_oneshot_pair_on_one_gpu", "dsv3_p2p_destroy", "dsv3_set_num_sms",
     "dsv3_latent_write", "dsv3_latent_read", "dsv3_latent_keep", "dsv3_latent_attention_workspace_bytes", "dsv3_latent_attention",
+    "dsv3_expanded_attention_workspace_bytes", "dsv3_expanded_attention", "dsv3_attention_join", "dsv3_rotary_table", "dsv3_rotary",
 )
 
 

@@ -395,6 +395,85 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
                           float* lse, void* workspace, size_t workspace_bytes, dsv3_stream_t stream);
 
 /*
+ * Attention of a prompt's queries over expanded keys and values -- the scores, softmax and weighted sum of model.py:486-494 as its `naive` branch
+ * (model.py:472-478, 487, 493) has them: every head has keys and values of its own, which `wkv_b` makes of the latents, and the rotated part of the keys is shared:
+ *   x[t, h, p] = q_nope[t, h] . k_nope[p, h] + q_rope[t, h] . k_rope[p]
+ *   out[t, h]  = sum over the keys p that t sees of softmax_p(softmax_scale * x[t, h, p]) v[p, h]
+ *   lse[t, h]  = log of the sum of exp(softmax_scale * x) (natural; optional: null)
+ * 2 * (192 + 128) operations per head, query and key, where absorbed queries take 2 * (576 + 512): the form for prompts and chunks of them.
+ *   q_nope bf16 [tokens, heads, 128], q_rope [tokens, heads, 64]; k_nope [kv_tokens, heads, 128], k_rope [kv_tokens, 64], v [kv_tokens, heads, 128]: last dimensions
+ *     contiguous, rows 16-byte aligned, strides of tokens and heads multiples of 8 elements, not negative; 1 <= heads <= 1024
+ *   cu_seqlens_q, cu_seqlens_k: int32 [n_seqs + 1] in device memory, not decreasing: sequence b owns queries [cu_q[b], cu_q[b + 1]) and keys [cu_k[b], cu_k[b + 1]).
+ *     Null: tokens / n_seqs queries, kv_tokens / n_seqs keys each.  Rows of out and lse before cu_q[0], and at and beyond cu_q[n_seqs], are left as they are; what keys and values
+ *     hold there does not matter.
+ *   causal : a sequence's queries are its last keys, each sees itself and all before it.  0: each sees all of its sequence's keys.
+ *   softmax_scale: positive
+ *   out bf16 [tokens, heads, 128], lse fp32 [tokens, heads], contiguous.  A query that sees nothing: zeros, and -inf.
+ * A key that is not finite makes the results of the queries that see it NaN, a value that is not finite makes them NaN or infinite in its dimension at least; others are not touched by it.
+ * workspace: dsv3_expanded_attention_workspace_bytes() bytes (ragged: cu_seqlens_q is not null), 16-byte aligned, not shared by calls that can overlap; its contents do not matter.  The size is that of
+ * exactly these arguments on the current device, 0 for most; dsv3_set_num_sms does not change it.
+ */
+#define DSV3_NOPE_DIM 128
+#define DSV3_VALUE_DIM 128
+typedef struct dsv3_expanded_attention {
+    const void* q_nope;
+    int64_t q_nope_token_stride, q_nope_head_stride;
+    const void* q_rope;
+    int64_t q_rope_token_stride, q_rope_head_stride;
+    const void* k_nope;
+    int64_t k_nope_token_stride, k_nope_head_stride;
+    const void* k_rope;
+    int64_t k_rope_token_stride;
+    const void* v;
+    int64_t v_token_stride, v_head_stride;
+    int64_t tokens, kv_tokens;
+    int heads, n_seqs;
+    const int32_t* cu_seqlens_q;
+    const int32_t* cu_seqlens_k;
+    int causal;
+    float softmax_scale;
+    void* out;
+    float* lse;
+} dsv3_expanded_attention_t;
+size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged);
+int dsv3_expanded_attention(const dsv3_expanded_attention_t* args, void* workspace, size_t workspace_bytes, dsv3_stream_t stream);
+
+/*
+ * The results of the same queries over several pieces of their keys (of a long prefix, say; of dsv3_expanded_attention or dsv3_latent_attention), joined:
+ *   lse = log sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
+ *   outs : host array of `parts` (1 .. 32) pointers to bf16 [rows, dim], contiguous, 16-byte aligned; dim a multiple of 8, up to 2048
+ *   lses : host array of pointers to fp32 [rows].  Where a part's is -inf (it sees nothing) its row is not read; where all are: zeros, and -inf
+ *   out  : bf16 [rows, dim], may be one of the parts; lse: fp32 [rows], may be one of the parts' (or null)
+ */
+int dsv3_attention_join(const void* const* outs, const float* const* lses, int parts, int64_t rows, int dim, void* out, float* lse, dsv3_stream_t stream);
+
+/*
+ * Angles of rotary positions -- precompute_freqs_cis, model.py:297-375: for positions start .. start + length - 1 and i < dim / 2
+ *   out[position, i] = exp(1j * position * f_i),  f_i = theta^(-2 i / dim), and for a factor other than 1 (contexts longer than original_length, that the model was trained on)
+ *   f_i / factor * ramp + f_i * (1 - ramp),  ramp = (i - low) / (high - low) held to 0 .. 1, low and high the indices (rounded down and up, held to 0 .. dim - 1) of the angles
+ *   that turn beta_fast and beta_slow times over original_length: dim log(original_length / (2 pi beta)) / (2 log theta)
+ * complex64 [length, dim / 2]; angles are formed in 64 bits (the reference: 32, which at position 100000 is off by 0.004).  dim even, at most 256.
+ */
+int dsv3_rotary_table(int dim, double theta, double factor, int64_t original_length, double beta_fast, double beta_slow, int64_t start, int64_t length,
+                      float* out, dsv3_stream_t stream);
+
+/*
+ * Rotation of heads, or of a part of them -- apply_rotary_emb, model.py:378-393: values offset .. offset + rotated - 1 of every head are pairs (a, b), which become
+ * (a c - b s, a s + b c), c + i s being freqs[position]; inverse: with -s (which turns back, and is the gradient).  Pairs are neighbours, or (half_layout) value i of
+ * the part and value i + rotated / 2.  Other values are copied.  Arithmetic in fp32, rounded once.
+ *   x, out    : [tokens, heads, dim] of dtype, last dimension contiguous, heads 16-byte aligned; strides in elements.  out may be x (with x's strides: in place), and
+ *               otherwise does not overlap it.  dim and offset multiples of 8, rotated of 16; dim at most 1024, rotated 256
+ *   freqs     : complex64 [n_positions, rotated / 2], contiguous
+ *   positions : int64 [tokens]; null: token t is at position t mod per.  A token at a position that the table does not hold becomes NaN (the rotated part)
+ */
+#define DSV3_BF16 0
+#define DSV3_FP16 1
+#define DSV3_FP32 2
+int dsv3_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, int dtype,
+                int64_t tokens, int heads, int dim, const float* freqs, int64_t n_positions, const int64_t* positions, int64_t per, int offset, int rotated,
+                int half_layout, int inverse, dsv3_stream_t stream);
+
+/*
  * One-shot all-reduce of a decode-sized bf16 tensor over peer-mapped buffers -- replaces `dist.all_reduce(y)` after
  * a row-parallel Linear and after the MoE expert loop (model.py:263-264, 691-692) for small y, where a ring or tree
  * collective is bound by latency.  One process per GPU; every rank
