@@ -331,7 +331,7 @@ int dsv3_check_device_status(dsv3_stream_t stream, uint32_t detail[4]) {
     DSV3_CUDA_TRY(cudaMemcpy(dptr, zero, sizeof(zero), cudaMemcpyHostToDevice));
     set_last_error("device wait gave up: kind=%u (1 smem-empty, 2 smem-full, 3 tmem-empty, 4 tmem-full, 7/8 scale table, "
                    "9 self-test, 10 all-reduce peer signal, 11-15 latent attention's weights, room for weights, queries, room for sums, lists, "
-                   "16-21 expanded attention's weights, sums, queries, looked-at values, items, halves) counter=%u cta=%u",
+                   "16-22 expanded attention's weights, sums, queries, looked-at values, items, room for rows, room for weights) counter=%u cta=%u",
                    host[1], host[2], host[3]);
     return DSV3_ERR_DEVICE_TIMEOUT;
 }

@@ -33,20 +33,24 @@ constexpr int kHalf = 128, kBlock = 2 * kHalf;   // queries
 constexpr int kTile = 128;                       // keys
 // Operands lie as rows of 64 values (128 bytes, swizzled).  Keys and values come through a ring of slots of 16 KB: three to a tile of keys (64 dimensions of 128 keys
 // each), two to one of values (64 keys of 128 dimensions each): beside the queries there is room for eight, one and a half tiles of both.
-constexpr int kSlots = 8, kSlotBytes = 16384, kKeySlots = 3, kValueSlots = 2, kTileSlots = kKeySlots + kValueSlots;
+constexpr int kSlots = 8, kSlotBytes = 16384, kKeySlots = 3, kValueSlots = 2;
+// A tile's keys, or its values, are a unit, which is waited for and given back as a whole; no more than four of either are on their way.
+constexpr int kUnits = 4;
 constexpr int kQueryBytes = kKeySlots * kSlotBytes;
 constexpr int kOperandBytes = kSlots * kSlotBytes + 2 * kQueryBytes;
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10, kThreads = 384;
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
-static_assert(kSoftmaxRegs * 256 + kOtherRegs * 128 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
-constexpr int kTmemScores = 0, kTmemSums = 2 * kTile, kTmemCols = 512;
-constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 2;
+constexpr int kSoftmaxWarps = 8, kScoreWarp = 8, kLoadWarp = 9, kGuardWarp = 10, kSumWarp = 11, kFinishWarp = 12, kFinishWarps = 4, kThreads = 512;
+constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
+static_assert(kSoftmaxRegs * 256 + kOtherRegs * 256 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
+constexpr int kTmemScores = 0, kTmemWeights = kTile, kTmemSums = 2 * kTile, kTmemCols = 512;   // columns; weights: 64 to a half, sums: 128
+constexpr int kAhead = 1;                        // tiles that scores are ahead of sums (twice as many where halves take turns)
+constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 3 + kFinishWarps;
 constexpr int kLanes = 32;                       // sequences that are put in order of their length
 // What a wait that gave up was for (kinds of dsv3_check_device_status)
-constexpr uint32_t kRoom = 1, kTileThere = 2, kScoresThere = 4, kWeightsThere = 16, kSumsThere = 17, kQueriesThere = 18, kGuarded = 19, kItems = 20, kHalves = 21;
+constexpr uint32_t kRoom = 1, kTileThere = 2, kScoresRoom = 3, kScoresThere = 4, kWeightsThere = 16, kSumsThere = 17, kQueriesThere = 18, kGuarded = 19, kItems = 20, kRowsRoom = 21, kWeightsRoom = 22;
 constexpr uint64_t kItemLimitNs = 100 * kWaitLimitNs;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kSlack = 8.0f;
+// A row's reference moves where a weight would pass 2^kSlack: bf16 weights and fp32 sums have the range for more, and the same bits wherever they are.
+constexpr float kSlack = 32.0f;
 
 struct Params {
     int tokens, kv_tokens, heads, n_seqs;
@@ -75,12 +79,12 @@ struct Item {
 };
 
 struct Small {
-    uint64_t full[kSlots], empty[kSlots];
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], guarded[2], item_full[kItemSlots], item_empty[kItemSlots], halves_full, halves_done, taken;
+    uint64_t k_full[kUnits], k_empty[kUnits], v_full[kUnits], v_empty[kUnits];
+    uint64_t q_full[2], q_empty[2], s_full[2], s_empty, p_full[2][kValueSlots], p_empty[2], o_full[2], guarded[2], item_full[kItemSlots], item_empty[kItemSlots], row_full[2], row_empty[2], o_empty[2], taken;
     Item item[kItemSlots];
     int not_finite[kItemSlots];           // first key whose values are not finite, of those in tiles that are not seen as a whole
     alignas(16) uint32_t answer[4];
-    float2 row[2][kHalf];                 // reference and sum of the halves' rows, where they are joined
+    float2 row[2][kHalf];                 // reference and sum of the halves' rows
     Control ctl;
 };
 constexpr int kSmallBytes = 3072, kSmemBytes = kSmallBytes + kOperandBytes;
@@ -118,6 +122,12 @@ __device__ __forceinline__ void tc_st_x32(uint32_t taddr, const uint32_t* r) {
         "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tc_st_x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+                 "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int x, int head, int row, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x),
@@ -142,6 +152,37 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "=f"(r.x), "=f"(r.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {    // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 16 N bytes of each of the warp's 32 rows, `stride` bytes apart, of which this lane has one (w) and writes 16 bytes of N: a store of 16 bytes to 32 rows takes 32 passes
+// through the L1, one of N neighbouring lanes to a row 32 / N.  Rows at and beyond `rows` are not written.
+template <int kWords>
+__device__ __forceinline__ void store_rows(uint32_t (&w)[kWords], void* first, int64_t stride, int rows) {
+    constexpr int N = kWords / 4;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int a = 0; a < N; ++a) {
+            if (a & o) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t &lo = w[4 * a + k], &hi = w[4 * (a + o) + k];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, o);
+                if (up) lo = got;
+                else hi = got;
+            }
+        }
+    }
+    char* const to = static_cast<char*>(first) + (lane & ~(N - 1)) * stride + (lane & (N - 1)) * 16;
+#pragma unroll
+    for (int r = 0; r < N; ++r)
+        if ((lane & ~(N - 1)) + r < rows) *reinterpret_cast<uint4*>(to + r * stride) = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
 }
 // Takes the place of a CTA of the grid that has not started; the answer (16 bytes) says whose.
 __device__ __forceinline__ void try_cancel(uint32_t answer, uint32_t bar) {
@@ -299,10 +340,25 @@ struct List {
     }
 };
 
-// Slots of an item's tiles, from its first on, in the order in which the MMAs come to them: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 ... where tiles alternate.
-__device__ __forceinline__ uint32_t key_slot(const Item& it, int t) { return it.alternate && t > 0 ? kTileSlots * t - kValueSlots : kTileSlots * t; }
-__device__ __forceinline__ uint32_t value_slot(const Item& it, int t) {
-    return it.alternate && t + 1 < it.n ? kTileSlots * (t + 1) + 1 : kTileSlots * t + kKeySlots;
+// An item's units in the order in which they are loaded and the MMAs come to them: K0 K1 V0 K2 V1 ... V(n-1), or K0 K1 K2 V0 K3 V1 ... where tiles alternate.
+struct Unit {
+    bool keys;
+    int tile;
+};
+__device__ __forceinline__ Unit unit_of(const Item& it, int u) {
+    const int ahead = min(it.alternate ? 2 * kAhead : kAhead, it.n);
+    if (u < ahead) return {true, u};
+    u -= ahead;
+    const int both = 2 * (it.n - ahead);                             // units that come in pairs
+    if (u < both) return {(u & 1) == 0, (u >> 1) + ((u & 1) == 0 ? ahead : 0)};
+    return {false, u - (it.n - ahead)};
+}
+
+// The slot of tile t's keys or values, from the item's first on.
+__device__ __forceinline__ uint32_t unit_slot(bool alternate, int n, int t, bool keys) {
+    const int ahead = min(alternate ? 2 * kAhead : kAhead, n);
+    if (keys) return kKeySlots * t + (t >= ahead ? kValueSlots * (t - ahead) : 0);
+    return kKeySlots * min(t + ahead + 1, n) + kValueSlots * t;
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -318,30 +374,35 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
 
     griddep_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kSlots; ++i) {
-            mbar_init(bar(sm.full[i]), 1);
-            mbar_init(bar(sm.empty[i]), 2);                          // the MMAs, and the warp that looks at values
+        for (int i = 0; i < kUnits; ++i) {
+            mbar_init(bar(sm.k_full[i]), 1);
+            mbar_init(bar(sm.k_empty[i]), 1);
+            mbar_init(bar(sm.v_full[i]), 1);
+            mbar_init(bar(sm.v_empty[i]), 2);                        // the MMAs, and the warp that looks at values
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(sm.q_full[i]), 1);
             mbar_init(bar(sm.q_empty[i]), 1);
             mbar_init(bar(sm.s_full[i]), 1);
-            mbar_init(bar(sm.p_full[i]), kSoftmaxWarps / 2);
+            for (int j = 0; j < kValueSlots; ++j) mbar_init(bar(sm.p_full[i][j]), kSoftmaxWarps / 2);
+            mbar_init(bar(sm.p_empty[i]), 1);
             mbar_init(bar(sm.o_full[i]), 1);
             mbar_init(bar(sm.guarded[i]), 1);
+            mbar_init(bar(sm.row_full[i]), kSoftmaxWarps / 2);
+            mbar_init(bar(sm.row_empty[i]), kFinishWarps);
+            mbar_init(bar(sm.o_empty[i]), kFinishWarps);
         }
         for (int i = 0; i < kItemSlots; ++i) {
             mbar_init(bar(sm.item_full[i]), 1);
             mbar_init(bar(sm.item_empty[i]), kItemReaders);
         }
-        mbar_init(bar(sm.halves_full), kSoftmaxWarps);
-        mbar_init(bar(sm.halves_done), kSoftmaxWarps);
+        mbar_init(bar(sm.s_empty), kSoftmaxWarps / 2);
         mbar_init(bar(sm.taken), 1);
         mbar_fence_init();
         ctl->abort_flag = (ring & 1023u) != 0 ? 1u : 0u;             // (dynamic shared memory begins at a multiple of 1024; swizzled tiles rely on it)
         if (ctl->abort_flag && atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = kRoom, status[2] = 0xFFFFFFFFu, status[3] = blockIdx.x;
     }
-    if (warp == kMmaWarp) tc_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+    if (warp == kScoreWarp) tc_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
     if (warp == kLoadWarp && lane == 0) {
         tma_prefetch_desc(&map_qn);
         tma_prefetch_desc(&map_qr);
@@ -357,7 +418,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
     const bool well = ctl->abort_flag == 0;
     // Whole warp: the item in the next slot of the list's ring, or one without rows.
     const auto wait = [&](const uint64_t& b, uint32_t parity, uint32_t what, uint32_t count) -> bool {
-        return __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, count));
+        return __all_sync(0xffffffffu, mbar_try_wait(bar(b), parity)) || __all_sync(0xffffffffu, bounded_wait(bar(b), parity, ctl, status, what, count));
     };
     const auto next_item = [&](uint32_t count, bool& ok) -> Item {
         Item it = {};
@@ -365,6 +426,9 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         if (ok) it = sm.item[count % kItemSlots];
         return it;
     };
+    // The same in all lanes, and known to be: branches and addresses that depend on it stay uniform, which the tensor core's instructions want (their operands are uniform registers: those of
+    // a lane go there one by one, 30 cycles an MMA more than it takes).
+    const auto uniform = [](int x) -> int { return __shfl_sync(0xffffffffu, x, 0); };
     const auto item_done = [&](uint32_t count) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(sm.item_empty[count % kItemSlots]));
@@ -379,15 +443,30 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             // ------------------------------------------------------------ the list, and the loads
             List list;
             list.begin(p);
-            uint32_t slot = 0, active = 0, taken = 0;                    // slots filled; items with tiles
+            uint32_t slot = 0, unit = 0, active = 0, taken = 0;      // slots and units filled; items with tiles
+            uint32_t freed = 0, back = 0, keys = 0;                  // slots and units given back; which of the last 32 units are keys
+            uint32_t k_loaded = 0, v_loaded = 0, k_back = 0, v_back = 0;
             bool ok = true;
             int at = static_cast<int>(blockIdx.x);
-            const auto fill = [&](auto&& copy) {
-                const uint32_t s = slot % kSlots;
-                ok = ok && wait(sm.empty[s], ((slot / kSlots) & 1) ^ 1, kRoom, slot);
+            const auto one_back = [&](uint32_t newest) {             // the oldest unit on its way is given back
+                if (keys >> (newest - back) & 1) {
+                    ok = wait(sm.k_empty[k_back % kUnits], (k_back / kUnits) & 1, kRoom, back);
+                    freed += kKeySlots;
+                    ++k_back;
+                } else {
+                    ok = wait(sm.v_empty[v_back % kUnits], (v_back / kUnits) & 1, kRoom, back);
+                    freed += kValueSlots;
+                    ++v_back;
+                }
+                ++back;
+            };
+            // a slot of the unit at hand, when there is room for it
+            const auto fill = [&](bool first, const uint64_t& full, int slots, auto&& copy) {
+                if (first) keys = keys << 1 | (slots == kKeySlots ? 1u : 0u);
+                while (ok && slot + 1 - freed > kSlots) one_back(unit);
                 if (ok && elect_one()) {
-                    mbar_arrive_expect_tx(bar(sm.full[s]), kSlotBytes);
-                    copy(ring + s * kSlotBytes, bar(sm.full[s]));
+                    if (first) mbar_arrive_expect_tx(bar(full), slots * kSlotBytes);
+                    copy(ring + slot % kSlots * kSlotBytes, bar(full));
                 }
                 __syncwarp();
                 ++slot;
@@ -404,12 +483,15 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 }
                 __syncwarp();
                 if (it.rows == 0) break;
-                const bool more = p.dynamic;
-                if (more && elect_one()) {
-                    mbar_arrive_expect_tx(bar(sm.taken), 16);
-                    try_cancel(smem_u32(sm.answer), bar(sm.taken));
-                }
-                __syncwarp();
+                // The next item is asked for as late as its loads allow: who asks early takes work that another SM would be free for.
+                const auto ask = [&]() {
+                    if (p.dynamic && elect_one()) {
+                        mbar_arrive_expect_tx(bar(sm.taken), 16);
+                        try_cancel(smem_u32(sm.answer), bar(sm.taken));
+                    }
+                    __syncwarp();
+                };
+                if (it.n == 0) ask();
                 if (it.n > 0) {
                     const auto load_queries = [&](int h) {
                         ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
@@ -429,36 +511,39 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     };
                     const auto load_keys = [&](int t) {
                         const int row = it.k0 + (it.tile + t) * kTile;
-                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 0, it.head, row, full); });
-                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 64, it.head, row, full); });
-                        fill([&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kr, 0, 0, row, full); });
+                        const uint64_t& there = sm.k_full[k_loaded % kUnits];
+                        fill(true, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 0, it.head, row, full); });
+                        fill(false, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 64, it.head, row, full); });
+                        fill(false, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kr, 0, 0, row, full); });
+                        ++k_loaded;
+                        ++unit;
                     };
                     const auto load_values = [&](int t) {
 #pragma unroll
                         for (int i = 0; i < kValueSlots; ++i) {
                             const int row = it.k0 + (it.tile + t) * kTile + i * 64;
-                            fill([&](uint32_t to, uint32_t full) {
+                            fill(i == 0, sm.v_full[v_loaded % kUnits], kValueSlots, [&](uint32_t to, uint32_t full) {
                                 tma_load_3d(to, &map_v, 0, it.head, row, full);
                                 tma_load_3d(to + kSlotBytes / 2, &map_v, 64, it.head, row, full);
                             });
                         }
+                        ++v_loaded;
+                        ++unit;
                     };
                     load_queries(0);
-                    load_keys(0);
-                    load_queries(1);
-                    if (it.alternate && it.n > 1) load_keys(1);
-                    for (int t = 0; t < it.n && ok; ++t) {
-                        load_values(t);
-                        const int ahead = t + (it.alternate ? 2 : 1);
-                        if (ahead < it.n && ok) load_keys(ahead);
+                    for (int u = 0; u < 2 * it.n && ok; ++u) {
+                        const Unit w = unit_of(it, u);
+                        if (u == 2 * it.n - 2) ask();
+                        if (w.keys) load_keys(w.tile);
+                        else load_values(w.tile);
+                        if (u == 0) load_queries(1);
                     }
                     ++active;
                 }
-                if (more) {
-                    // (waited for in any case: the answer may not arrive in the shared memory of another CTA)
-                    const bool there = wait(sm.taken, taken & 1, kItems, taken);
+                if (!ok) break;
+                if (p.dynamic) {
+                    ok = wait(sm.taken, taken & 1, kItems, taken);
                     ++taken;
-                    ok = ok && there;
                     if (ok) {
                         at = cancelled_cta(smem_u32(sm.answer));
                         fence_proxy_async_shared();
@@ -469,196 +554,247 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 }
             }
             // none of the arrivals on empty[] may be in flight when the CTA leaves its shared memory to another
-            for (uint32_t s = slot > kSlots ? slot - kSlots : 0u; ok && s < slot; ++s) ok = wait(sm.empty[s % kSlots], (s / kSlots) & 1, kRoom, s);
+            while (ok && back < unit) one_back(unit - 1);
             for (int h = 0; h < 2 && ok && active > 0; ++h) ok = wait(sm.q_empty[h], (active - 1) & 1, kQueriesThere, active);
-        } else if (warp == kMmaWarp) {
-            // ------------------------------------------------------------ the MMAs.  The warp stays converged and elects a lane for them alone.
-            uint32_t slot = 0, active = 0, edges = 0, scores0 = 0, scores1 = 0;
+        } else if (warp == kScoreWarp) {
+            // ------------------------------------------------------------ the MMAs of the scores.  Those of the sums have a warp of their own: an MMA takes 64 cycles, and what lies between
+            // two groups of them (waits that need not wait, 100 cycles each; addresses) as long as several.  The warps stay converged and elect a lane for the MMAs alone.
+            uint32_t slot = 0, keys = 0, active = 0, scored = 0;
+            const uint64_t ring_desc = umma_desc_k_major_sw128(ring), query_desc = umma_desc_k_major_sw128(queries);
             bool ok = true;
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
-                if (!ok || it.rows == 0) break;
+                const int n = uniform(it.n), n0 = uniform(it.n0), step = uniform(it.alternate);
+                if (!ok || uniform(it.rows) == 0) break;
                 item_done(count);
-                if (it.n == 0) continue;
-                const auto slot_at = [&](uint32_t i) { return (slot + i) % kSlots; };
-                const auto await = [&](uint32_t first, int n) {
-                    for (int i = 0; i < n; ++i) ok = ok && wait(sm.full[slot_at(first + i)], ((slot + first + i) / kSlots) & 1, kTileThere, slot + first + i);
-                };
-                // scores of tile t for half h; `done`: the tile's keys are not needed any more, `all`: nor the half's queries
-                const auto score = [&](int h, int t, bool done, bool all) {
-                    const uint32_t first = key_slot(it, t), d = tmem + kTmemScores + h * kTile, q = queries + (it.alternate ? 0 : h * kQueryBytes);
-                    if (elect_one()) {
+                if (n == 0) continue;
+                for (int h = 0; h < 2; ++h) ok = ok && wait(sm.q_full[h], active & 1, kQueriesThere, active);
+#pragma unroll 1
+                for (int t = 0, u = 0; t < n && ok; ++t, ++keys) {
+                    u = unit_slot(step != 0, n, t, true);
+                    ok = wait(sm.k_full[keys % kUnits], (keys / kUnits) & 1, kTileThere, keys);
+                    // both halves, the first one only where it sees the tile; or every other tile's
+#pragma unroll 1
+                    for (int h = step ? t & 1 : t < n0 ? 0 : 1, end = step ? h + 1 : 2; h < end && ok; ++h, ++scored) {
+                        ok = wait(sm.s_empty, (scored & 1) ^ 1, kScoresRoom, scored);      // (the softmax has the scores before)
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t a = query_desc + (step ? 0 : h * (kQueryBytes >> 4));
+                        if (elect_one()) {
 #pragma unroll
-                        for (int c = 0; c < kKeySlots; ++c) {
-                            const uint32_t s = slot_at(first + c);
-                            const uint64_t a = umma_desc_k_major_sw128(q + c * kSlotBytes), b = umma_desc_k_major_sw128(ring + s * kSlotBytes);
+                            for (int c = 0; c < kKeySlots; ++c) {
+                                const uint64_t b = ring_desc + (slot + u + c) % kSlots * (kSlotBytes >> 4);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) tc_mma_bf16(d, a + 2 * k, b + 2 * k, kIdescScores, (c | k) != 0);
-                            if (done) tc_commit(bar(sm.empty[s]));
+                                for (int k = 0; k < 4; ++k) tc_mma_bf16(tmem + kTmemScores, a + c * (kSlotBytes >> 4) + 2 * k, b + 2 * k, kIdescScores, (c | k) != 0);
+                            }
+                            tc_commit(bar(sm.s_full[h]));
                         }
-                        tc_commit(bar(sm.s_full[h]));
-                        if (all) tc_commit(bar(sm.q_empty[h]));
-                        if (all && it.alternate) tc_commit(bar(sm.q_empty[h ^ 1]));
+                        __syncwarp();
                     }
+                    if (elect_one()) tc_commit(bar(sm.k_empty[keys % kUnits]));
                     __syncwarp();
-                };
-                const auto sum = [&](int h, int t, bool first, bool done, bool last) {
-                    const uint32_t at = value_slot(it, t), d = tmem + kTmemSums + h * kValue, a = tmem + kTmemScores + h * kTile;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int i = 0; i < kValueSlots; ++i) {
-                            const uint32_t s = slot_at(at + i);
-                            const uint64_t b = umma_desc_values(ring + s * kSlotBytes);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) tc_mma_bf16_ts(d, a + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), kIdescSums, !first || (i | k) != 0);
-                            if (done) tc_commit(bar(sm.empty[s]));
-                        }
-                        if (last) tc_commit(bar(sm.o_full[h]));
-                    }
-                    __syncwarp();
-                };
-                const auto weights = [&](int h) {
-                    const uint32_t count = h == 0 ? scores0 : scores1;
-                    ok = ok && wait(sm.p_full[h], (count - 1) & 1, kWeightsThere, count);
-                };
-                const auto values = [&](int t) {                         // (once a tile)
-                    await(value_slot(it, t), kValueSlots);
-                    if (it.tile + t >= it.edge) {
+                }
+                if (elect_one()) {
+                    tc_commit(bar(sm.q_empty[0]));
+                    tc_commit(bar(sm.q_empty[1]));
+                }
+                __syncwarp();
+                slot += (kKeySlots + kValueSlots) * n;
+                ++active;
+            }
+        } else if (warp == kSumWarp) {
+            // ------------------------------------------------------------ the MMAs of the sums
+            uint32_t slot = 0, values = 0, edges = 0, summed0 = 0, summed1 = 0;
+            const uint64_t ring_desc = umma_desc_values(ring);
+            bool ok = true;
+            for (uint32_t count = 0; ok; ++count) {
+                const Item it = next_item(count, ok);
+                const int n = uniform(it.n), n0 = uniform(it.n0), n1 = uniform(it.n1), step = uniform(it.alternate), edge = uniform(it.edge) - uniform(it.tile);
+                if (!ok || uniform(it.rows) == 0) break;
+                item_done(count);
+                // (the sums of the item before are read: waited for with every item, or the parities would not tell)
+                const auto sums_room = [&](int h) { ok = ok && wait(sm.o_empty[h], (count & 1) ^ 1, kSumsThere, count); };
+                if (n0 == 0) sums_room(0);
+                if (n1 == 0) sums_room(1);
+#pragma unroll 1
+                for (int t = 0; t < n && ok; ++t, ++values) {
+                    const uint32_t u = slot + unit_slot(step != 0, n, t, false);
+                    ok = wait(sm.v_full[values % kUnits], (values / kUnits) & 1, kTileThere, values);
+                    if (t >= edge) {
                         ok = ok && wait(sm.guarded[edges & 1], (edges >> 1) & 1, kGuarded, edges);
                         ++edges;
                     }
-                };
-                for (int h = 0; h < 2; ++h) ok = ok && wait(sm.q_full[h], active & 1, kQueriesThere, active);
-                if (it.alternate) {
-                    // half t & 1 takes tile t
-                    for (int t = 0; t < min(2, it.n) && ok; ++t) {
-                        await(key_slot(it, t), kKeySlots);
-                        if (!ok) break;
-                        tc_fence_after();
-                        score(t, t, true, t + 1 == it.n);
-                        t == 0 ? ++scores0 : ++scores1;
-                    }
-                    for (int t = 0; t < it.n && ok; ++t) {
-                        const int h = t & 1;
-                        weights(h);
-                        values(t);
-                        if (!ok) break;
-                        tc_fence_after();
-                        sum(h, t, t < 2, true, t + 2 >= it.n);
-                        if (t + 2 < it.n) {
-                            await(key_slot(it, t + 2), kKeySlots);
+#pragma unroll 1
+                    for (int h = step ? t & 1 : t < n0 ? 0 : 1, end = step ? h + 1 : 2; h < end && ok; ++h) {
+                        const uint32_t tile = h == 0 ? summed0 : summed1, d = tmem + kTmemSums + h * kValue, weights = tmem + kTmemWeights + h * (kTile / 2);
+                        // (as the weights arrive: those of 64 keys, and then the others)
+#pragma unroll
+                        for (int i = 0; i < kValueSlots; ++i) {
+                            const bool adds = t > step || i > 0;
+                            if (!adds) sums_room(h);
+                            ok = ok && wait(sm.p_full[h][i], tile & 1, kWeightsThere, tile);
                             if (!ok) break;
                             tc_fence_after();
-                            score(h, t + 2, true, t + 3 == it.n);
-                            h == 0 ? ++scores0 : ++scores1;
+                            const uint64_t b = ring_desc + (u + i) % kSlots * (kSlotBytes >> 4);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) tc_mma_bf16_ts(d, weights + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), kIdescSums, adds || k != 0);
+                                if (i + 1 == kValueSlots) {
+                                    tc_commit(bar(sm.p_empty[h]));
+                                    if (t + step + 1 >= (step ? n : h == 0 ? n0 : n1)) tc_commit(bar(sm.o_full[h]));
+                                }
+                            }
+                            __syncwarp();
                         }
+                        h == 0 ? ++summed0 : ++summed1;
                     }
-                } else {
-                    const int n0 = it.n0, n1 = it.n1;      // (n0 <= n1: the second half sees what the first one does)
-                    await(0, kKeySlots);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (n0 > 0) {
-                        score(0, 0, false, n0 == 1);
-                        ++scores0;
-                    } else if (elect_one()) {
-                        tc_commit(bar(sm.q_empty[0]));
-                    }
-                    score(1, 0, true, n1 == 1);
-                    ++scores1;
-                    for (int t = 0; t < n1 && ok; ++t) {
-                        const bool first_too = t < n0;
-                        if (first_too) weights(0);
-                        values(t);
-                        if (!ok) break;
-                        if (first_too) {
-                            tc_fence_after();
-                            sum(0, t, t == 0, false, t + 1 == n0);
-                        }
-                        if (t + 1 < n1) await(key_slot(it, t + 1), kKeySlots);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (t + 1 < n0) {
-                            score(0, t + 1, false, t + 2 == n0);
-                            ++scores0;
-                        }
-                        weights(1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        sum(1, t, t == 0, true, t + 1 == n1);
-                        if (t + 1 < n1) {
-                            score(1, t + 1, true, t + 2 == n1);
-                            ++scores1;
-                        }
-                    }
+                    if (elect_one()) tc_commit(bar(sm.v_empty[values % kUnits]));
+                    __syncwarp();
                 }
-                slot += kTileSlots * it.n;
-                ++active;
+                slot += (kKeySlots + kValueSlots) * n;
             }
         } else if (warp == kGuardWarp) {
-            // ------------------------------------------------------------ values that the MMA must not see.  The warp follows the ring slot by slot (a wait by parity is exact only
-            // for who has seen the phase before), and works on the tiles that are not seen as a whole by all queries.
+            // ------------------------------------------------------------ values that the MMA must not see.  The warp follows all values (a wait by parity is exact only for who has
+            // seen the phase before; so none are given back without it), and works on the tiles that are not seen as a whole by all queries.
             uint8_t* const base = smem + kSmallBytes;
-            uint32_t slot = 0, edges = 0;
+            uint32_t slot = 0, values = 0, edges = 0;
             bool ok = true;
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
                 if (!ok || it.rows == 0) break;
-                const uint32_t end = slot + kTileSlots * it.n, start = slot;
-                int t = 0;                                               // tile whose values come next
-                while (slot < end && ok) {
-                    const bool is_value = t < it.n && slot - start >= value_slot(it, t);
-                    const int n = is_value ? kValueSlots : kKeySlots;
-                    const bool look = is_value && it.tile + t >= it.edge;
-                    for (int i = 0; i < n && ok; ++i, ++slot) {
-                        const uint32_t s = slot % kSlots;
-                        ok = wait(sm.full[s], (slot / kSlots) & 1, kTileThere, slot);
-                        if (!ok) break;
-                        if (look) {
-                            const int key0 = (it.tile + t) * kTile + i * 64;
-                            uint4* const at = reinterpret_cast<uint4*>(base + s * kSlotBytes);
-                            // 64 keys x 8 pieces of 16 bytes, twice; rows are keys, and a row's pieces stay in it
-                            __nv_bfloat162 seen = __floats2bfloat162_rn(0.0f, 0.0f);
-                            const __nv_bfloat162 zero = seen;
+                for (int t = 0; t < it.n; ++t, ++values) {
+                    const bool look = it.tile + t >= it.edge;
+                    ok = wait(sm.v_full[values % kUnits], (values / kUnits) & 1, kTileThere, values);
+                    if (!ok) break;
+                    const uint32_t u = slot + unit_slot(it.alternate, it.n, t, false);
+                    for (int i = 0; i < kValueSlots && look; ++i) {
+                        const int key0 = (it.tile + t) * kTile + i * 64;
+                        uint4* const at = reinterpret_cast<uint4*>(base + (u + i) % kSlots * kSlotBytes);
+                        // 64 keys x 8 pieces of 16 bytes, twice; rows are keys, and a row's pieces stay in it
+                        __nv_bfloat162 seen = __floats2bfloat162_rn(0.0f, 0.0f);
+                        const __nv_bfloat162 zero = seen;
 #pragma unroll 8
+                        for (int j = 0; j < kSlotBytes / 512; ++j) {
+                            const int key = key0 + ((j * 32 + lane) >> 3 & 63);
+                            if (key >= it.len) {
+                                at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                            } else {
+                                const uint4 v = at[j * 32 + lane];
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) seen = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, seen);   // NaN stays
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, __hisnan(seen.x) || __hisnan(seen.y))) {
+                            int bad = 0x7FFFFFFF;
                             for (int j = 0; j < kSlotBytes / 512; ++j) {
                                 const int key = key0 + ((j * 32 + lane) >> 3 & 63);
-                                if (key >= it.len) {
+                                const uint4 v = at[j * 32 + lane];
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                bool finite = true;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) finite = finite && (w[e] & 0x7F80u) != 0x7F80u && (w[e] & 0x7F800000u) != 0x7F800000u;
+                                if (!finite) {
+                                    bad = min(bad, key);
                                     at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
-                                } else {
-                                    const uint4 v = at[j * 32 + lane];
-                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) seen = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, seen);   // NaN stays
                                 }
                             }
-                            if (__any_sync(0xffffffffu, __hisnan(seen.x) || __hisnan(seen.y))) {
-                                int bad = 0x7FFFFFFF;
-                                for (int j = 0; j < kSlotBytes / 512; ++j) {
-                                    const int key = key0 + ((j * 32 + lane) >> 3 & 63);
-                                    const uint4 v = at[j * 32 + lane];
-                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                                    bool finite = true;
+                            bad = __reduce_min_sync(0xffffffffu, bad);
+                            if (lane == 0) atomicMin(&sm.not_finite[count % kItemSlots], bad);
+                        }
+                    }
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (look) mbar_arrive(bar(sm.guarded[edges & 1]));
+                        mbar_arrive(bar(sm.v_empty[values % kUnits]));
+                    }
+                    if (look) ++edges;
+                }
+                slot += (kKeySlots + kValueSlots) * it.n;
+                item_done(count);
+            }
+        } else if (warp >= kFinishWarp) {
+            // ------------------------------------------------------------ results: sums divided and written, while the softmax goes on with the next item.  (By the softmax' own warps:
+            // 4000 cycles an item that they did not work.)
+            const int quarter = warp - kFinishWarp;
+            const uint32_t sums_at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemSums;
+            const float c = p.scale;
+            uint32_t sums0 = 0, sums1 = 0;
+            bool ok = true;
+            for (uint32_t count = 0; ok; ++count) {
+                const Item it = next_item(count, ok);
+                if (!ok || it.rows == 0) break;
+                const int not_finite_at = static_cast<int>(count % kItemSlots);
+                const auto half_there = [&](int h) {
+                    ok = ok && wait(sm.row_full[h], count & 1, kSumsThere, count);
+                    if ((h == 0 ? it.n0 : it.n1) == 0) return;
+                    uint32_t& sums = h == 0 ? sums0 : sums1;
+                    ok = ok && wait(sm.o_full[h], sums & 1, kSumsThere, sums);
+                    ++sums;
+                };
+                const auto half_done = [&](int h) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bar(sm.row_empty[h]));
+                        mbar_arrive(bar(sm.o_empty[h]));
+                    }
+                };
+#pragma unroll 1
+                for (int h = 0; h < (it.alternate ? 1 : 2) && ok; ++h) {
+                    half_there(h);
+                    if (it.alternate) half_there(1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int row0 = h * kHalf + quarter * 32, row = row0 + lane;
+                    float2 stats = sm.row[h][quarter * 32 + lane];   // reference and sum
+                    float f = 1.0f, other = 0.0f;                    // factors of the half's sums, and of the other one's
+                    if (it.alternate) {
+                        const float2 theirs = sm.row[1][quarter * 32 + lane];
+                        const float both = fmaxf(stats.x, theirs.x), ref = both == -INFINITY ? 0.0f : both;
+                        f = ex2((stats.x - ref) * c);
+                        other = ex2((theirs.x - ref) * c);
+                        stats = make_float2(both, stats.y * f + theirs.y * other);
+                    }
+                    const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);
+                    const bool nothing = stats.x == -INFINITY && !isnan(stats.y);
+                    const bool spoilt = last >= *static_cast<volatile int*>(&sm.not_finite[not_finite_at]);
+                    const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / stats.y;
+                    const float2 f2 = make_float2(f * inv, f * inv), other2 = make_float2(other * inv, other * inv), zero2 = make_float2(0.0f, 0.0f);
+                    const int64_t place = static_cast<int64_t>(it.q0 + row0) * p.heads + it.head, part = static_cast<int64_t>(it.split) * p.tokens * p.heads + place;
+                    const int rows = it.rows - row0;
+                    if (lane < rows) {
+                        const float lse = nothing ? -INFINITY : (stats.x * c + log2f(stats.y)) * kLn2;
+                        if (p.partial) p.partial_lse[part + static_cast<int64_t>(lane) * p.heads] = lse;
+                        else if (p.lse) p.lse[place + static_cast<int64_t>(lane) * p.heads] = lse;
+                    }
+                    const int n = h == 0 ? it.n0 : it.n1;
+                    const bool two = it.alternate && it.n1 > 0;
+#pragma unroll 1
+                    for (int i = 0; i < kValue; i += 16) {
+                        uint32_t o[16] = {}, o2[16] = {};
+                        if (n > 0) tc_ld_x16(sums_at + h * kValue + i, o);
+                        if (two) tc_ld_x16(sums_at + kValue + i, o2);
+                        tc_wait_ld();
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) finite = finite && (w[e] & 0x7F80u) != 0x7F80u && (w[e] & 0x7F800000u) != 0x7F800000u;
-                                    if (!finite) {
-                                        bad = min(bad, key);
-                                        at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
-                                    }
-                                }
-                                bad = __reduce_min_sync(0xffffffffu, bad);
-                                if (lane == 0) *static_cast<volatile int*>(&sm.not_finite[count % kItemSlots]) = min(bad, sm.not_finite[count % kItemSlots]);
-                            }
-                            fence_proxy_async_shared();
+                        for (int j = 0; j < 16; j += 2) {
+                            float2 v = fma2(make_float2(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), f2, zero2);
+                            if (two) v = fma2(make_float2(__uint_as_float(o2[j]), __uint_as_float(o2[j + 1])), other2, v);
+                            o[j] = __float_as_uint(v.x), o[j + 1] = __float_as_uint(v.y);
+                        }
+                        if (p.partial) {
+                            store_rows(o, p.partial + part * kValue + i, static_cast<int64_t>(p.heads) * kValue * 4, rows);
+                        } else {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+                            store_rows(w, p.out + place * kValue + i, static_cast<int64_t>(p.heads) * kValue * 2, rows);
                         }
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar(sm.empty[s]));
                     }
-                    if (look && ok) {
-                        if (lane == 0) mbar_arrive(bar(sm.guarded[edges & 1]));
-                        ++edges;
-                    }
-                    if (is_value) ++t;
+                    half_done(h);
+                    if (it.alternate) half_done(1);
                 }
                 item_done(count);
             }
@@ -667,9 +803,9 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ------------------------------------------------------------ softmax: a thread to a query
         const int h = warp >> 2, quarter = warp & 3;
-        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, scores_at = tmem + lanes + kTmemScores + h * kTile;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, scores_at = tmem + lanes + kTmemScores, weights_at = tmem + lanes + kTmemWeights + h * (kTile / 2);
         const float c = p.scale;
-        uint32_t tiles = 0, sums = 0, joins = 0;
+        uint32_t tiles = 0;
         bool ok = true;
         for (uint32_t count = 0; ok; ++count) {
             const Item it = next_item(count, ok);
@@ -684,30 +820,40 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 ok = wait(sm.s_full[h], tiles & 1, kScoresThere, tiles);
                 if (!ok) break;
                 tc_fence_after();
+                // the last column that is the query's, the last that is all the warp's
+                const int visible = last - key0, visible0 = last0 - key0;
                 uint32_t x[kTile];
 #pragma unroll
                 for (int i = 0; i < kTile; i += 32) tc_ld_x32(scores_at + i, x + i);
                 tc_wait_ld();
-                if (key0 + kTile - 1 > last0) {
-                    const int visible = last - key0;                 // columns beyond are none of the query's
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sm.s_empty));
+                if (visible0 < kTile - 1) {
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) x[i] = i > visible ? 0xFF800000u : x[i];
                 }
                 float m[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) m[i] = fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 4]));
+                for (int i = 0; i < 4; ++i) m[i] = max3(__uint_as_float(x[i]), __uint_as_float(x[i + 4]), __uint_as_float(x[i + 8]));
 #pragma unroll
-                for (int i = 8; i < kTile; i += 8) {
+                for (int i = 12; i < kTile - 4; i += 8) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(m[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + j + 4]));
+                    for (int j = 0; j < 4; ++j) m[j] = max3(m[j], __uint_as_float(x[i + j]), __uint_as_float(x[i + j + 4]));
                 }
-                const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                // a weight would pass 2^8 (or nothing was seen so far): the reference moves
-                const bool moves = most * c > top * c + kSlack || (top == -INFINITY && most > -INFINITY);
+                static_assert((kTile - 16) % 8 == 0, "four columns are left");
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m[j] = max3(m[j], __uint_as_float(x[kTile - 4 + j]), -INFINITY);
+                const float most = max3(max3(m[0], m[1], m[2]), m[3], -INFINITY);
+                // (the sums of the tile before are complete: weights may be overwritten, sums rescaled)
+                ok = wait(sm.p_empty[h], (tiles & 1) ^ 1, kWeightsRoom, tiles);
+                if (!ok) break;
+                tc_fence_after();
+                // a weight would pass 2^kSlack, nothing was seen so far, or something is not a number: the reference moves
+                const bool moves = !(most * c <= top * c + kSlack);
                 if (t == 0) {
                     top = most;
                 } else if (__any_sync(0xffffffffu, moves)) {
-                    // (the scores' arrival says that the sums before them are complete)
                     const float f = moves ? (top == -INFINITY ? 0.0f : ex2((top - most) * c)) : 1.0f;
                     if (moves) top = most;
                     sum2.x *= f, sum2.y *= f;
@@ -725,107 +871,30 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 const float ref = top == -INFINITY ? 0.0f : -top * c;
                 const float2 c2 = make_float2(c, c), ref2 = make_float2(ref, ref);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    uint32_t w[32];
+                for (int first = 0; first < kTile; first += 32) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int at = g * 64 + 2 * i;
-                        const float2 y = fma2(make_float2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, ref2);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = fma2(make_float2(__uint_as_float(x[first + 2 * i]), __uint_as_float(x[first + 2 * i + 1])), c2, ref2);
                         const float2 e = make_float2(ex2(y.x), ex2(y.y));
                         sum2 = add2(sum2, e);
                         w[i] = pack_bf16x2(e.x, e.y);
                     }
-                    tc_st_x32(scores_at + g * 32, w);
+                    tc_st_x16(weights_at + first / 2, w);
+                    if (first & 32) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(sm.p_full[h][first >> 6]));
+                    }
                 }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(sm.p_full[h]));
             }
             if (!ok) break;
-            float sum = sum2.x + sum2.y;
-            if (n > 0) {
-                ok = wait(sm.o_full[h], sums & 1, kSumsThere, sums);
-                ++sums;
-                if (!ok) break;
-                tc_fence_after();
-            }
-            // Where the halves have the same queries, each takes half of the columns of their common result.
-            const bool joins_halves = it.alternate && it.n > 1;
-            float f = 1.0f, other = 0.0f;                            // factors of the half's sums, and of the other one's
-            if (joins_halves) {
-                sm.row[h][quarter * 32 + lane] = make_float2(top, sum);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(sm.halves_full));
-                ok = wait(sm.halves_full, joins & 1, kHalves, joins);
-                if (!ok) break;
-                tc_fence_after();
-                const float2 theirs = sm.row[h ^ 1][quarter * 32 + lane];
-                const float both = fmaxf(top, theirs.x), ref = both == -INFINITY ? 0.0f : both;
-                f = ex2((top - ref) * c);
-                other = ex2((theirs.x - ref) * c);
-                sum = sum * f + theirs.y * other;
-                top = both;
-            }
-            const bool nothing = sum == 0.0f;
-            const bool spoilt = last >= *static_cast<volatile int*>(&sm.not_finite[count % kItemSlots]);
-            const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / sum;
-            f *= inv, other *= inv;
-            const bool writes = row < it.rows && (h == 0 || !it.alternate || joins_halves);
-            const int64_t place = static_cast<int64_t>(it.q0 + row) * p.heads + it.head;
-            const int64_t part = static_cast<int64_t>(it.split) * p.tokens * p.heads + place;
-            const int first = joins_halves ? h * (kValue / 2) : 0, end = joins_halves ? first + kValue / 2 : kValue;
-            if (h == 0 || !it.alternate || joins_halves) {
-#pragma unroll 1
-                for (int i = first; i < end; i += 32) {
-                    uint32_t o[32];
-                    if (n > 0) {
-                        tc_ld_x32(tmem + lanes + kTmemSums + h * kValue + i, o);
-                        if (joins_halves) {
-                            uint32_t o2[32];
-                            tc_ld_x32(tmem + lanes + kTmemSums + (h ^ 1) * kValue + i, o2);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f + __uint_as_float(o2[j]) * other);
-                        } else {
-                            tc_wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        }
-                    }
-                    if (nothing) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = spoilt ? 0x7FC00000u : 0u;
-                    }
-                    if (writes && p.partial) {
-                        uint4* const to = reinterpret_cast<uint4*>(p.partial + part * kValue + i);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) to[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    } else if (writes) {
-                        uint4* const to = reinterpret_cast<uint4*>(p.out + place * kValue + i);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const auto two = [&](int k) { return pack_bf16x2(__uint_as_float(o[8 * j + 2 * k]), __uint_as_float(o[8 * j + 2 * k + 1])); };
-                            to[j] = make_uint4(two(0), two(1), two(2), two(3));
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-            if (writes && (h == 0 || !it.alternate)) {
-                const float lse = nothing ? -INFINITY : (top * c + log2f(sum)) * kLn2;
-                if (p.partial) p.partial_lse[part] = lse;
-                else if (p.lse) p.lse[place] = lse;
-            }
-            if (joins_halves) {                                      // (the other half still reads this one's sums)
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(sm.halves_done));
-                ok = wait(sm.halves_done, joins & 1, kHalves, joins);
-                ++joins;
-                if (!ok) break;
-            }
+            ok = wait(sm.row_empty[h], (count & 1) ^ 1, kRowsRoom, count);
+            if (!ok) break;
+            sm.row[h][quarter * 32 + lane] = make_float2(top, sum2.x + sum2.y);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(sm.row_full[h]));
             item_done(count);
         }
     }
@@ -840,7 +909,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == kMmaWarp) {
+    if (warp == kScoreWarp) {
         tc_fence_after();
         tc_dealloc(tmem, kTmemCols);
     }
@@ -875,7 +944,7 @@ int prepare_kernel() {
         // (the warps that ask for more registers wait for those that the block does not have)
         cudaFuncAttributes attr = {};
         DSV3_CUDA_TRY(cudaFuncGetAttributes(&attr, expanded_attention_kernel));
-        if (attr.numRegs * kThreads < kSoftmaxRegs * 256 + kOtherRegs * 128) {
+        if (attr.numRegs * kThreads < kSoftmaxRegs * 256 + kOtherRegs * 256) {
             set_last_error("expanded_attention: built with %d registers a thread, too few to share out", attr.numRegs);
             return DSV3_ERR_UNSUPPORTED;
         }

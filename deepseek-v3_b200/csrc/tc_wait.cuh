@@ -36,7 +36,7 @@ __device__ __forceinline__ bool bounded_wait_ns(uint32_t bar, uint32_t parity, C
             } else if (now - t0 > limit_ns) {
                 ctl->abort_flag = 1;
                 if (atomicCAS(&status[0], 0u, 1u) == 0u) {
-                    status[1] = what;        // 1 empty, 2 full, 3 tmem-empty, 4 tmem-full, 7-8 scale table, 9 self-test, 11-15 latent attention, 16-21 expanded attention
+                    status[1] = what;        // 1 empty, 2 full, 3 tmem-empty, 4 tmem-full, 7-8 scale table, 9 self-test, 11-15 latent attention, 16-22 expanded attention
                     status[2] = g;           // chunk / unit counter of the waiting role
                     status[3] = k2d ? blockIdx.y * gridDim.x + blockIdx.x : blockIdx.x;
                 }
