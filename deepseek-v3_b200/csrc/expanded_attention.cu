@@ -43,6 +43,7 @@ constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(kSoftmaxRegs * 256 + kOtherRegs * 256 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
 constexpr int kTmemScores = 0, kTmemWeights = kTile, kTmemSums = 2 * kTile, kTmemCols = 512;   // columns; weights: 64 to a half, sums: 128
 constexpr int kAhead = 1;                        // tiles that scores are ahead of sums (twice as many where halves take turns)
+constexpr int kAskEarly = 5, kAnswerEarly = 2;   // units before an item's last at which the next item is asked for, and the answer read
 constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 3 + kFinishWarps;
 constexpr int kLanes = 32;                       // sequences that are put in order of their length
 // What a wait that gave up was for (kinds of dsv3_check_device_status)
@@ -60,6 +61,7 @@ struct Params {
     float scale;                          // softmax_scale log2(e)
     int head_group;
     int splits;
+    FastDiv by_splits, by_group, by_last_group;      // ... and by the heads of the last group
     bool dynamic;                         // CTAs take the place of those that have not started; else every gridDim.x-th item
     __nv_bfloat16* out;
     float* lse;
@@ -250,9 +252,12 @@ struct List {
     int blocks, behind;                   // its blocks; steps of two tiles by which it is shorter than the longest
     int total, last_step;                 // blocks in all; steps in which blocks come up
     int chunk, before;                    // beyond 32 sequences: first of the 32 at hand, blocks before those
+    uint32_t group, group_first;          // group of heads of the item found last, the first item of it (but for parts)
+    int step;                             // ... and the step in which its block came up
     __device__ __forceinline__ void begin(const Params& p) {
         const int lane = threadIdx.x & 31;
-        chunk = before = 0;
+        chunk = before = step = 0;
+        group = group_first = 0;
         mine = load_seq(p, lane);
         blocks = blocks_of(mine.queries);
         const int tiles = blocks > 0 ? (mine.keys + kTile - 1) / kTile : 0;
@@ -268,26 +273,30 @@ struct List {
     __device__ __forceinline__ Item find(const Params& p, uint32_t at) {
         Item it = {};
         if (at >= static_cast<uint32_t>(total) * p.heads * p.splits) return it;
-        const uint32_t unsplit = at / p.splits;
+        const uint32_t unsplit = fast_div(at, p.by_splits);
         it.split = static_cast<int>(at - unsplit * p.splits);
-        const uint32_t group = unsplit / (static_cast<uint32_t>(total) * p.head_group), in_group = unsplit - group * (static_cast<uint32_t>(total) * p.head_group);
-        const uint32_t heads = min(p.head_group, p.heads - static_cast<int>(group) * p.head_group);
-        const int place = static_cast<int>(in_group / heads);
+        // (items are asked for in ascending order, as a rule: from where the last one was it is not far)
+        const uint32_t group_items = static_cast<uint32_t>(total) * p.head_group;
+        if (unsplit < group_first) group = group_first = 0, step = 0;
+        while (unsplit - group_first >= group_items) group_first += group_items, ++group, step = 0;
+        const uint32_t in_group = unsplit - group_first, heads = min(p.head_group, p.heads - static_cast<int>(group) * p.head_group);
+        const int place = static_cast<int>(fast_div(in_group, static_cast<int>(heads) == p.head_group ? p.by_group : p.by_last_group));
         it.head = static_cast<int>(group * p.head_group + in_group - place * heads);
         Seq s;
         int block;
         if (p.n_seqs <= kLanes) {
-            int lo = 0, hi = last_step;                              // first step that comes up to more than `place` blocks
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (up_to(mid) > place) hi = mid;
-                else lo = mid + 1;
+            int earlier = up_to(step - 1);                           // blocks that come up before the step
+            if (earlier > place) step = earlier = 0;
+            for (;;) {
+                const int here = up_to(step);
+                if (here > place || step >= last_step) break;
+                earlier = here;
+                ++step;
             }
-            const int nth = place - (lo > 0 ? up_to(lo - 1) : 0);
-            uint32_t there = __ballot_sync(0xffffffffu, lo >= behind && lo < behind + blocks);
-            for (int i = 0; i < nth; ++i) there &= there - 1;
+            uint32_t there = __ballot_sync(0xffffffffu, step >= behind && step < behind + blocks);
+            for (int i = earlier; i < place; ++i) there &= there - 1;
             const int from = __ffs(there) - 1;
-            block = __shfl_sync(0xffffffffu, blocks - 1 - (lo - behind), from);
+            block = __shfl_sync(0xffffffffu, blocks - 1 - (step - behind), from);
             s = {__shfl_sync(0xffffffffu, mine.q0, from), __shfl_sync(0xffffffffu, mine.queries, from), __shfl_sync(0xffffffffu, mine.k0, from),
                  __shfl_sync(0xffffffffu, mine.keys, from)};
         } else {
@@ -471,27 +480,50 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 __syncwarp();
                 ++slot;
             };
-            for (uint32_t count = 0; ok; ++count) {
+            // item number `at`, for the others to read
+            uint32_t listed = 0;
+            const auto publish = [&]() -> Item {
                 const Item it = at < 0 ? Item{} : list.find(p, static_cast<uint32_t>(at));
-                const uint32_t place = count % kItemSlots;
-                ok = __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_empty[place]), ((count / kItemSlots) & 1) ^ 1, ctl, status, kItems, count, kItemLimitNs));
-                if (!ok) break;
-                if (lane == 0) {
+                const uint32_t place = listed % kItemSlots;
+                ok = ok && __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_empty[place]), ((listed / kItemSlots) & 1) ^ 1, ctl, status, kItems, listed, kItemLimitNs));
+                if (ok && lane == 0) {
                     sm.item[place] = it;
                     sm.not_finite[place] = 0x7FFFFFFF;
                     mbar_arrive(bar(sm.item_full[place]));
                 }
                 __syncwarp();
-                if (it.rows == 0) break;
-                // The next item is asked for as late as its loads allow: who asks early takes work that another SM would be free for.
-                const auto ask = [&]() {
-                    if (p.dynamic && elect_one()) {
-                        mbar_arrive_expect_tx(bar(sm.taken), 16);
-                        try_cancel(smem_u32(sm.answer), bar(sm.taken));
-                    }
+                ++listed;
+                return it;
+            };
+            // The next item is asked for as late as the loads allow: who asks early takes work that another SM would be free for.
+            const auto ask = [&]() {
+                if (p.dynamic && elect_one()) {
+                    mbar_arrive_expect_tx(bar(sm.taken), 16);
+                    try_cancel(smem_u32(sm.answer), bar(sm.taken));
+                }
+                __syncwarp();
+            };
+            const auto answer = [&]() {
+                if (!p.dynamic) {
+                    at = at > 0x7FFFFFFF - static_cast<int>(gridDim.x) ? -1 : at + static_cast<int>(gridDim.x);
+                    return;
+                }
+                ok = ok && wait(sm.taken, taken & 1, kItems, taken);
+                ++taken;
+                if (ok) {
+                    at = cancelled_cta(smem_u32(sm.answer));
+                    fence_proxy_async_shared();
                     __syncwarp();
-                };
-                if (it.n == 0) ask();
+                }
+            };
+            Item it = publish();
+            while (ok && it.rows > 0) {
+                Item following = {};
+                if (it.n == 0) {
+                    ask();
+                    answer();
+                    following = publish();
+                }
                 if (it.n > 0) {
                     const auto load_queries = [&](int h) {
                         ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
@@ -530,28 +562,24 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                         ++v_loaded;
                         ++unit;
                     };
-                    load_queries(0);
+                    const int ask_at = max(0, 2 * it.n - kAskEarly), answer_at = max(ask_at, 2 * it.n - kAnswerEarly);
                     for (int u = 0; u < 2 * it.n && ok; ++u) {
                         const Unit w = unit_of(it, u);
-                        if (u == 2 * it.n - 2) ask();
+                        if (u == ask_at) ask();
+                        if (u == answer_at) {
+                            answer();
+                            following = publish();
+                        }
                         if (w.keys) load_keys(w.tile);
                         else load_values(w.tile);
-                        if (u == 0) load_queries(1);
+                        if (u == 0) {
+                            load_queries(0);
+                            load_queries(1);
+                        }
                     }
                     ++active;
                 }
-                if (!ok) break;
-                if (p.dynamic) {
-                    ok = wait(sm.taken, taken & 1, kItems, taken);
-                    ++taken;
-                    if (ok) {
-                        at = cancelled_cta(smem_u32(sm.answer));
-                        fence_proxy_async_shared();
-                        __syncwarp();
-                    }
-                } else {
-                    at = at > 0x7FFFFFFF - static_cast<int>(gridDim.x) ? -1 : at + static_cast<int>(gridDim.x);
-                }
+                it = following;
             }
             // none of the arrivals on empty[] may be in flight when the CTA leaves its shared memory to another
             while (ok && back < unit) one_back(unit - 1);
@@ -591,14 +619,14 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                         }
                         __syncwarp();
                     }
-                    if (elect_one()) tc_commit(bar(sm.k_empty[keys % kUnits]));
+                    if (elect_one()) {
+                        tc_commit(bar(sm.k_empty[keys % kUnits]));
+                        // (what is not needed any more: the first half may be done a tile before the second)
+                        if (t == max(0, (step ? n : n0) - 1)) tc_commit(bar(sm.q_empty[0]));
+                        if (t == n - 1) tc_commit(bar(sm.q_empty[1]));
+                    }
                     __syncwarp();
                 }
-                if (elect_one()) {
-                    tc_commit(bar(sm.q_empty[0]));
-                    tc_commit(bar(sm.q_empty[1]));
-                }
-                __syncwarp();
                 slot += (kKeySlots + kValueSlots) * n;
                 ++active;
             }
@@ -671,21 +699,21 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                         const int key0 = (it.tile + t) * kTile + i * 64;
                         uint4* const at = reinterpret_cast<uint4*>(base + (u + i) % kSlots * kSlotBytes);
                         // 64 keys x 8 pieces of 16 bytes, twice; rows are keys, and a row's pieces stay in it
-                        __nv_bfloat162 seen = __floats2bfloat162_rn(0.0f, 0.0f);
-                        const __nv_bfloat162 zero = seen;
+                        const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
+                        __nv_bfloat162 seen[4] = {zero, zero, zero, zero};
+                        if (key0 + 63 >= it.len) {
+                            for (int j = 0; j < kSlotBytes / 512; ++j)
+                                if (key0 + ((j * 32 + lane) >> 3 & 63) >= it.len) at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                        }
 #pragma unroll 8
                         for (int j = 0; j < kSlotBytes / 512; ++j) {
-                            const int key = key0 + ((j * 32 + lane) >> 3 & 63);
-                            if (key >= it.len) {
-                                at[j * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
-                            } else {
-                                const uint4 v = at[j * 32 + lane];
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                            const uint4 v = at[j * 32 + lane];
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) seen = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, seen);   // NaN stays
-                            }
+                            for (int e = 0; e < 4; ++e) seen[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, seen[e]);         // NaN stays
                         }
-                        if (__any_sync(0xffffffffu, __hisnan(seen.x) || __hisnan(seen.y))) {
+                        const __nv_bfloat162 all = __hadd2(__hadd2(seen[0], seen[1]), __hadd2(seen[2], seen[3]));
+                        if (__any_sync(0xffffffffu, __hisnan(all.x) || __hisnan(all.y))) {
                             int bad = 0x7FFFFFFF;
                             for (int j = 0; j < kSlotBytes / 512; ++j) {
                                 const int key = key0 + ((j * 32 + lane) >> 3 & 63);
@@ -1032,6 +1060,8 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
     p.causal = a->causal != 0;
     p.scale = a->softmax_scale * kLog2e;
     p.head_group = pl.head_group, p.splits = pl.splits, p.dynamic = dynamic;
+    p.by_splits = make_fast_div(pl.splits), p.by_group = make_fast_div(pl.head_group);
+    p.by_last_group = make_fast_div(a->heads % pl.head_group ? a->heads % pl.head_group : pl.head_group);
     p.out = static_cast<__nv_bfloat16*>(a->out), p.lse = a->lse;
     p.partial = partial, p.partial_lse = need ? partial + pl.splits * rows * kValue : nullptr;
     const int64_t grid = dynamic ? items : std::min<int64_t>(items, num_sms());
