@@ -2,7 +2,8 @@
 //
 //   lse = log sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
 //
-// HBM bounds it: every part is read once.  dim / 8 neighbouring threads to a row, eight values each, up to four parts on their way at once.
+// HBM bounds it: every part is read once.  dim / 8 neighbouring threads to a row, eight values each.  Up to four parts everything of a row is asked for at once, sums and weights
+// (whether a part saw anything or not: waiting for that first takes a second trip to memory).
 #include <algorithm>
 
 #include "attention_join.cuh"
@@ -26,53 +27,78 @@ struct Parts {
     int n_seqs, heads;
 };
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_bits_to_float(u[i] & 0xFFFFu), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-}
-__device__ __forceinline__ void load8(const float* p, float* v) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
+// Eight values as they lie in memory.
 template <typename T>
+struct Eight;
+template <>
+struct Eight<__nv_bfloat16> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void get(float* v) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = bf16_bits_to_float(u[i] & 0xFFFFu), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+};
+template <>
+struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ __forceinline__ void get(float* v) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+};
+
+// kN: at most so many parts, or 0 for any number, kAtOnce of them on their way.
+template <typename T, int kN>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ Parts p) {
     griddep_launch_dependents();
     griddep_wait();
     const uint32_t slot = fast_div(threadIdx.x, p.row_threads), at = threadIdx.x - slot * p.row_threads.d;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * p.block_rows + slot;
     if (static_cast<int>(slot) >= p.block_rows || row >= p.rows) return;
-    if (p.cu && (row < static_cast<int64_t>(p.cu[0]) * p.heads || row >= static_cast<int64_t>(p.cu[p.n_seqs]) * p.heads)) return;
     const int64_t from = (row * p.row_threads.d + at) * 8;
+    constexpr int kHeld = kN ? kN : kAtOnce;
+    Eight<T> v[kHeld];
+    float w[kHeld];
+    const auto fetch = [&](int first) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            w[k] = -INFINITY;
+            if (first + k < p.n) {
+                w[k] = p.lse[first + k][row];
+                v[k].load(static_cast<const T*>(p.out[first + k]) + from);
+            }
+        }
+    };
+    fetch(0);
+    if (p.cu && (row < static_cast<int64_t>(p.cu[0]) * p.heads || row >= static_cast<int64_t>(p.cu[p.n_seqs]) * p.heads)) return;
     float top = -INFINITY;
     bool nan = false;
-    for (int i = 0; i < p.n; ++i) {
-        const float v = p.lse[i][row];
-        nan = nan || isnan(v);
-        top = fmaxf(top, v);
+    const auto see = [&](float x) {
+        nan = nan || isnan(x);
+        top = fmaxf(top, x);
+    };
+    if constexpr (kN != 0) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) see(w[k]);
+    } else {
+        for (int i = 0; i < p.n; ++i) see(p.lse[i][row]);
     }
     const float ref = top == -INFINITY ? 0.0f : top;
     float acc[8] = {}, sum = 0.0f;
-    for (int i0 = 0; i0 < p.n; i0 += kAtOnce) {
-        float v[kAtOnce][8], w[kAtOnce];
+    for (int first = 0;;) {
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            if (i0 + k >= p.n) break;
-            w[k] = p.lse[i0 + k][row];
-            // (what a part that sees nothing left there does not matter)
-            if (w[k] != -INFINITY) load8(static_cast<const T*>(p.out[i0 + k]) + from, v[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            if (i0 + k >= p.n) break;
-            if (w[k] == -INFINITY) continue;
+        for (int k = 0; k < kHeld; ++k) {
+            if (w[k] == -INFINITY) continue;                         // (what a part that sees nothing left there does not matter)
             const float e = exp2f((w[k] - ref) * kLog2e);
+            float x[8];
+            v[k].get(x);
             sum += e;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = fmaf(e, v[k][j], acc[j]);
+            for (int j = 0; j < 8; ++j) acc[j] = fmaf(e, x[j], acc[j]);
         }
+        first += kHeld;
+        if (kN != 0 || first >= p.n) break;
+        fetch(first);
     }
     const float inv = nan ? __uint_as_float(0x7FC00000u) : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -90,7 +116,8 @@ int launch(const void* const* outs, const float* const* lses, int n, int64_t row
     p.n = n, p.rows = rows, p.row_threads = make_fast_div(row_threads), p.block_rows = block_rows;
     p.to = static_cast<__nv_bfloat16*>(out), p.to_lse = lse;
     p.cu = cu, p.n_seqs = n_seqs, p.heads = heads;
-    DSV3_CUDA_TRY(launch_dependent(attention_join_kernel<T>, dim3(static_cast<unsigned>((rows + block_rows - 1) / block_rows)), dim3(kThreads), 0, stream, p));
+    const auto go = [&](auto kern) { return launch_dependent(kern, dim3(static_cast<unsigned>((rows + block_rows - 1) / block_rows)), dim3(kThreads), 0, stream, p); };
+    DSV3_CUDA_TRY(n <= 2 ? go(attention_join_kernel<T, 2>) : n <= 4 ? go(attention_join_kernel<T, 4>) : go(attention_join_kernel<T, 0>));
     return DSV3_OK;
 }
 

@@ -949,14 +949,21 @@ struct Plan {
     int splits, head_group;
 };
 constexpr int kLeastTiles = 4;            // of a part
+constexpr int64_t kGroupBytes = 32ll << 20;
 Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, int sms) {
     Plan pl;
     const int64_t each = ragged ? 0 : tokens / n_seqs;
     const int64_t seqs = std::min(n_seqs, tokens);                   // that have queries
     pl.blocks = ragged ? (tokens - seqs) / kBlock + seqs : n_seqs * ((each + kBlock - 1) / kBlock);
-    const int64_t items = pl.blocks * heads, tiles = kv_tokens / n_seqs / kTile;
-    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxJoinParts, sms / items, tiles / kLeastTiles})));
-    pl.head_group = static_cast<int>(n_seqs > kLanes ? heads : std::min<int64_t>(heads, std::max<int64_t>(1, (2 * sms + pl.blocks - 1) / pl.blocks)));
+    const int64_t items = pl.blocks * heads;
+    // Where there are fewer items than SMs their keys are cut, in as many parts as fill the SMs once (a second round would cost what it gains).
+    const int64_t most = (kv_tokens / n_seqs + kTile - 1) / kTile;
+    // (`blocks` is more than there are, as a rule, where sequences are ragged)
+    const int64_t room = ragged && n_seqs > 1 ? sms + sms / 8 : sms;
+    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxJoinParts, room / items, most / kLeastTiles})));
+    // Groups of heads, equal ones: as few as keep a group's keys and values in the L2, and no more than leave each of them two items to an SM.
+    const int64_t bytes = heads * kv_tokens * 2 * (kNope + kValue), groups = n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, items / (2 * sms)));
+    pl.head_group = static_cast<int>((heads + groups - 1) / groups);
     return pl;
 }
 size_t partial_bytes(const Plan& pl, int64_t tokens, int64_t heads) {

@@ -1,6 +1,7 @@
 // Rotary positions (see include/dsv3_b200.h): the table of angles, and the rotation of queries or keys by them.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -8,30 +9,36 @@ namespace dsv3 {
 namespace {
 
 // ---------------------------------------------------------------- the table
-constexpr int kMaxPairs = 128, kTableThreads = 256, kTableUnroll = 4;
+constexpr int kMaxPairs = 128, kTableThreads = 256, kTableUnroll = 8;
 struct QuarterTurns {
     double per_position[kMaxPairs];       // of an angle: radians * 2 / pi
 };
 
-// A thread to kTableUnroll angles.  The angle is reduced to an eighth of a turn either side of a multiple of a quarter turn in 64 bits, so that position
-// 163840 is as exact as position 1, and what is left is an argument of ordinary size for fp32: both values are right to 2^-23.
-__global__ void __launch_bounds__(kTableThreads) rotary_table_kernel(const __grid_constant__ QuarterTurns f, FastDiv pairs, int64_t start, int64_t total,
+// A thread to one angle of kTableUnroll positions.  The angle is reduced to an eighth of a turn either side of a multiple of a quarter turn in 64 bits, so that position
+// 163840 is as exact as position 1; of what is left (r quarters, |r| <= 1/2) sine and cosine are polynomials in r^2, those of their degree whose largest error is least (Remez' exchange: 2^-27 and 2^-34).
+//   HBM bounds what is large, a launch what is small.  Conversions between 64-bit numbers and whole ones are what costs time here (one a cycle and SM): the nearest whole number comes from
+// adding 1.5 * 2^52, and only r is converted.
+__global__ void __launch_bounds__(kTableThreads) rotary_table_kernel(const __grid_constant__ QuarterTurns f, FastDiv pairs, int block_rows, int64_t start, int64_t length,
                                                                      float2* __restrict__ out) {
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kTableThreads * kTableUnroll) + threadIdx.x;
+    const uint32_t slot = fast_div(threadIdx.x, pairs), pair = threadIdx.x - slot * pairs.d;
+    if (static_cast<int>(slot) >= block_rows) return;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * block_rows * kTableUnroll + slot;
+    const double per = f.per_position[pair], step = static_cast<double>(block_rows);
+    double position = static_cast<double>(start + row);
 #pragma unroll
-    for (int u = 0; u < kTableUnroll; ++u) {
-        const int64_t i = at + u * kTableThreads;
-        if (i >= total) return;
-        const uint32_t row = fast_div(static_cast<uint32_t>(i), pairs), pair = static_cast<uint32_t>(i) - row * pairs.d;
-        const double quarters = static_cast<double>(start + row) * f.per_position[pair], whole = rint(quarters);
-        const int q = static_cast<int>(static_cast<long long>(whole)) & 3;
-        float sine, cosine;
-        sincospif(0.5f * static_cast<float>(quarters - whole), &sine, &cosine);
+    for (int u = 0; u < kTableUnroll; ++u, row += block_rows, position += step) {
+        if (row >= length) return;
+        constexpr double kWhole = 6755399441055744.0;                // 1.5 * 2^52: a sum with it has no fraction, and the whole number in its low bits
+        const double sum = fma(position, per, kWhole);
+        const float r = static_cast<float>(fma(position, per, kWhole - sum)), y = r * r;
+        const int q = __double2loint(sum);
+        const float sine = r * fmaf(y, fmaf(y, fmaf(y, -0x1.2d9bb8p-8f, 0x1.465ec6p-4f), -0x1.4abbbap-1f), 0x1.921fb6p+0f);
+        const float cosine = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 0x1.d9c364p-11f, -0x1.55c57cp-6f), 0x1.03c1dcp-2f), -0x1.3bd3ccp+0f), 1.0f);
         float2 z = q & 1 ? make_float2(-sine, cosine) : make_float2(cosine, sine);
         if (q & 2) z.x = -z.x, z.y = -z.y;
-        out[i] = z;
+        out[row * pairs.d + pair] = z;
     }
 }
 
@@ -55,46 +62,52 @@ struct Rows {
     float sign;                                         // of the sines
 };
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// Eight values of a head as they lie in memory.
+template <typename T>
+struct Eight {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+    __device__ __forceinline__ void get(float* v) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_bits_to_float(u[i] & 0xFFFFu), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-}
-__device__ __forceinline__ void load8(const __half* p, float* v) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = bf16_bits_to_float(u[i] & 0xFFFFu), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            }
+        }
     }
-}
-__device__ __forceinline__ void load8(const float* p, float* v) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(__half* p, const float* v) {
-    uint32_t u[4];
+    __device__ __forceinline__ void set(const float* v) {
+        uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                u[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            }
+        }
+        w = make_uint4(u[0], u[1], u[2], u[3]);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-}
-__device__ __forceinline__ void store8(float* p, const float* v) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
+};
+template <>
+struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ __forceinline__ void store(float* p) const { reinterpret_cast<float4*>(p)[0] = a, reinterpret_cast<float4*>(p)[1] = b; }
+    __device__ __forceinline__ void get(float* v) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+    __device__ __forceinline__ void set(const float* v) { a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]); }
+};
 
 // A unit is 16 values of a head in the layout of halves (eight from either half), else 8: four or eight pairs.  A thread keeps its unit's angles in registers and
-// takes every `teams`-th head of its token, kUnroll heads on their way at once.  Reads of a unit come before its writes, so that out may be x.
+// takes every `teams`-th head of its token.  HBM bounds it: heads are asked for kUnroll at once, before the angles, which come by way of the position.  Reads of a unit come before its
+// writes, so that out may be x.
 template <typename T, bool kHalf>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Rows r) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (kHalf ? 4 : 5) : kHalf ? 2 : 3) rotary_kernel(const Rows r) {
     griddep_launch_dependents();
     griddep_wait();
     const uint32_t slot = fast_div(threadIdx.x, r.token_threads), rest = threadIdx.x - slot * r.token_threads.d;
@@ -110,6 +123,20 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rows r) {
         at = (static_cast<int>(unit) - r.turned) * 8;
         if (at >= r.offset) at += rotated;
     }
+    const T* const x = static_cast<const T*>(r.x) + token * r.x_token + at;
+    T* const out = static_cast<T*>(r.out) + token * r.out_token + at;
+    const int second = rotated / 2;
+    Eight<T> v[kUnroll], v2[kHalf ? kUnroll : 1];
+    const auto fetch = [&](int head) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int h = head + u * r.teams;
+            if (h >= r.heads) break;
+            v[u].load(x + h * r.x_head);
+            if (kHalf && turns) v2[kHalf ? u : 0].load(x + h * r.x_head + second);
+        }
+    };
+    fetch(static_cast<int>(team));
     float2 f[kPairs];
     if (turns) {
         const int64_t position = r.positions ? r.positions[token] : static_cast<int64_t>(static_cast<uint32_t>(token) % r.per);
@@ -121,33 +148,34 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rows r) {
             f[i].y *= r.sign;
         }
     }
-    const T* const x = static_cast<const T*>(r.x) + token * r.x_token + at;
-    T* const out = static_cast<T*>(r.out) + token * r.out_token + at;
-    const int second = rotated / 2;
-    for (int head = static_cast<int>(team); head < r.heads; head += r.teams * kUnroll) {
-        float v[kUnroll][kHalf ? 16 : 8];
+    for (int head = static_cast<int>(team); head < r.heads;) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int h = head + u * r.teams;
             if (h >= r.heads) break;
-            load8(x + h * r.x_head, v[u]);
-            if (kHalf && turns) load8(x + h * r.x_head + second, v[u] + (kHalf ? 8 : 0));
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int h = head + u * r.teams;
-            if (h >= r.heads) break;
-            if (turns) {
-#pragma unroll
-                for (int i = 0; i < kPairs; ++i) {
-                    float &a = v[u][kHalf ? i : 2 * i], &b = v[u][kHalf ? 8 + i : 2 * i + 1];
-                    const float re = fmaf(a, f[i].x, -(b * f[i].y)), im = fmaf(a, f[i].y, b * f[i].x);
-                    a = re, b = im;
-                }
+            T* const to = out + h * r.out_head;
+            if (!turns) {
+                v[u].store(to);
+                continue;
             }
-            store8(out + h * r.out_head, v[u]);
-            if (kHalf && turns) store8(out + h * r.out_head + second, v[u] + (kHalf ? 8 : 0));
+            float a[8], b[8];
+            v[u].get(a);
+            if (kHalf) v2[kHalf ? u : 0].get(b);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                float &first = a[kHalf ? i : 2 * i], &other = kHalf ? b[i] : a[2 * i + 1];
+                const float re = fmaf(first, f[i].x, -(other * f[i].y)), im = fmaf(first, f[i].y, other * f[i].x);
+                first = re, other = im;
+            }
+            v[u].set(a);
+            v[u].store(to);
+            if (kHalf) {
+                v2[kHalf ? u : 0].set(b);
+                v2[kHalf ? u : 0].store(to + second);
+            }
         }
+        head += r.teams * kUnroll;
+        if (head < r.heads) fetch(head);
     }
 }
 
@@ -196,9 +224,10 @@ int dsv3_rotary_table(int dim, double theta, double factor, int64_t original_len
         }
         f.per_position[i] = per * (2.0 / kPi);
     }
-    const int64_t total = length * pairs, each = kTableThreads * kTableUnroll;
-    DSV3_CUDA_TRY(launch_dependent(rotary_table_kernel, dim3(static_cast<unsigned>((total + each - 1) / each)), dim3(kTableThreads), 0,
-                                   static_cast<cudaStream_t>(stream), f, make_fast_div(pairs), start, total, reinterpret_cast<float2*>(out)));
+    const int block_rows = kTableThreads / pairs;
+    const int64_t each = static_cast<int64_t>(block_rows) * kTableUnroll;
+    DSV3_CUDA_TRY(launch_dependent(rotary_table_kernel, dim3(static_cast<unsigned>((length + each - 1) / each)), dim3(kTableThreads), 0,
+                                   static_cast<cudaStream_t>(stream), f, make_fast_div(pairs), block_rows, start, length, reinterpret_cast<float2*>(out)));
     return DSV3_OK;
 }
 
