@@ -9,11 +9,15 @@ norm is called, and its bf16 result stored.
     import model, dsv3_b200
     dsv3_b200.install_mla(model)        # model.MLA.forward = mla_forward
     dsv3_b200.install_mla(model, release_buffers=True)        # ... and the modules' bf16 buffers give their memory back
+    dsv3_b200.install_mla(model, expand_from=256)             # ... and prompts of 256 tokens or more are attended to with expanded keys and values
 
 A module's cache is made on its first call (not in a captured graph), of the size of its bf16 buffers; ``mla_cache(module)`` gives it with its block table, for
 ``latent_cache_keep`` and ``latent_cache_read``.  Drafted tokens: with a tree of them, ``mask`` is the int64 ``[batch, tokens]`` of
 ``latent_attention``'s ``tree_mask`` and ``freqs_cis`` has a row per node, that of its depth.  Sequences of which different numbers of drafts were kept are of different
 lengths from then on: ``start_pos`` is then an integer tensor ``[batch]`` and ``freqs_cis`` ``[batch, tokens, 32]``.
+
+Prompts: ``expand_from`` says from how many new tokens on (to a sequence) the keys and values of all heads are expanded from the cached latents (model.py:472-478) and
+``expanded_attention`` reads those, with a third of the absorbed form's operations per token seen.  Both forms attend to the same cached tokens.
 """
 from __future__ import annotations
 
@@ -26,7 +30,8 @@ import torch
 from torch.nn.modules import module as _nn_module
 
 from ._lib import host
-from .latent import LATENT_DIM, ROPE_DIM, LatentCache, allocate_latent_cache, latent_attention, latent_cache_write
+from .expanded import NOPE_DIM, VALUE_DIM, attention_join, expanded_attention, rotary, rotary_table
+from .latent import LATENT_DIM, ROPE_DIM, LatentCache, allocate_latent_cache, latent_attention, latent_cache_read, latent_cache_write
 from .ops import weight_dequant
 
 PAGE = 64
@@ -149,11 +154,38 @@ def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
     return (mask.clamp(min=low) == causal).all()           # (few launches: a short prompt is bound by the host)
 
 
-def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128) -> torch.Tensor:
+_MOST_PARTS = 32        # of attention_join
+
+
+def _attend_expanded(q_nope, q_rope, cache: MlaCache, table, start_pos: int, weight, softmax_scale: float, expand_tokens: int) -> torch.Tensor:
+    """Causal attention of a chunk at ``start_pos`` to its sequences' cached tokens, expanded with ``weight`` ``[heads, 256, 512]``.  The tokens before the chunk's page are expanded and attended
+    to in pieces of whole pages, ``expand_tokens`` of all sequences together to a piece (512 bytes a head and token), and the pieces' results joined."""
+    bsz, seqlen, heads, _ = q_nope.shape
+
+    def attend(first, end, causal, with_lse):
+        tokens = end - first
+        ends = torch.arange(0, (bsz + 1) * tokens, tokens, dtype=torch.int32, device=q_nope.device)
+        latent, k_rope = latent_cache_read(cache.pool, table[:, first // PAGE:], ends, bsz * tokens)
+        kv = torch.nn.functional.linear(latent, weight.flatten(0, 1)).view(bsz, tokens, heads, -1)
+        return expanded_attention(q_nope, q_rope, kv[..., :NOPE_DIM], k_rope.view(bsz, tokens, -1), kv[..., NOPE_DIM:], softmax_scale, causal=causal, return_lse=with_lse)
+
+    before = start_pos // PAGE * PAGE                      # tokens that may be seen in pieces
+    end_pos = start_pos + seqlen
+    if bsz * end_pos <= expand_tokens or before == 0:
+        return attend(0, end_pos, True, False)
+    pages = before // PAGE
+    piece = max(1, expand_tokens // (bsz * PAGE), -(-pages // (_MOST_PARTS - 1))) * PAGE
+    parts = [attend(first, min(first + piece, before), False, True) for first in range(0, before, piece)] + [attend(before, end_pos, True, True)]
+    return attention_join([out for out, _ in parts], [lse for _, lse in parts])
+
+
+def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freqs_cis: torch.Tensor, mask: Optional[torch.Tensor], *, block_size: int = 128,
+                expand_from: Optional[int] = None, expand_tokens: int = 1 << 16) -> torch.Tensor:
     """``MLA.forward`` on the 8-bit latent cache.  ``mask``: None for one token, the reference's causal mask (of these tokens, or of all up to them), or
     int64 words of a tree of drafted tokens.  Masks of other shapes are refused; a floating mask that is not the causal one makes the result NaN (nothing is read back).
     ``start_pos``: one for all sequences, or an int32 or int64 tensor ``[batch]`` beside ``x``, which a captured step reads when it is replayed; a sequence whose tokens do not fit
-    its cache is then not stored, and its result NaN.  ``freqs_cis``: ``[tokens, 32]``, or ``[batch, tokens, 32]``."""
+    its cache is then not stored, and its result NaN.  ``freqs_cis``: ``[tokens, 32]``, or ``[batch, tokens, 32]``.  ``expand_from``: so many tokens, and more, of a causal mask are attended to with
+    expanded keys and values where ``start_pos`` is one for all and heads are of 128 and 64 values; ``expand_tokens`` bounds what is expanded at a time."""
     bsz, seqlen, _ = x.shape
     rope = self.qk_rope_head_dim
     if self.kv_lora_rank != LATENT_DIM or rope != ROPE_DIM:
@@ -208,6 +240,14 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
     if scale is not None:
         weight = weight_dequant(weight, scale, block_size)
     weight = weight.view(self.n_local_heads, -1, LATENT_DIM)
+    if (expand_from is not None and seqlen >= expand_from and mask is not None and tree is None and isinstance(start_pos, int)
+            and (self.qk_nope_head_dim, self.v_head_dim) == (NOPE_DIM, VALUE_DIM)):
+        angles = freqs_cis.reshape(-1, ROPE_DIM // 2)      # (of one sequence, or of all)
+        if valid is not None:
+            angles = torch.where(valid, angles, math.nan)
+        turned = rotary(q_rope, angles, None if len(angles) == seqlen else positions)
+        out = _attend_expanded(q_nope, turned, cache, table, start_pos, weight, self.softmax_scale, expand_tokens)
+        return self.wo(out.flatten(2))
     q_latent = torch.einsum("bshd,hdc->bshc", q_nope, weight[:, :self.qk_nope_head_dim])
     angles = freqs_cis.reshape(-1, seqlen, ROPE_DIM // 2)
     if valid is not None:
@@ -216,12 +256,33 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
     return self.wo(torch.einsum("bshc,hdc->bshd", out, weight[:, -self.v_head_dim:]).flatten(2))
 
 
-def install_mla(model_module, release_buffers: bool = False) -> None:
+def install_mla(model_module, release_buffers: bool = False, expand_from: Optional[int] = None, expand_tokens: int = 1 << 16) -> None:
     """Point ``model_module.MLA.forward`` at ``mla_forward``; ``model_module.block_size`` is read at call time, as in the reference.  ``release_buffers``: a module's
-    bf16 buffers give their memory back at its first call; without it they stay, 1152 bytes a token beside the 644 of the 8-bit cache, for a host that goes back to the old forward."""
+    bf16 buffers give their memory back at its first call; without it they stay, 1152 bytes a token beside the 644 of the 8-bit cache, for a host that goes back to the old forward.
+    ``expand_from``: prompts of so many tokens and more to a sequence are attended to with expanded keys and values (None: never), ``expand_tokens`` cached ones at a time."""
+    if (expand_from is not None and expand_from < 1) or expand_tokens < 1:
+        raise ValueError("expand_from and expand_tokens are numbers of tokens, from 1 on")
+
     def forward(self, x, start_pos, freqs_cis, mask):
         if release_buffers:
             _release_buffers(self)
-        return mla_forward(self, x, start_pos, freqs_cis, mask, block_size=getattr(model_module, "block_size", 128))
+        return mla_forward(self, x, start_pos, freqs_cis, mask, block_size=getattr(model_module, "block_size", 128), expand_from=expand_from, expand_tokens=expand_tokens)
     forward.__doc__ = mla_forward.__doc__
     model_module.MLA.forward = forward
+
+
+def install_rotary(model_module) -> None:
+    """Point ``model_module.apply_rotary_emb`` (model.py:378-393) and ``precompute_freqs_cis`` (model.py:297-375) at ``rotary`` and ``rotary_table``.
+
+    One launch to a rotation instead of five, any strides of tokens and heads; angles are formed in 64 bits.  The table is made on torch's default device, which has to be a CUDA device
+    (``with torch.device("cuda")``, as the reference's generate.py makes its model)."""
+    def precompute_freqs_cis(args):
+        factor = args.rope_factor if args.max_seq_len > args.original_seq_len else 1.0
+        return rotary_table(args.max_seq_len, args.qk_rope_head_dim, args.rope_theta, factor=factor, original_length=args.original_seq_len, beta_fast=args.beta_fast,
+                            beta_slow=args.beta_slow, device=torch.get_default_device())
+
+    def apply_rotary_emb(x, freqs_cis):
+        return rotary(x, freqs_cis)
+
+    model_module.precompute_freqs_cis = precompute_freqs_cis
+    model_module.apply_rotary_emb = apply_rotary_emb
