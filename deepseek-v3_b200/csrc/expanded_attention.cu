@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "attention_join.cuh"
 #include "tc_wait.cuh"
@@ -29,21 +30,33 @@ int make_tmap_heads(CUtensorMap* map, const void* base, int width, int64_t heads
 namespace {
 
 constexpr int kNope = DSV3_NOPE_DIM, kRope = DSV3_ROPE_DIM, kValue = DSV3_VALUE_DIM;
-constexpr int kHalf = 128, kBlock = 2 * kHalf;   // queries
+constexpr int kHalf = 128;                       // queries of a CTA's half of a block
 constexpr int kTile = 128;                       // keys
 // Operands lie as rows of 64 values (128 bytes, swizzled).  Keys and values come through a ring of slots of 16 KB: three to a tile of keys (64 dimensions of 128 keys
 // each), two to one of values (64 keys of 128 dimensions each): beside the queries there is room for eight, one and a half tiles of both.
-constexpr int kSlots = 8, kSlotBytes = 16384, kKeySlots = 3, kValueSlots = 2;
-// A tile's keys, or its values, are a unit, which is waited for and given back as a whole; no more than four of either are on their way.
-constexpr int kUnits = 4;
-constexpr int kQueryBytes = kKeySlots * kSlotBytes;
-constexpr int kOperandBytes = kSlots * kSlotBytes + 2 * kQueryBytes;
+constexpr int kKeySlots = 3, kValueSlots = 2;
+// A tile's keys, or its values, are a unit, which is waited for and given back as a whole.
+constexpr int kUnits = 8;                        // of either that can be on their way: a ring of a pair's slots has room for no more values
+constexpr int kRingBytes = 131072, kQueryPart = kHalf * 128, kQueryBytes = kKeySlots * kQueryPart;
+constexpr int kOperandBytes = kRingBytes + 2 * kQueryBytes;
+// One CTA, or a pair of them: both halves of a block have 128 queries in either, and either loads half of the keys' rows and half of the values' dimensions.
+template <int kCtas>
+struct Cfg {
+    static constexpr int kRows = kCtas * kHalf, kBlock = 2 * kRows;                  // queries of a half, of a block
+    static constexpr int kSlotBytes = 16384 / kCtas, kSlots = kRingBytes / kSlotBytes;
+    // (a wait by parity is exact for who has seen the phase before: a unit's barrier is not used again before the unit is given back)
+    static_assert(kSlots / std::min(kKeySlots, kValueSlots) <= kUnits, "units in the ring");
+    // bf16 x bf16 -> fp32
+    static constexpr uint32_t kIdescScores = umma_idesc_e4m3_f32(kRows, kTile) | (1u << 7) | (1u << 10);
+    static constexpr uint32_t kIdescSums = umma_idesc_e4m3_f32(kRows, kValue) | (1u << 7) | (1u << 10) | (1u << 16);      // B transposed
+};
 constexpr int kSoftmaxWarps = 8, kScoreWarp = 8, kLoadWarp = 9, kGuardWarp = 10, kSumWarp = 11, kFinishWarp = 12, kFinishWarps = 4, kThreads = 512;
 constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(kSoftmaxRegs * 256 + kOtherRegs * 256 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
 constexpr int kTmemScores = 0, kTmemWeights = kTile, kTmemSums = 2 * kTile, kTmemCols = 512;   // columns; weights: 64 to a half, sums: 128
 constexpr int kAhead = 1;                        // tiles that scores are ahead of sums (twice as many where halves take turns)
 constexpr int kAskEarly = 5, kAnswerEarly = 2;   // units before an item's last at which the next item is asked for, and the answer read
+constexpr int kNotFiniteSlots = 8;
 constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 3 + kFinishWarps;
 constexpr int kLanes = 32;                       // sequences that are put in order of their length
 // What a wait that gave up was for (kinds of dsv3_check_device_status)
@@ -81,11 +94,12 @@ struct Item {
 };
 
 struct Small {
-    uint64_t k_full[kUnits], k_empty[kUnits], v_full[kUnits], v_empty[kUnits];
-    uint64_t q_full[2], q_empty[2], s_full[2], s_empty, p_full[2][kValueSlots], p_empty[2], o_full[2], guarded[2], item_full[kItemSlots], item_empty[kItemSlots], row_full[2], row_empty[2], o_empty[2], taken;
+    uint64_t k_full[kUnits], k_empty[kUnits], v_full[kUnits], v_ready[kUnits], v_empty[kUnits];
+    uint64_t q_full[2], q_empty[2], s_full[2], s_empty, p_full[2][kValueSlots], p_empty[2], o_full[2], item_full[kItemSlots], item_empty[kItemSlots], row_full[2], row_empty[2], o_empty[2], taken;
     Item item[kItemSlots];
-    int not_finite[kItemSlots];           // first key whose values are not finite, of those in tiles that are not seen as a whole
+    int not_finite[kNotFiniteSlots];      // first key whose values are not finite, of those in tiles that are not seen as a whole
     alignas(16) uint32_t answer[4];
+    int next_at[4];                       // of a pair: what the first CTA was answered
     float2 row[2][kHalf];                 // reference and sum of the halves' rows
     Control ctl;
 };
@@ -114,6 +128,27 @@ __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem,
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// ... by a pair of CTAs: rows 0 .. 127 in the first one, the others in the second; either has half of B's columns
+__device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_bf16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 __device__ __forceinline__ void tc_st_x32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -136,6 +171,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int 
                  "r"(head), "r"(row), "r"(bar)
                  : "memory");
 }
+// ... whose completion is signalled on a barrier of the pair's first CTA (shared::cluster address)
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, int x, int head, int row, uint32_t bar_cluster) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x),
+                 "r"(head), "r"(row), "r"(bar_cluster)
+                 : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ int load_cluster(uint32_t at) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -208,7 +259,7 @@ __device__ __forceinline__ int cancelled_cta(uint32_t answer) {       // or -1: 
     return x;
 }
 
-// 64 keys of 128 values as two blocks of [64 keys][64 values], 128-byte swizzle, K (the keys) the slow dimension: groups of eight keys are 1024 bytes apart, the
+// 64 keys of 128 values as two blocks (of a pair: one) of [64 keys][64 values], 128-byte swizzle, K (the keys) the slow dimension: groups of eight keys are 1024 bytes apart, the
 // blocks 8192.
 __device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr) {
     uint64_t d = 0;
@@ -219,10 +270,6 @@ __device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr) {
     d |= static_cast<uint64_t>(2) << 61;
     return d;
 }
-// bf16 x bf16 -> fp32
-constexpr uint32_t kIdescScores = umma_idesc_e4m3_f32(kHalf, kTile) | (1u << 7) | (1u << 10);
-constexpr uint32_t kIdescSums = umma_idesc_e4m3_f32(kHalf, kValue) | (1u << 7) | (1u << 10) | (1u << 16);   // B transposed
-
 // ---------------------------------------------------------------- who works on what
 struct Seq {
     int q0, queries, k0, keys;
@@ -242,14 +289,16 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
     r.keys = max(0, min(k1, p.kv_tokens) - r.k0);
     return r;
 }
-__device__ __forceinline__ int blocks_of(int queries) { return (queries + kBlock - 1) / kBlock; }
 
 // The list of items: groups of heads, in those the blocks of queries, in those the heads of the group and the parts of the keys.  A group has so many heads that the CTAs
 // that work at one time share few heads' keys, which the L2 then holds.  Blocks with more keys come first (up to 32 sequences): an SM that is done
 // takes the next item of the list, and what is left for the end is short.
+template <int kCtas>
 struct List {
+    static constexpr int kBlock = Cfg<kCtas>::kBlock, kRows = Cfg<kCtas>::kRows;
+    static __device__ __forceinline__ int blocks_of(int queries) { return (queries + kBlock - 1) / kBlock; }
     Seq mine;                             // this lane's sequence (up to 32)
-    int blocks, behind;                   // its blocks; steps of two tiles by which it is shorter than the longest
+    int blocks, behind;                   // its blocks; by how many blocks' tiles it is shorter than the longest
     int total, last_step;                 // blocks in all; steps in which blocks come up
     int chunk, before;                    // beyond 32 sequences: first of the 32 at hand, blocks before those
     uint32_t group, group_first;          // group of heads of the item found last, the first item of it (but for parts)
@@ -261,7 +310,7 @@ struct List {
         mine = load_seq(p, lane);
         blocks = blocks_of(mine.queries);
         const int tiles = blocks > 0 ? (mine.keys + kTile - 1) / kTile : 0;
-        behind = (__reduce_max_sync(0xffffffffu, tiles) - tiles) >> 1;
+        behind = (__reduce_max_sync(0xffffffffu, tiles) - tiles) / (kBlock / kTile);
         last_step = __reduce_max_sync(0xffffffffu, blocks > 0 ? behind + blocks : 0) - 1;
         total = __reduce_add_sync(0xffffffffu, blocks);
         for (int s = kLanes; s < p.n_seqs; s += kLanes) total += __reduce_add_sync(0xffffffffu, blocks_of(load_seq(p, s + lane).queries));
@@ -331,7 +380,7 @@ struct List {
         it.k0 = s.k0;
         it.len = s.keys;
         it.limit = p.causal ? s.keys - s.queries + first : s.keys - 1;
-        it.alternate = it.rows <= kHalf;
+        it.alternate = it.rows <= kRows;
         const auto tiles_of_row = [&](int row) { return max(0, min(it.limit + (p.causal ? row : 0), s.keys - 1) + kTile) / kTile; };
         const int all = tiles_of_row(it.rows - 1);
         it.tile = static_cast<int>(static_cast<int64_t>(all) * it.split / p.splits);
@@ -341,7 +390,7 @@ struct List {
             it.n0 = (it.n + 1) >> 1;
             it.n1 = it.n >> 1;
         } else {
-            it.n0 = max(0, min(end, tiles_of_row(kHalf - 1)) - it.tile);
+            it.n0 = max(0, min(end, tiles_of_row(kRows - 1)) - it.tile);
             it.n1 = it.n;
         }
         it.edge = max(0, min(it.limit, s.keys - 1) + 1) / kTile;
@@ -371,15 +420,34 @@ __device__ __forceinline__ uint32_t unit_slot(bool alternate, int n, int t, bool
 }
 
 // ---------------------------------------------------------------- the kernel
+template <int kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
 expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qr, const __grid_constant__ CUtensorMap map_kn,
                           const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ CUtensorMap map_v, const Params p, unsigned int* status) {
+    using C = Cfg<kCtas>;
+    constexpr int kSlots = C::kSlots, kSlotBytes = C::kSlotBytes, kRows = C::kRows;
+    constexpr bool kPair = kCtas == 2;
     extern __shared__ __align__(1024) uint8_t smem[];
     Small& sm = *reinterpret_cast<Small*>(smem);
     Control* const ctl = &sm.ctl;
-    const uint32_t ring = smem_u32(smem) + kSmallBytes, queries = ring + kSlots * kSlotBytes;
+    const uint32_t ring = smem_u32(smem) + kSmallBytes, queries = ring + kRingBytes;
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const auto bar = [](const uint64_t& b) { return smem_u32(&b); };
+    // A pair's MMAs are the first CTA's: it waits for both, and both wait for it.
+    const uint32_t rank = kPair ? cluster_ctarank() : 0u;
+    const auto lead = [](const uint64_t& b) -> uint32_t { return kPair ? mapa_shared(smem_u32(&b), 0) : smem_u32(&b); };
+    const auto arrive_lead = [&](const uint64_t& b) {
+        if (kPair) mbar_arrive_cluster(lead(b));
+        else mbar_arrive(bar(b));
+    };
+    const auto commit = [](const uint64_t& b) {                      // the MMAs so far, to all CTAs
+        if (kPair) {
+            tc_commit_pair(smem_u32(&b));
+            tc_commit_pair(mapa_shared(smem_u32(&b), 1));
+        } else {
+            tc_commit(smem_u32(&b));
+        }
+    };
 
     griddep_launch_dependents();
     if (threadIdx.x == 0) {
@@ -387,31 +455,34 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             mbar_init(bar(sm.k_full[i]), 1);
             mbar_init(bar(sm.k_empty[i]), 1);
             mbar_init(bar(sm.v_full[i]), 1);
-            mbar_init(bar(sm.v_empty[i]), 2);                        // the MMAs, and the warp that looks at values
+            mbar_init(bar(sm.v_ready[i]), kCtas);                    // (looked at)
+            mbar_init(bar(sm.v_empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(sm.q_full[i]), 1);
             mbar_init(bar(sm.q_empty[i]), 1);
             mbar_init(bar(sm.s_full[i]), 1);
-            for (int j = 0; j < kValueSlots; ++j) mbar_init(bar(sm.p_full[i][j]), kSoftmaxWarps / 2);
+            for (int j = 0; j < kValueSlots; ++j) mbar_init(bar(sm.p_full[i][j]), kCtas * kSoftmaxWarps / 2);
             mbar_init(bar(sm.p_empty[i]), 1);
             mbar_init(bar(sm.o_full[i]), 1);
-            mbar_init(bar(sm.guarded[i]), 1);
             mbar_init(bar(sm.row_full[i]), kSoftmaxWarps / 2);
             mbar_init(bar(sm.row_empty[i]), kFinishWarps);
-            mbar_init(bar(sm.o_empty[i]), kFinishWarps);
+            mbar_init(bar(sm.o_empty[i]), kCtas * kFinishWarps);
         }
         for (int i = 0; i < kItemSlots; ++i) {
             mbar_init(bar(sm.item_full[i]), 1);
             mbar_init(bar(sm.item_empty[i]), kItemReaders);
         }
-        mbar_init(bar(sm.s_empty), kSoftmaxWarps / 2);
+        mbar_init(bar(sm.s_empty), kCtas * kSoftmaxWarps / 2);
         mbar_init(bar(sm.taken), 1);
         mbar_fence_init();
         ctl->abort_flag = (ring & 1023u) != 0 ? 1u : 0u;             // (dynamic shared memory begins at a multiple of 1024; swizzled tiles rely on it)
         if (ctl->abort_flag && atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = kRoom, status[2] = 0xFFFFFFFFu, status[3] = blockIdx.x;
     }
-    if (warp == kScoreWarp) tc_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+    if (warp == kScoreWarp) {
+        if (kPair) tc_alloc_pair(smem_u32(&ctl->tmem_base), kTmemCols);
+        else tc_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+    }
     if (warp == kLoadWarp && lane == 0) {
         tma_prefetch_desc(&map_qn);
         tma_prefetch_desc(&map_qr);
@@ -422,6 +493,10 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
     griddep_wait();
     tc_fence_before();
     __syncthreads();
+    if (kPair) {                                                     // (no signal before the other's barriers are set up)
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
     const bool well = ctl->abort_flag == 0;
@@ -450,13 +525,13 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kLoadWarp) {
             // ------------------------------------------------------------ the list, and the loads
-            List list;
+            List<kCtas> list;
             list.begin(p);
             uint32_t slot = 0, unit = 0, active = 0, taken = 0;      // slots and units filled; items with tiles
             uint32_t freed = 0, back = 0, keys = 0;                  // slots and units given back; which of the last 32 units are keys
             uint32_t k_loaded = 0, v_loaded = 0, k_back = 0, v_back = 0;
             bool ok = true;
-            int at = static_cast<int>(blockIdx.x);
+            int at = static_cast<int>(blockIdx.x) / kCtas;
             const auto one_back = [&](uint32_t newest) {             // the oldest unit on its way is given back
                 if (keys >> (newest - back) & 1) {
                     ok = wait(sm.k_empty[k_back % kUnits], (k_back / kUnits) & 1, kRoom, back);
@@ -470,12 +545,14 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 ++back;
             };
             // a slot of the unit at hand, when there is room for it
-            const auto fill = [&](bool first, const uint64_t& full, int slots, auto&& copy) {
-                if (first) keys = keys << 1 | (slots == kKeySlots ? 1u : 0u);
+            const auto fill = [&](bool first, bool of_keys, const uint64_t& full, auto&& copy) {
+                if (first) keys = keys << 1 | (of_keys ? 1u : 0u);
                 while (ok && slot + 1 - freed > kSlots) one_back(unit);
                 if (ok && elect_one()) {
-                    if (first) mbar_arrive_expect_tx(bar(full), slots * kSlotBytes);
-                    copy(ring + slot % kSlots * kSlotBytes, bar(full));
+                    // (keys: those of both CTAs arrive at the first one's barrier)
+                    if (first && !of_keys) mbar_arrive_expect_tx(bar(full), kValueSlots * kSlotBytes);
+                    if (first && of_keys && rank == 0) mbar_arrive_expect_tx(bar(full), kCtas * kKeySlots * kSlotBytes);
+                    copy(ring + slot % kSlots * kSlotBytes);
                 }
                 __syncwarp();
                 ++slot;
@@ -488,7 +565,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 ok = ok && __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_empty[place]), ((listed / kItemSlots) & 1) ^ 1, ctl, status, kItems, listed, kItemLimitNs));
                 if (ok && lane == 0) {
                     sm.item[place] = it;
-                    sm.not_finite[place] = 0x7FFFFFFF;
+                    sm.not_finite[listed % kNotFiniteSlots] = 0x7FFFFFFF;
                     mbar_arrive(bar(sm.item_full[place]));
                 }
                 __syncwarp();
@@ -497,7 +574,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             };
             // The next item is asked for as late as the loads allow: who asks early takes work that another SM would be free for.
             const auto ask = [&]() {
-                if (p.dynamic && elect_one()) {
+                if (p.dynamic && rank == 0 && elect_one()) {
                     mbar_arrive_expect_tx(bar(sm.taken), 16);
                     try_cancel(smem_u32(sm.answer), bar(sm.taken));
                 }
@@ -505,16 +582,27 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             };
             const auto answer = [&]() {
                 if (!p.dynamic) {
-                    at = at > 0x7FFFFFFF - static_cast<int>(gridDim.x) ? -1 : at + static_cast<int>(gridDim.x);
+                    const int step = static_cast<int>(gridDim.x) / kCtas;
+                    at = at > 0x7FFFFFFF - step ? -1 : at + step;
                     return;
                 }
                 ok = ok && wait(sm.taken, taken & 1, kItems, taken);
+                int& next_at = sm.next_at[taken % 4];
                 ++taken;
-                if (ok) {
+                if (!ok) return;
+                if (rank == 0) {
                     at = cancelled_cta(smem_u32(sm.answer));
+                    if (at > 0) at /= kCtas;
                     fence_proxy_async_shared();
-                    __syncwarp();
+                    if (kPair && lane == 0) {
+                        store_cluster(mapa_shared(smem_u32(&next_at), 1), at);
+                        mbar_arrive_cluster_release(mapa_shared(bar(sm.taken), 1));
+                    }
+                } else {
+                    fence_cluster();
+                    at = *static_cast<volatile int*>(&next_at);
                 }
+                __syncwarp();
             };
             Item it = publish();
             while (ok && it.rows > 0) {
@@ -525,28 +613,33 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     following = publish();
                 }
                 if (it.n > 0) {
+                    // (a pair's queries and keys arrive at the first CTA's barriers, values at the CTA's own)
+                    const auto copy = [&](uint32_t to, const CUtensorMap& map, int x, int head, int row, const uint64_t& full) {
+                        if (kPair) tma_load_3d_pair(to, &map, x, head, row, lead(full));
+                        else tma_load_3d(to, &map, x, head, row, bar(full));
+                    };
                     const auto load_queries = [&](int h) {
                         ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
                         if (ok && elect_one()) {
                             if (h == 1 && it.alternate) {
-                                mbar_arrive(bar(sm.q_full[h]));          // (both halves use the first one's)
+                                if (rank == 0) mbar_arrive(bar(sm.q_full[h]));          // (both halves use the first one's)
                             } else {
                                 const uint32_t to = queries + h * kQueryBytes;
-                                const int row = it.q0 + h * kHalf;
-                                mbar_arrive_expect_tx(bar(sm.q_full[h]), kQueryBytes);
-                                tma_load_3d(to, &map_qn, 0, it.head, row, bar(sm.q_full[h]));
-                                tma_load_3d(to + kSlotBytes, &map_qn, 64, it.head, row, bar(sm.q_full[h]));
-                                tma_load_3d(to + 2 * kSlotBytes, &map_qr, 0, it.head, row, bar(sm.q_full[h]));
+                                const int row = it.q0 + h * kRows + static_cast<int>(rank) * kHalf;
+                                if (rank == 0) mbar_arrive_expect_tx(bar(sm.q_full[h]), kCtas * kQueryBytes);
+                                copy(to, map_qn, 0, it.head, row, sm.q_full[h]);
+                                copy(to + kQueryPart, map_qn, 64, it.head, row, sm.q_full[h]);
+                                copy(to + 2 * kQueryPart, map_qr, 0, it.head, row, sm.q_full[h]);
                             }
                         }
                         __syncwarp();
                     };
                     const auto load_keys = [&](int t) {
-                        const int row = it.k0 + (it.tile + t) * kTile;
+                        const int row = it.k0 + (it.tile + t) * kTile + static_cast<int>(rank) * (kTile / kCtas);
                         const uint64_t& there = sm.k_full[k_loaded % kUnits];
-                        fill(true, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 0, it.head, row, full); });
-                        fill(false, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kn, 64, it.head, row, full); });
-                        fill(false, there, kKeySlots, [&](uint32_t to, uint32_t full) { tma_load_3d(to, &map_kr, 0, 0, row, full); });
+                        fill(true, true, there, [&](uint32_t to) { copy(to, map_kn, 0, it.head, row, there); });
+                        fill(false, true, there, [&](uint32_t to) { copy(to, map_kn, 64, it.head, row, there); });
+                        fill(false, true, there, [&](uint32_t to) { copy(to, map_kr, 0, 0, row, there); });
                         ++k_loaded;
                         ++unit;
                     };
@@ -554,9 +647,10 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
 #pragma unroll
                         for (int i = 0; i < kValueSlots; ++i) {
                             const int row = it.k0 + (it.tile + t) * kTile + i * 64;
-                            fill(i == 0, sm.v_full[v_loaded % kUnits], kValueSlots, [&](uint32_t to, uint32_t full) {
-                                tma_load_3d(to, &map_v, 0, it.head, row, full);
-                                tma_load_3d(to + kSlotBytes / 2, &map_v, 64, it.head, row, full);
+                            const uint64_t& there = sm.v_full[v_loaded % kUnits];
+                            fill(i == 0, false, there, [&](uint32_t to) {
+                                tma_load_3d(to, &map_v, static_cast<int>(rank) * 64, it.head, row, bar(there));
+                                if (!kPair) tma_load_3d(to + kSlotBytes / 2, &map_v, 64, it.head, row, bar(there));
                             });
                         }
                         ++v_loaded;
@@ -595,7 +689,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 const int n = uniform(it.n), n0 = uniform(it.n0), step = uniform(it.alternate);
                 if (!ok || uniform(it.rows) == 0) break;
                 item_done(count);
-                if (n == 0) continue;
+                if (n == 0 || rank != 0) continue;
                 for (int h = 0; h < 2; ++h) ok = ok && wait(sm.q_full[h], active & 1, kQueriesThere, active);
 #pragma unroll 1
                 for (int t = 0, u = 0; t < n && ok; ++t, ++keys) {
@@ -613,17 +707,21 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                             for (int c = 0; c < kKeySlots; ++c) {
                                 const uint64_t b = ring_desc + (slot + u + c) % kSlots * (kSlotBytes >> 4);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) tc_mma_bf16(tmem + kTmemScores, a + c * (kSlotBytes >> 4) + 2 * k, b + 2 * k, kIdescScores, (c | k) != 0);
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint64_t ak = a + c * (kQueryPart >> 4) + 2 * k;
+                                    if (kPair) tc_mma_bf16_pair(tmem + kTmemScores, ak, b + 2 * k, C::kIdescScores, (c | k) != 0);
+                                    else tc_mma_bf16(tmem + kTmemScores, ak, b + 2 * k, C::kIdescScores, (c | k) != 0);
+                                }
                             }
-                            tc_commit(bar(sm.s_full[h]));
+                            commit(sm.s_full[h]);
                         }
                         __syncwarp();
                     }
                     if (elect_one()) {
-                        tc_commit(bar(sm.k_empty[keys % kUnits]));
+                        commit(sm.k_empty[keys % kUnits]);
                         // (what is not needed any more: the first half may be done a tile before the second)
-                        if (t == max(0, (step ? n : n0) - 1)) tc_commit(bar(sm.q_empty[0]));
-                        if (t == n - 1) tc_commit(bar(sm.q_empty[1]));
+                        if (t == max(0, (step ? n : n0) - 1)) commit(sm.q_empty[0]);
+                        if (t == n - 1) commit(sm.q_empty[1]);
                     }
                     __syncwarp();
                 }
@@ -632,14 +730,15 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             }
         } else if (warp == kSumWarp) {
             // ------------------------------------------------------------ the MMAs of the sums
-            uint32_t slot = 0, values = 0, edges = 0, summed0 = 0, summed1 = 0;
+            uint32_t slot = 0, values = 0, summed0 = 0, summed1 = 0;
             const uint64_t ring_desc = umma_desc_values(ring);
             bool ok = true;
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
-                const int n = uniform(it.n), n0 = uniform(it.n0), n1 = uniform(it.n1), step = uniform(it.alternate), edge = uniform(it.edge) - uniform(it.tile);
+                const int n = uniform(it.n), n0 = uniform(it.n0), n1 = uniform(it.n1), step = uniform(it.alternate);
                 if (!ok || uniform(it.rows) == 0) break;
                 item_done(count);
+                if (rank != 0) continue;
                 // (the sums of the item before are read: waited for with every item, or the parities would not tell)
                 const auto sums_room = [&](int h) { ok = ok && wait(sm.o_empty[h], (count & 1) ^ 1, kSumsThere, count); };
                 if (n0 == 0) sums_room(0);
@@ -647,11 +746,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
 #pragma unroll 1
                 for (int t = 0; t < n && ok; ++t, ++values) {
                     const uint32_t u = slot + unit_slot(step != 0, n, t, false);
-                    ok = wait(sm.v_full[values % kUnits], (values / kUnits) & 1, kTileThere, values);
-                    if (t >= edge) {
-                        ok = ok && wait(sm.guarded[edges & 1], (edges >> 1) & 1, kGuarded, edges);
-                        ++edges;
-                    }
+                    ok = wait(sm.v_ready[values % kUnits], (values / kUnits) & 1, kGuarded, values);
 #pragma unroll 1
                     for (int h = step ? t & 1 : t < n0 ? 0 : 1, end = step ? h + 1 : 2; h < end && ok; ++h) {
                         const uint32_t tile = h == 0 ? summed0 : summed1, d = tmem + kTmemSums + h * kValue, weights = tmem + kTmemWeights + h * (kTile / 2);
@@ -666,26 +761,29 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                             const uint64_t b = ring_desc + (u + i) % kSlots * (kSlotBytes >> 4);
                             if (elect_one()) {
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) tc_mma_bf16_ts(d, weights + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), kIdescSums, adds || k != 0);
+                                for (int k = 0; k < 4; ++k) {
+                                    if (kPair) tc_mma_bf16_ts_pair(d, weights + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), C::kIdescSums, adds || k != 0);
+                                    else tc_mma_bf16_ts(d, weights + (i * 4 + k) * 8, b + k * (16 * 128 >> 4), C::kIdescSums, adds || k != 0);
+                                }
                                 if (i + 1 == kValueSlots) {
-                                    tc_commit(bar(sm.p_empty[h]));
-                                    if (t + step + 1 >= (step ? n : h == 0 ? n0 : n1)) tc_commit(bar(sm.o_full[h]));
+                                    commit(sm.p_empty[h]);
+                                    if (t + step + 1 >= (step ? n : h == 0 ? n0 : n1)) commit(sm.o_full[h]);
                                 }
                             }
                             __syncwarp();
                         }
                         h == 0 ? ++summed0 : ++summed1;
                     }
-                    if (elect_one()) tc_commit(bar(sm.v_empty[values % kUnits]));
+                    if (elect_one()) commit(sm.v_empty[values % kUnits]);
                     __syncwarp();
                 }
                 slot += (kKeySlots + kValueSlots) * n;
             }
         } else if (warp == kGuardWarp) {
-            // ------------------------------------------------------------ values that the MMA must not see.  The warp follows all values (a wait by parity is exact only for who has
-            // seen the phase before; so none are given back without it), and works on the tiles that are not seen as a whole by all queries.
+            // ------------------------------------------------------------ values that the MMA must not see.  The warp passes all values on to the MMAs, and works on the tiles that are
+            // not seen as a whole by all queries.
             uint8_t* const base = smem + kSmallBytes;
-            uint32_t slot = 0, values = 0, edges = 0;
+            uint32_t slot = 0, values = 0;
             bool ok = true;
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
@@ -698,7 +796,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     for (int i = 0; i < kValueSlots && look; ++i) {
                         const int key0 = (it.tile + t) * kTile + i * 64;
                         uint4* const at = reinterpret_cast<uint4*>(base + (u + i) % kSlots * kSlotBytes);
-                        // 64 keys x 8 pieces of 16 bytes, twice; rows are keys, and a row's pieces stay in it
+                        // 64 keys x 8 pieces of 16 bytes, for either 64 dimensions; rows are keys, and a row's pieces stay in it
                         const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
                         __nv_bfloat162 seen[4] = {zero, zero, zero, zero};
                         if (key0 + 63 >= it.len) {
@@ -728,16 +826,12 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                                 }
                             }
                             bad = __reduce_min_sync(0xffffffffu, bad);
-                            if (lane == 0) atomicMin(&sm.not_finite[count % kItemSlots], bad);
+                            if (lane == 0) atomicMin(&sm.not_finite[count % kNotFiniteSlots], bad);
                         }
                     }
-                    fence_proxy_async_shared();
+                    if (look) fence_proxy_async_shared();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (look) mbar_arrive(bar(sm.guarded[edges & 1]));
-                        mbar_arrive(bar(sm.v_empty[values % kUnits]));
-                    }
-                    if (look) ++edges;
+                    if (lane == 0) arrive_lead(sm.v_ready[values % kUnits]);
                 }
                 slot += (kKeySlots + kValueSlots) * it.n;
                 item_done(count);
@@ -753,7 +847,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
                 if (!ok || it.rows == 0) break;
-                const int not_finite_at = static_cast<int>(count % kItemSlots);
+                const int& not_finite = sm.not_finite[count % kNotFiniteSlots];
                 const auto half_there = [&](int h) {
                     ok = ok && wait(sm.row_full[h], count & 1, kSumsThere, count);
                     if ((h == 0 ? it.n0 : it.n1) == 0) return;
@@ -766,7 +860,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(bar(sm.row_empty[h]));
-                        mbar_arrive(bar(sm.o_empty[h]));
+                        arrive_lead(sm.o_empty[h]);
                     }
                 };
 #pragma unroll 1
@@ -775,7 +869,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     if (it.alternate) half_there(1);
                     if (!ok) break;
                     tc_fence_after();
-                    const int row0 = h * kHalf + quarter * 32, row = row0 + lane;
+                    const int row0 = h * kRows + static_cast<int>(rank) * kHalf + quarter * 32, row = row0 + lane;
                     float2 stats = sm.row[h][quarter * 32 + lane];   // reference and sum
                     float f = 1.0f, other = 0.0f;                    // factors of the half's sums, and of the other one's
                     if (it.alternate) {
@@ -787,7 +881,9 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     }
                     const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);
                     const bool nothing = stats.x == -INFINITY && !isnan(stats.y);
-                    const bool spoilt = last >= *static_cast<volatile int*>(&sm.not_finite[not_finite_at]);
+                    int bad = *static_cast<const volatile int*>(&not_finite);
+                    if (kPair) bad = min(bad, load_cluster(mapa_shared(smem_u32(&not_finite), rank ^ 1u)));      // (its slot is not used again before this item's sums are read)
+                    const bool spoilt = last >= bad;
                     const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / stats.y;
                     const float2 f2 = make_float2(f * inv, f * inv), other2 = make_float2(other * inv, other * inv), zero2 = make_float2(0.0f, 0.0f);
                     const int64_t place = static_cast<int64_t>(it.q0 + row0) * p.heads + it.head, part = static_cast<int64_t>(it.split) * p.tokens * p.heads + place;
@@ -838,7 +934,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         for (uint32_t count = 0; ok; ++count) {
             const Item it = next_item(count, ok);
             if (!ok || it.rows == 0) break;
-            const int n = h == 0 ? it.n0 : it.n1, row0 = (it.alternate ? 0 : h * kHalf) + quarter * 32, row = row0 + lane;
+            const int n = h == 0 ? it.n0 : it.n1, row0 = (it.alternate ? 0 : h * kRows) + static_cast<int>(rank) * kHalf + quarter * 32, row = row0 + lane;
             const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);           // key that the query sees last
             const int last0 = min(it.limit + (p.causal ? row0 : 0), it.len - 1);         // ... of the warp's first one
             float top = -INFINITY;
@@ -856,7 +952,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 tc_wait_ld();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(sm.s_empty));
+                if (lane == 0) arrive_lead(sm.s_empty);
                 if (visible0 < kTile - 1) {
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) x[i] = i > visible ? 0xFF800000u : x[i];
@@ -913,7 +1009,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                         tc_wait_st();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar(sm.p_full[h][first >> 6]));
+                        if (lane == 0) arrive_lead(sm.p_full[h][first >> 6]);
                     }
                 }
             }
@@ -925,6 +1021,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             if (lane == 0) mbar_arrive(bar(sm.row_full[h]));
             item_done(count);
         }
+        // (none of the signals of the MMAs may be on its way when the CTA leaves its shared memory to another)
+        if (ok && tiles > 0) wait(sm.p_empty[h], (tiles - 1) & 1, kWeightsRoom, tiles);
     }
 
     // ---------------------------------------------------------------- teardown
@@ -937,24 +1035,40 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
         __syncthreads();
     }
+    if (kPair) {                                                     // (no signal is on its way to a CTA that has gone)
+        cluster_arrive();
+        cluster_wait();
+    }
     if (warp == kScoreWarp) {
         tc_fence_after();
-        tc_dealloc(tmem, kTmemCols);
+        if (kPair) tc_dealloc_pair(tmem, kTmemCols);
+        else tc_dealloc(tmem, kTmemCols);
     }
 }
 
 // How a call is cut up.  What is known on the host is how many queries, keys and sequences there are, not which sequence has how many.
 struct Plan {
+    int ctas;                             // to a block of queries
     int64_t blocks;                       // at most
     int splits, head_group;
 };
 constexpr int kLeastTiles = 4;            // of a part
 constexpr int64_t kGroupBytes = 32ll << 20;
-Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, int sms) {
+// Whether CTAs work in pairs: a tile then takes 3.4 units of time where it takes a CTA alone 4.4, but a block's begin and end the time of 6.9 tiles where they take 3.4 (measured: 512 queries of 128
+// heads over 512, 2048 and 8192 keys 26.2, 79.3 and 290.9 us alone, 32.0, 72.9 and 250.3 in pairs), and blocks are filled up to 256 queries, not to 128.  A gain of 3 % or more is asked for: 2048 queries
+// of 128 heads over themselves 164.4 alone, 170.4 in pairs; 1024 over 4096 270.8 and 242.0; 1500 over 2500 202.9 and 195.8.
+bool pairs_pay(int64_t tokens, int64_t kv_tokens, int64_t n_seqs, bool causal) {
+    const double queries = std::max(1.0, static_cast<double>(tokens) / n_seqs), keys = static_cast<double>(kv_tokens) / n_seqs;
+    const double tiles = (causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (causal ? 0.5 : 0.0);
+    return 1.03 * std::ceil(queries / 256) * 2 * 3.41 * (tiles + 6.9) < std::ceil(queries / 128) * 4.42 * (tiles + 3.4);
+}
+Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, bool causal, int sms) {
     Plan pl;
-    const int64_t each = ragged ? 0 : tokens / n_seqs;
+    pl.ctas = sms > 1 && pairs_pay(tokens, kv_tokens, n_seqs, causal) ? 2 : 1;
+    const int64_t each = ragged ? 0 : tokens / n_seqs, rows = pl.ctas * 2 * kHalf;
     const int64_t seqs = std::min(n_seqs, tokens);                   // that have queries
-    pl.blocks = ragged ? (tokens - seqs) / kBlock + seqs : n_seqs * ((each + kBlock - 1) / kBlock);
+    pl.blocks = ragged ? (tokens - seqs) / rows + seqs : n_seqs * ((each + rows - 1) / rows);
+    sms /= pl.ctas;
     const int64_t items = pl.blocks * heads;
     // Where there are fewer items than SMs their keys are cut, in as many parts as fill the SMs once (a second round would cost what it gains).
     const int64_t most = (kv_tokens / n_seqs + kTile - 1) / kTile;
@@ -970,21 +1084,49 @@ size_t partial_bytes(const Plan& pl, int64_t tokens, int64_t heads) {
     return pl.splits > 1 ? static_cast<size_t>(pl.splits) * tokens * heads * (kValue + 1) * sizeof(float) : 0;
 }
 
+template <int kCtas>
 int prepare_kernel() {
     static std::atomic<uint64_t> prepared{0};                        // devices
     int device = 0;
     DSV3_CUDA_TRY(cudaGetDevice(&device));
     if (device >= 64 || !(prepared.load(std::memory_order_relaxed) >> device & 1)) {
-        DSV3_CUDA_TRY(cudaFuncSetAttribute(expanded_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        DSV3_CUDA_TRY(cudaFuncSetAttribute(expanded_attention_kernel<kCtas>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
         // (the warps that ask for more registers wait for those that the block does not have)
         cudaFuncAttributes attr = {};
-        DSV3_CUDA_TRY(cudaFuncGetAttributes(&attr, expanded_attention_kernel));
+        DSV3_CUDA_TRY(cudaFuncGetAttributes(&attr, expanded_attention_kernel<kCtas>));
         if (attr.numRegs * kThreads < kSoftmaxRegs * 256 + kOtherRegs * 256) {
             set_last_error("expanded_attention: built with %d registers a thread, too few to share out", attr.numRegs);
             return DSV3_ERR_UNSUPPORTED;
         }
         if (device < 64) prepared.fetch_or(1ull << device, std::memory_order_relaxed);
     }
+    return DSV3_OK;
+}
+
+template <int kCtas>
+int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, const CUtensorMap& kr, const CUtensorMap& v, const Params& p, int64_t items, unsigned int* status,
+           cudaStream_t stream) {
+    if (const int rc = prepare_kernel<kCtas>(); rc != DSV3_OK) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * kCtas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (kCtas > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = kCtas, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    DSV3_CUDA_TRY(cudaLaunchKernelEx(&cfg, expanded_attention_kernel<kCtas>, qn, qr, kn, kr, v, p, status));
     return DSV3_OK;
 }
 
@@ -995,9 +1137,9 @@ using namespace dsv3;
 
 extern "C" {
 
-size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged) {
+size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged, int causal) {
     if (tokens <= 0 || kv_tokens <= 0 || heads <= 0 || n_seqs <= 0) return 0;
-    return partial_bytes(plan_of(tokens, kv_tokens, heads, n_seqs, ragged != 0, device_sms()), tokens, heads);
+    return partial_bytes(plan_of(tokens, kv_tokens, heads, n_seqs, ragged != 0, causal != 0, device_sms()), tokens, heads);
 }
 
 int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace, size_t workspace_bytes, dsv3_stream_t stream) {
@@ -1029,8 +1171,8 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
         return DSV3_ERR_UNSUPPORTED;
     }
     const int sms = device_sms();
-    const Plan pl = plan_of(a->tokens, std::max<int64_t>(1, a->kv_tokens), a->heads, a->n_seqs, ragged, sms);
-    if (a->heads > 1024 || a->tokens > 0x7FFFFF00ll || a->kv_tokens > 0x7FFFFF00ll || pl.blocks * a->heads * pl.splits > 0x7FFFFFFFll) {
+    const Plan pl = plan_of(a->tokens, std::max<int64_t>(1, a->kv_tokens), a->heads, a->n_seqs, ragged, a->causal != 0, sms);
+    if (a->heads > 1024 || a->tokens > 0x7FFFFF00ll || a->kv_tokens > 0x7FFFFF00ll || pl.blocks * a->heads * pl.splits > 0x3FFFFFFFll) {
         set_last_error("expanded_attention: more than 1024 heads, or 2^31 queries, keys or blocks of queries");
         return DSV3_ERR_UNSUPPORTED;
     }
@@ -1041,7 +1183,6 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
     }
     unsigned int* const status = status_device_ptr();
     if (!status) return DSV3_ERR_CUDA;
-    if (const int rc = prepare_kernel(); rc != DSV3_OK) return rc;
     CUtensorMap qn, qr, kn, kr, v;
     // (without keys nothing is loaded; the maps then describe the queries)
     const bool keys = a->kv_tokens > 0;
@@ -1052,8 +1193,8 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
         kn = v = qn;
         kr = qr;
     } else {
-        if ((rc = make_tmap_heads(&kn, a->k_nope, kNope, a->heads, a->kv_tokens, a->k_nope_head_stride, a->k_nope_token_stride, kTile)) != DSV3_OK) return rc;
-        if ((rc = make_tmap_heads(&kr, a->k_rope, kRope, 1, a->kv_tokens, 0, a->k_rope_token_stride, kTile)) != DSV3_OK) return rc;
+        if ((rc = make_tmap_heads(&kn, a->k_nope, kNope, a->heads, a->kv_tokens, a->k_nope_head_stride, a->k_nope_token_stride, kTile / pl.ctas)) != DSV3_OK) return rc;
+        if ((rc = make_tmap_heads(&kr, a->k_rope, kRope, 1, a->kv_tokens, 0, a->k_rope_token_stride, kTile / pl.ctas)) != DSV3_OK) return rc;
         if ((rc = make_tmap_heads(&v, a->v, kValue, a->heads, a->kv_tokens, a->v_head_stride, a->v_token_stride, kTile / 2)) != DSV3_OK) return rc;
     }
     const int64_t items = pl.blocks * a->heads * pl.splits, rows = a->tokens * a->heads;
@@ -1071,9 +1212,9 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
     p.by_last_group = make_fast_div(a->heads % pl.head_group ? a->heads % pl.head_group : pl.head_group);
     p.out = static_cast<__nv_bfloat16*>(a->out), p.lse = a->lse;
     p.partial = partial, p.partial_lse = need ? partial + pl.splits * rows * kValue : nullptr;
-    const int64_t grid = dynamic ? items : std::min<int64_t>(items, num_sms());
-    DSV3_CUDA_TRY(launch_dependent(expanded_attention_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kSmemBytes, static_cast<cudaStream_t>(stream), qn, qr, kn,
-                                   kr, v, p, status));
+    const int64_t grid = dynamic ? items : std::min<int64_t>(items, std::max(1, num_sms() / pl.ctas));
+    const auto go = pl.ctas == 2 ? launch<2> : launch<1>;
+    if (rc = go(qn, qr, kn, kr, v, p, grid, status, static_cast<cudaStream_t>(stream)); rc != DSV3_OK) return rc;
     if (!need) return DSV3_OK;
     return join_partials(partial, p.partial_lse, pl.splits, rows, kValue, p.cu_q, a->n_seqs, a->heads, a->out, a->lse, static_cast<cudaStream_t>(stream));
 }

@@ -71,7 +71,7 @@ PyObject* py_expanded_attention(PyObject*, PyObject* const* args, Py_ssize_t n) 
         if (with_lse) lse = new_cuda(sizes, at::kFloat, dev);
         c10::cuda::OptionalCUDAGuard guard;                                    // (the size is that of the current device)
         if (dev.index() != c10::cuda::current_device()) guard.set_device(dev);
-        const size_t need = dsv3_expanded_attention_workspace_bytes(q.tokens, k.tokens, static_cast<int>(q.heads), static_cast<int>(n_seqs), cu_q != nullptr);
+        const size_t need = dsv3_expanded_attention_workspace_bytes(q.tokens, k.tokens, static_cast<int>(q.heads), static_cast<int>(n_seqs), cu_q != nullptr, causal);
         // (given back after the launches: torch hands the memory out again in the stream's order)
         const at::Tensor ws = need ? new_cuda({static_cast<int64_t>(need)}, at::kByte, dev) : at::Tensor();
         const dsv3_expanded_attention_t a = {qn.const_data_ptr(), q.token_stride, q.head_stride, qr.const_data_ptr(), r.token_stride, r.head_stride,

@@ -435,7 +435,7 @@ typedef struct dsv3_expanded_attention {
     void* out;
     float* lse;
 } dsv3_expanded_attention_t;
-size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged);
+size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged, int causal);
 int dsv3_expanded_attention(const dsv3_expanded_attention_t* args, void* workspace, size_t workspace_bytes, dsv3_stream_t stream);
 
 /*

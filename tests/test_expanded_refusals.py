@@ -17,7 +17,7 @@ def _lib():
     from dsv3_b200 import _lib
     lib = ctypes.CDLL(_lib.LIB_PATH)
     lib.dsv3_expanded_attention.argtypes = [vp, vp, ctypes.c_size_t, vp]
-    lib.dsv3_expanded_attention_workspace_bytes.argtypes = [i64, i64, ci, ci, ci]
+    lib.dsv3_expanded_attention_workspace_bytes.argtypes = [i64, i64, ci, ci, ci, ci]
     lib.dsv3_expanded_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.dsv3_attention_join.argtypes = [vp, vp, ci, i64, ci, vp, vp, vp]
     lib.dsv3_rotary_table.argtypes = [ci, ctypes.c_double, ctypes.c_double, i64, ctypes.c_double, ctypes.c_double, i64, i64, vp, vp]
@@ -52,13 +52,13 @@ def test_attention_of_nothing_and_workspaces():
     assert lib.dsv3_expanded_attention(_args(tokens=0), None, 0, None) == names.OK
     assert lib.dsv3_expanded_attention(_args(heads=0), None, 0, None) == names.OK
     # few queries over many keys leave parts behind
-    need = lib.dsv3_expanded_attention_workspace_bytes(8, 8000, 2, 1, 0)
+    need = lib.dsv3_expanded_attention_workspace_bytes(8, 8000, 2, 1, 0, 1)
     assert need > 0 and need % (8 * 2 * 129 * 4) == 0
     assert lib.dsv3_expanded_attention(_args(kv_tokens=8000), None, 0, None) == names.ERR_WORKSPACE
     assert lib.dsv3_expanded_attention(_args(kv_tokens=8000), 256, need - 1, None) == names.ERR_WORKSPACE
     assert lib.dsv3_expanded_attention(_args(kv_tokens=8000), 264, need, None) == names.ERR_WORKSPACE
-    assert lib.dsv3_expanded_attention_workspace_bytes(100000, 100000, 128, 1, 0) == 0
-    assert lib.dsv3_expanded_attention_workspace_bytes(0, 8000, 2, 1, 0) == 0
+    assert lib.dsv3_expanded_attention_workspace_bytes(100000, 100000, 128, 1, 0, 1) == 0
+    assert lib.dsv3_expanded_attention_workspace_bytes(0, 8000, 2, 1, 0, 1) == 0
 
 
 def test_joins_that_are_refused():

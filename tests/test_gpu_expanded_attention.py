@@ -182,6 +182,39 @@ def test_a_budget_of_sms_changes_nothing(sms):
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
 
 
+@pytest.mark.parametrize("q, k, heads, causal", [([1700], [2600], 40, True), ([1536, 1400, 1000], [6000, 1400, 7000], 24, True), ([512, 700], [3000, 4001], 37, False), ([2100], [5000], 9, True),
+                                                 ([1000], [8000], 3, True), ([1024], [1300], 1, False)])
+@pytest.mark.parametrize("sms", [0, 7, 60])
+def test_long_chunks_over_many_keys(q, k, heads, causal, sms):
+    """What CTAs work on in pairs: several blocks to a pair, blocks of fewer queries than a pair has room for among them, and keys that are cut."""
+    from dsv3_b200 import set_num_sms
+    args = inputs(q, k, heads, seed=sms)
+    set_num_sms(sms)
+    try:
+        out, lse = _run(args, q, k, causal)
+    finally:
+        set_num_sms(0)
+    for b in range(len(q)):
+        rows, keys = slice(sum(q[:b]), sum(q[:b + 1])), slice(sum(k[:b]), sum(k[:b + 1]))
+        for h in range(0, heads, 4):
+            part = [args[0][rows, h:h + 4], args[1][rows, h:h + 4], args[2][keys, h:h + 4], args[3][keys], args[4][keys, h:h + 4]]
+            want, want_lse, bound, lse_bound = reference(*part, q[b:b + 1], k[b:b + 1], causal)
+            check(out[rows, h:h + 4], want, bound)
+            check(lse[rows, h:h + 4], want_lse, lse_bound, "lse")
+
+
+def test_values_that_are_not_finite_in_a_pairs_tiles():
+    """Either CTA of a pair looks at half of the values' dimensions; what one finds both know."""
+    q, k = [1536], [6000]
+    for column in (5, 100):
+        for bad in (4600, 5990):
+            args = [t.clone() for t in inputs(q, k, 2)]
+            args[4][bad, 1, column] = math.inf
+            out, _ = _run(args, q, k)
+            sees = torch.arange(1536, device="cuda") + 6000 - 1536 >= bad
+            assert bool(out[:, 0].isfinite().all()) and bool(out[~sees].isfinite().all()) and not out[sees][:, 1, column].isfinite().any()
+
+
 def test_offsets_beyond_32_bits():
     """Keys whose last sequence begins more than 2^31 values, and 2^32 bytes, behind the first."""
     heads, tokens = 128, 70000

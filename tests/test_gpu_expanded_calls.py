@@ -36,7 +36,7 @@ def test_rows_that_belong_to_no_sequence_are_left_as_they_are(q, k, heads):
     tokens = front + sum(q) + back
     out = torch.full((tokens, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
     lse = torch.full((tokens, heads), 7.0, device="cuda")
-    need = lib.dsv3_expanded_attention_workspace_bytes(tokens, args[2].shape[0], heads, len(q), 1)
+    need = lib.dsv3_expanded_attention_workspace_bytes(tokens, args[2].shape[0], heads, len(q), 1, 1)
     ws = torch.full((max(need, 1),), 0xFF, dtype=torch.uint8, device="cuda")
     c = _c_args(*args, out, lse, cu_q, cu_k, len(q))
     assert lib.dsv3_expanded_attention(ctypes.byref(c), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == names.OK
