@@ -55,7 +55,7 @@ constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(kSoftmaxRegs * 256 + kOtherRegs * 256 <= 65536 / kThreads / 8 * 8 * kThreads, "what the block was launched with");
 constexpr int kTmemScores = 0, kTmemWeights = kTile, kTmemSums = 2 * kTile, kTmemCols = 512;   // columns; weights: 64 to a half, sums: 128
 constexpr int kAhead = 1;                        // tiles that scores are ahead of sums (twice as many where halves take turns)
-constexpr int kAskEarly = 5, kAnswerEarly = 2;   // units before an item's last at which the next item is asked for, and the answer read
+constexpr int kAskEarly = 2;                     // tiles before an item's end at which the next item is asked for
 constexpr int kNotFiniteSlots = 8;
 constexpr int kItemSlots = 2, kItemReaders = kSoftmaxWarps + 3 + kFinishWarps;
 constexpr int kLanes = 32;                       // sequences that are put in order of their length
@@ -398,20 +398,7 @@ struct List {
     }
 };
 
-// An item's units in the order in which they are loaded and the MMAs come to them: K0 K1 V0 K2 V1 ... V(n-1), or K0 K1 K2 V0 K3 V1 ... where tiles alternate.
-struct Unit {
-    bool keys;
-    int tile;
-};
-__device__ __forceinline__ Unit unit_of(const Item& it, int u) {
-    const int ahead = min(it.alternate ? 2 * kAhead : kAhead, it.n);
-    if (u < ahead) return {true, u};
-    u -= ahead;
-    const int both = 2 * (it.n - ahead);                             // units that come in pairs
-    if (u < both) return {(u & 1) == 0, (u >> 1) + ((u & 1) == 0 ? ahead : 0)};
-    return {false, u - (it.n - ahead)};
-}
-
+// An item's units are loaded as the MMAs come to them: K0 K1 V0 K2 V1 ... V(n-1), or K0 K1 K2 V0 K3 V1 ... where tiles alternate.
 // The slot of tile t's keys or values, from the item's first on.
 __device__ __forceinline__ uint32_t unit_slot(bool alternate, int n, int t, bool keys) {
     const int ahead = min(alternate ? 2 * kAhead : kAhead, n);
@@ -527,35 +514,21 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             // ------------------------------------------------------------ the list, and the loads
             List<kCtas> list;
             list.begin(p);
-            uint32_t slot = 0, unit = 0, active = 0, taken = 0;      // slots and units filled; items with tiles
-            uint32_t freed = 0, back = 0, keys = 0;                  // slots and units given back; which of the last 32 units are keys
+            // (This warp sets the pace: an MMA's 64 cycles are what a few instructions take here.  A unit is armed and copied by one lane in one go.)
+            uint32_t slot = 0, active = 0, taken = 0;                // slots filled; items with tiles
+            uint32_t freed = 0, back = 0, keys = 0, loaded = 0;      // slots and units given back; which of the last 32 units are keys; units
             uint32_t k_loaded = 0, v_loaded = 0, k_back = 0, v_back = 0;
             bool ok = true;
             int at = static_cast<int>(blockIdx.x) / kCtas;
-            const auto one_back = [&](uint32_t newest) {             // the oldest unit on its way is given back
-                if (keys >> (newest - back) & 1) {
-                    ok = wait(sm.k_empty[k_back % kUnits], (k_back / kUnits) & 1, kRoom, back);
-                    freed += kKeySlots;
-                    ++k_back;
-                } else {
-                    ok = wait(sm.v_empty[v_back % kUnits], (v_back / kUnits) & 1, kRoom, back);
-                    freed += kValueSlots;
-                    ++v_back;
-                }
+            const auto one_back = [&]() {                            // the oldest unit on its way is given back
+                const bool of_keys = keys >> (loaded - 1 - back) & 1;
+                const uint32_t i = of_keys ? k_back++ : v_back++;
+                ok = wait((of_keys ? sm.k_empty : sm.v_empty)[i % kUnits], (i / kUnits) & 1, kRoom, back);
+                freed += of_keys ? kKeySlots : kValueSlots;
                 ++back;
             };
-            // a slot of the unit at hand, when there is room for it
-            const auto fill = [&](bool first, bool of_keys, const uint64_t& full, auto&& copy) {
-                if (first) keys = keys << 1 | (of_keys ? 1u : 0u);
-                while (ok && slot + 1 - freed > kSlots) one_back(unit);
-                if (ok && elect_one()) {
-                    // (keys: those of both CTAs arrive at the first one's barrier)
-                    if (first && !of_keys) mbar_arrive_expect_tx(bar(full), kValueSlots * kSlotBytes);
-                    if (first && of_keys && rank == 0) mbar_arrive_expect_tx(bar(full), kCtas * kKeySlots * kSlotBytes);
-                    copy(ring + slot % kSlots * kSlotBytes);
-                }
-                __syncwarp();
-                ++slot;
+            const auto room = [&](int slots) {
+                while (ok && slot + slots - freed > kSlots) one_back();
             };
             // item number `at`, for the others to read
             uint32_t listed = 0;
@@ -634,49 +607,60 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                         }
                         __syncwarp();
                     };
+                    const int head = uniform(it.head), n = uniform(it.n), ahead = uniform(it.alternate) != 0 ? 2 * kAhead : kAhead, row0 = uniform(it.k0 + it.tile * kTile);
                     const auto load_keys = [&](int t) {
-                        const int row = it.k0 + (it.tile + t) * kTile + static_cast<int>(rank) * (kTile / kCtas);
+                        const int row = row0 + t * kTile + static_cast<int>(rank) * (kTile / kCtas);
                         const uint64_t& there = sm.k_full[k_loaded % kUnits];
-                        fill(true, true, there, [&](uint32_t to) { copy(to, map_kn, 0, it.head, row, there); });
-                        fill(false, true, there, [&](uint32_t to) { copy(to, map_kn, 64, it.head, row, there); });
-                        fill(false, true, there, [&](uint32_t to) { copy(to, map_kr, 0, 0, row, there); });
-                        ++k_loaded;
-                        ++unit;
+                        room(kKeySlots);
+                        if (ok && elect_one()) {
+                            if (rank == 0) mbar_arrive_expect_tx(bar(there), kCtas * kKeySlots * kSlotBytes);
+                            copy(ring + slot % kSlots * kSlotBytes, map_kn, 0, head, row, there);
+                            copy(ring + (slot + 1) % kSlots * kSlotBytes, map_kn, 64, head, row, there);
+                            copy(ring + (slot + 2) % kSlots * kSlotBytes, map_kr, 0, 0, row, there);
+                        }
+                        __syncwarp();
+                        keys = keys << 1 | 1u;
+                        slot += kKeySlots;
+                        ++k_loaded, ++loaded;
                     };
                     const auto load_values = [&](int t) {
+                        const int row = row0 + t * kTile;
+                        const uint64_t& there = sm.v_full[v_loaded % kUnits];
+                        room(kValueSlots);
+                        if (ok && elect_one()) {
+                            mbar_arrive_expect_tx(bar(there), kValueSlots * kSlotBytes);
 #pragma unroll
-                        for (int i = 0; i < kValueSlots; ++i) {
-                            const int row = it.k0 + (it.tile + t) * kTile + i * 64;
-                            const uint64_t& there = sm.v_full[v_loaded % kUnits];
-                            fill(i == 0, false, there, [&](uint32_t to) {
-                                tma_load_3d(to, &map_v, static_cast<int>(rank) * 64, it.head, row, bar(there));
-                                if (!kPair) tma_load_3d(to + kSlotBytes / 2, &map_v, 64, it.head, row, bar(there));
-                            });
+                            for (int i = 0; i < kValueSlots; ++i) {
+                                const uint32_t to = ring + (slot + i) % kSlots * kSlotBytes;
+                                tma_load_3d(to, &map_v, static_cast<int>(rank) * 64, head, row + i * 64, bar(there));
+                                if (!kPair) tma_load_3d(to + kSlotBytes / 2, &map_v, 64, head, row + i * 64, bar(there));
+                            }
                         }
-                        ++v_loaded;
-                        ++unit;
+                        __syncwarp();
+                        keys <<= 1;
+                        slot += kValueSlots;
+                        ++v_loaded, ++loaded;
                     };
-                    const int ask_at = max(0, 2 * it.n - kAskEarly), answer_at = max(ask_at, 2 * it.n - kAnswerEarly);
-                    for (int u = 0; u < 2 * it.n && ok; ++u) {
-                        const Unit w = unit_of(it, u);
-                        if (u == ask_at) ask();
-                        if (u == answer_at) {
-                            answer();
-                            following = publish();
-                        }
-                        if (w.keys) load_keys(w.tile);
-                        else load_values(w.tile);
-                        if (u == 0) {
+                    const int ask_at = max(-ahead, n - kAskEarly);
+#pragma unroll 1
+                    for (int t = -ahead; t < n && ok; ++t) {
+                        if (t == ask_at) ask();
+                        if (t + ahead < n) load_keys(t + ahead);
+                        if (t == -ahead) {
                             load_queries(0);
                             load_queries(1);
                         }
+                        if (t >= 0) load_values(t);
                     }
                     ++active;
+                    // (the MMAs still have some tiles to go)
+                    answer();
+                    following = publish();
                 }
                 it = following;
             }
             // none of the arrivals on empty[] may be in flight when the CTA leaves its shared memory to another
-            while (ok && back < unit) one_back(unit - 1);
+            while (ok && back < loaded) one_back();
             for (int h = 0; h < 2 && ok && active > 0; ++h) ok = wait(sm.q_empty[h], (active - 1) & 1, kQueriesThere, active);
         } else if (warp == kScoreWarp) {
             // ------------------------------------------------------------ the MMAs of the scores.  Those of the sums have a warp of their own: an MMA takes 64 cycles, and what lies between
