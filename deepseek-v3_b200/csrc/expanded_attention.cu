@@ -103,8 +103,8 @@ struct Small {
     float2 row[2][kHalf];                 // reference and sum of the halves' rows
     Control ctl;
 };
-constexpr int kSmallBytes = 3072, kSmemBytes = kSmallBytes + kOperandBytes;
-static_assert(sizeof(Small) <= kSmallBytes && kSmemBytes <= 232448, "shared memory of a CTA");
+constexpr int kSmallBytes = (sizeof(Small) + 1023) / 1024 * 1024, kSmemBytes = kSmallBytes + kOperandBytes;
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 // ---------------------------------------------------------------- PTX
 __device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -1038,21 +1038,13 @@ struct Plan {
 };
 constexpr int kLeastTiles = 4;            // of a part
 constexpr int64_t kGroupBytes = 32ll << 20;
-// Whether CTAs work in pairs: a tile then takes 3.4 units of time where it takes a CTA alone 4.4, but a block's begin and end the time of 6.9 tiles where they take 3.4 (measured: 512 queries of 128
-// heads over 512, 2048 and 8192 keys 26.2, 79.3 and 290.9 us alone, 32.0, 72.9 and 250.3 in pairs), and blocks are filled up to 256 queries, not to 128.  A gain of 3 % or more is asked for: 2048 queries
-// of 128 heads over themselves 164.4 alone, 170.4 in pairs; 1024 over 4096 270.8 and 242.0; 1500 over 2500 202.9 and 195.8.
-bool pairs_pay(int64_t tokens, int64_t kv_tokens, int64_t n_seqs, bool causal) {
-    const double queries = std::max(1.0, static_cast<double>(tokens) / n_seqs), keys = static_cast<double>(kv_tokens) / n_seqs;
-    const double tiles = (causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (causal ? 0.5 : 0.0);
-    return 1.03 * std::ceil(queries / 256) * 2 * 3.41 * (tiles + 6.9) < std::ceil(queries / 128) * 4.42 * (tiles + 3.4);
-}
-Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, bool causal, int sms) {
+Plan plan_for(int ctas, int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, int sms) {
     Plan pl;
-    pl.ctas = sms > 1 && pairs_pay(tokens, kv_tokens, n_seqs, causal) ? 2 : 1;
-    const int64_t each = ragged ? 0 : tokens / n_seqs, rows = pl.ctas * 2 * kHalf;
+    pl.ctas = ctas;
+    const int64_t each = ragged ? 0 : tokens / n_seqs, rows = ctas * 2 * kHalf;
     const int64_t seqs = std::min(n_seqs, tokens);                   // that have queries
     pl.blocks = ragged ? (tokens - seqs) / rows + seqs : n_seqs * ((each + rows - 1) / rows);
-    sms /= pl.ctas;
+    sms /= ctas;
     const int64_t items = pl.blocks * heads;
     // Where there are fewer items than SMs their keys are cut, in as many parts as fill the SMs once (a second round would cost what it gains).
     const int64_t most = (kv_tokens / n_seqs + kTile - 1) / kTile;
@@ -1063,6 +1055,23 @@ Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, b
     const int64_t bytes = heads * kv_tokens * 2 * (kNope + kValue), groups = n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, items / (2 * sms)));
     pl.head_group = static_cast<int>((heads + groups - 1) / groups);
     return pl;
+}
+// How long a plan takes, in times that half a block of a CTA alone takes for a tile (1.17 us): what there is to do, spread over all SMs, or the longest item, whichever is more.  A pair's tile takes
+// 0.785 of that and its block's begin and end as long as 4.1 of its tiles, not 2, and its blocks are filled up to 256 queries, not to 128.  Fitted to 52 calls of 2 to 128 heads, 64 to 16001 queries
+// and up to 16384 keys; where the two differ by more than 3 % it picks the faster but for two of them (5 % and 3 %).  Alone / in pairs: 512 queries of 128 heads over 512 keys 24.0 / 28.9 us, over 2048
+// 79.4 / 70.6, over 8192 298 / 250; 515 of 16 heads over 4099 35.4 / 39.7; 1000 over 8000 78.1 / 67.0; 300 and 500 over 3000 and 2500 37.7 / 47.3; 16001 over themselves 942 / 836.
+double time_of(const Plan& pl, int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool causal, int sms) {
+    const double queries = std::max(1.0, static_cast<double>(tokens) / n_seqs), keys = static_cast<double>(kv_tokens) / n_seqs;
+    const double tiles = (causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (causal ? 0.5 : 0.0);
+    const double a_tile = pl.ctas == 2 ? 0.785 : 1.0, ends = pl.ctas == 2 ? 4.1 : 2.0, halves = std::ceil(queries / (pl.ctas * kHalf));
+    const double all = heads * n_seqs * halves * (tiles + ends * pl.splits) / (sms / pl.ctas), longest = std::min(2.0, halves) * (keys / kTile / pl.splits + ends);
+    return a_tile * std::max(all, longest);
+}
+Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, bool causal, int sms) {
+    const Plan alone = plan_for(1, tokens, kv_tokens, heads, n_seqs, ragged, sms);
+    if (sms < 2) return alone;
+    const Plan pairs = plan_for(2, tokens, kv_tokens, heads, n_seqs, ragged, sms);
+    return time_of(pairs, tokens, kv_tokens, heads, n_seqs, causal, sms) < time_of(alone, tokens, kv_tokens, heads, n_seqs, causal, sms) ? pairs : alone;
 }
 size_t partial_bytes(const Plan& pl, int64_t tokens, int64_t heads) {
     return pl.splits > 1 ? static_cast<size_t>(pl.splits) * tokens * heads * (kValue + 1) * sizeof(float) : 0;

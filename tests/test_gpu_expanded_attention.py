@@ -183,7 +183,8 @@ def test_a_budget_of_sms_changes_nothing(sms):
 
 
 @pytest.mark.parametrize("q, k, heads, causal", [([1700], [2600], 40, True), ([1536, 1400, 1000], [6000, 1400, 7000], 24, True), ([512, 700], [3000, 4001], 37, False), ([2100], [5000], 9, True),
-                                                 ([1000], [8000], 3, True), ([1024], [1300], 1, False)])
+                                                 ([1000], [8000], 3, True), ([1024], [1300], 1, False),
+                                                 ([1000], [8000], 16, True), ([700], [5000], 33, False)])
 @pytest.mark.parametrize("sms", [0, 7, 60])
 def test_long_chunks_over_many_keys(q, k, heads, causal, sms):
     """What CTAs work on in pairs: several blocks to a pair, blocks of fewer queries than a pair has room for among them, and keys that are cut."""
@@ -203,12 +204,13 @@ def test_long_chunks_over_many_keys(q, k, heads, causal, sms):
             check(lse[rows, h:h + 4], want_lse, lse_bound, "lse")
 
 
-def test_values_that_are_not_finite_in_a_pairs_tiles():
+@pytest.mark.parametrize("heads", [2, 24])
+def test_values_that_are_not_finite_in_a_pairs_tiles(heads):
     """Either CTA of a pair looks at half of the values' dimensions; what one finds both know."""
     q, k = [1536], [6000]
     for column in (5, 100):
         for bad in (4600, 5990):
-            args = [t.clone() for t in inputs(q, k, 2)]
+            args = [t.clone() for t in inputs(q, k, heads)]
             args[4][bad, 1, column] = math.inf
             out, _ = _run(args, q, k)
             sees = torch.arange(1536, device="cuda") + 6000 - 1536 >= bad
