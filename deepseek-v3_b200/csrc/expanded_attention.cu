@@ -299,6 +299,7 @@ struct List {
     static __device__ __forceinline__ int blocks_of(int queries) { return (queries + kBlock - 1) / kBlock; }
     Seq mine;                             // this lane's sequence (up to 32)
     int blocks, behind;                   // its blocks; by how many blocks' tiles it is shorter than the longest
+    int short_at;                         // its last block's place in their order, if the halves share the tiles: it takes half the time
     int total, last_step;                 // blocks in all; steps in which blocks come up
     int chunk, before;                    // beyond 32 sequences: first of the 32 at hand, blocks before those
     uint32_t group, group_first;          // group of heads of the item found last, the first item of it (but for parts)
@@ -311,6 +312,8 @@ struct List {
         blocks = blocks_of(mine.queries);
         const int tiles = blocks > 0 ? (mine.keys + kTile - 1) / kTile : 0;
         behind = (__reduce_max_sync(0xffffffffu, tiles) - tiles) / (kBlock / kTile);
+        const bool is_short = blocks > 0 && mine.queries - (blocks - 1) * kBlock <= kRows;
+        short_at = !is_short ? 0 : p.causal ? min(blocks - 1, tiles / 2 / (kBlock / kTile)) : blocks - 1;
         last_step = __reduce_max_sync(0xffffffffu, blocks > 0 ? behind + blocks : 0) - 1;
         total = __reduce_add_sync(0xffffffffu, blocks);
         for (int s = kLanes; s < p.n_seqs; s += kLanes) total += __reduce_add_sync(0xffffffffu, blocks_of(load_seq(p, s + lane).queries));
@@ -345,7 +348,8 @@ struct List {
             uint32_t there = __ballot_sync(0xffffffffu, step >= behind && step < behind + blocks);
             for (int i = earlier; i < place; ++i) there &= there - 1;
             const int from = __ffs(there) - 1;
-            block = __shfl_sync(0xffffffffu, blocks - 1 - (step - behind), from);
+            const int i = step - behind;
+            block = __shfl_sync(0xffffffffu, i < short_at ? blocks - 2 - i : i == short_at ? blocks - 1 : blocks - 1 - i, from);
             s = {__shfl_sync(0xffffffffu, mine.q0, from), __shfl_sync(0xffffffffu, mine.queries, from), __shfl_sync(0xffffffffu, mine.k0, from),
                  __shfl_sync(0xffffffffu, mine.keys, from)};
         } else {
@@ -813,7 +817,10 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                             if (lane == 0) atomicMin(&sm.not_finite[count % kNotFiniteSlots], bad);
                         }
                     }
-                    if (look) fence_proxy_async_shared();
+                    if (look) {
+                        fence_proxy_async_shared();
+                        if (kPair) fence_cluster();                  // (the other CTA's warps read not_finite)
+                    }
                     __syncwarp();
                     if (lane == 0) arrive_lead(sm.v_ready[values % kUnits]);
                 }
@@ -866,6 +873,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);
                     const bool nothing = stats.x == -INFINITY && !isnan(stats.y);
                     int bad = *static_cast<const volatile int*>(&not_finite);
+                    if (kPair) fence_cluster();
                     if (kPair) bad = min(bad, load_cluster(mapa_shared(smem_u32(&not_finite), rank ^ 1u)));      // (its slot is not used again before this item's sums are read)
                     const bool spoilt = last >= bad;
                     const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / stats.y;
@@ -1030,7 +1038,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
     }
 }
 
-// How a call is cut up.  What is known on the host is how many queries, keys and sequences there are, not which sequence has how many.
+// How a call is cut up: whether CTAs work in pairs, and in how many parts the keys of a block of queries are cut.  What is known on the host is how many queries, keys and sequences there are, not
+// which sequence has how many.
 struct Plan {
     int ctas;                             // to a block of queries
     int64_t blocks;                       // at most
@@ -1038,40 +1047,44 @@ struct Plan {
 };
 constexpr int kLeastTiles = 4;            // of a part
 constexpr int64_t kGroupBytes = 32ll << 20;
-Plan plan_for(int ctas, int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, int sms) {
-    Plan pl;
-    pl.ctas = ctas;
-    const int64_t each = ragged ? 0 : tokens / n_seqs, rows = ctas * 2 * kHalf;
-    const int64_t seqs = std::min(n_seqs, tokens);                   // that have queries
-    pl.blocks = ragged ? (tokens - seqs) / rows + seqs : n_seqs * ((each + rows - 1) / rows);
-    sms /= ctas;
-    const int64_t items = pl.blocks * heads;
-    // Where there are fewer items than SMs their keys are cut, in as many parts as fill the SMs once (a second round would cost what it gains).
-    const int64_t most = (kv_tokens / n_seqs + kTile - 1) / kTile;
-    // (`blocks` is more than there are, as a rule, where sequences are ragged)
-    const int64_t room = ragged && n_seqs > 1 ? sms + sms / 8 : sms;
-    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxJoinParts, room / items, most / kLeastTiles})));
+struct Call {
+    int64_t tokens, kv_tokens, heads, n_seqs;
+    bool ragged, causal;
+};
+// How long a plan takes, in times that half a block of a CTA alone takes for a tile (1.03 us): what there is to do, spread over all SMs, or its longest item; where all items are about as long, as many
+// rounds of them as there are.  A pair's tile takes 0.807 of that, an item's begin and end as long as 2.5 of its half's tiles (of a pair's 4.5), a join 5.9 and 56 more for a million partial rows.
+// Fitted to 78 calls of 1 to 16001 queries and 37 to 16384 keys, alone and in pairs, 26 of them in up to 12 parts.  Of those it picks the fastest or one at most 6 % slower.
+//   Parts of 2, 3 and 4: 515 queries of 16 heads over 4099 keys 45.2, 36.5 and 41.5 us; 512 over 8192 in pairs 65.9, 51.5 and 44.6; 2 heads of 16001 tokens in pairs 121, 130 and 133, and 195 in one.
+// Alone / in pairs: 512 queries of 128 heads over 512 keys 24.0 / 28.9 us, over 2048 79.4 / 70.6, over 8192 298 / 250; 1000 of 16 over 8000 78.7 / 69.3; 16001 of 16 over themselves 942 / 836.
+double time_of(const Call& c, int ctas, int splits, int sms) {
+    const double slots = sms / ctas, queries = std::max(1.0, static_cast<double>(c.tokens) / c.n_seqs), keys = static_cast<double>(c.kv_tokens) / c.n_seqs;
+    const double longest = keys / kTile, tiles = (c.causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (c.causal ? 0.5 : 0.0);
+    const double a_tile = ctas == 2 ? 0.807 : 1.0, ends = ctas == 2 ? 4.5 : 2.5;
+    const double halves = std::ceil(queries / (ctas * kHalf)), items = c.heads * c.n_seqs * std::max(1.0, halves / 2) * splits;
+    const double all = c.heads * c.n_seqs * halves * (tiles + ends * splits) / slots, one = std::min(2.0, halves) * (longest / splits + ends);
+    const double alike = std::pow(std::max(0.0, std::min(1.0, 2 * tiles / longest - 1)), 0.75);       // 0: of all lengths up to the longest
+    const double time = std::max({all, one, all + (std::ceil(items / slots) * one - all) * alike});
+    return a_tile * time + (splits > 1 ? 5.9 + 56e-6 * splits * c.tokens * c.heads : 0.0);
+}
+Plan plan_of(const Call& c, int sms) {
+    // (the tiles of a sequence, if all have as many)
+    const int64_t most = (c.kv_tokens / c.n_seqs + kTile - 1) / kTile;
+    const int last = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxJoinParts, most / kLeastTiles)));
+    Plan pl = {1, 0, 1, 0};
+    double best = time_of(c, 1, 1, sms);
+    // (blocks of a pair that are not half full gain nothing: 64 queries of 128 heads over 4000 keys 55.9 us alone, 75.3 in pairs)
+    for (int ctas = 1; ctas <= (sms > 1 && c.tokens / c.n_seqs >= 2 * kHalf ? 2 : 1); ++ctas)
+        for (int splits = 1; splits <= last; ++splits) {
+            const double time = time_of(c, ctas, splits, sms) * (ctas == 2 ? 1.04 : 1.0);        // (what is as good is not worth a pair)
+            if (time < best) best = time, pl.ctas = ctas, pl.splits = splits;
+        }
+    const int64_t each = c.ragged ? 0 : c.tokens / c.n_seqs, rows = pl.ctas * 2 * kHalf, seqs = std::min(c.n_seqs, c.tokens);      // (that have queries)
+    pl.blocks = c.ragged ? (c.tokens - seqs) / rows + seqs : c.n_seqs * ((each + rows - 1) / rows);
     // Groups of heads, equal ones: as few as keep a group's keys and values in the L2, and no more than leave each of them two items to an SM.
-    const int64_t bytes = heads * kv_tokens * 2 * (kNope + kValue), groups = n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, items / (2 * sms)));
-    pl.head_group = static_cast<int>((heads + groups - 1) / groups);
+    const int64_t bytes = c.heads * c.kv_tokens * 2 * (kNope + kValue);
+    const int64_t groups = c.n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, pl.blocks * c.heads / (2 * std::max(1, sms / pl.ctas))));
+    pl.head_group = static_cast<int>((c.heads + groups - 1) / groups);
     return pl;
-}
-// How long a plan takes, in times that half a block of a CTA alone takes for a tile (1.17 us): what there is to do, spread over all SMs, or the longest item, whichever is more.  A pair's tile takes
-// 0.785 of that and its block's begin and end as long as 4.1 of its tiles, not 2, and its blocks are filled up to 256 queries, not to 128.  Fitted to 52 calls of 2 to 128 heads, 64 to 16001 queries
-// and up to 16384 keys; where the two differ by more than 3 % it picks the faster but for two of them (5 % and 3 %).  Alone / in pairs: 512 queries of 128 heads over 512 keys 24.0 / 28.9 us, over 2048
-// 79.4 / 70.6, over 8192 298 / 250; 515 of 16 heads over 4099 35.4 / 39.7; 1000 over 8000 78.1 / 67.0; 300 and 500 over 3000 and 2500 37.7 / 47.3; 16001 over themselves 942 / 836.
-double time_of(const Plan& pl, int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool causal, int sms) {
-    const double queries = std::max(1.0, static_cast<double>(tokens) / n_seqs), keys = static_cast<double>(kv_tokens) / n_seqs;
-    const double tiles = (causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (causal ? 0.5 : 0.0);
-    const double a_tile = pl.ctas == 2 ? 0.785 : 1.0, ends = pl.ctas == 2 ? 4.1 : 2.0, halves = std::ceil(queries / (pl.ctas * kHalf));
-    const double all = heads * n_seqs * halves * (tiles + ends * pl.splits) / (sms / pl.ctas), longest = std::min(2.0, halves) * (keys / kTile / pl.splits + ends);
-    return a_tile * std::max(all, longest);
-}
-Plan plan_of(int64_t tokens, int64_t kv_tokens, int64_t heads, int64_t n_seqs, bool ragged, bool causal, int sms) {
-    const Plan alone = plan_for(1, tokens, kv_tokens, heads, n_seqs, ragged, sms);
-    if (sms < 2) return alone;
-    const Plan pairs = plan_for(2, tokens, kv_tokens, heads, n_seqs, ragged, sms);
-    return time_of(pairs, tokens, kv_tokens, heads, n_seqs, causal, sms) < time_of(alone, tokens, kv_tokens, heads, n_seqs, causal, sms) ? pairs : alone;
 }
 size_t partial_bytes(const Plan& pl, int64_t tokens, int64_t heads) {
     return pl.splits > 1 ? static_cast<size_t>(pl.splits) * tokens * heads * (kValue + 1) * sizeof(float) : 0;
@@ -1132,7 +1145,7 @@ extern "C" {
 
 size_t dsv3_expanded_attention_workspace_bytes(int64_t tokens, int64_t kv_tokens, int heads, int n_seqs, int ragged, int causal) {
     if (tokens <= 0 || kv_tokens <= 0 || heads <= 0 || n_seqs <= 0) return 0;
-    return partial_bytes(plan_of(tokens, kv_tokens, heads, n_seqs, ragged != 0, causal != 0, device_sms()), tokens, heads);
+    return partial_bytes(plan_of({tokens, kv_tokens, heads, n_seqs, ragged != 0, causal != 0}, device_sms()), tokens, heads);
 }
 
 int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace, size_t workspace_bytes, dsv3_stream_t stream) {
@@ -1164,7 +1177,7 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
         return DSV3_ERR_UNSUPPORTED;
     }
     const int sms = device_sms();
-    const Plan pl = plan_of(a->tokens, std::max<int64_t>(1, a->kv_tokens), a->heads, a->n_seqs, ragged, a->causal != 0, sms);
+    const Plan pl = plan_of({a->tokens, std::max<int64_t>(1, a->kv_tokens), a->heads, a->n_seqs, ragged, a->causal != 0}, sms);
     if (a->heads > 1024 || a->tokens > 0x7FFFFF00ll || a->kv_tokens > 0x7FFFFF00ll || pl.blocks * a->heads * pl.splits > 0x3FFFFFFFll) {
         set_last_error("expanded_attention: more than 1024 heads, or 2^31 queries, keys or blocks of queries");
         return DSV3_ERR_UNSUPPORTED;
