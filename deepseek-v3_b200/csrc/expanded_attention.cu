@@ -95,11 +95,11 @@ struct Item {
 
 struct Small {
     uint64_t k_full[kUnits], k_empty[kUnits], v_full[kUnits], v_ready[kUnits], v_empty[kUnits];
-    uint64_t q_full[2], q_empty[2], s_full[2], s_empty, p_full[2][kValueSlots], p_empty[2], o_full[2], item_full[kItemSlots], item_empty[kItemSlots], row_full[2], row_empty[2], o_empty[2], taken;
+    uint64_t q_full[2], q_empty[2], s_full[2], s_empty, p_full[2][kValueSlots], p_empty[2], o_full[2], item_full[kItemSlots], item_empty[kItemSlots], row_full[2], row_empty[2], o_empty[2], taken, seen;
     Item item[kItemSlots];
     int not_finite[kNotFiniteSlots];      // first key whose values are not finite, of those in tiles that are not seen as a whole
     alignas(16) uint32_t answer[4];
-    int next_at[4];                       // of a pair: what the first CTA was answered
+    int next_at;                          // of a pair: what the first CTA was answered
     float2 row[2][kHalf];                 // reference and sum of the halves' rows
     Control ctl;
 };
@@ -303,10 +303,10 @@ struct List {
     int total, last_step;                 // blocks in all; steps in which blocks come up
     int chunk, before;                    // beyond 32 sequences: first of the 32 at hand, blocks before those
     uint32_t group, group_first;          // group of heads of the item found last, the first item of it (but for parts)
-    int step;                             // ... and the step in which its block came up
+    int step, earlier;                    // ... the step in which its block came up, and the blocks of the steps before
     __device__ __forceinline__ void begin(const Params& p) {
         const int lane = threadIdx.x & 31;
-        chunk = before = step = 0;
+        chunk = before = step = earlier = 0;
         group = group_first = 0;
         mine = load_seq(p, lane);
         blocks = blocks_of(mine.queries);
@@ -329,15 +329,14 @@ struct List {
         it.split = static_cast<int>(at - unsplit * p.splits);
         // (items are asked for in ascending order, as a rule: from where the last one was it is not far)
         const uint32_t group_items = static_cast<uint32_t>(total) * p.head_group;
-        if (unsplit < group_first) group = group_first = 0, step = 0;
-        while (unsplit - group_first >= group_items) group_first += group_items, ++group, step = 0;
+        if (unsplit < group_first) group = group_first = 0, step = earlier = 0;
+        while (unsplit - group_first >= group_items) group_first += group_items, ++group, step = earlier = 0;
         const uint32_t in_group = unsplit - group_first, heads = min(p.head_group, p.heads - static_cast<int>(group) * p.head_group);
         const int place = static_cast<int>(fast_div(in_group, static_cast<int>(heads) == p.head_group ? p.by_group : p.by_last_group));
         it.head = static_cast<int>(group * p.head_group + in_group - place * heads);
         Seq s;
         int block;
         if (p.n_seqs <= kLanes) {
-            int earlier = up_to(step - 1);                           // blocks that come up before the step
             if (earlier > place) step = earlier = 0;
             for (;;) {
                 const int here = up_to(step);
@@ -387,8 +386,8 @@ struct List {
         it.alternate = it.rows <= kRows;
         const auto tiles_of_row = [&](int row) { return max(0, min(it.limit + (p.causal ? row : 0), s.keys - 1) + kTile) / kTile; };
         const int all = tiles_of_row(it.rows - 1);
-        it.tile = static_cast<int>(static_cast<int64_t>(all) * it.split / p.splits);
-        const int end = static_cast<int>(static_cast<int64_t>(all) * (it.split + 1) / p.splits);
+        it.tile = static_cast<int>(fast_div(static_cast<uint32_t>(all) * it.split, p.by_splits));              // (2^24 tiles, 32 parts)
+        const int end = static_cast<int>(fast_div(static_cast<uint32_t>(all) * (it.split + 1), p.by_splits));
         it.n = end - it.tile;
         if (it.alternate) {
             it.n0 = (it.n + 1) >> 1;
@@ -466,6 +465,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         }
         mbar_init(bar(sm.s_empty), kCtas * kSoftmaxWarps / 2);
         mbar_init(bar(sm.taken), 1);
+        mbar_init(bar(sm.seen), 1);
+        for (int i = 0; i < kNotFiniteSlots; ++i) sm.not_finite[i] = 0x7FFFFFFF;
         mbar_fence_init();
         ctl->abort_flag = (ring & 1023u) != 0 ? 1u : 0u;             // (dynamic shared memory begins at a multiple of 1024; swizzled tiles rely on it)
         if (ctl->abort_flag && atomicCAS(&status[0], 0u, 1u) == 0u) status[1] = kRoom, status[2] = 0xFFFFFFFFu, status[3] = blockIdx.x;
@@ -542,7 +543,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 ok = ok && __all_sync(0xffffffffu, bounded_wait_ns(bar(sm.item_empty[place]), ((listed / kItemSlots) & 1) ^ 1, ctl, status, kItems, listed, kItemLimitNs));
                 if (ok && lane == 0) {
                     sm.item[place] = it;
-                    sm.not_finite[listed % kNotFiniteSlots] = 0x7FFFFFFF;
+                    sm.not_finite[(listed + kNotFiniteSlots / 2) % kNotFiniteSlots] = 0x7FFFFFFF;      // (a pair's other CTA may be an item ahead)
                     mbar_arrive(bar(sm.item_full[place]));
                 }
                 __syncwarp();
@@ -564,21 +565,25 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     return;
                 }
                 ok = ok && wait(sm.taken, taken & 1, kItems, taken);
-                int& next_at = sm.next_at[taken % 4];
-                ++taken;
                 if (!ok) return;
                 if (rank == 0) {
                     at = cancelled_cta(smem_u32(sm.answer));
                     if (at > 0) at /= kCtas;
                     fence_proxy_async_shared();
-                    if (kPair && lane == 0) {
-                        store_cluster(mapa_shared(smem_u32(&next_at), 1), at);
-                        mbar_arrive_cluster_release(mapa_shared(bar(sm.taken), 1));
+                    if (kPair) {
+                        ok = wait(sm.seen, (taken & 1) ^ 1, kItems, taken);      // (the other one has read the answer before)
+                        if (ok && lane == 0) {
+                            store_cluster(mapa_shared(smem_u32(&sm.next_at), 1), at);
+                            mbar_arrive_cluster_release(mapa_shared(bar(sm.taken), 1));
+                        }
                     }
                 } else {
                     fence_cluster();
-                    at = *static_cast<volatile int*>(&next_at);
+                    at = *static_cast<volatile int*>(&sm.next_at);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_release(lead(sm.seen));
                 }
+                ++taken;
                 __syncwarp();
             };
             Item it = publish();
@@ -727,10 +732,14 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 if (!ok || uniform(it.rows) == 0) break;
                 item_done(count);
                 if (rank != 0) continue;
-                // (the sums of the item before are read: waited for with every item, or the parities would not tell)
+                // (the sums of the item before are read: waited for, and the end signalled, with every item, so that neither side gets ahead of what parities tell)
                 const auto sums_room = [&](int h) { ok = ok && wait(sm.o_empty[h], (count & 1) ^ 1, kSumsThere, count); };
-                if (n0 == 0) sums_room(0);
-                if (n1 == 0) sums_room(1);
+                for (int h = 0; h < 2; ++h) {
+                    if ((h == 0 ? n0 : n1) > 0) continue;
+                    sums_room(h);
+                    if (ok && elect_one()) commit(sm.o_full[h]);
+                    __syncwarp();
+                }
 #pragma unroll 1
                 for (int t = 0; t < n && ok; ++t, ++values) {
                     const uint32_t u = slot + unit_slot(step != 0, n, t, false);
@@ -833,18 +842,13 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             const int quarter = warp - kFinishWarp;
             const uint32_t sums_at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemSums;
             const float c = p.scale;
-            uint32_t sums0 = 0, sums1 = 0;
             bool ok = true;
             for (uint32_t count = 0; ok; ++count) {
                 const Item it = next_item(count, ok);
                 if (!ok || it.rows == 0) break;
                 const int& not_finite = sm.not_finite[count % kNotFiniteSlots];
                 const auto half_there = [&](int h) {
-                    ok = ok && wait(sm.row_full[h], count & 1, kSumsThere, count);
-                    if ((h == 0 ? it.n0 : it.n1) == 0) return;
-                    uint32_t& sums = h == 0 ? sums0 : sums1;
-                    ok = ok && wait(sm.o_full[h], sums & 1, kSumsThere, sums);
-                    ++sums;
+                    ok = ok && wait(sm.row_full[h], count & 1, kSumsThere, count) && wait(sm.o_full[h], count & 1, kSumsThere, count);
                 };
                 const auto half_done = [&](int h) {
                     tc_fence_before();

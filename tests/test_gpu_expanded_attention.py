@@ -204,6 +204,23 @@ def test_long_chunks_over_many_keys(q, k, heads, causal, sms):
             check(lse[rows, h:h + 4], want_lse, lse_bound, "lse")
 
 
+def test_long_sequences_among_those_that_see_little():
+    """Blocks of a pair, some of which have no tiles at all, or only one half of them has."""
+    q, k, heads = [1500, 1500, 700, 1300, 900], [4000, 0, 6000, 100, 1700], 24
+    args = inputs(q, k, heads)
+    first, first_lse = _run(args, q, k)
+    for b in range(len(q)):
+        rows, keys = slice(sum(q[:b]), sum(q[:b + 1])), slice(sum(k[:b]), sum(k[:b + 1]))
+        for h in range(0, heads, 8):
+            part = [args[0][rows, h:h + 8], args[1][rows, h:h + 8], args[2][keys, h:h + 8], args[3][keys], args[4][keys, h:h + 8]]
+            want, want_lse, bound, lse_bound = reference(*part, q[b:b + 1], k[b:b + 1], True)
+            check(first[rows, h:h + 8], want, bound)
+            check(first_lse[rows, h:h + 8], want_lse, lse_bound, "lse")
+    for _ in range(20):
+        out, lse = _run(args, q, k)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
 @pytest.mark.parametrize("heads", [2, 24])
 def test_values_that_are_not_finite_in_a_pairs_tiles(heads):
     """Either CTA of a pair looks at half of the values' dimensions; what one finds both know."""
