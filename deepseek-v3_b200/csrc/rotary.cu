@@ -62,12 +62,20 @@ struct Rows {
     float sign;                                         // of the sines
 };
 
-// Eight values of a head as they lie in memory.
+// Eight values of a head as they lie in memory: side by side, or four and four.
 template <typename T>
 struct Eight {
     uint4 w;
     __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+    __device__ __forceinline__ void load(const T* p, int second) {
+        const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + second);
+        w = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    __device__ __forceinline__ void store(T* p, int second) const {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w.x, w.y);
+        *reinterpret_cast<uint2*>(p + second) = make_uint2(w.z, w.w);
+    }
     __device__ __forceinline__ void get(float* v) const {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -99,15 +107,17 @@ struct Eight<float> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
     __device__ __forceinline__ void store(float* p) const { reinterpret_cast<float4*>(p)[0] = a, reinterpret_cast<float4*>(p)[1] = b; }
+    __device__ __forceinline__ void load(const float* p, int second) { a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + second); }
+    __device__ __forceinline__ void store(float* p, int second) const { *reinterpret_cast<float4*>(p) = a, *reinterpret_cast<float4*>(p + second) = b; }
     __device__ __forceinline__ void get(float* v) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
     __device__ __forceinline__ void set(const float* v) { a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]); }
 };
 
-// A unit is 16 values of a head in the layout of halves (eight from either half), else 8: four or eight pairs.  A thread keeps its unit's angles in registers and
+// A unit is eight values of a head, four pairs if they turn: side by side, or in the layout of halves four of either half.  A thread keeps its unit's angles in registers and
 // takes every `teams`-th head of its token.  HBM bounds it: heads are asked for kUnroll at once, before the angles, which come by way of the position.  Reads of a unit come before its
 // writes, so that out may be x.
 template <typename T, bool kHalf>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (kHalf ? 4 : 5) : kHalf ? 2 : 3) rotary_kernel(const Rows r) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 3) rotary_kernel(const Rows r) {
     griddep_launch_dependents();
     griddep_wait();
     const uint32_t slot = fast_div(threadIdx.x, r.token_threads), rest = threadIdx.x - slot * r.token_threads.d;
@@ -115,25 +125,24 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (kHalf ? 4 : 5) : k
     if (static_cast<int>(slot) >= r.block_tokens || token >= r.tokens) return;
     const uint32_t team = fast_div(rest, r.units), unit = rest - team * r.units.d;
     const bool turns = static_cast<int>(unit) < r.turned;
-    constexpr int kPairs = kHalf ? 8 : 4;
+    constexpr int kPairs = 4;
     // where the unit begins in a head, and (halves) how far behind it the other values are
-    const int width = kHalf ? 16 : 8, rotated = r.turned * width;
-    int at = r.offset + static_cast<int>(unit) * 8;
+    const int rotated = r.turned * 8, second = rotated / 2;
+    int at = r.offset + static_cast<int>(unit) * (kHalf ? 4 : 8);
     if (!turns) {
         at = (static_cast<int>(unit) - r.turned) * 8;
         if (at >= r.offset) at += rotated;
     }
     const T* const x = static_cast<const T*>(r.x) + token * r.x_token + at;
     T* const out = static_cast<T*>(r.out) + token * r.out_token + at;
-    const int second = rotated / 2;
-    Eight<T> v[kUnroll], v2[kHalf ? kUnroll : 1];
+    Eight<T> v[kUnroll];
     const auto fetch = [&](int head) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int h = head + u * r.teams;
             if (h >= r.heads) break;
-            v[u].load(x + h * r.x_head);
-            if (kHalf && turns) v2[kHalf ? u : 0].load(x + h * r.x_head + second);
+            if (kHalf && turns) v[u].load(x + h * r.x_head, second);
+            else v[u].load(x + h * r.x_head);
         }
     };
     fetch(static_cast<int>(team));
@@ -141,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (kHalf ? 4 : 5) : k
     if (turns) {
         const int64_t position = r.positions ? r.positions[token] : static_cast<int64_t>(static_cast<uint32_t>(token) % r.per);
         const bool there = position >= 0 && position < r.n_positions;
-        const float2* const row = r.freqs + (there ? position : 0) * (rotated / 2) + unit * kPairs;
+        const float2* const row = r.freqs + (there ? position : 0) * second + unit * kPairs;
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
             f[i] = there ? row[i] : make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
@@ -158,21 +167,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (kHalf ? 4 : 5) : k
                 v[u].store(to);
                 continue;
             }
-            float a[8], b[8];
+            float a[8];
             v[u].get(a);
-            if (kHalf) v2[kHalf ? u : 0].get(b);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-                float &first = a[kHalf ? i : 2 * i], &other = kHalf ? b[i] : a[2 * i + 1];
+                float &first = a[kHalf ? i : 2 * i], &other = a[kHalf ? 4 + i : 2 * i + 1];
                 const float re = fmaf(first, f[i].x, -(other * f[i].y)), im = fmaf(first, f[i].y, other * f[i].x);
                 first = re, other = im;
             }
             v[u].set(a);
-            v[u].store(to);
-            if (kHalf) {
-                v2[kHalf ? u : 0].set(b);
-                v2[kHalf ? u : 0].store(to + second);
-            }
+            if (kHalf) v[u].store(to, second);
+            else v[u].store(to);
         }
         head += r.teams * kUnroll;
         if (head < r.heads) fetch(head);
@@ -267,7 +272,7 @@ int dsv3_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, vo
         set_last_error("rotary: 2^31 tokens or more");
         return DSV3_ERR_UNSUPPORTED;
     }
-    const int turned = rotated / (half_layout ? 16 : 8);
+    const int turned = rotated / 8;
     // (in place what is not rotated stays where it is)
     const int units = turned + (x == out ? 0 : (dim - rotated) / 8);
     if (units == 0) return DSV3_OK;
