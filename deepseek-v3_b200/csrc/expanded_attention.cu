@@ -3,14 +3,20 @@
 //   x[r, p] = q_nope[r] . k_nope[p] + q_rope[r] . k_rope[p]          r: a query of one head, p: a key; k_rope is shared by the heads
 //   out[r]  = sum_p 2^(c x - m) v[p] / sum_p 2^(c x - m)             c: softmax_scale log2(e), m: a running reference of the row
 //
-// One pass over the keys.  A CTA works on 256 queries of a head as two halves of 128 (the M of an MMA), a lane of TMEM and a softmax thread to a query; keys
-// come in tiles of 128, which both halves use.  Scores (128 columns of TMEM) and sums (128 more) of either half fill TMEM: while one half's
-// weights are formed the tensor core works for the other.  Weights go back to TMEM in bf16, over the scores they come from, as the A operand of the second product: they
-// never see shared memory, which the first product's operands keep busy (96 KB a tile and half at 128 bytes a cycle, as long as its MMAs take).
-//   The reference m of a row moves only where a weight would pass 2^8, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
+// One pass over the keys.  A CTA works on 256 queries of a head as two halves of 128 (the M of an MMA), a lane of TMEM and a softmax thread to a query; keys come in tiles of 128,
+// which both halves use.  In TMEM lie the scores of one half's tile at a time (128 columns: the softmax takes them to registers at once, so that the halves take turns), both halves'
+// weights (64 columns each, two bf16 to a column) and both halves' sums (128 each).  Weights are the A operand of the second product from TMEM: they never see shared memory, which the
+// operands of the first keep busy.
+//   Long chunks are worked on by CTAs in pairs (cta_group::2): halves of 256 queries, 128 in either CTA, and either loads half of the keys' rows and half of the values' dimensions for both.
+// The ring of keys and values then holds three tiles, not one and a half, and loads half as much: 16001 tokens of 16 heads 836 us, 942 by CTAs alone.
+//   The reference m of a row moves only where a weight would pass 2^32, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
 // (2^-9), sums and statistics are fp32.
-//   Blocks of at most 128 queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
+//   Blocks of at most half as many queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
 // than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
+//   What bounds it: the tensor cores on long sequences.  8192 queries and keys of 32 heads, each query seeing all keys: 851 us, 1615 TFLOP/s, as much as a large matrix product reaches (seeing
+// those before it: 467 us, the tensor pipe 83 % busy).  In a row of calls that lasts, the power limit lowers the clock: 985 us for 16001 tokens of 16 heads, 1330 TFLOP/s.  A block's begin
+// and end take as long as 2.5 tiles of a half (4.5 of a pair's): 4096 tokens of 128 heads 518 us, 1327 TFLOP/s; 515 of 16 heads over 4099 keys 36 us, 570.  Few queries: HBM, 64 of 128 heads over
+// 4000 keys 55 us, 4.9 TB/s.  A single short block: what one tile takes from end to end, 37 tokens 8.3 us.
 //
 // Keys and values behind a sequence's end belong to another one, or to nobody: what they score is replaced, and their values are cleared in shared memory before the MMA
 // that would multiply them by zero (0 * NaN).  The same warp looks at the tiles that some queries of a block see only in part for values that are not finite.
@@ -32,8 +38,8 @@ namespace {
 constexpr int kNope = DSV3_NOPE_DIM, kRope = DSV3_ROPE_DIM, kValue = DSV3_VALUE_DIM;
 constexpr int kHalf = 128;                       // queries of a CTA's half of a block
 constexpr int kTile = 128;                       // keys
-// Operands lie as rows of 64 values (128 bytes, swizzled).  Keys and values come through a ring of slots of 16 KB: three to a tile of keys (64 dimensions of 128 keys
-// each), two to one of values (64 keys of 128 dimensions each): beside the queries there is room for eight, one and a half tiles of both.
+// Operands lie as rows of 64 values (128 bytes, swizzled).  Keys and values come through a ring of slots: three to a tile of keys (64 dimensions of 128 keys
+// each), two to one of values (64 keys of 128 dimensions each).  A slot is 16 KB, of a pair's CTA 8: beside the queries there is room for eight or sixteen, one and a half or three tiles of both.
 constexpr int kKeySlots = 3, kValueSlots = 2;
 // A tile's keys, or its values, are a unit, which is waited for and given back as a whole.
 constexpr int kUnits = 8;                        // of either that can be on their way: a ring of a pair's slots has room for no more values
@@ -502,8 +508,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         if (ok) it = sm.item[count % kItemSlots];
         return it;
     };
-    // The same in all lanes, and known to be: branches and addresses that depend on it stay uniform, which the tensor core's instructions want (their operands are uniform registers: those of
-    // a lane go there one by one, 30 cycles an MMA more than it takes).
+    // The same in all lanes, and known to be: branches and addresses that depend on it stay uniform, which the tensor core's instructions want (with addresses that were a lane's own, MMAs came half as
+    // fast).
     const auto uniform = [](int x) -> int { return __shfl_sync(0xffffffffu, x, 0); };
     const auto item_done = [&](uint32_t count) {
         __syncwarp();
