@@ -80,6 +80,7 @@ struct Params {
     float scale;                          // softmax_scale log2(e)
     int head_group;
     int splits;
+    int blocks;                           // at most, of offsets that ascend
     FastDiv by_splits, by_group, by_last_group;      // ... and by the heads of the last group
     bool dynamic;                         // CTAs take the place of those that have not started; else every gridDim.x-th item
     __nv_bfloat16* out;
@@ -323,6 +324,7 @@ struct List {
         last_step = __reduce_max_sync(0xffffffffu, blocks > 0 ? behind + blocks : 0) - 1;
         total = __reduce_add_sync(0xffffffffu, blocks);
         for (int s = kLanes; s < p.n_seqs; s += kLanes) total += __reduce_add_sync(0xffffffffu, blocks_of(load_seq(p, s + lane).queries));
+        total = max(0, min(total, p.blocks));                        // (offsets that do not ascend: some blocks are left out, none is looked for that the grid does not have)
     }
     __device__ __forceinline__ int up_to(int step) const {           // blocks that come up in steps 0 .. step
         return __reduce_add_sync(0xffffffffu, max(0, min(step - behind + 1, blocks)));
@@ -1066,26 +1068,35 @@ struct Call {
 // Fitted to 78 calls of 1 to 16001 queries and 37 to 16384 keys, alone and in pairs, 26 of them in up to 12 parts.  Of those it picks the fastest or one at most 6 % slower.
 //   Parts of 2, 3 and 4: 515 queries of 16 heads over 4099 keys 45.2, 36.5 and 41.5 us; 512 over 8192 in pairs 65.9, 51.5 and 44.6; 2 heads of 16001 tokens in pairs 121, 130 and 133, and 195 in one.
 // Alone / in pairs: 512 queries of 128 heads over 512 keys 24.0 / 28.9 us, over 2048 79.4 / 70.6, over 8192 298 / 250; 1000 of 16 over 8000 78.7 / 69.3; 16001 of 16 over themselves 942 / 836.
-double time_of(const Call& c, int ctas, int splits, int sms) {
-    const double slots = sms / ctas, queries = std::max(1.0, static_cast<double>(c.tokens) / c.n_seqs), keys = static_cast<double>(c.kv_tokens) / c.n_seqs;
-    const double longest = keys / kTile, tiles = (c.causal ? keys > queries ? keys - queries / 2 : keys / 2 : keys) / kTile + (c.causal ? 0.5 : 0.0);
-    const double a_tile = ctas == 2 ? 0.807 : 1.0, ends = ctas == 2 ? 4.5 : 2.5;
-    const double halves = std::ceil(queries / (ctas * kHalf)), items = c.heads * c.n_seqs * std::max(1.0, halves / 2) * splits;
-    const double all = c.heads * c.n_seqs * halves * (tiles + ends * splits) / slots, one = std::min(2.0, halves) * (longest / splits + ends);
-    const double alike = std::pow(std::max(0.0, std::min(1.0, 2 * tiles / longest - 1)), 0.75);       // 0: of all lengths up to the longest
-    const double time = std::max({all, one, all + (std::ceil(items / slots) * one - all) * alike});
-    return a_tile * time + (splits > 1 ? 5.9 + 56e-6 * splits * c.tokens * c.heads : 0.0);
+struct Work {
+    double queries, longest, tiles;       // of a sequence: queries, tiles of keys, those that a query sees
+    double alike;                         // 1: items are as long, 0: of all lengths up to the longest
+    double heads, rows;                   // of all sequences
+};
+double time_of(const Work& w, int ctas, int splits, int sms) {
+    const double slots = sms / ctas, a_tile = ctas == 2 ? 0.807 : 1.0, ends = ctas == 2 ? 4.5 : 2.5;
+    const double halves = std::ceil(w.queries / (ctas * kHalf)), items = w.heads * std::max(1.0, halves / 2) * splits;
+    const double all = w.heads * halves * (w.tiles + ends * splits) / slots, one = std::min(2.0, halves) * (w.longest / splits + ends);
+    const double time = std::max({all, one, all + (std::ceil(items / slots) * one - all) * w.alike});
+    return a_tile * time + (splits > 1 ? 5.9 + 56e-6 * splits * w.rows : 0.0);
 }
 Plan plan_of(const Call& c, int sms) {
-    // (the tiles of a sequence, if all have as many)
+    Work w;
+    const double keys = static_cast<double>(c.kv_tokens) / c.n_seqs;                 // (if all sequences have as many)
+    w.queries = std::max(1.0, static_cast<double>(c.tokens) / c.n_seqs);
+    w.longest = keys / kTile;
+    w.tiles = (c.causal ? keys > w.queries ? keys - w.queries / 2 : keys / 2 : keys) / kTile + (c.causal ? 0.5 : 0.0);
+    w.alike = std::pow(std::max(0.0, std::min(1.0, 2 * w.tiles / w.longest - 1)), 0.75);
+    w.heads = static_cast<double>(c.heads) * c.n_seqs;
+    w.rows = static_cast<double>(c.tokens) * c.heads;
     const int64_t most = (c.kv_tokens / c.n_seqs + kTile - 1) / kTile;
     const int last = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxJoinParts, most / kLeastTiles)));
     Plan pl = {1, 0, 1, 0};
-    double best = time_of(c, 1, 1, sms);
+    double best = time_of(w, 1, 1, sms);
     // (blocks of a pair that are not half full gain nothing: 64 queries of 128 heads over 4000 keys 55.9 us alone, 75.3 in pairs)
     for (int ctas = 1; ctas <= (sms > 1 && c.tokens / c.n_seqs >= 2 * kHalf ? 2 : 1); ++ctas)
-        for (int splits = 1; splits <= last; ++splits) {
-            const double time = time_of(c, ctas, splits, sms) * (ctas == 2 ? 1.04 : 1.0);        // (what is as good is not worth a pair)
+        for (int splits = 1; splits <= last && (splits == 1 || w.heads * splits <= 8.0 * sms); ++splits) {          // (more than some rounds of items gain nothing)
+            const double time = time_of(w, ctas, splits, sms) * (ctas == 2 ? 1.04 : 1.0);        // (what is as good is not worth a pair)
             if (time < best) best = time, pl.ctas = ctas, pl.splits = splits;
         }
     const int64_t each = c.ragged ? 0 : c.tokens / c.n_seqs, rows = pl.ctas * 2 * kHalf, seqs = std::min(c.n_seqs, c.tokens);      // (that have queries)
@@ -1223,7 +1234,7 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* a, void* workspace,
     p.per_q = ragged ? 0 : static_cast<int>(a->tokens / a->n_seqs), p.per_k = a->cu_seqlens_k ? 0 : static_cast<int>(a->kv_tokens / a->n_seqs);
     p.causal = a->causal != 0;
     p.scale = a->softmax_scale * kLog2e;
-    p.head_group = pl.head_group, p.splits = pl.splits, p.dynamic = dynamic;
+    p.head_group = pl.head_group, p.splits = pl.splits, p.blocks = static_cast<int>(pl.blocks), p.dynamic = dynamic;
     p.by_splits = make_fast_div(pl.splits), p.by_group = make_fast_div(pl.head_group);
     p.by_last_group = make_fast_div(a->heads % pl.head_group ? a->heads % pl.head_group : pl.head_group);
     p.out = static_cast<__nv_bfloat16*>(a->out), p.lse = a->lse;

@@ -57,6 +57,17 @@ def test_offsets_that_lead_out_of_the_tensors_are_cut_off():
     check(out, want, bound)
 
 
+@pytest.mark.parametrize("sequences", [3, 5, 50])
+def test_offsets_that_do_not_ascend_end(sequences):
+    """Sequences over one another, more blocks than there are queries for: results are anything, but of the keys, and the call ends without an error."""
+    from dsv3_b200 import expanded_attention
+    args = inputs([700], [900], 3)
+    cu = lambda n: torch.tensor([n * (i % 2) for i in range(sequences + 1)], dtype=torch.int32, device="cuda")  # noqa: E731
+    expanded_attention(*args, SCALE, cu(700), cu(900))
+    want, _, bound, _ = reference(*args, [700], [900])
+    check(expanded_attention(*args, SCALE, offsets([700]), offsets([900])), want, bound)
+
+
 @pytest.mark.parametrize("tokens, keys, heads", [(400, 900, 4), (30, 5000, 2)])
 def test_a_captured_call_follows_the_lengths(tokens, keys, heads):
     """One graph, other lengths at every replay; beside another graph and eager calls."""
