@@ -185,10 +185,9 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap,
                  : "memory");
 }
 __device__ __forceinline__ void store_cluster(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
-__device__ __forceinline__ int load_cluster(uint32_t at) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void min_cluster(uint32_t at, int v) {
+    int old;
+    asm volatile("atom.shared::cluster.min.s32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t bar_cluster) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
@@ -197,6 +196,11 @@ __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cl
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -518,17 +522,23 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
         if (lane == 0) mbar_arrive(bar(sm.item_empty[count % kItemSlots]));
     };
 
+    // (a pair's queries and keys arrive at the first CTA's barriers, values at the CTA's own)
+    const auto copy = [&](uint32_t to, const CUtensorMap& map, int x, int head, int row, const uint64_t& full) {
+        if (kPair) tma_load_3d_pair(to, &map, x, head, row, lead(full));
+        else tma_load_3d(to, &map, x, head, row, bar(full));
+    };
+
     // (in the branches of the roles themselves: behind a common point the compiler counts on the lesser of both numbers)
     if (!well) {
         // nothing is started
     } else if (warp >= kSoftmaxWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kLoadWarp) {
-            // ------------------------------------------------------------ the list, and the loads
+            // ------------------------------------------------------------ the list, and the loads of keys and values
             List<kCtas> list;
             list.begin(p);
             // (This warp sets the pace: an MMA's 64 cycles are what a few instructions take here.  A unit is armed and copied by one lane in one go.)
-            uint32_t slot = 0, active = 0, taken = 0;                // slots filled; items with tiles
+            uint32_t slot = 0, taken = 0;                            // slots filled; answers
             uint32_t freed = 0, back = 0, keys = 0, loaded = 0;      // slots and units given back; which of the last 32 units are keys; units
             uint32_t k_loaded = 0, v_loaded = 0, k_back = 0, v_back = 0;
             bool ok = true;
@@ -603,27 +613,6 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     following = publish();
                 }
                 if (it.n > 0) {
-                    // (a pair's queries and keys arrive at the first CTA's barriers, values at the CTA's own)
-                    const auto copy = [&](uint32_t to, const CUtensorMap& map, int x, int head, int row, const uint64_t& full) {
-                        if (kPair) tma_load_3d_pair(to, &map, x, head, row, lead(full));
-                        else tma_load_3d(to, &map, x, head, row, bar(full));
-                    };
-                    const auto load_queries = [&](int h) {
-                        ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
-                        if (ok && elect_one()) {
-                            if (h == 1 && it.alternate) {
-                                if (rank == 0) mbar_arrive(bar(sm.q_full[h]));          // (both halves use the first one's)
-                            } else {
-                                const uint32_t to = queries + h * kQueryBytes;
-                                const int row = it.q0 + h * kRows + static_cast<int>(rank) * kHalf;
-                                if (rank == 0) mbar_arrive_expect_tx(bar(sm.q_full[h]), kCtas * kQueryBytes);
-                                copy(to, map_qn, 0, it.head, row, sm.q_full[h]);
-                                copy(to + kQueryPart, map_qn, 64, it.head, row, sm.q_full[h]);
-                                copy(to + 2 * kQueryPart, map_qr, 0, it.head, row, sm.q_full[h]);
-                            }
-                        }
-                        __syncwarp();
-                    };
                     const int head = uniform(it.head), n = uniform(it.n), ahead = uniform(it.alternate) != 0 ? 2 * kAhead : kAhead, row0 = uniform(it.k0 + it.tile * kTile);
                     const auto load_keys = [&](int t) {
                         const int row = row0 + t * kTile + static_cast<int>(rank) * (kTile / kCtas);
@@ -663,13 +652,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     for (int t = -ahead; t < n && ok; ++t) {
                         if (t == ask_at) ask();
                         if (t + ahead < n) load_keys(t + ahead);
-                        if (t == -ahead) {
-                            load_queries(0);
-                            load_queries(1);
-                        }
                         if (t >= 0) load_values(t);
                     }
-                    ++active;
                     // (the MMAs still have some tiles to go)
                     answer();
                     following = publish();
@@ -678,9 +662,8 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
             }
             // none of the arrivals on empty[] may be in flight when the CTA leaves its shared memory to another
             while (ok && back < loaded) one_back();
-            for (int h = 0; h < 2 && ok && active > 0; ++h) ok = wait(sm.q_empty[h], (active - 1) & 1, kQueriesThere, active);
         } else if (warp == kScoreWarp) {
-            // ------------------------------------------------------------ the MMAs of the scores.  Those of the sums have a warp of their own: an MMA takes 64 cycles, and what lies between
+            // ------------------------------------------------------------ queries, and the MMAs of the scores.  Those of the sums have a warp of their own: an MMA takes 64 cycles, and what lies between
             // two groups of them (waits that need not wait, 100 cycles each; addresses) as long as several.  The warps stay converged and elect a lane for the MMAs alone.
             uint32_t slot = 0, keys = 0, active = 0, scored = 0;
             const uint64_t ring_desc = umma_desc_k_major_sw128(ring), query_desc = umma_desc_k_major_sw128(queries);
@@ -690,7 +673,29 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 const int n = uniform(it.n), n0 = uniform(it.n0), step = uniform(it.alternate);
                 if (!ok || uniform(it.rows) == 0) break;
                 item_done(count);
-                if (n == 0 || rank != 0) continue;
+                if (n == 0) continue;
+                // (this warp has nothing to do before they are there, and the one that loads keys has)
+                const int head = uniform(it.head), row0 = uniform(it.q0) + static_cast<int>(rank) * kHalf;
+                for (int h = 0; h < 2; ++h) {
+                    ok = ok && wait(sm.q_empty[h], (active & 1) ^ 1, kQueriesThere, active);
+                    if (ok && elect_one()) {
+                        if (h == 1 && step != 0) {
+                            if (rank == 0) mbar_arrive(bar(sm.q_full[h]));              // (both halves use the first one's)
+                        } else {
+                            const uint32_t to = queries + h * kQueryBytes;
+                            const int row = row0 + h * kRows;
+                            if (rank == 0) mbar_arrive_expect_tx(bar(sm.q_full[h]), kCtas * kQueryBytes);
+                            copy(to, map_qn, 0, head, row, sm.q_full[h]);
+                            copy(to + kQueryPart, map_qn, 64, head, row, sm.q_full[h]);
+                            copy(to + 2 * kQueryPart, map_qr, 0, head, row, sm.q_full[h]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (rank != 0) {
+                    ++active;
+                    continue;
+                }
                 for (int h = 0; h < 2; ++h) ok = ok && wait(sm.q_full[h], active & 1, kQueriesThere, active);
 #pragma unroll 1
                 for (int t = 0, u = 0; t < n && ok; ++t, ++keys) {
@@ -729,6 +734,7 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                 slot += (kKeySlots + kValueSlots) * n;
                 ++active;
             }
+            for (int h = 0; h < 2 && ok && active > 0; ++h) ok = wait(sm.q_empty[h], (active - 1) & 1, kQueriesThere, active);
         } else if (warp == kSumWarp) {
             // ------------------------------------------------------------ the MMAs of the sums
             uint32_t slot = 0, values = 0, summed0 = 0, summed1 = 0;
@@ -831,13 +837,17 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                                 }
                             }
                             bad = __reduce_min_sync(0xffffffffu, bad);
-                            if (lane == 0) atomicMin(&sm.not_finite[count % kNotFiniteSlots], bad);
+                            if (lane == 0) {
+                                int& worst = sm.not_finite[count % kNotFiniteSlots];
+                                atomicMin(&worst, bad);
+                                if (kPair) {
+                                    min_cluster(mapa_shared(smem_u32(&worst), rank ^ 1u), bad);
+                                    fence_cluster();
+                                }
+                            }
                         }
                     }
-                    if (look) {
-                        fence_proxy_async_shared();
-                        if (kPair) fence_cluster();                  // (the other CTA's warps read not_finite)
-                    }
+                    if (look) fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) arrive_lead(sm.v_ready[values % kUnits]);
                 }
@@ -884,19 +894,11 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     }
                     const int last = min(it.limit + (p.causal ? row : 0), it.len - 1);
                     const bool nothing = stats.x == -INFINITY && !isnan(stats.y);
-                    int bad = *static_cast<const volatile int*>(&not_finite);
-                    if (kPair) fence_cluster();
-                    if (kPair) bad = min(bad, load_cluster(mapa_shared(smem_u32(&not_finite), rank ^ 1u)));      // (its slot is not used again before this item's sums are read)
-                    const bool spoilt = last >= bad;
-                    const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : 1.0f / stats.y;
+                    const bool spoilt = last >= *static_cast<const volatile int*>(&not_finite);
+                    const float inv = spoilt ? __uint_as_float(0x7FC00000u) : nothing ? 0.0f : rcp(stats.y);
                     const float2 f2 = make_float2(f * inv, f * inv), other2 = make_float2(other * inv, other * inv), zero2 = make_float2(0.0f, 0.0f);
                     const int64_t place = static_cast<int64_t>(it.q0 + row0) * p.heads + it.head, part = static_cast<int64_t>(it.split) * p.tokens * p.heads + place;
                     const int rows = it.rows - row0;
-                    if (lane < rows) {
-                        const float lse = nothing ? -INFINITY : (stats.x * c + log2f(stats.y)) * kLn2;
-                        if (p.partial) p.partial_lse[part + static_cast<int64_t>(lane) * p.heads] = lse;
-                        else if (p.lse) p.lse[place + static_cast<int64_t>(lane) * p.heads] = lse;
-                    }
                     const int n = h == 0 ? it.n0 : it.n1;
                     const bool two = it.alternate && it.n1 > 0;
 #pragma unroll 1
@@ -923,6 +925,11 @@ expanded_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __gr
                     }
                     half_done(h);
                     if (it.alternate) half_done(1);
+                    if (lane < rows) {
+                        const float lse = nothing ? -INFINITY : (stats.x * c + log2f(stats.y)) * kLn2;
+                        if (p.partial) p.partial_lse[part + static_cast<int64_t>(lane) * p.heads] = lse;
+                        else if (p.lse) p.lse[place + static_cast<int64_t>(lane) * p.heads] = lse;
+                    }
                 }
                 item_done(count);
             }
