@@ -8,15 +8,15 @@
 // weights (64 columns each, two bf16 to a column) and both halves' sums (128 each).  Weights are the A operand of the second product from TMEM: they never see shared memory, which the
 // operands of the first keep busy.
 //   Long chunks are worked on by CTAs in pairs (cta_group::2): halves of 256 queries, 128 in either CTA, and either loads half of the keys' rows and half of the values' dimensions for both.
-// The ring of keys and values then holds three tiles, not one and a half, and loads half as much: 16001 tokens of 16 heads 836 us, 942 by CTAs alone.
+// The ring of keys and values then holds three tiles, not one and a half, and loads half as much: 16001 tokens of 16 heads 844 us, 942 by CTAs alone.
 //   The reference m of a row moves only where a weight would pass 2^32, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
 // (2^-9), sums and statistics are fp32.
 //   Blocks of at most half as many queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
 // than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
-//   What bounds it: the tensor cores on long sequences.  8192 queries and keys of 32 heads, each query seeing all keys: 851 us, 1615 TFLOP/s, as much as a large matrix product reaches (seeing
-// those before it: 467 us, the tensor pipe 83 % busy).  In a row of calls that lasts, the power limit lowers the clock: 985 us for 16001 tokens of 16 heads, 1330 TFLOP/s.  A block's begin
-// and end take as long as 2.5 tiles of a half (4.5 of a pair's): 4096 tokens of 128 heads 518 us, 1327 TFLOP/s; 515 of 16 heads over 4099 keys 36 us, 570.  Few queries: HBM, 64 of 128 heads over
-// 4000 keys 55 us, 4.9 TB/s.  A single short block: what one tile takes from end to end, 37 tokens 8.3 us.
+//   What bounds it: the tensor cores on long sequences.  8192 queries and keys of 32 heads, each query seeing all keys: 855 us, 1607 TFLOP/s, as much as a large matrix product reaches (seeing
+// those before it: 467 us, the tensor pipe 83 % busy).  In a row of calls that lasts, the power limit lowers the clock: 976 us for 16001 tokens of 16 heads, 1343 TFLOP/s.  A block's begin
+// and end take as long as 2.5 tiles of a half (4.5 of a pair's): 4096 tokens of 128 heads 518 us, 1327 TFLOP/s; 515 of 16 heads over 4099 keys 35.4 us, 572.  Few queries: HBM, 64 of 128 heads over
+// 4000 keys 55 us, 4.8 TB/s.  A single short block: what one tile takes from end to end, 37 tokens 7.9 us.
 //
 // Keys and values behind a sequence's end belong to another one, or to nobody: what they score is replaced, and their values are cleared in shared memory before the MMA
 // that would multiply them by zero (0 * NaN).  The same warp looks at the tiles that some queries of a block see only in part for values that are not finite.
