@@ -16,7 +16,7 @@ struct QuarterTurns {
 
 // A thread to one angle of kTableUnroll positions.  The angle is reduced to an eighth of a turn either side of a multiple of a quarter turn in 64 bits, so that position
 // 163840 is as exact as position 1; of what is left (r quarters, |r| <= 1/2) sine and cosine are polynomials in r^2, those of their degree whose largest error is least (Remez' exchange: 2^-27 and 2^-34).
-//   HBM bounds what is large (163840 positions of 32 angles 9.4 us, 4.5 TB/s), a launch what is small (4096: 6.7 us).  Conversions between 64-bit numbers and whole ones are what costs time here (one a cycle and SM): the nearest whole number comes from
+//   HBM bounds what is large (163840 positions of 32 angles 9.4 us, 4.5 TB/s), a launch what is small (4096: 1.8 us in a graph).  Conversions between 64-bit numbers and whole ones are what costs time here (one a cycle and SM): the nearest whole number comes from
 // adding 1.5 * 2^52, and only r is converted.
 __global__ void __launch_bounds__(kTableThreads) rotary_table_kernel(const __grid_constant__ QuarterTurns f, FastDiv pairs, int block_rows, int64_t start, int64_t length,
                                                                      float2* __restrict__ out) {
@@ -116,7 +116,7 @@ struct Eight<float> {
 // A unit is eight values of a head, four pairs if they turn: side by side, or in the layout of halves four of either half.  A thread keeps its unit's angles in registers and
 // takes every `teams`-th head of its token.  HBM bounds it: heads are asked for kUnroll at once, before the angles, which come by way of the position.  Reads of a unit come before its
 // writes, so that out may be x.  4099 tokens of 128 heads of 64: 21.6 us, 22.2 in halves, 6.2 TB/s of what is read and written (from a cold L2 23.8); a part of 2047 tokens of 32 heads of 192 10.4 us
-// (units of eight values of either half: 12.7); 64 tokens 2.9 us, a launch.
+// (units of eight values of either half: 12.7); 64 tokens of 16 heads 1.6 us in a graph, a launch.
 template <typename T, bool kHalf>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 3) rotary_kernel(const Rows r) {
     griddep_launch_dependents();
