@@ -158,8 +158,8 @@ int dsv3_fp8_gemm_static(const void* a, const float* a_s, const void* b, const f
 int dsv3_set_gemm_policy(int kernel, int split_k);
 
 /*
- * SMs the persistent tcgen05 GEMM kernels (and the plans that size split-K for them) and latent attention may occupy; 0 = all
- * (default).  No counterpart in the reference.  For hosts that run a collective next to the GEMMs: a persistent
+ * SMs the persistent tcgen05 GEMM kernels (and the plans that size split-K for them), latent attention and expanded attention (two at least;
+ * not the kernel that joins its parts) may occupy; 0 = all (default).  No counterpart in the reference.  For hosts that run a collective next to the GEMMs: a persistent
  * kernel that fills every SM keeps the collective's CTAs waiting until it ends, and the GEMM launched after that
  * finds SMs taken and runs a straggling round; leaving the collective its SMs (about as many as it has
  * channels) avoids both.  The two-launch form of the expert layer (dsv3_few_*) does not keep to it, and
