@@ -1108,9 +1108,11 @@ Plan plan_of(const Call& c, int sms) {
         }
     const int64_t each = c.ragged ? 0 : c.tokens / c.n_seqs, rows = pl.ctas * 2 * kHalf, seqs = std::min(c.n_seqs, c.tokens);      // (that have queries)
     pl.blocks = c.ragged ? (c.tokens - seqs) / rows + seqs : c.n_seqs * ((each + rows - 1) / rows);
-    // Groups of heads, equal ones: as few as keep a group's keys and values in the L2, and no more than leave each of them two items to an SM.
+    // Groups of heads, equal ones: as few as keep a group's keys and values in the L2, and no more than leave each of them an item to an SM (or pair).  In long rows of calls, in groups of 16 MB, 32, 64 or all
+    // heads at once: 4096 tokens of 128 heads 607, 606, 622 and 675 us; 16001 of 16 heads, which then are too few to a group, 1050, 980, 1005 and 1004; 515 of 128 heads over 4099 keys 221, 221, 221
+    // and 234 (with two items to an SM at least, 233 for 32 MB).
     const int64_t bytes = c.heads * c.kv_tokens * 2 * (kNope + kValue);
-    const int64_t groups = c.n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, pl.blocks * c.heads / (2 * std::max(1, sms / pl.ctas))));
+    const int64_t groups = c.n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, pl.blocks * c.heads / std::max(1, sms / pl.ctas)));
     pl.head_group = static_cast<int>((c.heads + groups - 1) / groups);
     return pl;
 }
