@@ -14,7 +14,7 @@
 //   Blocks of at most half as many queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
 // than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
 //   What bounds it: the tensor cores on long sequences.  8192 queries and keys of 32 heads, each query seeing all keys: 855 us, 1607 TFLOP/s, as much as a large matrix product reaches (seeing
-// those before it: 467 us, the tensor pipe 83 % busy).  In a row of calls that lasts, the power limit lowers the clock: 976 us for 16001 tokens of 16 heads, 1343 TFLOP/s.  A block's begin
+// those before it: 462 us, the tensor pipe 84 % busy).  In a row of calls that lasts, the power limit lowers the clock: 986 us for 16001 tokens of 16 heads, 1330 TFLOP/s.  A block's begin
 // and end take as long as 2.5 tiles of a half (4.5 of a pair's): 4096 tokens of 128 heads 518 us, 1327 TFLOP/s; 515 of 16 heads over 4099 keys 35.4 us, 572.  Few queries: HBM, 64 of 128 heads over
 // 4000 keys 55 us, 4.8 TB/s.  A single short block: what one tile takes from end to end, 37 tokens 7.4 us in a graph.
 //
