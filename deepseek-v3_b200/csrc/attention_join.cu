@@ -24,6 +24,7 @@ struct Parts {
     int block_rows;
     __nv_bfloat16* to;
     float* to_lse;
+    bool lse_in_place;        // to_lse is a part's
     const int32_t* cu;        // or null; rows of tokens before cu[0], and from cu[n_seqs] on, are left as they are
     int n_seqs, heads;
 };
@@ -105,6 +106,8 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] *= inv;
     *reinterpret_cast<uint4*>(p.to + from) = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+    // (every thread of a row, which can be in several warps, has read the parts' before one writes.  Threads that have left do not keep the barrier waiting.)
+    if (p.lse_in_place) __syncthreads();
     if (p.to_lse && at == 0) p.to_lse[row] = nan ? inv : sum == 0.0f ? -INFINITY : top + log2f(sum) * kLn2;
 }
 
@@ -113,7 +116,10 @@ int launch(const void* const* outs, const float* const* lses, int n, int64_t row
            cudaStream_t stream) {
     const int row_threads = dim / 8, block_rows = kThreads / row_threads;
     Parts p = {};
-    for (int i = 0; i < n; ++i) p.out[i] = outs[i], p.lse[i] = lses[i];
+    for (int i = 0; i < n; ++i) {
+        p.out[i] = outs[i], p.lse[i] = lses[i];
+        p.lse_in_place = p.lse_in_place || lses[i] == lse;
+    }
     p.n = n, p.rows = rows, p.row_threads = make_fast_div(row_threads), p.block_rows = block_rows;
     p.to = static_cast<__nv_bfloat16*>(out), p.to_lse = lse;
     p.cu = cu, p.n_seqs = n_seqs, p.heads = heads;
