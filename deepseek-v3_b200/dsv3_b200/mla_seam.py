@@ -159,15 +159,38 @@ _MOST_PARTS = 32        # of attention_join
 
 def _attend_expanded(q_nope, q_rope, cache: MlaCache, table, start_pos: int, weight, softmax_scale: float, expand_tokens: int) -> torch.Tensor:
     """Causal attention of a chunk at ``start_pos`` to its sequences' cached tokens, expanded with ``weight`` ``[heads, 256, 512]``.  The tokens before the chunk's page are expanded and attended
-    to in pieces of whole pages, ``expand_tokens`` of all sequences together to a piece (512 bytes a head and token), and the pieces' results joined."""
+    to in pieces of whole pages, ``expand_tokens`` of all sequences together to a piece, and the pieces' results joined (each is rounded to bf16 first, as a result is; the join's sums are fp32).
+    Of what is more than that at a time (the chunk itself; pieces, of which there are ``_MOST_PARTS`` at most) fewer heads are expanded at once, and of one head fewer sequences: heads and sequences
+    do not depend on one another, so that nothing is rounded for it."""
     bsz, seqlen, heads, _ = q_nope.shape
 
     def attend(first, end, causal, with_lse):
         tokens = end - first
         ends = torch.arange(0, (bsz + 1) * tokens, tokens, dtype=torch.int32, device=q_nope.device)
         latent, k_rope = latent_cache_read(cache.pool, table[:, first // PAGE:], ends, bsz * tokens)
-        kv = torch.nn.functional.linear(latent, weight.flatten(0, 1)).view(bsz, tokens, heads, -1)
-        return expanded_attention(q_nope, q_rope, kv[..., :NOPE_DIM], k_rope.view(bsz, tokens, -1), kv[..., NOPE_DIM:], softmax_scale, causal=causal, return_lse=with_lse)
+        latent, k_rope = latent.view(bsz, tokens, -1), k_rope.view(bsz, tokens, -1)
+
+        def some(seqs, some_heads):
+            kv = torch.nn.functional.linear(latent[seqs], weight[some_heads].flatten(0, 1)).unflatten(-1, (-1, NOPE_DIM + VALUE_DIM))
+            return expanded_attention(q_nope[seqs, :, some_heads], q_rope[seqs, :, some_heads], kv[..., :NOPE_DIM], k_rope[seqs], kv[..., NOPE_DIM:], softmax_scale, causal=causal,
+                                      return_lse=with_lse)
+
+        def in_steps(count, most):                          # equal ones
+            steps = -(-count // max(1, most))
+            return [slice(count * i // steps, count * (i + 1) // steps) for i in range(steps)]
+
+        room = expand_tokens * heads                       # of tokens times heads
+        if bsz * tokens * heads <= room:
+            return some(slice(None), slice(None))
+        out = q_nope.new_empty(bsz, seqlen, heads, VALUE_DIM)
+        lse = q_nope.new_empty(bsz, seqlen, heads, dtype=torch.float32) if with_lse else None
+        for seqs in in_steps(bsz, room // tokens):
+            for some_heads in in_steps(heads, room // ((seqs.stop - seqs.start) * tokens)):
+                if with_lse:
+                    out[seqs, :, some_heads], lse[seqs, :, some_heads] = some(seqs, some_heads)
+                else:
+                    out[seqs, :, some_heads] = some(seqs, some_heads)
+        return (out, lse) if with_lse else out
 
     before = start_pos // PAGE * PAGE                      # tokens that may be seen in pieces
     end_pos = start_pos + seqlen
@@ -185,7 +208,8 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
     int64 words of a tree of drafted tokens.  Masks of other shapes are refused; a floating mask that is not the causal one makes the result NaN (nothing is read back).
     ``start_pos``: one for all sequences, or an int32 or int64 tensor ``[batch]`` beside ``x``, which a captured step reads when it is replayed; a sequence whose tokens do not fit
     its cache is then not stored, and its result NaN.  ``freqs_cis``: ``[tokens, 32]``, or ``[batch, tokens, 32]``.  ``expand_from``: so many tokens, and more, of a causal mask are attended to with
-    expanded keys and values where ``start_pos`` is one for all and heads are of 128 and 64 values; ``expand_tokens`` bounds what is expanded at a time."""
+    expanded keys and values where ``start_pos`` is one for all and heads are of 128 and 64 values; keys and values of ``expand_tokens`` tokens with all heads (512 bytes a token and head) are held at a time at
+    most, or, if that is more, one head's of one sequence."""
     bsz, seqlen, _ = x.shape
     rope = self.qk_rope_head_dim
     if self.kv_lora_rank != LATENT_DIM or rope != ROPE_DIM:
@@ -259,7 +283,8 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
 def install_mla(model_module, release_buffers: bool = False, expand_from: Optional[int] = None, expand_tokens: int = 1 << 16) -> None:
     """Point ``model_module.MLA.forward`` at ``mla_forward``; ``model_module.block_size`` is read at call time, as in the reference.  ``release_buffers``: a module's
     bf16 buffers give their memory back at its first call; without it they stay, 1152 bytes a token beside the 644 of the 8-bit cache, for a host that goes back to the old forward.
-    ``expand_from``: prompts of so many tokens and more to a sequence are attended to with expanded keys and values (None: never), ``expand_tokens`` cached ones at a time."""
+    ``expand_from``: prompts of so many tokens and more to a sequence are attended to with expanded keys and values (None: never), with the keys and values of ``expand_tokens`` tokens at a time, cached and new
+    ones of all sequences (or those of one head of one sequence, if that is more)."""
     if (expand_from is not None and expand_from < 1) or expand_tokens < 1:
         raise ValueError("expand_from and expand_tokens are numbers of tokens, from 1 on")
 
