@@ -9,7 +9,7 @@
 // operands of the first keep busy.
 //   Long chunks are worked on by CTAs in pairs (cta_group::2): halves of 256 queries, 128 in either CTA, and either loads half of the keys' rows and half of the values' dimensions for both.
 // The ring of keys and values then holds three tiles, not one and a half, and loads half as much: 16001 tokens of 16 heads 844 us, 942 by CTAs alone.
-//   The reference m of a row moves only where a weight would pass 2^32, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
+//   The reference m of a row moves only where a weight would pass 2^8, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
 // (2^-9), sums and statistics are fp32.
 //   Blocks of at most half as many queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
 // than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
@@ -69,8 +69,9 @@ constexpr int kLanes = 32;                       // sequences that are put in or
 constexpr uint32_t kRoom = 1, kTileThere = 2, kScoresRoom = 3, kScoresThere = 4, kWeightsThere = 16, kSumsThere = 17, kQueriesThere = 18, kGuarded = 19, kItems = 20, kRowsRoom = 21, kWeightsRoom = 22;
 constexpr uint64_t kItemLimitNs = 100 * kWaitLimitNs;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-// A row's reference moves where a weight would pass 2^kSlack: bf16 weights and fp32 sums have the range for more, and the same bits wherever they are.
-constexpr float kSlack = 32.0f;
+// A row's reference moves where a weight would pass 2^kSlack: bf16 weights and fp32 sums have the same bits wherever they are.  What weights are larger by is range that values lose: sums of n of them pass
+// fp32's largest for values beyond 2^(120 - log2 n).  (With 32 instead of 8 each of 25 calls took the same time within 0.6 %, and values of 2^95 could overflow.)
+constexpr float kSlack = 8.0f;
 
 struct Params {
     int tokens, kv_tokens, heads, n_seqs;
