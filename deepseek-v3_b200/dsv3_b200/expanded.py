@@ -42,7 +42,7 @@ def attention_join(outs: Sequence[torch.Tensor], lses: Sequence[torch.Tensor],
                    return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """The results of the same queries over several pieces of their keys (up to 32), as over all of them: bf16 ``[..., dim]``, and with ``return_lse`` fp32 ``[...]``.
 
-    ``outs`` and ``lses`` are what ``expanded_attention`` or ``latent_attention`` return with ``return_lse``.  Sums in fp32, rounded once; a part that sees nothing (-inf) is not read."""
+    ``outs`` and ``lses`` are what ``expanded_attention`` or ``latent_attention`` return with ``return_lse``.  Sums in fp32, rounded once; what a part that sees nothing (-inf) holds does not count."""
     return host.attention_join(tuple(outs), tuple(lses), return_lse)
 
 

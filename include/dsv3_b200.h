@@ -443,7 +443,7 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* args, void* workspa
  * The results of the same queries over several pieces of their keys (of a long prefix, say; of dsv3_expanded_attention or dsv3_latent_attention), joined:
  *   lse = log sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
  *   outs : host array of `parts` (1 .. 32) pointers to bf16 [rows, dim], contiguous, 16-byte aligned; dim a multiple of 8, up to 2048
- *   lses : host array of pointers to fp32 [rows].  Where a part's is -inf (it sees nothing) its row is not read; where all are: zeros, and -inf
+ *   lses : host array of pointers to fp32 [rows].  Where a part's is -inf (it sees nothing) its row does not count, whatever it holds (it may be read all the same); where all are: zeros, and -inf
  *   out  : bf16 [rows, dim], may be one of the parts; lse: fp32 [rows], may be one of the parts' (or null)
  */
 int dsv3_attention_join(const void* const* outs, const float* const* lses, int parts, int64_t rows, int dim, void* out, float* lse, dsv3_stream_t stream);
