@@ -33,8 +33,8 @@ def expanded_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch
     ``q_nope`` bf16 ``[tokens, heads, 128]``, ``q_rope`` ``[tokens, heads, 64]``, rotated; ``k_nope`` and ``v`` ``[keys, heads, 128]``, ``k_rope`` ``[keys, 64]``; or all
     with the sequences in front.  Strides of tokens and heads are free (multiples of 8).  ``cu_seqlens_q`` and ``cu_seqlens_k`` int32 ``[sequences + 1]``: where the sequences' queries
     and keys begin; without them the batch is the sequences, or all is one.  ``causal``: a sequence's queries are its last keys, and see themselves and all before; else they see all of
-    its keys.  A query that sees nothing gives zeros and -inf.  A key or value that is not
-    finite spoils the results of the queries that see it, and no others."""
+    its keys.  A query that sees nothing gives zeros and -inf.  A score of NaN or +inf, or a value that is
+    not finite, spoils the results of the queries that see its key, and no others; a score of -inf weighs nothing."""
     return host.expanded_attention(q_nope, q_rope, k_nope, k_rope, v, softmax_scale, cu_seqlens_q, cu_seqlens_k, causal, return_lse)
 
 

@@ -410,7 +410,8 @@ int dsv3_latent_attention(const dsv3_latent_cache_t* cache, const void* q_latent
  *   softmax_scale: positive
  *   out bf16 [tokens, heads, 128], lse fp32 [tokens, heads], contiguous.  A query that sees nothing: zeros, and -inf.
  * Sums are fp32, over weights of up to 2^8: values beyond 2^119 / (keys that a query sees) in magnitude can make its results infinite or NaN.
- * A key that is not finite makes the results of the queries that see it NaN, a value that is not finite makes them NaN or infinite in its dimension at least; others are not touched by it.
+ * Not finite: a score of NaN or +inf makes the query's results NaN, one of -inf (an infinite component of the key against one of the query) weighs nothing, and a query all of whose scores are -inf gives
+ * zeros and -inf as if it saw nothing.  A value that is not finite makes the results of the queries that see its key NaN or infinite in its dimension at least.  Other queries are not touched by either.
  * workspace: dsv3_expanded_attention_workspace_bytes() bytes (ragged: cu_seqlens_q is not null), 16-byte aligned, not shared by calls that can overlap; its contents do not matter.  The size is that of
  * exactly these arguments on the current device, 0 for most; dsv3_set_num_sms does not change it.
  */
