@@ -15,9 +15,10 @@ struct QuarterTurns {
 };
 
 // A thread to one angle of kTableUnroll positions.  The angle is reduced to an eighth of a turn either side of a multiple of a quarter turn in 64 bits, so that position
-// 163840 is as exact as position 1; of what is left (r quarters, |r| <= 1/2) sine and cosine are polynomials in r^2, those of their degree whose largest error is least (Remez' exchange: 2^-27 and 2^-34).
-//   HBM bounds what is large (163840 positions of 32 angles 9.4 us, 4.5 TB/s), a launch what is small (4096: 1.8 us in a graph).  Conversions between 64-bit numbers and whole ones are what costs time here (one a cycle and SM): the nearest whole number comes from
-// adding 1.5 * 2^52, and only r is converted.
+// 163840 is as exact as position 1; of what is left (r quarters, |r| <= 1/2) sine and cosine are polynomials in r^2, those of their degree whose largest error is least (Remez' exchange: 2^-29.6 and 2^-34.1), in
+// 64 bits as well, and rounded once: off by 0.52 * 2^-24 at most.  (In 32 bits, which took as long, by 1.7 * 2^-24, and 43 % of the sines were not the rounded ones.)
+//   HBM bounds what is large (163840 positions of 32 angles 9.1 us, 4.6 TB/s), a launch what is small (4096: 2.0 us in a graph).  Conversions between 64-bit numbers and whole ones
+// would cost more than all of that (one a cycle and SM; 40 us): the nearest whole number comes from adding 1.5 * 2^52.
 __global__ void __launch_bounds__(kTableThreads) rotary_table_kernel(const __grid_constant__ QuarterTurns f, FastDiv pairs, int block_rows, int64_t start, int64_t length,
                                                                      float2* __restrict__ out) {
     griddep_launch_dependents();
@@ -32,10 +33,10 @@ __global__ void __launch_bounds__(kTableThreads) rotary_table_kernel(const __gri
         if (row >= length) return;
         constexpr double kWhole = 6755399441055744.0;                // 1.5 * 2^52: a sum with it has no fraction, and the whole number in its low bits
         const double sum = fma(position, per, kWhole);
-        const float r = static_cast<float>(fma(position, per, kWhole - sum)), y = r * r;
+        const double r = fma(position, per, kWhole - sum), y = r * r;
         const int q = __double2loint(sum);
-        const float sine = r * fmaf(y, fmaf(y, fmaf(y, -0x1.2d9bb8p-8f, 0x1.465ec6p-4f), -0x1.4abbbap-1f), 0x1.921fb6p+0f);
-        const float cosine = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 0x1.d9c364p-11f, -0x1.55c57cp-6f), 0x1.03c1dcp-2f), -0x1.3bd3ccp+0f), 1.0f);
+        const float sine = static_cast<float>(r * fma(y, fma(y, fma(y, -0x1.2cf5d364ef498p-8, 0x1.465a3d5891be3p-4), -0x1.4abba77bb6abfp-1), 0x1.921fb4e70509bp+0));
+        const float cosine = static_cast<float>(fma(y, fma(y, fma(y, fma(y, 0x1.d9f7bc182813bp-11, -0x1.55c6643b6d261p-6), 0x1.03c1decc705bap-2), -0x1.3bd3cc7ec2b97p+0), 1.0));
         float2 z = q & 1 ? make_float2(-sine, cosine) : make_float2(cosine, sine);
         if (q & 2) z.x = -z.x, z.y = -z.y;
         out[row * pairs.d + pair] = z;

@@ -51,8 +51,8 @@ def rotary_table(length: int, dim: int = 64, theta: float = 10000.0, factor: flo
     """Angles of positions ``start`` ... ``start + length - 1`` as complex64 ``[length, dim / 2]`` (``precompute_freqs_cis``, model.py:297-375).
 
     With a ``factor`` other than 1 slow angles are divided by it, for contexts that many times as long as the ``original_length`` of the training; those that turn more than
-    ``beta_fast`` times over it stay, those that turn between ``beta_slow`` and ``beta_fast`` times are divided by degrees.  Formed in 64 bits and rounded once, so that far
-    positions are as exact as near ones."""
+    ``beta_fast`` times over it stay, those that turn between ``beta_slow`` and ``beta_fast`` times are divided by degrees.  Formed in 64 bits and rounded once (2^-24, and
+    2^-51 of the angle), so that far positions are as exact as near ones."""
     if device is not None:
         device = torch.device(device)
         if device.type != "cuda":

@@ -454,7 +454,8 @@ int dsv3_attention_join(const void* const* outs, const float* const* lses, int p
  *   out[position, i] = exp(1j * position * f_i),  f_i = theta^(-2 i / dim), and for a factor other than 1 (contexts longer than original_length, that the model was trained on)
  *   f_i / factor * ramp + f_i * (1 - ramp),  ramp = (i - low) / (high - low) held to 0 .. 1, low and high the indices (rounded down and up, held to 0 .. dim - 1) of the angles
  *   that turn beta_fast and beta_slow times over original_length: dim log(original_length / (2 pi beta)) / (2 log theta)
- * complex64 [length, dim / 2]; angles are formed in 64 bits (the reference: 32, which at position 100000 is off by 0.004).  dim even, at most 256.
+ * complex64 [length, dim / 2]; angles, sines and cosines are formed in 64 bits and rounded once: off by 2^-24 at most, and 2^-51 of the angle (the reference: 32 bits, which at position 100000 is off by
+ * 0.004).  dim even, at most 256; start at most 2^40.
  */
 int dsv3_rotary_table(int dim, double theta, double factor, int64_t original_length, double beta_fast, double beta_slow, int64_t start, int64_t length,
                       float* out, dsv3_stream_t stream);
