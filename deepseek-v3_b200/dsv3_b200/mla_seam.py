@@ -307,7 +307,8 @@ def install_rotary(model_module) -> None:
                             beta_slow=args.beta_slow, device=torch.get_default_device())
 
     def apply_rotary_emb(x, freqs_cis):
-        return rotary(x, freqs_cis)
+        # (as there: a table that is not of x's tokens and width is an error, not a part of either)
+        return rotary(x, freqs_cis.view(x.size(1), x.size(-1) // 2))
 
     model_module.precompute_freqs_cis = precompute_freqs_cis
     model_module.apply_rotary_emb = apply_rotary_emb
