@@ -65,7 +65,7 @@ def rotary(x: torch.Tensor, freqs_cis: torch.Tensor, positions: Optional[torch.T
            inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` with a part of every head rotated by the angles of its token's position (``apply_rotary_emb``, model.py:378-393).
 
-    ``x`` bf16, fp16 or fp32 ``[tokens, heads, dim]``, or with the sequences in front, of any strides of tokens and heads; ``freqs_cis`` complex64 ``[positions, rotated / 2]``:
+    ``x`` bf16, fp16 or fp32 ``[tokens, heads, dim]`` of any strides of tokens and heads (multiples of 16 bytes), or with the sequences in front, whose tokens are then all one stride apart; ``freqs_cis`` complex64 ``[positions, rotated / 2]``:
     values ``offset`` ... ``offset + rotated - 1`` of a head turn, the others are copied.  ``layout``: ``"interleaved"`` (neighbours are a pair) or ``"half"`` (value ``i`` and value
     ``i + rotated / 2`` of the part).  ``positions`` int64, one per token; without it a sequence's tokens are at 0, 1, ...  A token at a position that the table does not hold
     becomes NaN.  ``inverse`` turns back: the gradient of the rotation.  ``out``: a tensor to write to; ``x`` itself to rotate in place, which leaves the rest of the heads alone."""

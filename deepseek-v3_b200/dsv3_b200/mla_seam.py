@@ -296,10 +296,22 @@ def install_mla(model_module, release_buffers: bool = False, expand_from: Option
     model_module.MLA.forward = forward
 
 
+def _in_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` ``[batch, tokens, heads, dim]``, or a copy of it where ``rotary`` does not take its strides: tokens of a batch that are not one stride apart (a cut from longer sequences), rows that are not contiguous or
+    do not begin at multiples of 16 bytes."""
+    batch, tokens, heads, _ = x.shape
+    b, t, h, last = x.stride()
+    size = x.element_size()
+    lies = (last == 1 and (batch <= 1 or tokens <= 1 or b == tokens * t) and x.data_ptr() % 16 == 0 and (heads <= 1 or h * size % 16 == 0)
+            and (batch * tokens <= 1 or (t if tokens > 1 else b) * size % 16 == 0))
+    return x if lies else x.contiguous()
+
+
 def install_rotary(model_module) -> None:
     """Point ``model_module.apply_rotary_emb`` (model.py:378-393) and ``precompute_freqs_cis`` (model.py:297-375) at ``rotary`` and ``rotary_table``.
 
-    One launch to a rotation instead of five, any strides of tokens and heads; angles are formed in 64 bits.  The table is made on torch's default device, which has to be a CUDA device
+    One launch to a rotation instead of five; angles are formed in 64 bits.  ``x`` is bf16, fp16 or fp32 on a CUDA device, heads of a multiple of 16 values up to 256; of any strides, though rows that are not 16-byte aligned and
+    a batch cut from longer sequences are copied first.  The table is made on torch's default device, which has to be a CUDA device
     (``with torch.device("cuda")``, as the reference's generate.py makes its model)."""
     def precompute_freqs_cis(args):
         factor = args.rope_factor if args.max_seq_len > args.original_seq_len else 1.0
@@ -308,7 +320,7 @@ def install_rotary(model_module) -> None:
 
     def apply_rotary_emb(x, freqs_cis):
         # (as there: a table that is not of x's tokens and width is an error, not a part of either)
-        return rotary(x, freqs_cis.view(x.size(1), x.size(-1) // 2))
+        return rotary(_in_rows(x), freqs_cis.view(x.size(1), x.size(-1) // 2).contiguous())
 
     model_module.precompute_freqs_cis = precompute_freqs_cis
     model_module.apply_rotary_emb = apply_rotary_emb

@@ -33,7 +33,8 @@ def _check(got, x, f):
     want = _want(x, f)
     assert got.dtype == x.dtype and got.shape == x.shape
     # (two products and a sum in fp32, each rounded, and the result; a product is x's largest at most)
-    check(got, want, want.abs() * STEP[x.dtype] + 3 * 2.0 ** -24 * 2 * x.double().abs().amax() + (2.0 ** -24 if x.dtype == torch.float16 else 0.0))
+    most = x.double().abs().amax() if x.numel() else 0.0
+    check(got, want, want.abs() * STEP[x.dtype] + 3 * 2.0 ** -24 * 2 * most + (2.0 ** -24 if x.dtype == torch.float16 else 0.0))
 
 
 def test_a_table_of_other_tokens_or_another_width_is_an_error():
@@ -45,3 +46,30 @@ def test_a_table_of_other_tokens_or_another_width_is_an_error():
     for wrong in (f, f[:29], f[:31], f[:30, :16].contiguous(), f[:30].repeat(1, 2)):
         with pytest.raises(RuntimeError):
             apply(x, wrong)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_strides_that_the_function_it_replaces_takes(dtype):
+    """Cuts from longer sequences, single tokens of them, rows at odd places, dimensions in other orders, values for several heads or sequences in one place, angles with strides."""
+    apply = _apply()
+    whole, f = torch.randn(3, 40, 4, 192, device="cuda").to(dtype), _angles(40, 64)
+    odd = torch.randn(3 * 40 * 4 * 67 + 1, device="cuda").to(dtype)[1:].view(3, 40, 4, 67)
+    cases = [(whole[..., 128:], f), (whole[:, 7:20, :, 128:], f[7:20]), (whole[:, 5:6, :, 128:], f[5:6]), (whole[1:2, 7:20, 1:3, 64:128], f[7:20]), (whole[:, ::2, :, :64], f[::2]),
+             (odd[..., 3:], f), (whole.transpose(1, 2)[..., 128:], f[:4]), (whole[..., :64].transpose(1, 3).contiguous().transpose(1, 3), f), (whole[:, :, :1, 128:].expand(-1, -1, 4, -1), f),
+             (whole[:1, :, :, :64].expand(3, -1, -1, -1), f), (whole[:, :0, :, :64], f[:0]), (whole[:0, :, :, :64], f)]
+    for x, angles in cases:
+        before = x.clone()
+        _check(apply(x, angles), x, angles)
+        assert torch.equal(x, before)
+    _check(apply(whole[..., :64], f.t().contiguous().t()), whole[..., :64], f)
+
+
+def test_what_it_does_not_take():
+    apply = _apply()
+    x, f = torch.randn(1, 3, 2, 64, device="cuda"), _angles(3, 64)
+    with pytest.raises(NotImplementedError):
+        apply(x.double(), f)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        apply(x.cpu(), f.cpu())
+    with pytest.raises(ValueError):
+        apply(x[0], f)
