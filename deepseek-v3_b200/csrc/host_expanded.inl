@@ -152,11 +152,12 @@ std::pair<const char*, const char*> extent(const at::Tensor& t) {
     return {p, p + (last + 1) * static_cast<int64_t>(t.element_size())};
 }
 
-// (x, freqs, positions or None, half_layout, offset, inverse, out or None) -> out
+// (x, freqs, positions or None, half_layout, offset, inverse, out or None) -> out, or None where autograd is to have a gradient, which is the caller's part
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want_args(n, 7);
         const at::Tensor &x = tensor_arg(args[0]), &f = tensor_arg(args[1]);
+        if (c10::GradMode::is_enabled() && (x.requires_grad() || f.requires_grad() || (args[6] != Py_None && tensor_arg(args[6]).requires_grad()))) Py_RETURN_NONE;
         const int half = PyObject_IsTrue(args[3]), inverse = PyObject_IsTrue(args[5]);
         if (half < 0 || inverse < 0) throw PythonError{};
         const int64_t offset = int_arg(args[4]);

@@ -61,6 +61,23 @@ def rotary_table(length: int, dim: int = 64, theta: float = 10000.0, factor: flo
     return host.rotary_table(length, dim, theta, factor, original_length, beta_fast, beta_slow, start, device)
 
 
+class _Rotary(torch.autograd.Function):
+    """A rotation whose gradient is the gradient turned back (and the other way round: the gradient of that is a rotation again)."""
+
+    @staticmethod
+    def forward(ctx, x, freqs_cis, positions, half, offset, inverse):
+        ctx.save_for_backward(freqs_cis, positions)
+        ctx.how = half, offset, inverse
+        return host.rotary(x, freqs_cis, positions, half, offset, inverse, None)
+
+    @staticmethod
+    def backward(ctx, grad):
+        half, offset, inverse = ctx.how
+        # (a gradient may be one number in many places, or lie as whatever made it left it)
+        grad = grad.contiguous() if grad.data_ptr() % 16 == 0 else grad.clone(memory_format=torch.contiguous_format)
+        return _Rotary.apply(grad, *ctx.saved_tensors, half, offset, not inverse), None, None, None, None, None
+
+
 def rotary(x: torch.Tensor, freqs_cis: torch.Tensor, positions: Optional[torch.Tensor] = None, layout: str = "interleaved", offset: int = 0,
            inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` with a part of every head rotated by the angles of its token's position (``apply_rotary_emb``, model.py:378-393).
@@ -68,7 +85,15 @@ def rotary(x: torch.Tensor, freqs_cis: torch.Tensor, positions: Optional[torch.T
     ``x`` bf16, fp16 or fp32 ``[tokens, heads, dim]`` of any strides of tokens and heads (multiples of 16 bytes), or with the sequences in front, whose tokens are then all one stride apart; ``freqs_cis`` complex64 ``[positions, rotated / 2]``:
     values ``offset`` ... ``offset + rotated - 1`` of a head turn, the others are copied.  ``layout``: ``"interleaved"`` (neighbours are a pair) or ``"half"`` (value ``i`` and value
     ``i + rotated / 2`` of the part).  ``positions`` int64, one per token; without it a sequence's tokens are at 0, 1, ...  A token at a position that the table does not hold
-    becomes NaN.  ``inverse`` turns back: the gradient of the rotation.  ``out``: a tensor to write to; ``x`` itself to rotate in place, which leaves the rest of the heads alone."""
+    becomes NaN.  ``inverse`` turns back: the gradient of the rotation, which ``x`` has where autograd asks for one (``freqs_cis`` has none).  ``out``: a tensor to write to; ``x`` itself to rotate in place, which leaves
+    the rest of the heads alone; as everywhere, not where a gradient is asked for."""
     if layout not in ("interleaved", "half"):
         raise ValueError(f"layout must be 'interleaved' or 'half', not {layout!r}")
-    return host.rotary(x, freqs_cis, positions, layout == "half", offset, inverse, out)
+    turned = host.rotary(x, freqs_cis, positions, layout == "half", offset, inverse, out)
+    if turned is None:                                      # (nothing was done: a gradient is asked for)
+        if freqs_cis.requires_grad:
+            raise NotImplementedError("rotary has no gradient for freqs_cis")
+        if out is not None:
+            raise RuntimeError("rotary: a result that is written to out has no gradient")
+        return _Rotary.apply(x, freqs_cis, positions, layout == "half", offset, inverse)
+    return turned
