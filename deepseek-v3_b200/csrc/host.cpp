@@ -911,6 +911,7 @@ PyMethodDef methods[] = {
     {"attention_join", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_attention_join)), METH_FASTCALL, "(outs, lses, return_lse)"},
     {"rotary_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_rotary_table)), METH_FASTCALL,
      "(length, dim, theta, factor, original_length, beta_fast, beta_slow, start, device)"},
+    {"rotary_takes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_rotary_takes)), METH_FASTCALL, "(x, freqs)"},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_rotary)), METH_FASTCALL, "(x, freqs, positions, half_layout, offset, inverse, out)"},
     {"set_stats", py_set_stats, METH_O, "dict whose counters linear() keeps"},
     {"forget", py_forget, METH_NOARGS, "drop the remembered quantisations"},

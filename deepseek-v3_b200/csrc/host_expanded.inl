@@ -152,6 +152,19 @@ std::pair<const char*, const char*> extent(const at::Tensor& t) {
     return {p, p + (last + 1) * static_cast<int64_t>(t.element_size())};
 }
 
+// (x, freqs) -> whether rotary takes a batch [batch, tokens, heads, dim] as it lies, with the angles [tokens, dim / 2] of all of its heads' values: tokens one stride apart, rows at multiples of 16 bytes
+PyObject* py_rotary_takes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want_args(n, 2);
+        const at::Tensor &x = tensor_arg(args[0]), &f = tensor_arg(args[1]);
+        if (x.dim() != 4) raise(PyExc_ValueError, "x must be [batch, tokens, heads, dim]");
+        const int64_t batch = x.size(0), tokens = x.size(1), each = 16 / std::max<int64_t>(1, static_cast<int64_t>(x.element_size())), step = tokens > 1 ? x.stride(1) : x.stride(0);
+        return PyBool_FromLong(f.dim() == 2 && f.size(0) == tokens && f.size(1) == x.size(3) / 2 && f.is_contiguous() && x.stride(3) == 1 &&
+                               (batch <= 1 || tokens <= 1 || x.stride(0) == tokens * step) && (batch * tokens <= 1 || step % each == 0) && (x.size(2) <= 1 || x.stride(2) % each == 0) &&
+                               reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0);
+    });
+}
+
 // (x, freqs, positions or None, half_layout, offset, inverse, out or None) -> out, or None where autograd is to have a gradient, which is the caller's part
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {

@@ -296,17 +296,6 @@ def install_mla(model_module, release_buffers: bool = False, expand_from: Option
     model_module.MLA.forward = forward
 
 
-def _in_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` ``[batch, tokens, heads, dim]``, or a copy of it where ``rotary`` does not take its strides: tokens of a batch that are not one stride apart (a cut from longer sequences), rows that are not contiguous or
-    do not begin at multiples of 16 bytes."""
-    batch, tokens, heads, _ = x.shape
-    b, t, h, last = x.stride()
-    size = x.element_size()
-    lies = (last == 1 and (batch <= 1 or tokens <= 1 or b == tokens * t) and x.data_ptr() % 16 == 0 and (heads <= 1 or h * size % 16 == 0)
-            and (batch * tokens <= 1 or (t if tokens > 1 else b) * size % 16 == 0))
-    return x if lies else x.contiguous()
-
-
 def install_rotary(model_module) -> None:
     """Point ``model_module.apply_rotary_emb`` (model.py:378-393) and ``precompute_freqs_cis`` (model.py:297-375) at ``rotary`` and ``rotary_table``.
 
@@ -319,8 +308,12 @@ def install_rotary(model_module) -> None:
                             beta_slow=args.beta_slow, device=torch.get_default_device())
 
     def apply_rotary_emb(x, freqs_cis):
-        # (as there: a table that is not of x's tokens and width is an error, not a part of either)
-        return rotary(_in_rows(x), freqs_cis.view(x.size(1), x.size(-1) // 2).contiguous())
+        if not host.rotary_takes(x, freqs_cis):
+            # (as there: a table that is not of x's tokens and width is an error, not a part of either)
+            freqs_cis = freqs_cis.view(x.size(1), x.size(3) // 2).contiguous()
+            if not host.rotary_takes(x, freqs_cis):
+                x = x.clone(memory_format=torch.contiguous_format)
+        return rotary(x, freqs_cis)
 
     model_module.precompute_freqs_cis = precompute_freqs_cis
     model_module.apply_rotary_emb = apply_rotary_emb
