@@ -1112,8 +1112,11 @@ Plan plan_of(const Call& c, int sms) {
     // Groups of heads, equal ones: as few as keep a group's keys and values in the L2, and no more than leave each of them an item to an SM (or pair).  In long rows of calls, in groups of 16 MB, 32, 64 or all
     // heads at once: 4096 tokens of 128 heads 607, 606, 622 and 675 us; 16001 of 16 heads, which then are too few to a group, 1050, 980, 1005 and 1004; 515 of 128 heads over 4099 keys 221, 221, 221
     // and 234 (with two items to an SM at least, 233 for 32 MB).
+    //   Two items where lengths may differ: the longest come first within a group only, so that a group with few of them ends with SMs that wait, the last one above all.  Seven prompts of 16 heads, 70 to 2050 queries
+    // over up to 4610 keys, 130 us with two and 154 with one; eleven of 32 heads, one of them of 4000 tokens, 198 and 218; four of 64 heads 214 and 229; three of 24 heads 181 and 195.  The other way round 800 and
+    // 3000 queries of 32 heads 345 and 335; three times 1024 of 128 heads over 3000 keys 505 and 492; 600, 70 and 1200 of 128 heads 282 and 275.  Of 21 batches 6 gain 3 to 16 %, 4 lose 2 to 3 %, 11 stay.
     const int64_t bytes = c.heads * c.kv_tokens * 2 * (kNope + kValue);
-    const int64_t groups = c.n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, pl.blocks * c.heads / std::max(1, sms / pl.ctas)));
+    const int64_t groups = c.n_seqs > kLanes ? 1 : std::max<int64_t>(1, std::min(bytes / kGroupBytes, pl.blocks * c.heads / ((c.ragged && c.n_seqs > 1 ? 2 : 1) * std::max(1, sms / pl.ctas))));
     pl.head_group = static_cast<int>((c.heads + groups - 1) / groups);
     return pl;
 }
