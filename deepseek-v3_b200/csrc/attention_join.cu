@@ -153,7 +153,11 @@ extern "C" int dsv3_attention_join(const void* const* outs, const float* const* 
                        parts, static_cast<long long>(rows), dim);
         return DSV3_ERR_UNSUPPORTED;
     }
-    if (rows == 0 || dim == 0) return DSV3_OK;
+    if (rows == 0 || (dim == 0 && !lse)) return DSV3_OK;
+    if (dim == 0) {
+        set_last_error("attention_join: rows without values have no threads that would join their logarithms");
+        return DSV3_ERR_UNSUPPORTED;
+    }
     for (int i = 0; i < parts; ++i) {
         if (!outs[i] || !lses[i] || !out) {
             set_last_error("attention_join: null pointer");

@@ -108,8 +108,9 @@ PyObject* py_attention_join(PyObject*, PyObject* const* args, Py_ssize_t n) {
             if (o.scalar_type() != at::kBFloat16 || l.scalar_type() != at::kFloat) raise(PyExc_NotImplementedError, "attention_join takes bfloat16 parts and float32 lses");
             outs[i] = o.const_data_ptr(), lses[i] = static_cast<const float*>(l.const_data_ptr());
         }
-        const int64_t dim = first.size(-1), rows = dim > 0 ? first.numel() / dim : 0;
+        const int64_t dim = first.size(-1), rows = dim > 0 ? first.numel() / dim : 0, l_rows = tensor_arg(PyTuple_GET_ITEM(args[1], 0)).numel();
         if (dim > 2048) raise(PyExc_NotImplementedError, "attention_join takes at most 2048 values a row");
+        if (dim == 0 && with_lse && l_rows > 0) raise(PyExc_NotImplementedError, "attention_join does not join the logarithms of rows without values");
         c10::SmallVector<int64_t, 6> sizes(first.sizes().begin(), first.sizes().end());
         at::Tensor out = new_cuda(sizes, at::kBFloat16, dev), lse;
         sizes.pop_back();

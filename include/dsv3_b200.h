@@ -443,7 +443,7 @@ int dsv3_expanded_attention(const dsv3_expanded_attention_t* args, void* workspa
 /*
  * The results of the same queries over several pieces of their keys (of a long prefix, say; of dsv3_expanded_attention or dsv3_latent_attention), joined:
  *   lse = log sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
- *   outs : host array of `parts` (1 .. 32) pointers to bf16 [rows, dim], contiguous, 16-byte aligned; dim a multiple of 8, up to 2048
+ *   outs : host array of `parts` (1 .. 32) pointers to bf16 [rows, dim], contiguous, 16-byte aligned; dim a multiple of 8, up to 2048 (of 0 there is nothing to do, and no lse)
  *   lses : host array of pointers to fp32 [rows].  Where a part's is -inf (it sees nothing) its row does not count, whatever it holds (it may be read all the same); where all are: zeros, and -inf
  *   out  : bf16 [rows, dim], may be one of the parts; lse: fp32 [rows], may be one of the parts' (or null)
  */
