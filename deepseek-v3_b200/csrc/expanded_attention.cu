@@ -9,8 +9,8 @@
 // operands of the first keep busy.
 //   Long chunks are worked on by CTAs in pairs (cta_group::2): halves of 256 queries, 128 in either CTA, and either loads half of the keys' rows and half of the values' dimensions for both.
 // The ring of keys and values then holds three tiles, not one and a half, and loads half as much: 16001 tokens of 16 heads 844 us, 942 by CTAs alone.
-//   The reference m of a row moves only where a weight would pass 2^8, so that sums are hardly ever rescaled; weights are rounded to bf16, relative to themselves
-// (2^-9), sums and statistics are fp32.
+//   The reference m of a row moves only where a weight would pass 2^8, so that sums are hardly ever rescaled; weights are rounded to bf16 (by 2^-8 of themselves
+// at most: the tensor cores' type, and what the reference rounds its scores to), sums and statistics are fp32.
 //   Blocks of at most half as many queries give both halves the same queries and every other tile of the keys, and join the halves at the end; where there are fewer blocks
 // than SMs, the keys of each are cut in parts for as many CTAs, and a second kernel joins those.
 //   What bounds it: the tensor cores on long sequences.  8192 queries and keys of 32 heads, each query seeing all keys: 855 us, 1607 TFLOP/s, as much as a large matrix product reaches (seeing
@@ -1073,7 +1073,9 @@ struct Call {
 };
 // How long a plan takes, in times that half a block of a CTA alone takes for a tile (1.03 us): what there is to do, spread over all SMs, or its longest item; where all items are about as long, as many
 // rounds of them as there are.  A pair's tile takes 0.807 of that, an item's begin and end as long as 2.5 of its half's tiles (of a pair's 4.5), a join 5.9 and 56 more for a million partial rows.
-// Fitted to 78 calls of 1 to 16001 queries and 37 to 16384 keys, alone and in pairs, 26 of them in up to 12 parts.  Of those it picks the fastest or one at most 6 % slower.
+// Fitted to 78 calls of 1 to 16001 queries and 37 to 16384 keys, alone and in pairs, 26 of them in up to 12 parts.  Held against either kind of CTAs and up to 32 parts of 45 calls it picks the fastest, or one at
+// most 4 % slower, for 35 of them; farthest off are 768 queries of 16 heads over themselves (alone 18.2 us, in pairs 15.1), 3000 of 5 heads (four parts alone 34.8, three in pairs 29.6), 64 of 16 heads over 8192 keys (nine
+// parts 25.0, eight 22.4) and 200 of 16 heads over themselves (10.2, in pairs 9.3).
 //   Parts of 2, 3 and 4: 515 queries of 16 heads over 4099 keys 45.2, 36.5 and 41.5 us; 512 over 8192 in pairs 65.9, 51.5 and 44.6; 2 heads of 16001 tokens in pairs 121, 130 and 133, and 195 in one.
 // Alone / in pairs: 512 queries of 128 heads over 512 keys 24.0 / 28.9 us, over 2048 79.4 / 70.6, over 8192 298 / 250; 1000 of 16 over 8000 78.7 / 69.3; 16001 of 16 over themselves 942 / 836.
 struct Work {

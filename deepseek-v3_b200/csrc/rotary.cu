@@ -117,7 +117,8 @@ struct Eight<float> {
 // A unit is eight values of a head, four pairs if they turn: side by side, or in the layout of halves four of either half.  A thread keeps its unit's angles in registers and
 // takes every `teams`-th head of its token.  HBM bounds it: heads are asked for kUnroll at once, before the angles, which come by way of the position.  Reads of a unit come before its
 // writes, so that out may be x.  4099 tokens of 128 heads of 64: 21.6 us, 22.2 in halves, 6.2 TB/s of what is read and written (from a cold L2 23.8); a part of 2047 tokens of 32 heads of 192 10.4 us
-// (units of eight values of either half: 12.7); 64 tokens of 16 heads 1.6 us in a graph, a launch.
+// (units of eight values of either half: 12.7); 64 tokens of 16 heads 1.6 us in a graph, a launch.  fp32 values take 71 to 74 registers, three blocks to an SM: 4099 tokens of 128 heads, cut from heads of 192, 46.3 us, 41.8 in
+// halves, 5.8 and 6.4 TB/s (16 bits: 22.2 and 23.7 of such).
 template <typename T, bool kHalf>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 3) rotary_kernel(const Rows r) {
     griddep_launch_dependents();
