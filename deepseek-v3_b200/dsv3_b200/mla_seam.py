@@ -157,6 +157,29 @@ def _is_causal(mask: torch.Tensor, start_pos: int) -> torch.Tensor:
 _MOST_PARTS = 32        # of attention_join
 
 
+def _steps(count: int, most: int):
+    """``count`` things in equal steps of ``most`` at most (and of one at least)."""
+    steps = -(-count // max(1, most))
+    return [slice(count * i // steps, count * (i + 1) // steps) for i in range(steps)]
+
+
+def _attend_in_steps(q_nope, q_rope, latent, k_rope, weight, room: int, softmax_scale: float, causal: bool, with_lse: bool):
+    """Attention to cached tokens that are expanded for some heads, and of one head for some sequences, at a time: ``room`` tokens times heads."""
+    bsz, seqlen, heads, _ = q_nope.shape
+    tokens = latent.size(1)
+    out = q_nope.new_empty(bsz, seqlen, heads, VALUE_DIM)
+    lse = q_nope.new_empty(bsz, seqlen, heads, dtype=torch.float32) if with_lse else None
+    for seqs in _steps(bsz, room // tokens):
+        for some in _steps(heads, room // ((seqs.stop - seqs.start) * tokens)):
+            kv = torch.nn.functional.linear(latent[seqs], weight[some].flatten(0, 1)).unflatten(-1, (-1, NOPE_DIM + VALUE_DIM))
+            got = expanded_attention(q_nope[seqs, :, some], q_rope[seqs, :, some], kv[..., :NOPE_DIM], k_rope[seqs], kv[..., NOPE_DIM:], softmax_scale, causal=causal, return_lse=with_lse)
+            out[seqs, :, some] = got[0] if with_lse else got
+            if with_lse:
+                lse[seqs, :, some] = got[1]
+            del kv, got
+    return (out, lse) if with_lse else out
+
+
 def _attend_expanded(q_nope, q_rope, cache: MlaCache, table, start_pos: int, weight, softmax_scale: float, expand_tokens: int) -> torch.Tensor:
     """Causal attention of a chunk at ``start_pos`` to its sequences' cached tokens, expanded with ``weight`` ``[heads, 256, 512]``.  The tokens before the chunk's page are expanded and attended
     to in pieces of whole pages, ``expand_tokens`` of all sequences together to a piece, and the pieces' results joined (each is rounded to bf16 first, as a result is; the join's sums are fp32).
@@ -168,29 +191,11 @@ def _attend_expanded(q_nope, q_rope, cache: MlaCache, table, start_pos: int, wei
         tokens = end - first
         ends = torch.arange(0, (bsz + 1) * tokens, tokens, dtype=torch.int32, device=q_nope.device)
         latent, k_rope = latent_cache_read(cache.pool, table[:, first // PAGE:], ends, bsz * tokens)
-        latent, k_rope = latent.view(bsz, tokens, -1), k_rope.view(bsz, tokens, -1)
-
-        def some(seqs, some_heads):
-            kv = torch.nn.functional.linear(latent[seqs], weight[some_heads].flatten(0, 1)).unflatten(-1, (-1, NOPE_DIM + VALUE_DIM))
-            return expanded_attention(q_nope[seqs, :, some_heads], q_rope[seqs, :, some_heads], kv[..., :NOPE_DIM], k_rope[seqs], kv[..., NOPE_DIM:], softmax_scale, causal=causal,
-                                      return_lse=with_lse)
-
-        def in_steps(count, most):                          # equal ones
-            steps = -(-count // max(1, most))
-            return [slice(count * i // steps, count * (i + 1) // steps) for i in range(steps)]
-
-        room = expand_tokens * heads                       # of tokens times heads
-        if bsz * tokens * heads <= room:
-            return some(slice(None), slice(None))
-        out = q_nope.new_empty(bsz, seqlen, heads, VALUE_DIM)
-        lse = q_nope.new_empty(bsz, seqlen, heads, dtype=torch.float32) if with_lse else None
-        for seqs in in_steps(bsz, room // tokens):
-            for some_heads in in_steps(heads, room // ((seqs.stop - seqs.start) * tokens)):
-                if with_lse:
-                    out[seqs, :, some_heads], lse[seqs, :, some_heads] = some(seqs, some_heads)
-                else:
-                    out[seqs, :, some_heads] = some(seqs, some_heads)
-        return (out, lse) if with_lse else out
+        k_rope = k_rope.view(bsz, tokens, -1)
+        if bsz * tokens > expand_tokens:
+            return _attend_in_steps(q_nope, q_rope, latent.view(bsz, tokens, -1), k_rope, weight, expand_tokens * heads, softmax_scale, causal, with_lse)
+        kv = torch.nn.functional.linear(latent, weight.flatten(0, 1)).view(bsz, tokens, heads, -1)
+        return expanded_attention(q_nope, q_rope, kv[..., :NOPE_DIM], k_rope, kv[..., NOPE_DIM:], softmax_scale, causal=causal, return_lse=with_lse)
 
     before = start_pos // PAGE * PAGE                      # tokens that may be seen in pieces
     end_pos = start_pos + seqlen
@@ -269,7 +274,8 @@ def mla_forward(self, x: torch.Tensor, start_pos: Union[int, torch.Tensor], freq
         angles = freqs_cis.reshape(-1, ROPE_DIM // 2)      # (of one sequence, or of all)
         if valid is not None:
             angles = torch.where(valid, angles, math.nan)
-        turned = rotary(q_rope, angles, None if len(angles) == seqlen else positions)
+        # (the attention has no gradient)
+        turned = rotary(q_rope.detach() if q_rope.requires_grad else q_rope, angles, None if len(angles) == seqlen else positions)
         out = _attend_expanded(q_nope, turned, cache, table, start_pos, weight, self.softmax_scale, expand_tokens)
         return self.wo(out.flatten(2))
     q_latent = torch.einsum("bshd,hdc->bshc", q_nope, weight[:, :self.qk_nope_head_dim])
